@@ -68,6 +68,7 @@ enum {
     GHIP_TYPE_IQ4_NL = 20,
     GHIP_TYPE_IQ4_XS = 23,
     GHIP_TYPE_I32 = 26,
+    GHIP_TYPE_I64 = 27,
     GHIP_TYPE_IQ2_XXS = 16,
     GHIP_TYPE_IQ2_XS = 17,
     GHIP_TYPE_IQ3_XXS = 18,
@@ -261,6 +262,89 @@ ghip_status ghip_mul_mat_id_subsums(ghip_context *ctx, const ghip_tensor *as, co
 ghip_status ghip_flash_attn_ext(ghip_context *ctx, const ghip_tensor *q, const ghip_tensor *k, const ghip_tensor *v,
                                 const ghip_tensor *mask, const ghip_tensor *sinks, const ghip_tensor *dst,
                                 void *stream);
+
+/* ---- Serving: rotary positions, a paged KV cache, attention over it.
+ *
+ * The cache of one layer is kv [2 D, H_kv, page, pages], F16 or BF16: row j % page
+ * of page table[j / page] holds key j of a sequence, for each KV head its D key
+ * elements and then its D value elements.  Slot `page * i + r` is row r of page i.
+ * All three calls read lengths, slots and pages on the device, allocate nothing
+ * beyond the workspace and can be captured into a graph whose tables change
+ * between replays. */
+
+/* enum ggml_rope_type */
+enum {
+    GHIP_ROPE_NORM = 0,    /* pairs (2 i, 2 i + 1) */
+    GHIP_ROPE_NEOX = 2,    /* pairs (i, i + n_dims / 2) */
+    GHIP_ROPE_MROPE = 8,   /* NEOX pairs, several axes: sections[a] pairs in turn follow axis a */
+    GHIP_ROPE_VISION = 24, /* pairs (i, i + n_dims); each axis starts at the first frequency */
+    GHIP_ROPE_IMROPE = 40, /* NEOX pairs; pair i follows axis i % 3 (axis 3 past its 3 * sections[axis] pairs) */
+};
+
+/* A rotation: pair i turns by pos[axis] * freq_base^(-2 i / n_dims) * freq_scale
+ * / factors[i].  Elements past the pairs are left as they are.  With several
+ * axes the pairs repeat the sections (time, height, width, extra) in turn.
+ * ext_factor != 0 keeps short wavelengths unscaled: pairs that turn more than
+ * beta_fast times over n_ctx_orig positions keep their frequency, those below
+ * beta_slow take freq_scale, with a ramp between, and cos and sin grow by
+ * 1 + 0.1 ln(1 / freq_scale).  attn_factor multiplies both. */
+typedef struct ghip_rope_params {
+    int32_t n_dims;      /* even; 2..256 (VISION: ..128, and 2 n_dims <= D) */
+    int32_t mode;        /* GHIP_ROPE_* */
+    int32_t sections[4]; /* MROPE, IMROPE, VISION */
+    double freq_base, freq_scale; /* 64 bits: what they are off by grows with the position */
+    double ext_factor, attn_factor, beta_fast, beta_slow;
+    int32_t n_ctx_orig;
+} ghip_rope_params;
+
+/* dst = x rotated.
+ *   x, dst:  F32 | F16 | BF16 [D, H, T], the same type (nb0 == the element, any
+ *            other strides); dst may be x itself
+ *   pos:     I32 [T] or, with several axes, I32 [T, axes] (nb0 == 4)
+ *   factors: F32 [pairs] or NULL
+ * Angles are formed in 64 bits and outputs rounded once.  */
+ghip_status ghip_rope(ghip_context *ctx, const ghip_tensor *x, const ghip_tensor *pos, const ghip_tensor *factors,
+                      const ghip_rope_params *rope, const ghip_tensor *dst, void *stream);
+
+/* Write T tokens' keys and values into a paged cache, the keys rotated on the
+ * way (rope NULL: as they are; then pos and factors are NULL too).
+ *   k, v:  F32, or both of kv's type, [D, H_kv, T] (nb0 == the element), D <= 256
+ *   slots: I64 [T]; a negative slot (padding) or one outside the cache writes
+ *          nothing.  Slots of one call must differ.
+ *   kv:    F16 | BF16 [2 D, H_kv, page, pages] (nb0 == 2)
+ * k and v must not overlap kv. */
+ghip_status ghip_kv_append(ghip_context *ctx, const ghip_tensor *k, const ghip_tensor *v, const ghip_tensor *slots,
+                           const ghip_tensor *pos, const ghip_tensor *factors, const ghip_rope_params *rope,
+                           const ghip_tensor *kv, void *stream);
+
+typedef struct ghip_paged_params {
+    float scale;      /* of q . k */
+    int32_t window;   /* keys a row sees, its own among them; 0: all */
+    int32_t n_first;  /* keys at the start that every row sees, whatever the window */
+    int32_t n_shared; /* keys at the start that all sequences have in common; 0: none */
+    int32_t max_q;    /* the most query rows of a sequence */
+} ghip_paged_params;
+
+/* dst = attention of a batch of sequences over a paged cache.
+ *   q, dst: F32 [D, H, T] (nb0 == 4), D a multiple of 8 up to 256, H % H_kv == 0;
+ *           dst apart from q
+ *   kv:     F16 | BF16 [2 D, H_kv, page, pages], data and strides multiples of 16 bytes
+ *   seqs:   I32 [3 + per, B] (nb0 == 4): for each sequence its first row in q, its
+ *           number of rows nq, its number of keys nkv (those of its rows among
+ *           them, the last nq) and the pages of its keys in order
+ *   sinks:  F32 [H] or NULL: one more logit of each head, below the line only
+ * Row i of a sequence is at position p = nkv - nq + i and sees the keys j <= p
+ * with j > p - window or j < n_first.  A row that sees nothing gives 0; rows of
+ * q that no sequence names are not written.  n_shared > 0 says that the first
+ * n_shared keys of every sequence hold the same values: they are read through
+ * the first sequence's pages, once for the batch.
+ * Pages of keys that no row sees are not looked at, and what the cache holds
+ * there, NaN included, does not matter.  A row that sees a key on a page outside
+ * [0, pages), or past its table row, gives NaN.  Rows past max_q are not
+ * computed. */
+ghip_status ghip_flash_attn_paged(ghip_context *ctx, const ghip_tensor *q, const ghip_tensor *kv, const ghip_tensor *seqs,
+                                  const ghip_tensor *sinks, const ghip_paged_params *params, const ghip_tensor *dst,
+                                  void *stream);
 
 /* One node of a graph: the op, its sources in ggml order (MUL_MAT: src0,
  * src1; MUL_MAT_ID: as, b, ids; FLASH_ATTN_EXT: q, k, v, mask|NULL,

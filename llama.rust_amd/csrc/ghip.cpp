@@ -20,7 +20,7 @@
 
 namespace {
 
-const char *const kModules[] = {"ghip_quant.hsaco", "ghip_kq.hsaco", "ghip_gemv.hsaco", "ghip_wquant.hsaco", "ghip_gemm.hsaco", "ghip_fa.hsaco", "ghip_moe.hsaco", "ghip_skinny.hsaco", "ghip_iq.hsaco", "ghip_dense.hsaco"};
+const char *const kModules[] = {"ghip_quant.hsaco", "ghip_kq.hsaco", "ghip_gemv.hsaco", "ghip_wquant.hsaco", "ghip_gemm.hsaco", "ghip_fa.hsaco", "ghip_moe.hsaco", "ghip_skinny.hsaco", "ghip_iq.hsaco", "ghip_dense.hsaco", "ghip_rope.hsaco", "ghip_fap.hsaco"};
 
 struct TypeInfo {
     int blck;
@@ -52,6 +52,7 @@ TypeInfo type_info(int t) {
     case GHIP_TYPE_Q6_K: return {256, 210};
     case GHIP_TYPE_Q8_K: return {256, 292};
     case GHIP_TYPE_I32: return {1, 4};
+    case GHIP_TYPE_I64: return {1, 8};
     case GHIP_TYPE_MXFP4: return {32, 17};
     case GHIP_TYPE_IQ4_NL: return {32, 18};
     case GHIP_TYPE_IQ4_XS: return {256, 136};
@@ -2995,6 +2996,398 @@ ghip_status ghip_quantize_chunk(ghip_context *ctx, int type, const float *src, v
     const unsigned tpb = ti.blck == 256 ? 64 : 256;
     const unsigned grid = (unsigned)((nblocks + tpb - 1) / tpb);
     return ctx->launch(name, dim3(grid), dim3(tpb), 0, (hipStream_t)stream, src, nblocks, (uint8_t *)dst);
+}
+
+}  // extern "C"
+
+// ------------------------------------------------- rotary positions, KV append
+
+namespace {
+
+// Mirrors of the kernels' argument structs in ghip_rope.hip.
+struct RopeTab {
+    double rev[128];
+    uint8_t axis[128];
+    float mscale;
+};
+struct RopeParams {
+    const void *x;
+    void *y;
+    int64_t x_nb1, x_nb2, y_nb1, y_nb2;
+    const int32_t *pos;
+    int64_t pos_nb1;
+    const float *factors;
+    int T, H, D, P;
+    int U, UR, HG;
+    RopeTab tab;
+};
+struct AppendParams {
+    const void *k, *v;
+    int64_t k_nb1, k_nb2, v_nb1, v_nb2;
+    void *kv;
+    int64_t kv_head, kv_row, kv_page;
+    const int64_t *slots;
+    int64_t n_slots;
+    int64_t page;
+    const int32_t *pos;
+    int64_t pos_nb1;
+    const float *factors;
+    int T, H, D, P, U, UR, HG;
+    RopeTab tab;
+};
+
+bool float_type(int t) { return t == GHIP_TYPE_F32 || t == GHIP_TYPE_F16 || t == GHIP_TYPE_BF16; }
+const char *float_name(int t) { return t == GHIP_TYPE_F32 ? "f32" : t == GHIP_TYPE_F16 ? "f16" : "bf16"; }
+// rows of elements, strides in whole elements
+bool elem_rows(const ghip_tensor *t, uint64_t e) {
+    return t->nb[0] == e && t->nb[1] % e == 0 && t->nb[2] % e == 0 && t->nb[3] % e == 0;
+}
+size_t byte_extent(const ghip_tensor *t, uint64_t e) {
+    uint64_t n = e;
+    for (int d = 0; d < 4; d++) {
+        if (t->ne[d] <= 0) return 0;
+        n += (uint64_t)(t->ne[d] - 1) * t->nb[d];
+    }
+    return n;
+}
+
+// The rotation of rows of D elements: its pairs, each pair's axis and turns per
+// position.  The frequencies base^(-2 i / n_dims) come from one power and a
+// running product in long double (off by less than 2^-56 after 128 of them).
+// Context extension mixes the frequency and the scaled one over the pairs whose
+// wavelength lies between n_ctx_orig / beta_fast and n_ctx_orig / beta_slow.
+// Returns the reason it is refused, or null.
+const char *rope_table(const ghip_rope_params &r, int64_t D, RopeTab &tab, int &P, int &axes) {
+    const bool vision = r.mode == GHIP_ROPE_VISION;
+    const bool multi = vision || r.mode == GHIP_ROPE_MROPE || r.mode == GHIP_ROPE_IMROPE;
+    if (!multi && r.mode != GHIP_ROPE_NORM && r.mode != GHIP_ROPE_NEOX) return "mode must be one of GHIP_ROPE_*";
+    if (r.n_dims < 2 || r.n_dims % 2 || r.n_dims > 256) return "n_dims must be even, 2..256";
+    if ((vision ? 2 : 1) * (int64_t)r.n_dims > D) return "n_dims (twice it for VISION) must not pass the head size";
+    if (vision && r.n_dims > 128) return "n_dims of VISION must be at most 128";
+    if (!(r.freq_base > 0.0) || !std::isfinite(r.freq_base)) return "freq_base must be positive";
+    if (!(r.freq_scale > 0.0) || !std::isfinite(r.freq_scale)) return "freq_scale must be positive";
+    if (!std::isfinite(r.ext_factor) || !std::isfinite(r.attn_factor)) return "ext_factor and attn_factor must be finite";
+    int64_t sum = 0;
+    for (int k = 0; k < 4; k++) {
+        if (multi && (r.sections[k] < 0 || r.sections[k] > 256)) return "sections must be 0..256";
+        sum += r.sections[k];
+    }
+    if (multi && sum <= 0) return "sections must not all be 0";
+    P = vision ? r.n_dims : r.n_dims / 2;
+    axes = 1;
+    const long double step = std::pow((long double)r.freq_base, -2.0L / r.n_dims), turn = 6.283185307179586476925L;
+    double low = 0, high = 0;
+    if (r.ext_factor != 0.0) {
+        if (r.n_ctx_orig < 1 || !(r.beta_fast > 0.0) || !(r.beta_slow > 0.0) || r.freq_base == 1.0)
+            return "ext_factor needs n_ctx_orig, beta_fast and beta_slow > 0 and a freq_base other than 1";
+        auto dim = [&](double beta) {
+            return r.n_dims * std::log(r.n_ctx_orig / (beta * (double)turn)) / (2.0 * std::log(r.freq_base));
+        };
+        low = std::max(0.0, std::floor(dim(r.beta_fast)));
+        high = std::min((double)r.n_dims - 1, std::ceil(dim(r.beta_slow)));
+    }
+    long double f = 1.0L;
+    int prev_axis = 0;
+    for (int i = 0; i < P; i++) {
+        int axis = 0;
+        if (multi) {
+            const int j = (int)(i % sum);
+            if (r.mode == GHIP_ROPE_IMROPE) {
+                axis = j % 3;
+                if (j >= 3 * r.sections[axis]) axis = 3;
+            } else {
+                int end = r.sections[0];
+                while (j >= end) end += r.sections[++axis];
+                // each axis of VISION starts at the first frequency
+                if (vision && (axis != prev_axis || j == 0)) f = 1.0L;
+            }
+        }
+        prev_axis = axis;
+        axes = std::max(axes, axis + 1);
+        double scale = r.freq_scale;
+        if (r.ext_factor != 0.0) {
+            const double ramp = std::min(1.0, std::max(0.0, (i - low) / std::max(0.001, high - low)));
+            const double mix = (1.0 - ramp) * r.ext_factor;
+            scale = scale * (1.0 - mix) + mix;
+        }
+        tab.rev[i] = (double)(f * scale / turn);
+        tab.axis[i] = (uint8_t)axis;
+        f *= step;
+    }
+    tab.mscale = (float)r.attn_factor;
+    if (r.ext_factor != 0.0) tab.mscale = (float)(r.attn_factor * (1.0 + 0.1 * std::log(1.0 / r.freq_scale)));
+    return nullptr;
+}
+
+// positions and frequency factors of T tokens; the reason they are refused, or null
+const char *rope_operands(const ghip_tensor *pos, const ghip_tensor *factors, int64_t T, int P, int axes) {
+    if (!pos || pos->type != GHIP_TYPE_I32 || pos->nb[0] != 4 || pos->nb[1] % 4) return "pos must be I32 rows";
+    if (pos->ne[0] < T) return "pos has fewer positions than there are tokens";
+    if (axes > 1 && pos->ne[1] < axes) return "pos needs a row for each axis";
+    if (factors && (factors->type != GHIP_TYPE_F32 || factors->nb[0] != 4 || factors->ne[0] < P))
+        return "factors must be F32, one for each pair";
+    return nullptr;
+}
+
+// Units of 4 pairs where the pairs and what is not rotated divide into them
+// (loads need no alignment beyond the element's).  One head a thread while that
+// leaves too few threads to cover the loads' latency on 256 CUs (8 wavefronts
+// each), else four, which share their angles.
+struct RopeShape {
+    int vec, hn, U, UR, HG;
+    unsigned grid;
+};
+bool rope_shape(int64_t T, int64_t H, int64_t D, int P, RopeShape &r) {
+    r.vec = P % 4 == 0 && D % 8 == 0 ? 4 : 1;
+    r.UR = P / r.vec;
+    r.U = r.UR + (int)((D - 2 * P + 2 * r.vec - 1) / (2 * r.vec));
+    r.hn = T * ((H + 3) / 4) * r.U >= 256 * 8 * 64 ? 4 : 1;
+    r.HG = (int)((H + r.hn - 1) / r.hn);
+    const int64_t n = T * r.HG * r.U;
+    r.grid = (unsigned)((n + 255) / 256);
+    return n < (1ll << 32) - 256;
+}
+
+}  // namespace
+
+extern "C" {
+
+ghip_status ghip_rope(ghip_context *ctx, const ghip_tensor *x, const ghip_tensor *pos, const ghip_tensor *factors,
+                      const ghip_rope_params *rope, const ghip_tensor *dst, void *stream) {
+    if (!ctx) return GHIP_STATUS_BACKEND_ERROR;
+    std::lock_guard<std::mutex> lock(ctx->mu);
+    auto bad = [&](const char *why) { return ctx->fail(GHIP_STATUS_BACKEND_ERROR, "rope: %s", why); };
+    if (!x || !pos || !rope || !dst) return bad("null operand");
+    if (!float_type(x->type) || dst->type != x->type) return bad("x must be F32, F16 or BF16, and dst of its type");
+    const uint64_t e = type_info(x->type).bytes;
+    if (!elem_rows(x, e) || !elem_rows(dst, e)) return bad("x and dst must be rows of elements");
+    for (int d = 0; d < 4; d++)
+        if (x->ne[d] != dst->ne[d] || x->ne[d] < 0) return bad("dst must have the shape of x");
+    if (x->ne[3] != 1) return bad("x must be [D, H, T]");
+    const int64_t D = x->ne[0], H = x->ne[1], T = x->ne[2];
+    if (D > INT32_MAX || H > INT32_MAX || T > INT32_MAX) return bad("dimension too large");
+    RopeParams p;
+    int axes;
+    if (const char *why = rope_table(*rope, D, p.tab, p.P, axes)) return bad(why);
+    if (const char *why = rope_operands(pos, factors, T, p.P, axes)) return bad(why);
+    if (T == 0 || H == 0) return GHIP_STATUS_SUCCESS;
+    if (!x->data || !dst->data || !pos->data) return bad("null data");
+    if (x->data != dst->data && overlaps(x, dst)) return bad("dst must be x itself or lie apart from it");
+    if (x->data == dst->data && (x->nb[1] != dst->nb[1] || x->nb[2] != dst->nb[2]))
+        return bad("dst in the place of x must have its strides");
+    RopeShape r;
+    if (!rope_shape(T, H, D, p.P, r)) return bad("x too large");
+    hipStream_t s = (hipStream_t)stream;
+    if (!ctx->set_device()) return ctx->fail(GHIP_STATUS_BACKEND_ERROR, "hipSetDevice failed");
+    ghip_status st = ctx->begin(s);
+    if (st != GHIP_STATUS_SUCCESS) return st;
+    p.x = x->data;
+    p.y = dst->data;
+    p.x_nb1 = (int64_t)(x->nb[1] / e);
+    p.x_nb2 = (int64_t)(x->nb[2] / e);
+    p.y_nb1 = (int64_t)(dst->nb[1] / e);
+    p.y_nb2 = (int64_t)(dst->nb[2] / e);
+    p.pos = (const int32_t *)pos->data;
+    p.pos_nb1 = (int64_t)(pos->nb[1] / 4);
+    p.factors = factors ? (const float *)factors->data : nullptr;
+    p.T = (int)T;
+    p.H = (int)H;
+    p.D = (int)D;
+    p.U = r.U;
+    p.UR = r.UR;
+    p.HG = r.HG;
+    ctx->allow(dst->data, byte_extent(dst, e), "dst");
+    ctx->expect(p.y, (size_t)(((T - 1) * p.y_nb2 + (H - 1) * p.y_nb1 + D) * (int64_t)e), "dst");
+    char name[64];
+    snprintf(name, sizeof name, "ghip_rope_%s_%s_v%d_h%d", float_name(x->type),
+             rope->mode == GHIP_ROPE_NORM ? "norm" : "half", r.vec, r.hn);
+    return ctx->launch(name, dim3(r.grid), dim3(256), 0, s, p);
+}
+
+ghip_status ghip_kv_append(ghip_context *ctx, const ghip_tensor *k, const ghip_tensor *v, const ghip_tensor *slots,
+                           const ghip_tensor *pos, const ghip_tensor *factors, const ghip_rope_params *rope,
+                           const ghip_tensor *kv, void *stream) {
+    if (!ctx) return GHIP_STATUS_BACKEND_ERROR;
+    std::lock_guard<std::mutex> lock(ctx->mu);
+    auto bad = [&](const char *why) { return ctx->fail(GHIP_STATUS_BACKEND_ERROR, "kv_append: %s", why); };
+    if (!k || !v || !slots || !kv) return bad("null operand");
+    if (kv->type != GHIP_TYPE_F16 && kv->type != GHIP_TYPE_BF16) return bad("kv must be F16 or BF16");
+    if ((k->type != GHIP_TYPE_F32 && k->type != kv->type) || v->type != k->type)
+        return bad("k and v must both be F32 or both of kv's type");
+    const uint64_t e = type_info(k->type).bytes;
+    if (!elem_rows(k, e) || !elem_rows(v, e)) return bad("k and v must be rows of elements");
+    for (int d = 0; d < 4; d++)
+        if (k->ne[d] != v->ne[d] || k->ne[d] < 0) return bad("k and v must have the same shape");
+    if (k->ne[3] != 1) return bad("k and v must be [D, H_kv, T]");
+    const int64_t D = k->ne[0], H = k->ne[1], T = k->ne[2];
+    if (D < 1 || D > 256) return bad("head size must be 1..256");
+    if (H > INT32_MAX || T > INT32_MAX) return bad("dimension too large");
+    if (!elem_rows(kv, 2) || kv->ne[0] != 2 * D || kv->ne[1] != H || kv->ne[2] < 1 || kv->ne[3] < 0)
+        return bad("kv must be [2 D, H_kv, page, pages]");
+    if (kv->ne[2] > INT32_MAX || kv->ne[3] > INT32_MAX) return bad("dimension too large");
+    if (slots->type != GHIP_TYPE_I64 || slots->nb[0] != 8 || slots->ne[0] < T) return bad("slots must be I64, one for each token");
+    AppendParams p;
+    p.P = 0;
+    p.pos = nullptr;
+    p.pos_nb1 = 0;
+    p.factors = nullptr;
+    if (rope) {
+        int axes;
+        if (const char *why = rope_table(*rope, D, p.tab, p.P, axes)) return bad(why);
+        if (const char *why = rope_operands(pos, factors, T, p.P, axes)) return bad(why);
+        p.pos = (const int32_t *)pos->data;
+        p.pos_nb1 = (int64_t)(pos->nb[1] / 4);
+        p.factors = factors ? (const float *)factors->data : nullptr;
+    } else if (pos || factors) {
+        return bad("pos and factors need a rotation");
+    }
+    if (T == 0 || H == 0) return GHIP_STATUS_SUCCESS;
+    if (!k->data || !v->data || !slots->data || (!kv->data && kv->ne[3]) || (rope && !pos->data)) return bad("null data");
+    if (kv->ne[3] && (overlaps(k, kv) || overlaps(v, kv))) return bad("k and v must lie apart from kv");
+    RopeShape r;
+    if (!rope_shape(T, H, D, p.P, r)) return bad("k too large");
+    hipStream_t s = (hipStream_t)stream;
+    if (!ctx->set_device()) return ctx->fail(GHIP_STATUS_BACKEND_ERROR, "hipSetDevice failed");
+    ghip_status st = ctx->begin(s);
+    if (st != GHIP_STATUS_SUCCESS) return st;
+    p.k = k->data;
+    p.v = v->data;
+    p.k_nb1 = (int64_t)(k->nb[1] / e);
+    p.k_nb2 = (int64_t)(k->nb[2] / e);
+    p.v_nb1 = (int64_t)(v->nb[1] / e);
+    p.v_nb2 = (int64_t)(v->nb[2] / e);
+    p.kv = kv->data;
+    p.kv_head = (int64_t)(kv->nb[1] / 2);
+    p.kv_row = (int64_t)(kv->nb[2] / 2);
+    p.kv_page = (int64_t)(kv->nb[3] / 2);
+    p.slots = (const int64_t *)slots->data;
+    p.n_slots = kv->ne[2] * kv->ne[3];
+    p.page = p.kv_page == p.kv_row * kv->ne[2] ? 0 : kv->ne[2];
+    p.T = (int)T;
+    p.H = (int)H;
+    p.D = (int)D;
+    p.U = r.U;
+    p.UR = r.UR;
+    p.HG = r.HG;
+    ctx->allow(kv->data, byte_extent(kv, 2), "kv");
+    if (p.n_slots)
+        ctx->expect(p.kv, (size_t)(2 * ((kv->ne[3] - 1) * p.kv_page + (kv->ne[2] - 1) * p.kv_row + (H - 1) * p.kv_head + 2 * D)), "kv");
+    char name[64];
+    snprintf(name, sizeof name, "ghip_append_%s_%s_%s_v%d_h%d", float_name(k->type), float_name(kv->type),
+             rope && rope->mode != GHIP_ROPE_NORM ? "half" : "norm", r.vec, r.hn);
+    return ctx->launch(name, dim3(r.grid), dim3(256), 0, s, p);
+}
+
+}  // extern "C"
+
+// ------------------------------------------------ attention over a paged KV cache
+
+namespace {
+
+// Mirror of FapParams in ghip_fap.hip.
+struct FapParams {
+    const float *q;
+    int64_t q_nb1, q_nb2;
+    const uint16_t *kv;
+    int64_t kv_head, kv_row, kv_page;
+    int n_pages, page;
+    const int32_t *seqs;
+    int64_t seq_nb1;
+    int per, B;
+    const float *sinks;
+    float *dst;
+    int64_t d_nb1, d_nb2;
+    int T, H, H_kv, D;
+    float scale;
+    int window, n_first, n_shared, max_q;
+};
+
+bool plan_fap(ghip_context *ctx, const ghip_tensor *q, const ghip_tensor *kv, const ghip_tensor *seqs,
+              const ghip_tensor *sinks, const ghip_tensor *d, const ghip_paged_params *pp, FapParams &p, ghip_status &st) {
+    st = GHIP_STATUS_BACKEND_ERROR;
+    auto bad = [&](const char *why) { st = ctx->fail(GHIP_STATUS_BACKEND_ERROR, "flash_attn_paged: %s", why); return false; };
+    if (!q || !kv || !seqs || !d || !pp) return bad("null operand");
+    if (q->type != GHIP_TYPE_F32 || !elem_rows(q, 4) || d->type != GHIP_TYPE_F32 || !elem_rows(d, 4))
+        return bad("q and dst must be F32 rows");
+    for (int i = 0; i < 4; i++)
+        if (q->ne[i] != d->ne[i] || q->ne[i] < 0) return bad("dst must have the shape of q");
+    const int64_t D = q->ne[0], H = q->ne[1], T = q->ne[2];
+    if (q->ne[3] != 1) return bad("q must be [D, H, T]");
+    if (D < 8 || D > 256 || D % 8) return bad("head size must be a multiple of 8, 8..256");
+    if (kv->type != GHIP_TYPE_F16 && kv->type != GHIP_TYPE_BF16) return bad("kv must be F16 or BF16");
+    if (kv->nb[0] != 2 || kv->ne[0] != 2 * D || kv->ne[1] < 1 || kv->ne[2] < 1 || kv->ne[3] < 0)
+        return bad("kv must be [2 D, H_kv, page, pages]");
+    if (kv->nb[1] % 16 || kv->nb[2] % 16 || kv->nb[3] % 16 || (uintptr_t)kv->data % 16)
+        return bad("kv and its strides must be multiples of 16 bytes");
+    const int64_t H_kv = kv->ne[1], page = kv->ne[2];
+    if (H % H_kv) return bad("H % H_kv != 0");
+    if (H > 65535 || T > INT32_MAX || page > INT32_MAX || kv->ne[3] > INT32_MAX) return bad("dimension too large");
+    if (seqs->type != GHIP_TYPE_I32 || seqs->nb[0] != 4 || seqs->nb[1] % 4 || seqs->ne[0] < 3 || seqs->ne[1] < 0 ||
+        seqs->ne[2] != 1 || seqs->ne[3] != 1)
+        return bad("seqs must be I32 [3 + pages of a sequence, sequences]");
+    const int64_t per = seqs->ne[0] - 3, B = seqs->ne[1];
+    if (per * page > INT32_MAX || B > INT32_MAX) return bad("dimension too large");
+    if (sinks && (sinks->type != GHIP_TYPE_F32 || sinks->nb[0] != 4 || sinks->ne[0] < H)) return bad("sinks must be F32 [H]");
+    if (!std::isfinite(pp->scale)) return bad("scale must be finite");
+    if (pp->window < 0 || pp->n_first < 0) return bad("window and n_first must not be negative");
+    if (pp->n_shared < 0 || pp->n_shared > per * page) return bad("n_shared must be 0 .. the keys of a table row");
+    if (pp->max_q < 0) return bad("max_q must not be negative");
+    if (T && H && B) {
+        if (!q->data || !d->data || !seqs->data || (!kv->data && kv->ne[3])) return bad("null data");
+        if (overlaps(q, d)) return bad("dst must lie apart from q");
+    }
+    p.q = (const float *)q->data;
+    p.q_nb1 = (int64_t)(q->nb[1] / 4);
+    p.q_nb2 = (int64_t)(q->nb[2] / 4);
+    p.kv = (const uint16_t *)kv->data;
+    p.kv_head = (int64_t)(kv->nb[1] / 2);
+    p.kv_row = (int64_t)(kv->nb[2] / 2);
+    p.kv_page = (int64_t)(kv->nb[3] / 2);
+    p.n_pages = (int)kv->ne[3];
+    p.page = (int)page;
+    p.seqs = (const int32_t *)seqs->data;
+    p.seq_nb1 = (int64_t)(seqs->nb[1] / 4);
+    p.per = (int)per;
+    p.B = (int)B;
+    p.sinks = sinks ? (const float *)sinks->data : nullptr;
+    p.dst = (float *)d->data;
+    p.d_nb1 = (int64_t)(d->nb[1] / 4);
+    p.d_nb2 = (int64_t)(d->nb[2] / 4);
+    p.T = (int)T;
+    p.H = (int)H;
+    p.H_kv = (int)H_kv;
+    p.D = (int)D;
+    p.scale = pp->scale;
+    p.window = pp->window;
+    p.n_first = pp->n_first;
+    p.n_shared = pp->n_shared;
+    p.max_q = (int)std::min<int64_t>(pp->max_q, T);
+    st = GHIP_STATUS_SUCCESS;
+    return true;
+}
+
+}  // namespace
+
+extern "C" {
+
+ghip_status ghip_flash_attn_paged(ghip_context *ctx, const ghip_tensor *q, const ghip_tensor *kv, const ghip_tensor *seqs,
+                                  const ghip_tensor *sinks, const ghip_paged_params *params, const ghip_tensor *dst,
+                                  void *stream) {
+    if (!ctx) return GHIP_STATUS_BACKEND_ERROR;
+    std::lock_guard<std::mutex> lock(ctx->mu);
+    FapParams p;
+    ghip_status st;
+    if (!plan_fap(ctx, q, kv, seqs, sinks, dst, params, p, st)) return st;
+    if (p.max_q == 0 || p.H == 0 || p.B == 0) return GHIP_STATUS_SUCCESS;
+    hipStream_t s = (hipStream_t)stream;
+    if (!ctx->set_device()) return ctx->fail(GHIP_STATUS_BACKEND_ERROR, "hipSetDevice failed");
+    st = ctx->begin(s);
+    if (st != GHIP_STATUS_SUCCESS) return st;
+    ctx->allow(dst->data, byte_extent(dst, 4), "dst");
+    ctx->expect(p.dst, (size_t)(4 * ((p.T - 1) * p.d_nb2 + (p.H - 1) * p.d_nb1 + p.D)), "dst");
+    const int64_t n = (int64_t)p.B * p.max_q * p.H;
+    if (n > INT32_MAX) return ctx->fail(GHIP_STATUS_BACKEND_ERROR, "flash_attn_paged: too many rows");
+    return ctx->launch(kv->type == GHIP_TYPE_F16 ? "ghip_fap_rows_f16" : "ghip_fap_rows_bf16", dim3((unsigned)n), dim3(64), 0, s, p);
 }
 
 }  // extern "C"

@@ -101,6 +101,9 @@ void *reg_proc_address(const ggml_hip_backend_reg *, const char *name) {
         {"ghip_mul_mat_id", (void *)&ghip_mul_mat_id},
         {"ghip_mul_mat_id_subsums", (void *)&ghip_mul_mat_id_subsums},
         {"ghip_flash_attn_ext", (void *)&ghip_flash_attn_ext},
+        {"ghip_rope", (void *)&ghip_rope},
+        {"ghip_kv_append", (void *)&ghip_kv_append},
+        {"ghip_flash_attn_paged", (void *)&ghip_flash_attn_paged},
         {"ghip_quantize_chunk", (void *)&ghip_quantize_chunk},
         {"ghip_graph_compute", (void *)&ghip_graph_compute},
         {"ghip_set_workspace", (void *)&ghip_set_workspace},

@@ -19,10 +19,12 @@ Q2_K, Q3_K = 10, 11
 IQ4_NL, IQ4_XS, NVFP4 = 20, 23, 40
 Q1_0, Q2_0 = 41, 42
 BF16 = 30
+I64 = 27
 IQ2_XXS, IQ2_XS, IQ3_XXS, IQ1_S, IQ3_S, IQ2_S, IQ1_M = 16, 17, 18, 19, 21, 22, 29
+ROPE_NORM, ROPE_NEOX, ROPE_MROPE, ROPE_VISION, ROPE_IMROPE = 0, 2, 8, 24, 40
 OP_MUL_MAT, OP_MUL_MAT_ID, OP_FLASH_ATTN_EXT = 1, 2, 3
 BLOCK = {Q4_0: (32, 18), Q5_0: (32, 22), Q8_0: (32, 34), Q4_K: (256, 144), Q5_K: (256, 176), Q6_K: (256, 210),
-         Q8_K: (256, 292), MXFP4: (32, 17), F32: (1, 4), F16: (1, 2), I32: (1, 4),
+         Q8_K: (256, 292), MXFP4: (32, 17), F32: (1, 4), F16: (1, 2), I32: (1, 4), I64: (1, 8),
          Q4_1: (32, 20), Q5_1: (32, 24), Q8_1: (32, 36), Q2_K: (256, 84), Q3_K: (256, 110),
          IQ4_NL: (32, 18), IQ4_XS: (256, 136), NVFP4: (64, 36), Q1_0: (128, 18), Q2_0: (64, 18), BF16: (1, 2),
          IQ2_XXS: (256, 66), IQ2_XS: (256, 74), IQ2_S: (256, 82), IQ3_XXS: (256, 98), IQ3_S: (256, 110),
@@ -47,6 +49,29 @@ class Tensor(C.Structure):
 class GNode(C.Structure):
     """struct ghip_node"""
     _fields_ = [("op", C.c_int32), ("src", C.POINTER(Tensor) * 5), ("dst", C.POINTER(Tensor))]
+
+
+class RopeParams(C.Structure):
+    """struct ghip_rope_params"""
+    _fields_ = [("n_dims", C.c_int32), ("mode", C.c_int32), ("sections", C.c_int32 * 4), ("freq_base", C.c_double),
+                ("freq_scale", C.c_double), ("ext_factor", C.c_double), ("attn_factor", C.c_double),
+                ("beta_fast", C.c_double), ("beta_slow", C.c_double), ("n_ctx_orig", C.c_int32)]
+
+
+class PagedParams(C.Structure):
+    """struct ghip_paged_params"""
+    _fields_ = [("scale", C.c_float), ("window", C.c_int32), ("n_first", C.c_int32), ("n_shared", C.c_int32),
+                ("max_q", C.c_int32)]
+
+
+class Rope:
+    """A rotation of head rows by their positions, made once for a model."""
+
+    def __init__(self, n_dims, mode=ROPE_NEOX, freq_base=10000.0, freq_scale=1.0, sections=(0, 0, 0, 0), ext_factor=0.0,
+                 attn_factor=1.0, beta_fast=32.0, beta_slow=1.0, n_ctx_orig=0):
+        self.params = RopeParams(n_dims, mode, (C.c_int32 * 4)(*sections), freq_base, freq_scale, ext_factor,
+                                 attn_factor, beta_fast, beta_slow, n_ctx_orig)
+        self._ref = C.byref(self.params)
 
 
 class Node:
@@ -85,7 +110,8 @@ def row_size(ty, n):
 
 _PACK = struct.Struct("=i4x4q4QQ64x").pack  # a Tensor's bytes (op_params zero)
 assert struct.calcsize("=i4x4q4QQ64x") == C.sizeof(Tensor)
-_PLAIN = frozenset((F32, F16, BF16, I32))
+_PLAIN = frozenset((F32, F16, BF16, I32, I64))
+_TYPE_OF = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16, torch.int32: I32, torch.int64: I64}
 
 
 def describe(t, ty, ne0=None):
@@ -117,6 +143,22 @@ def describe(t, ty, ne0=None):
     while len(nb) < 4:
         nb.append(nb[-1] * ne[len(nb) - 1])
     return Tensor.from_buffer_copy(_PACK(ty, *ne, *nb[:4], t.data_ptr()))
+
+
+def _view(t):
+    """describe() of a tensor of its own type; None stays None"""
+    if t is None:
+        return None
+    ty = _TYPE_OF.get(t.dtype)
+    if ty is None:
+        raise GhipError(f"dtype {t.dtype} not supported")
+    if not t.is_cuda:
+        raise GhipError("tensors must be on the GPU")
+    return describe(t, ty)
+
+
+def _ref(t):
+    return C.byref(t) if t is not None else None
 
 
 _lib = None
@@ -166,6 +208,13 @@ def lib():
         L.ghip_weight_cache_stats.argtypes = [C.c_void_p] + [C.POINTER(C.c_size_t)] * 3
         L.ghip_flash_attn_ext.restype = C.c_int
         L.ghip_flash_attn_ext.argtypes = [C.c_void_p, P, P, P, P, P, P, C.c_void_p]
+        R = C.POINTER(RopeParams)
+        L.ghip_rope.restype = C.c_int
+        L.ghip_rope.argtypes = [C.c_void_p, P, P, P, R, P, C.c_void_p]
+        L.ghip_kv_append.restype = C.c_int
+        L.ghip_kv_append.argtypes = [C.c_void_p, P, P, P, P, P, R, P, C.c_void_p]
+        L.ghip_flash_attn_paged.restype = C.c_int
+        L.ghip_flash_attn_paged.argtypes = [C.c_void_p, P, P, P, P, C.POINTER(PagedParams), P, C.c_void_p]
         _lib = L
     return _lib
 
@@ -308,6 +357,36 @@ class Backend:
         ref = lambda t: C.byref(t) if t is not None else None
         self._check(lib().ghip_flash_attn_ext(self._ctx, ref(tq), ref(tk), ref(tv), ref(tm), ref(ts), ref(td),
                                               _stream()), "ghip_flash_attn_ext")
+        return out
+
+    # ---- rotary positions, paged KV cache
+    def rope(self, x, pos, rope, factors=None, out=None):
+        """x [T, H, D] f32 / f16 / bf16 rotated by `rope` (a Rope) at pos [T] or
+        [axes, T] int32; factors [pairs] f32.  out may be x."""
+        if out is None:
+            out = torch.empty_like(x)
+        a, b, f, d = _view(x), _view(pos), _view(factors), _view(out)
+        self._check(lib().ghip_rope(self._ctx, _ref(a), _ref(b), _ref(f), rope._ref, _ref(d), _stream()), "ghip_rope")
+        return out
+
+    def kv_append(self, k, v, slots, kv, pos=None, rope=None, factors=None):
+        """Write k / v [T, H_kv, D] (f32 or kv's type) into rows `slots` [T] int64
+        (negative: skipped) of kv [pages, page, H_kv, 2 D], k rotated by `rope`."""
+        a, b, c, d, f, e = _view(k), _view(v), _view(slots), _view(pos), _view(factors), _view(kv)
+        self._check(lib().ghip_kv_append(self._ctx, _ref(a), _ref(b), _ref(c), _ref(d), _ref(f),
+                                         rope._ref if rope is not None else None, _ref(e), _stream()), "ghip_kv_append")
+        return kv
+
+    def flash_attn_paged(self, q, kv, seqs, scale=1.0, sinks=None, window=0, n_first=0, n_shared=0, max_q=None, out=None):
+        """q [T, H, D] f32 over kv [pages, page, H_kv, 2 D] f16 / bf16; seqs
+        [B, 3 + per] int32 rows (first row in q, rows, keys, pages ..); sinks [H]
+        f32.  max_q: the most rows of a sequence (T where None) -> [T, H, D] f32."""
+        if out is None:
+            out = torch.empty_like(q)
+        a, b, c, s, d = _view(q), _view(kv), _view(seqs), _view(sinks), _view(out)
+        pp = PagedParams(scale, window, n_first, n_shared, q.shape[0] if max_q is None else max_q)
+        self._check(lib().ghip_flash_attn_paged(self._ctx, _ref(a), _ref(b), _ref(c), _ref(s), C.byref(pp), _ref(d),
+                                                _stream()), "ghip_flash_attn_paged")
         return out
 
     # ---- graph
