@@ -42,6 +42,7 @@ EXTRA_FLAGS = {
     "ghip_gemm": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "ghip_kq": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "ghip_dense": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "ghip_fap": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "ghip_skinny": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }
 

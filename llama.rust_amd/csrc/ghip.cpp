@@ -2,6 +2,7 @@
 // validation, workspace management and kernel dispatch behind include/ghip.h.
 #include "../../include/ghip.h"
 #include "ghip_internal.h"
+#include "ghip_paged.h"
 
 #include <hip/hip_runtime.h>
 
@@ -3300,6 +3301,9 @@ struct FapParams {
     int T, H, H_kv, D;
     float scale;
     int window, n_first, n_shared, max_q;
+    PagedDiv by_page;
+    int nb_sh, zs_sh, nb_own, zs_own, wg_sh, least;
+    float *part, *stat;
 };
 
 bool plan_fap(ghip_context *ctx, const ghip_tensor *q, const ghip_tensor *kv, const ghip_tensor *seqs,
@@ -3321,12 +3325,14 @@ bool plan_fap(ghip_context *ctx, const ghip_tensor *q, const ghip_tensor *kv, co
         return bad("kv and its strides must be multiples of 16 bytes");
     const int64_t H_kv = kv->ne[1], page = kv->ne[2];
     if (H % H_kv) return bad("H % H_kv != 0");
-    if (H > 65535 || T > INT32_MAX || page > INT32_MAX || kv->ne[3] > INT32_MAX) return bad("dimension too large");
+    // the kernels count rows in 32 bits, 256 sequences of them at a time
+    if (H > 65535 || T >= (1 << 23) || T * H >= (1ll << 29) || page > INT32_MAX || kv->ne[3] > INT32_MAX)
+        return bad("dimension too large");
     if (seqs->type != GHIP_TYPE_I32 || seqs->nb[0] != 4 || seqs->nb[1] % 4 || seqs->ne[0] < 3 || seqs->ne[1] < 0 ||
         seqs->ne[2] != 1 || seqs->ne[3] != 1)
         return bad("seqs must be I32 [3 + pages of a sequence, sequences]");
     const int64_t per = seqs->ne[0] - 3, B = seqs->ne[1];
-    if (per * page > INT32_MAX || B > INT32_MAX) return bad("dimension too large");
+    if (per * page >= (1ll << 30) || B >= (1 << 23)) return bad("dimension too large");
     if (sinks && (sinks->type != GHIP_TYPE_F32 || sinks->nb[0] != 4 || sinks->ne[0] < H)) return bad("sinks must be F32 [H]");
     if (!std::isfinite(pp->scale)) return bad("scale must be finite");
     if (pp->window < 0 || pp->n_first < 0) return bad("window and n_first must not be negative");
@@ -3358,12 +3364,56 @@ bool plan_fap(ghip_context *ctx, const ghip_tensor *q, const ghip_tensor *kv, co
     p.H_kv = (int)H_kv;
     p.D = (int)D;
     p.scale = pp->scale;
-    p.window = pp->window;
-    p.n_first = pp->n_first;
-    p.n_shared = pp->n_shared;
+    // a window or first keys past the table are as good as all of it
+    p.window = pp->window > per * page ? 0 : pp->window;
+    p.n_first = (int)std::min<int64_t>(pp->n_first, per * page);
+    p.n_shared = B > 1 ? pp->n_shared : 0;
+    p.by_page = paged_divisor((uint32_t)page);
     p.max_q = (int)std::min<int64_t>(pp->max_q, T);
     st = GHIP_STATUS_SUCCESS;
     return true;
+}
+
+// Which kernels run, how their keys are split, and the workspace of the splits.
+struct FapLayout {
+    bool few;
+    int DP, rows;
+    size_t ws_bytes;
+};
+FapLayout fap_layout(FapParams &p) {
+    FapLayout L;
+    const int G = p.H / p.H_kv;
+    L.DP = p.D <= 64 ? 64 : p.D <= 96 ? 96 : p.D <= 128 ? 128 : 256;
+    L.few = (int64_t)p.max_q * G <= 16;
+    L.rows = L.DP == 256 ? 64 : 128;
+    const int64_t table = (int64_t)p.per * p.page;
+    // the most keys that one block of rows goes through outside the shared prefix
+    int64_t keys = table - p.n_shared;
+    if (p.window) keys = std::min(keys, (int64_t)p.window + p.max_q - 1 + p.n_first);
+    p.least = 4;
+    auto splits = [&](int64_t wgs, int64_t want, int64_t n) {
+        return (int)std::max<int64_t>(1, std::min<int64_t>({(want + wgs - 1) / wgs, n, 32}));
+    };
+    if (L.few) {
+        p.nb_own = p.B;
+        p.zs_own = splits((int64_t)p.nb_own * p.H_kv, env_int("GHIP_FAP_WGS", 1024), (keys + 127) / 128);
+    } else {
+        p.nb_own = (int64_t)p.max_q * G <= L.rows ? p.B : (int)((int64_t)p.T * G / L.rows + p.B);
+        p.zs_own = splits((int64_t)p.nb_own * p.H_kv, env_int("GHIP_FAP_WGS", 1024) / 2, (keys + 255) / 256);
+    }
+    p.nb_sh = p.zs_sh = p.wg_sh = 0;
+    if (p.n_shared) {
+        const int64_t rows = std::min((int64_t)p.T, (int64_t)p.B * p.max_q) * G;
+        p.nb_sh = (int)((rows + L.rows - 1) / L.rows);
+        int64_t shk = p.n_shared;
+        if (p.window) shk = std::min(shk, (int64_t)p.n_first + p.window + table);
+        p.zs_sh = splits((int64_t)p.nb_sh * p.H_kv, env_int("GHIP_FAP_WGS", 1024) / 2, (shk + 255) / 256);
+        p.wg_sh = p.nb_sh * p.H_kv * p.zs_sh;
+    }
+    const int nz = p.zs_sh + p.zs_own;
+    const size_t n = (size_t)p.T * p.H * nz;
+    L.ws_bytes = nz > 1 ? n * (p.D + 2) * sizeof(float) : 0;
+    return L;
 }
 
 }  // namespace
@@ -3384,10 +3434,52 @@ ghip_status ghip_flash_attn_paged(ghip_context *ctx, const ghip_tensor *q, const
     st = ctx->begin(s);
     if (st != GHIP_STATUS_SUCCESS) return st;
     ctx->allow(dst->data, byte_extent(dst, 4), "dst");
+    const FapLayout L = fap_layout(p);
+    p.part = p.stat = nullptr;
+    if (L.ws_bytes) {
+        void *ws = nullptr;
+        st = ctx->workspace(L.ws_bytes, s, &ws);
+        if (st != GHIP_STATUS_SUCCESS) return st;
+        const size_t n = (size_t)p.T * p.H * (p.zs_sh + p.zs_own);
+        p.part = (float *)ws;
+        p.stat = p.part + n * p.D;
+    }
+    // no pages: keys that rows see are all missing; what is read in their place
+    // (and not used) is q's first row, which is as long as a cache row
+    if (p.n_pages == 0) {
+        p.kv = (const uint16_t *)((uintptr_t)p.q & ~(uintptr_t)15);
+        p.kv_head = p.kv_row = p.kv_page = 0;
+    }
+    auto expect = [&]() {
+        if (p.part) {
+            const size_t n = (size_t)p.T * p.H * (p.zs_sh + p.zs_own);
+            ctx->expect(p.part, n * p.D * 4, "partials");
+            ctx->expect(p.stat, n * 2 * 4, "statistics");
+        } else {
+            ctx->expect(p.dst, (size_t)(4 * ((p.T - 1) * p.d_nb2 + (p.H - 1) * p.d_nb1 + p.D)), "dst");
+        }
+    };
+    char name[48];
+    const char *ty = float_name(kv->type);
+    const int64_t own = (int64_t)p.nb_own * p.H_kv * p.zs_own, joins = ((int64_t)p.B * p.max_q * p.H + 3) / 4;
+    if (own + p.wg_sh > INT32_MAX || joins > INT32_MAX)
+        return ctx->fail(GHIP_STATUS_BACKEND_ERROR, "flash_attn_paged: too many rows");
+    const int64_t tiles = p.wg_sh + (L.few ? 0 : own);
+    if (tiles) {
+        expect();
+        snprintf(name, sizeof name, "ghip_fap_tile_%s_%d", ty, L.DP);
+        st = ctx->launch(name, dim3((unsigned)tiles), dim3(256), 0, s, p);
+        if (st != GHIP_STATUS_SUCCESS) return st;
+    }
+    if (L.few) {
+        expect();
+        snprintf(name, sizeof name, "ghip_fap_few_%s_%d", ty, L.DP);
+        st = ctx->launch(name, dim3((unsigned)own), dim3(256), 0, s, p);
+        if (st != GHIP_STATUS_SUCCESS) return st;
+    }
+    if (!p.part) return GHIP_STATUS_SUCCESS;
     ctx->expect(p.dst, (size_t)(4 * ((p.T - 1) * p.d_nb2 + (p.H - 1) * p.d_nb1 + p.D)), "dst");
-    const int64_t n = (int64_t)p.B * p.max_q * p.H;
-    if (n > INT32_MAX) return ctx->fail(GHIP_STATUS_BACKEND_ERROR, "flash_attn_paged: too many rows");
-    return ctx->launch(kv->type == GHIP_TYPE_F16 ? "ghip_fap_rows_f16" : "ghip_fap_rows_bf16", dim3((unsigned)n), dim3(64), 0, s, p);
+    return ctx->launch("ghip_fap_join", dim3((unsigned)joins), dim3(256), 0, s, p);
 }
 
 }  // extern "C"

@@ -6,12 +6,70 @@
 // of them):  o = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m),  s_j = scale q . k_j;
 // a sink adds e^(sink - m) below the line.  A row that sees nothing gives 0.
 // Key j is row j % page of page table[j / page]; a row that sees a key whose
-// page does not exist gives NaN, and no key that no row sees is read.
+// page does not exist gives NaN.
+//
+// Both kernels walk the keys once with a running maximum and sum, on the matrix
+// cores (v_mfma_f32_16x16x32): S^T = K Q^T leaves a query row in 4 lanes (n, n +
+// 16, n + 32, n + 48), whose scores are the B operand of O^T += V^T P^T as they
+// are.  q is 32-bit and the output too, so q and p are split into NQ / NP terms
+// of the cache's type that add up to them (f16: 2 terms, 22 bits; bf16: 3 terms,
+// 24 bits), each a product of its own on the same K or V fragment; sums are 32-bit.
+//
+//  * ghip_fap_few: up to 16 rows of a KV head (generation: the G = H / H_kv query
+//    heads that share it, times a few rows).  Bound by reading K and V once: each
+//    of the 4 wavefronts streams its own 32-key tiles and they meet at the end.
+//  * ghip_fap_tile: up to 128 rows; the 4 wavefronts hold 32 rows each and share
+//    64-key tiles.  Bound by the matrix cores and the softmax's vector work.
+//
+// K and V go straight from memory into LDS, 16 bytes a lane.  A row's 16-byte
+// chunks are swapped about by its number so that the fragment reads meet no bank
+// twice (k_swz, v_swz).  The loads are inline assembly: the compiler would wait
+// for all of them before any LDS read.  Everything the loops load is counted by
+// hand, in the order of issue.
 #include "ghip_common.h"
 #include "ghip_paged.h"
 
 typedef _Float16 f16;
 typedef __bf16 bf16;
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v2f __attribute__((ext_vector_type(2)));
+
+template <typename E> struct Frag;
+template <> struct Frag<f16> {
+    typedef _Float16 v8 __attribute__((ext_vector_type(8)));
+    typedef _Float16 v4 __attribute__((ext_vector_type(4)));
+    typedef _Float16 v2 __attribute__((ext_vector_type(2)));
+    typedef __fp16 tr __attribute__((__vector_size__(8)));
+    static constexpr int NQ = 2, NP = 2;
+    static __device__ __forceinline__ v4f mfma(v8 a, v8 b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ v4 read_tr(const f16 *p) {
+        return __builtin_bit_cast(v4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) tr *)p));
+    }
+};
+template <> struct Frag<bf16> {
+    typedef __bf16 v8 __attribute__((ext_vector_type(8)));
+    typedef __bf16 v4 __attribute__((ext_vector_type(4)));
+    typedef __bf16 v2 __attribute__((ext_vector_type(2)));
+    static constexpr int NQ = 3, NP = 3;
+    static __device__ __forceinline__ v4f mfma(v8 a, v8 b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ v4 read_tr(const bf16 *p) {
+        return __builtin_bit_cast(v4, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) v4 *)p));
+    }
+};
+
+// x as N terms of E: each the rest of the ones before, rounded to nearest
+template <typename E, int N>
+DEV void split_pair(float x0, float x1, typename Frag<E>::v2 (&t)[N]) {
+    v2f x = {x0, x1};
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        t[i] = __builtin_convertvector(x, typename Frag<E>::v2);
+        if (i + 1 < N) {
+            x[0] -= (float)t[i][0];
+            x[1] -= (float)t[i][1];
+        }
+    }
+}
 
 struct FapParams {
     const float *q;
@@ -26,72 +84,830 @@ struct FapParams {
     float *dst;
     int64_t d_nb1, d_nb2;  // floats: head, token
     int T, H, H_kv, D;
-    float scale;
+    float scale;  // times log2 e: scores are kept in log2 units
     int window, n_first, n_shared, max_q;
+    PagedDiv by_page;
+    // launch: the first wg_sh workgroups take the shared prefix (nb_sh blocks of
+    // rows, zs_sh splits), the others each sequence's own keys (nb_own, zs_own)
+    int nb_sh, zs_sh, nb_own, zs_own, wg_sh, least;
+    // partials of row (token, head), split z (shared prefix first): part[.. + z][D]
+    // and stat[.. + z][2] = (maximum, sum); null where zs_sh + zs_own == 1
+    float *part, *stat;
 };
 
-// One wavefront a row of one head: 64 keys at a time, a lane scoring one key;
-// then every lane owns dims lane, lane + 64, .. of the output.
-template <typename E>
-DEV void fap_rows(const FapParams &p) {
-    __shared__ float qs[256];
-    const int lane = threadIdx.x;
-    const int h = blockIdx.x % p.H;
-    const int bi = blockIdx.x / p.H, b = bi / p.max_q, i = bi - b * p.max_q;
-    const int32_t *row = p.seqs + (int64_t)b * p.seq_nb1;
-    const PagedSeq s = paged_seq(row[0], row[1], row[2], p.T, p.max_q);
-    if (i >= s.nq) return;
-    const int64_t t = s.q0 + i, pos = s.pos0 + i;
-    for (int d = lane; d < p.D; d += 64) qs[d] = p.q[t * p.q_nb2 + h * p.q_nb1 + d] * p.scale;
-    __syncthreads();
-    const E *kv = (const E *)p.kv + (h / (p.H / p.H_kv)) * p.kv_head;
-    const PagedKeys kr = paged_keys(pos, pos, p.window, p.n_first);
-    const int64_t table = (int64_t)p.per * p.page;
-    float m = -__builtin_inff(), l = 0.0f, o[4] = {0, 0, 0, 0};
-    bool bad = kr.hi > table;
-    for (int part = 0; part < 2; part++) {
-        const int64_t a = part ? kr.lo : 0, e = part ? min(kr.hi, table) : min(kr.first, table);
-        for (int64_t k0 = a; k0 < e; k0 += 64) {
-            const int64_t j = k0 + lane;
-            float x = -__builtin_inff();
-            int64_t at = -1;
-            if (j < e) {
-                const int32_t pg = row[3 + j / p.page];
-                if (pg >= 0 && pg < p.n_pages) {
-                    at = pg * p.kv_page + (j % p.page) * p.kv_row;
-                    x = 0.0f;
-                    for (int d = 0; d < p.D; d++) x = fmaf(qs[d], (float)kv[at + d], x);
-                } else {
-                    bad = true;
-                }
-            }
-            float mx = x;
-            for (int w = 32; w; w >>= 1) mx = fmaxf(mx, __shfl_xor(mx, w, 64));
-            const float mn = fmaxf(m, mx);
-            const float alpha = mn == -__builtin_inff() ? 1.0f : __expf(m - mn);
-            const float pr = x == -__builtin_inff() ? 0.0f : __expf(x - mn);
-            m = mn;
-            l = l * alpha + wave_sum(pr);
-            for (int u = 0; u < 4; u++) o[u] *= alpha;
-            for (int jj = 0; jj < 64; jj++) {
-                const float pj = __shfl(pr, jj, 64);
-                const int64_t aj = __shfl(at, jj, 64);
-                if (aj < 0) continue;
-                for (int u = 0; u < 4; u++)
-                    if (lane + 64 * u < p.D) o[u] = fmaf(pj, (float)kv[aj + p.D + lane + 64 * u], o[u]);
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int FEW_ROWS = 16, TILE_ROWS = 128;
+
+// LDS chunk (16 bytes) of a row of CH chunks that holds chunk c of row r.  Reads of
+// K take one chunk of 16 rows; reads of V 32 bytes of 8 rows at a time: both
+// touch each of the 64 banks once.
+template <int CH>
+DEV int k_swz(int r, int c) {
+    return CH == 8 ? c ^ ((r >> 1) & 7) : CH == 12 ? c ^ ((r >> 2) & 3) : c ^ (r & 15);
+}
+template <int CH>
+DEV int v_swz(int r, int c) {
+    return CH == 8 ? c ^ (((r >> 1) & 3) << 1) : CH == 12 ? c ^ (((r >> 2) & 1) << 1) : c ^ ((r & 7) << 1);
+}
+
+DEV uint32_t lds_addr(const void *p) { return (uint32_t)(uintptr_t)(lds_void *)p; }
+// 16 / 4 bytes a lane from memory to LDS at `to` (wave-uniform) + lane's place
+DEV void load16(const void *from, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory");
+}
+DEV void load4(const void *from, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(to), "v"(from) : "memory");
+}
+template <int N>
+DEV void wait_loads() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+DEV void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+// maximum / sum over the 4 lanes of a query row
+DEV float row_max(float x) {
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+DEV float row_sum(float x) {
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+
+// The wavefront's rows and what they hold: RW tiles of 16 rows.
+template <typename E, int DP, int RW>
+struct Rows {
+    typedef Frag<E> F;
+    typename F::v8 q[RW][DP / 32][F::NQ];
+    v4f o[RW][DP / 16];
+    v4f mneg[RW];   // minus the reference maximum (log2 units) four times: the scores' start; 0 while unset
+    float l[RW];    // this lane's share of the sum
+    int pos[RW];    // position of this lane's row; -1: there is none, or it sees nothing
+    bool set[RW];   // a key has been seen
+};
+
+template <typename E, int DP, int RW>
+DEV void rows_load(Rows<E, DP, RW> &R, int rt, const float *qr, int D, float scale, bool valid) {
+    const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+    for (int kk = 0; kk < DP / 32; kk++) {
+        const int d = 32 * kk + 8 * g;
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = 0.0f;
+        if (valid && d < D) __builtin_memcpy(x, qr + d, 32);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            typename Frag<E>::v2 t[Frag<E>::NQ];
+            split_pair<E, Frag<E>::NQ>(x[2 * e] * scale, x[2 * e + 1] * scale, t);
+#pragma unroll
+            for (int i = 0; i < Frag<E>::NQ; i++) {
+                R.q[rt][kk][i][2 * e] = t[i][0];
+                R.q[rt][kk][i][2 * e + 1] = t[i][1];
             }
         }
     }
-    if (p.sinks) {
-        const float sk = p.sinks[h], mn = fmaxf(m, sk);
-        const float alpha = mn == -__builtin_inff() ? 1.0f : __expf(m - mn);
-        l = l * alpha + (mn == -__builtin_inff() ? 0.0f : __expf(sk - mn));
-        for (int u = 0; u < 4; u++) o[u] *= alpha;
-    }
-    const bool nan = __ballot(bad) != 0;
-    for (int u = 0; u < 4; u++)
-        if (lane + 64 * u < p.D)
-            p.dst[t * p.d_nb2 + h * p.d_nb1 + lane + 64 * u] = nan ? __builtin_nanf("") : l > 0.0f ? o[u] / l : 0.0f;
+#pragma unroll
+    for (int dt = 0; dt < DP / 16; dt++) R.o[rt][dt] = v4f{0, 0, 0, 0};
+    R.mneg[rt] = v4f{0, 0, 0, 0};
+    R.l[rt] = 0.0f;
+    R.set[rt] = false;
 }
-extern "C" __global__ void __launch_bounds__(64) ghip_fap_rows_f16(FapParams p) { fap_rows<f16>(p); }
-extern "C" __global__ void __launch_bounds__(64) ghip_fap_rows_bf16(FapParams p) { fap_rows<bf16>(p); }
+
+// Scores of the NT 16-key tiles at Ks, less the reference maximum.
+template <typename E, int DP, int RW, int NT>
+DEV void scores(const Rows<E, DP, RW> &R, const E *Ks, v4f (&s)[NT][RW]) {
+    constexpr int CH = DP / 8;
+    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+#pragma unroll
+        for (int kk = 0; kk < DP / 32; kk++) {
+            const int r = 16 * t + n;
+            typename Frag<E>::v8 a;
+            __builtin_memcpy(&a, __builtin_assume_aligned(Ks + r * DP + 8 * k_swz<CH>(r, 4 * kk + g), 16), 16);
+#pragma unroll
+            for (int i = Frag<E>::NQ - 1; i >= 0; i--)
+#pragma unroll
+                for (int rt = 0; rt < RW; rt++)
+                    s[t][rt] = Frag<E>::mfma(a, R.q[rt][kk][i], kk == 0 && i == Frag<E>::NQ - 1 ? R.mneg[rt] : s[t][rt]);
+        }
+    }
+}
+
+// What of a tile is to be masked: keys k0 .. , of which [k0, ke) are the pass's,
+// `bad` of them on no page.  Key r = 16 t + 4 g + v of the tile is compared as
+// 16 t + v with limits less k0 + 4 g.
+template <typename E, int DP, int RW, int NT>
+DEV void mask_scores(const Rows<E, DP, RW> &R, v4f (&s)[NT][RW], int k0, int ke, uint64_t bad, int window, int n_first) {
+    const int at = k0 + 4 * ((threadIdx.x & 63) >> 4);
+#pragma unroll
+    for (int rt = 0; rt < RW; rt++) {
+        const int hi = min(R.pos[rt], ke - 1) - at, lo = window ? R.pos[rt] - window - at : -0x7fffffff, first = n_first - at;
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int v = 0; v < 4; v++) {
+                const int c = 16 * t + v;
+                if (!(c <= hi && (c > lo || c < first))) s[t][rt][v] = -__builtin_inff();
+            }
+    }
+    if (bad) {
+        const uint64_t mine = bad >> (4 * ((threadIdx.x & 63) >> 4));
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int v = 0; v < 4; v++)
+                if ((mine >> (16 * t + v)) & 1) {
+#pragma unroll
+                    for (int rt = 0; rt < RW; rt++)
+                        if (s[t][rt][v] > -__builtin_inff()) s[t][rt][v] = __builtin_nanf("");
+                }
+    }
+}
+
+// Scores -> probabilities.  The reference maximum moves only when a score passes
+// it by more than 8 (so p <= 256) or on a row's first key; o and l are rescaled
+// only then.
+template <typename E, int DP, int RW, int NT>
+DEV void softmax(Rows<E, DP, RW> &R, v4f (&s)[NT][RW]) {
+#pragma unroll
+    for (int rt = 0; rt < RW; rt++) {
+        float mx = -__builtin_inff();
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int v = 0; v < 4; v++) mx = fmaxf(mx, s[t][rt][v]);
+        if (__ballot(mx > 8.0f || !R.set[rt])) {
+            mx = row_max(mx);
+            if (mx > 8.0f || (!R.set[rt] && mx > -__builtin_inff())) {
+                const float alpha = R.set[rt] ? __builtin_amdgcn_exp2f(-mx) : 1.0f;
+                R.set[rt] = true;
+                R.mneg[rt] -= mx;
+                R.l[rt] *= alpha;
+#pragma unroll
+                for (int dt = 0; dt < DP / 16; dt++) R.o[rt][dt] *= alpha;
+#pragma unroll
+                for (int t = 0; t < NT; t++) s[t][rt] -= mx;
+            }
+        }
+        float sum = 0.0f;
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int v = 0; v < 4; v++) {
+                s[t][rt][v] = __builtin_amdgcn_exp2f(s[t][rt][v]);
+                sum += s[t][rt][v];
+            }
+        R.l[rt] += sum;
+    }
+}
+
+// fragment of V^T of the MFMA: dims 16 dt + (lane & 15), in slot e key 32 u + 4 g + e,
+// from slot 4 on 16 further (as the scores lie)
+template <typename E, int DP>
+DEV typename Frag<E>::v8 value_frag(const E *Vs, int u, int dt) {
+    constexpr int CH = DP / 8;
+    const int lane = threadIdx.x & 63, lj = lane & 15, g = lane >> 4;
+    const int r0 = 32 * u + 4 * g + (lj >> 2), c = 2 * dt + ((lj & 3) >> 1), h = 4 * (lj & 1);
+    const typename Frag<E>::v4 lo = Frag<E>::read_tr(Vs + r0 * DP + 8 * v_swz<CH>(r0, c) + h);
+    const typename Frag<E>::v4 hi = Frag<E>::read_tr(Vs + (r0 + 16) * DP + 8 * v_swz<CH>(r0 + 16, c) + h);
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+// O^T += V^T P^T over NT 16-key tiles at Vs
+template <typename E, int DP, int RW, int NT>
+DEV void values(Rows<E, DP, RW> &R, const E *Vs, const v4f (&s)[NT][RW]) {
+    constexpr int NP = Frag<E>::NP;
+    typename Frag<E>::v8 p[RW][NP];
+#pragma unroll
+    for (int u = 0; u < NT / 2; u++) {
+#pragma unroll
+        for (int rt = 0; rt < RW; rt++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                typename Frag<E>::v2 t[NP];
+                split_pair<E, NP>(s[2 * u + e / 2][rt][2 * (e & 1)], s[2 * u + e / 2][rt][2 * (e & 1) + 1], t);
+#pragma unroll
+                for (int i = 0; i < NP; i++) {
+                    p[rt][i][2 * e] = t[i][0];
+                    p[rt][i][2 * e + 1] = t[i][1];
+                }
+            }
+#pragma unroll
+        for (int dt = 0; dt < DP / 16; dt++) {
+            const typename Frag<E>::v8 a = value_frag<E, DP>(Vs, u, dt);
+#pragma unroll
+            for (int i = NP - 1; i >= 0; i--)
+#pragma unroll
+                for (int rt = 0; rt < RW; rt++) R.o[rt][dt] = Frag<E>::mfma(a, p[rt][i], R.o[rt][dt]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
+// Infinities and NaN among the values of a tile that some rows do not see in
+// full: there a product with p = 0 would be NaN.  Each output whose row has such
+// a value with p > 0 takes an infinity of that sign (NaN: both) from products of
+// p with flags; the values themselves are then set to 0 in the tile.
+template <typename E>
+DEV bool odd_pair(uint32_t x) {
+    constexpr uint32_t LO = Frag<E>::NQ == 2 ? 0x7c00u : 0x7f80u, HI = LO << 16;
+    return (x & LO) == LO || (x & HI) == HI;
+}
+template <typename E, int DP, int RW, int NT>
+DEV void add_odd(Rows<E, DP, RW> &R, const E *Vs, const v4f (&s)[NT][RW]) {
+#pragma unroll
+    for (int u = 0; u < NT / 2; u++)
+#pragma unroll
+        for (int rt = 0; rt < RW; rt++) {
+            typename Frag<E>::v8 p;
+#pragma unroll
+            for (int e = 0; e < 8; e++) p[e] = s[2 * u + e / 4][rt][e & 3] > 0.0f ? (E)1.0f : (E)0.0f;
+#pragma unroll
+            for (int dt = 0; dt < DP / 16; dt++) {
+                const typename Frag<E>::v8 a = value_frag<E, DP>(Vs, u, dt);
+                typename Frag<E>::v8 up, dn;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const float x = (float)a[e];
+                    const bool odd = !(fabsf(x) < __builtin_inff());
+                    up[e] = odd && !(x < 0.0f) ? (E)1.0f : (E)0.0f;
+                    dn[e] = odd && !(x > 0.0f) ? (E)1.0f : (E)0.0f;
+                }
+                const v4f zero = {0, 0, 0, 0};
+                const v4f nu = Frag<E>::mfma(up, p, zero), nd = Frag<E>::mfma(dn, p, zero);
+#pragma unroll
+                for (int v = 0; v < 4; v++) {
+                    if (nu[v] > 0.0f) R.o[rt][dt][v] += __builtin_inff();
+                    if (nd[v] > 0.0f) R.o[rt][dt][v] -= __builtin_inff();
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+}
+// chunks from + 64 i + lane, i < n, of a tile: do they hold one?  / set to 0
+template <typename E>
+DEV bool odd_chunks(const uint8_t *Vs, int from, int n) {
+    bool odd = false;
+#pragma unroll 1
+    for (int i = 0; i < n; i++) {
+        const uint4 x = *(const uint4 *)(Vs + 16 * (from + 64 * i + (threadIdx.x & 63)));
+        odd = odd || odd_pair<E>(x.x) || odd_pair<E>(x.y) || odd_pair<E>(x.z) || odd_pair<E>(x.w);
+    }
+    return __ballot(odd) != 0;
+}
+template <typename E>
+DEV void clear_odd(uint8_t *Vs, int from, int n) {
+    constexpr uint32_t LO = Frag<E>::NQ == 2 ? 0x7c00u : 0x7f80u, HI = LO << 16;
+#pragma unroll 1
+    for (int i = 0; i < n; i++) {
+        uint32_t *x = (uint32_t *)(Vs + 16 * (from + 64 * i + (threadIdx.x & 63)));
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            if ((x[k] & LO) == LO) x[k] &= 0xffff0000u;
+            if ((x[k] & HI) == HI) x[k] &= 0x0000ffffu;
+        }
+    }
+}
+
+// One pass of a workgroup: which rows, which keys.
+struct Pass {
+    const int32_t *row;  // table row of its pages
+    int hk, z, share;    // KV head, split, tiles of a split
+    int p0, p1;          // least and largest position of its rows
+    PagedTiles tl;
+    int zi;              // where its partials go
+};
+DEV int clip_pos(int64_t p, int64_t table) { return (int)(p < -1 ? -1 : p > table ? table : p); }
+
+struct Tile {
+    int k0, ke;
+};
+DEV Tile tile_at(const PagedTiles &tl, int t, int kt) {
+    Tile r;
+    r.k0 = t < tl.na ? tl.a0 + t * kt : tl.b0 + (t - tl.na) * kt;
+    r.ke = t < tl.na ? tl.a1 : tl.b1;
+    return r;
+}
+DEV bool tile_whole(const Tile &tile, int kt, const Pass &ps, int window, int n_first) {
+    return tile.k0 + kt <= tile.ke && tile.k0 + kt - 1 <= ps.p0 &&
+           (!window || tile.k0 > ps.p1 - window || tile.k0 + kt <= n_first);
+}
+
+// Rows' results to dst, or to this split's partials.  m, l: of this lane's row.
+DEV void finish_stat(const FapParams &p, int h, float &m, float &l, float &f) {
+    f = 1.0f;
+    if (p.sinks) {
+        const float sk = p.sinks[h] * kLog2e;
+        const float M = fmaxf(m, sk);
+        if (M > -__builtin_inff()) {
+            f = __builtin_amdgcn_exp2f(m - M);
+            l = l * f + __builtin_amdgcn_exp2f(sk - M);
+        }
+    }
+    f = l == 0.0f ? 0.0f : f / l;
+}
+
+// the statistics of a split that holds none of a row's keys (NaN: it has keys
+// past its table); its sums are not read
+DEV void stat_none(const FapParams &p, int64_t pi, bool nan) {
+    p.stat[2 * pi] = -__builtin_inff();
+    p.stat[2 * pi + 1] = nan ? __builtin_nanf("") : 0.0f;
+}
+
+// ---- up to 16 rows a KV head: 4 wavefronts, each its own 32-key tiles
+
+template <typename E, int DP>
+DEV void fap_few(const FapParams &p) {
+    constexpr int KT = 32, CH = DP / 8, NI = KT * CH / 64;  // loads of a K (or V) tile
+    constexpr int TB = KT * DP * 2;                         // bytes of one
+    __shared__ __attribute__((aligned(1024))) uint8_t kvs[4][2][TB];
+    __shared__ int32_t te[4][2][64];
+    __shared__ float ws[4][2][16];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
+    const int G = p.H / p.H_kv;
+    const int64_t table = (int64_t)p.per * p.page;
+    const int id = blockIdx.x, hk = id % p.H_kv, z = (id / p.H_kv) % p.zs_own, b = id / (p.H_kv * p.zs_own);
+    const int32_t *row = p.seqs + (int64_t)b * p.seq_nb1;
+    const PagedSeq sq = paged_seq(row[0], row[1], row[2], p.T, p.max_q);
+    if (sq.nq == 0) return;
+    Pass ps;
+    ps.row = row;
+    ps.p0 = clip_pos(sq.pos0, table);
+    ps.p1 = clip_pos(sq.pos0 + sq.nq - 1, table);
+    ps.tl = paged_tiles(ps.p0, ps.p1, p.window, p.n_first, p.n_shared, (int)table, KT);
+    const int share = paged_share(ps.tl.n, p.zs_own, p.least);
+    const int t0 = (int)min((int64_t)z * share, (int64_t)ps.tl.n), t1 = min(ps.tl.n, t0 + share);
+    const int i = n / G, hd = hk * G + n % G;
+    const bool valid = n < sq.nq * G;
+    const int64_t tok = sq.q0 + (valid ? i : 0);
+    const int64_t pi = (tok * p.H + hd) * (p.zs_sh + p.zs_own) + p.zs_sh + z;
+    if (t0 >= t1 && p.part) {  // nothing in this split
+        if (valid && w == 0 && g == 0) stat_none(p, pi, sq.pos0 + i >= table);
+        return;
+    }
+    Rows<E, DP, 1> R;
+    rows_load<E, DP, 1>(R, 0, p.q + tok * p.q_nb2 + hd * p.q_nb1, p.D, p.scale * kLog2e, valid);
+    R.pos[0] = valid ? clip_pos(sq.pos0 + i, table) : -1;
+    const E *kvh = (const E *)p.kv + hk * p.kv_head;
+    E *Ks = (E *)kvs[w][0], *Vs = (E *)kvs[w][1];
+    const uint32_t ka = lds_addr(Ks), va = lds_addr(Vs);
+
+    // page numbers of tile t's keys, a lane each
+    auto load_pages = [&](int t) {
+        const Tile tl = tile_at(ps.tl, min(t, t1 - 1), KT);
+        const int j = min(tl.k0 + lane, tl.ke - 1);
+        load4(row + 3 + paged_div((uint32_t)j, p.by_page), lds_addr(te[w][t >> 2 & 1]));
+    };
+    const E *at[NI];       // this lane's source of each load of the next tile
+    uint32_t ok = 0;       // its keys that are there
+    uint32_t bad = 0;      // those on no page
+    auto find_rows = [&](int t, uint32_t &okm, uint32_t &badm) {
+        const Tile tl = tile_at(ps.tl, t, KT);
+        const int32_t *pg = te[w][t >> 2 & 1];
+        const bool in = lane < KT && tl.k0 + lane < tl.ke;
+        const int my = in ? pg[lane] : 0;
+        const bool there = my >= 0 && my < p.n_pages;
+        okm = (uint32_t)__ballot(in && there);
+        badm = (uint32_t)__ballot(in && !there);
+#pragma unroll
+        for (int ii = 0; ii < NI; ii++) {
+            const int c = 64 * ii + lane, r = c / CH;
+            const uint32_t j = tl.k0 + r, page = pg[r];
+            const bool o = (okm >> r) & 1;
+            const int64_t off = o ? (int64_t)page * p.kv_page + (int64_t)(j - paged_div(j, p.by_page) * p.page) * p.kv_row : 0;
+            at[ii] = kvh + off;
+        }
+    };
+    auto load_k = [&]() {
+#pragma unroll
+        for (int ii = 0; ii < NI; ii++) {
+            const int c = 64 * ii + lane, r = c / CH, x = k_swz<CH>(r, c % CH);
+            load16(at[ii] + (8 * x < p.D ? 8 * x : 0), ka + 1024 * ii);
+        }
+    };
+    auto load_v = [&]() {
+#pragma unroll
+        for (int ii = 0; ii < NI; ii++) {
+            const int c = 64 * ii + lane, r = c / CH, x = v_swz<CH>(r, c % CH);
+            load16(at[ii] + p.D + (8 * x < p.D ? 8 * x : 0), va + 1024 * ii);
+        }
+    };
+    // in flight at the top of a step, oldest first: pages t + 4, K t, V t
+    const int first = t0 + w;
+    if (first < t1) {
+        load_pages(first);
+        wait_loads<0>();
+        find_rows(first, ok, bad);
+        load_pages(first + 4);
+        load_k();
+        load_v();
+    }
+    for (int t = first; t < t1; t += 4) {
+        const Tile tile = tile_at(ps.tl, t, KT);
+        const uint32_t okc = ok, badc = bad;
+        const bool more = t + 4 < t1;
+        wait_loads<NI>();
+        v4f s[2][1];
+        scores<E, DP, 1, 2>(R, Ks, s);
+        if (more) {
+            find_rows(t + 4, ok, bad);
+            wait_lds();
+            load_pages(t + 8);
+            load_k();
+        }
+        const bool part = !tile_whole(tile, KT, ps, p.window, p.n_first);
+        if (part || badc) mask_scores<E, DP, 1, 2>(R, s, tile.k0, tile.ke, badc, p.window, p.n_first);
+        softmax<E, DP, 1, 2>(R, s);
+        if (more) wait_loads<NI + 1>();
+        else wait_loads<0>();
+        if (okc != 0xffffffffu) {
+            // rows that were not there: no value of theirs may count
+#pragma unroll
+            for (int ii = 0; ii < NI; ii++) {
+                const int c = 64 * ii + lane;
+                if (!((okc >> (c / CH)) & 1)) *(uint4 *)(kvs[w][1] + 16 * c) = make_uint4(0, 0, 0, 0);
+            }
+            wait_lds();
+        }
+        if (part && ps.p0 != ps.p1 && odd_chunks<E>(kvs[w][1], 0, NI)) {
+            add_odd<E, DP, 1, 2>(R, Vs, s);
+            clear_odd<E>(kvs[w][1], 0, NI);
+        }
+        values<E, DP, 1, 2>(R, Vs, s);
+        if (more) {
+            wait_lds();
+            load_v();
+        }
+    }
+    // the 4 wavefronts' rows: everyone takes the common maximum, then thread
+    // (dims, row) adds the four
+    const float l = row_sum(R.l[0]), m = R.set[0] ? -R.mneg[0][0] : -__builtin_inff();
+    if (g == 0) {
+        ws[w][0][n] = m;
+        ws[w][1][n] = l;
+    }
+    __syncthreads();
+    float M = -__builtin_inff(), L = 0.0f;
+#pragma unroll
+    for (int u = 0; u < 4; u++) M = fmaxf(M, ws[u][0][n]);
+#pragma unroll
+    for (int u = 0; u < 4; u++) L += M > -__builtin_inff() ? ws[u][1][n] * __builtin_amdgcn_exp2f(ws[u][0][n] - M) : ws[u][1][n];
+    if (valid && R.pos[0] >= table) L = __builtin_nanf("");
+    const float f = M > -__builtin_inff() ? __builtin_amdgcn_exp2f(m - M) : 1.0f;
+    float *os = (float *)&kvs[0][0][0];  // [4][16][DP + 4]
+    static_assert(sizeof(kvs) >= 4 * 16 * (DP + 4) * 4, "the wavefronts' rows fit the tiles");
+    if (n < sq.nq * G) {
+#pragma unroll
+        for (int dt = 0; dt < DP / 16; dt++) *(v4f *)&os[(w * 16 + n) * (DP + 4) + 16 * dt + 4 * g] = R.o[0][dt] * f;
+    }
+    __syncthreads();
+    const bool direct = !p.part;
+    float fin = 1.0f, Mf = M, Lf = L;
+    if (direct) finish_stat(p, hd, Mf, Lf, fin);
+    // lanes of row n: wavefront w and lane group g take dims 16 w + 4 g + 64 k
+    if (valid) {
+        float *out = direct ? p.dst + tok * p.d_nb2 + hd * p.d_nb1 : p.part + pi * p.D;
+        for (int d = 16 * w + 4 * g; d < p.D; d += 64) {
+            v4f a = {0, 0, 0, 0};
+#pragma unroll
+            for (int u = 0; u < 4; u++) a += *(v4f *)&os[(u * 16 + n) * (DP + 4) + d];
+            a *= fin;
+            __builtin_memcpy(out + d, &a, 16);
+        }
+        if (!direct && w == 0 && g == 0) {
+            p.stat[2 * pi] = M;
+            p.stat[2 * pi + 1] = L;
+        }
+    }
+}
+
+// ---- up to 64 RW rows: 4 wavefronts of 16 RW rows, 64-key tiles for all
+
+// The rows of a workgroup: for each of its tokens the row of q (-1: none) and
+// its position.
+template <int R>
+struct RowList {
+    int tok[R + 1], pos[R + 1];
+    int sums[4], found[2];
+    int odd[2][4];  // by the tile's parity and the wavefront that loaded the part
+};
+// exclusive sum of v over the 256 threads; total: that of all
+template <int R>
+DEV int scan256(RowList<R> &ls, int v, int &total) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    int x = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_up(x, o, 64);
+        if (lane >= o) x += y;
+    }
+    __syncthreads();
+    if (lane == 63) ls.sums[w] = x;
+    __syncthreads();
+    int before = 0;
+    total = 0;
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+        if (u < w) before += ls.sums[u];
+        total += ls.sums[u];
+    }
+    return before + x - v;
+}
+DEV PagedSeq seq_of(const FapParams &p, int b) {
+    const int32_t *row = p.seqs + (int64_t)b * p.seq_nb1;
+    return paged_seq(row[0], row[1], row[2], p.T, p.max_q);
+}
+
+template <typename E, int DP, int RW>
+DEV void fap_tile(const FapParams &p) {
+    constexpr int KT = 64, R = 64 * RW, CH = DP / 8, NI = KT * CH / 256;  // loads of a K tile by each wavefront
+    constexpr int TB = KT * DP * 2;
+    __shared__ __attribute__((aligned(1024))) uint8_t kvs[2][2][TB];
+    __shared__ int32_t te[4][2][64];
+    __shared__ RowList<R> ls;
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, g = lane >> 4;
+    const int G = p.H / p.H_kv;
+    const int64_t table = (int64_t)p.per * p.page;
+    const bool shared = (int)blockIdx.x < p.wg_sh;
+    const int id = shared ? blockIdx.x : blockIdx.x - p.wg_sh, nz = shared ? p.zs_sh : p.zs_own;
+    const int hk = id % p.H_kv, z = (id / p.H_kv) % nz, blk = id / (p.H_kv * nz);
+    const int32_t *row = p.seqs;  // the pages: the first sequence's for the shared prefix
+    int x0, r0;  // first token of the list, first row of the block (rows of token x0 + k: G (x0 + k) ..)
+    if (shared) {
+        // tokens x0 .. of all sequences in order
+        r0 = blk * R;
+        x0 = r0 / G;
+        const int nx = (r0 + R - 1) / G - x0 + 1;
+        for (int k = tid; k < nx; k += 256) ls.tok[k] = -1;
+        __syncthreads();
+        if (p.max_q == 1) {  // one row a sequence: sequence x0 + k
+            for (int k = tid; k < nx && x0 + k < p.B; k += 256) {
+                const PagedSeq sq = seq_of(p, x0 + k);
+                ls.tok[k] = sq.nq ? sq.q0 : -1;
+                ls.pos[k] = clip_pos(sq.pos0, table);
+            }
+        } else {
+            int base = 0;
+            for (int b0 = 0; b0 < p.B && base < x0 + nx; b0 += 256) {
+                PagedSeq sq;
+                sq.nq = 0;
+                if (b0 + tid < p.B) sq = seq_of(p, b0 + tid);
+                int total;
+                const int at = base + scan256<R>(ls, sq.nq, total);
+                for (int k = max(at, x0); k < min(at + sq.nq, x0 + nx); k++) {
+                    ls.tok[k - x0] = sq.q0 + (k - at);
+                    ls.pos[k - x0] = clip_pos(sq.pos0 + (k - at), table);
+                }
+                base += total;
+            }
+        }
+    } else {
+        // block blk of the sequences' blocks of R rows
+        int b = blk, bb = 0;
+        if ((int64_t)p.max_q * G > R) {
+            if (tid == 0) ls.found[0] = -1;
+            int base = 0;
+            for (int b0 = 0; b0 < p.B && base <= blk; b0 += 256) {
+                int nb = 0;
+                if (b0 + tid < p.B) nb = (int)(((int64_t)seq_of(p, b0 + tid).nq * G + R - 1) / R);
+                int total;
+                const int at = base + scan256<R>(ls, nb, total);
+                if (at <= blk && blk < at + nb) {
+                    ls.found[0] = b0 + tid;
+                    ls.found[1] = at + nb - 1 - blk;  // the last rows, which see most keys, come first
+                }
+                base += total;
+            }
+            __syncthreads();
+            b = ls.found[0];
+            bb = ls.found[1];
+            if (b < 0) return;
+        }
+        r0 = bb * R;
+        x0 = r0 / G;
+        const PagedSeq sq = seq_of(p, b);
+        const int nx = (r0 + R - 1) / G - x0 + 1;
+        for (int k = tid; k < nx; k += 256) {
+            ls.tok[k] = x0 + k < sq.nq ? sq.q0 + x0 + k : -1;
+            ls.pos[k] = clip_pos(sq.pos0 + x0 + k, table);
+        }
+        row = p.seqs + (int64_t)b * p.seq_nb1;
+    }
+    __syncthreads();
+    Pass ps;
+    ps.p0 = 0x7fffffff;
+    ps.p1 = -1;
+    bool any = false;
+    for (int k = lane; k <= (r0 + R - 1) / G - x0; k += 64)
+        if (ls.tok[k] >= 0) {
+            ps.p0 = min(ps.p0, ls.pos[k]);
+            ps.p1 = max(ps.p1, ls.pos[k]);
+            any = true;
+        }
+    if (!__ballot(any)) return;
+#pragma unroll
+    for (int o = 32; o; o >>= 1) {
+        ps.p0 = min(ps.p0, __shfl_xor(ps.p0, o, 64));
+        ps.p1 = max(ps.p1, __shfl_xor(ps.p1, o, 64));
+    }
+    ps.p0 = __builtin_amdgcn_readfirstlane(ps.p0);
+    ps.p1 = __builtin_amdgcn_readfirstlane(ps.p1);
+    ps.tl = paged_tiles(ps.p0, ps.p1, p.window, p.n_first, shared ? 0 : p.n_shared, shared ? p.n_shared : (int)table, KT);
+    const int share = paged_share(ps.tl.n, nz, p.least);
+    const int t0 = (int)min((int64_t)z * share, (int64_t)ps.tl.n), t1 = min(ps.tl.n, t0 + share);
+    // this lane's rows
+    struct Row {
+        int hd, pos;
+        bool valid;
+        int64_t tok, pi;
+    };
+    auto row_of = [&](int rt) {
+        Row y;
+        const int r = r0 + 16 * (RW * w + rt) + n, k = r / G - x0;
+        y.hd = hk * G + r % G;
+        y.valid = ls.tok[k] >= 0;
+        y.tok = y.valid ? ls.tok[k] : 0;
+        y.pos = y.valid ? ls.pos[k] : -1;
+        y.pi = (y.tok * p.H + y.hd) * (p.zs_sh + p.zs_own) + (shared ? 0 : p.zs_sh) + z;
+        return y;
+    };
+    if (t0 >= t1 && p.part) {  // nothing in this split
+#pragma unroll
+        for (int rt = 0; rt < RW; rt++) {
+            const Row y = row_of(rt);
+            if (y.valid && g == 0) stat_none(p, y.pi, y.pos >= table);
+        }
+        return;
+    }
+    Rows<E, DP, RW> Q;
+    bool mine = false;
+#pragma unroll
+    for (int rt = 0; rt < RW; rt++) {
+        const Row y = row_of(rt);
+        rows_load<E, DP, RW>(Q, rt, p.q + y.tok * p.q_nb2 + y.hd * p.q_nb1, p.D, p.scale * kLog2e, y.valid);
+        Q.pos[rt] = y.pos;
+        mine = mine || y.valid;
+    }
+    const bool work = __ballot(mine) != 0;  // a wavefront without rows only loads
+    const E *kvh = (const E *)p.kv + hk * p.kv_head;
+
+    auto load_pages = [&](int t) {
+        const Tile tl = tile_at(ps.tl, min(t, t1 - 1), KT);
+        const int j = min(tl.k0 + lane, tl.ke - 1);
+        load4(row + 3 + paged_div((uint32_t)j, p.by_page), lds_addr(te[w][t & 1]));
+    };
+    uint64_t ok = 0, bad = 0;  // keys of the next tile that are there, those on no page
+    auto load_tile = [&](int t) {
+        const Tile tl = tile_at(ps.tl, t, KT);
+        const int32_t *pg = te[w][t & 1];
+        const bool in = tl.k0 + lane < tl.ke;
+        const int my = in ? pg[lane] : 0;
+        const bool there = my >= 0 && my < p.n_pages;
+        ok = __ballot(in && there);
+        bad = __ballot(in && !there);
+        const uint32_t ka = lds_addr(kvs[t & 1][0]), va = lds_addr(kvs[t & 1][1]);
+        const E *at[NI];
+#pragma unroll
+        for (int ii = 0; ii < NI; ii++) {
+            const int r = (64 * (NI * w + ii) + lane) / CH;
+            const uint32_t j = tl.k0 + r, page = pg[r];
+            const bool o = (ok >> r) & 1;
+            at[ii] = kvh + (o ? (int64_t)page * p.kv_page + (int64_t)(j - paged_div(j, p.by_page) * p.page) * p.kv_row : 0);
+        }
+        load_pages(t + 1);
+#pragma unroll
+        for (int ii = 0; ii < NI; ii++) {
+            const int c = 64 * (NI * w + ii) + lane, r = c / CH, x = k_swz<CH>(r, c % CH);
+            load16(at[ii] + (8 * x < p.D ? 8 * x : 0), ka + 1024 * (NI * w + ii));
+        }
+#pragma unroll
+        for (int ii = 0; ii < NI; ii++) {
+            const int c = 64 * (NI * w + ii) + lane, r = c / CH, x = v_swz<CH>(r, c % CH);
+            load16(at[ii] + p.D + (8 * x < p.D ? 8 * x : 0), va + 1024 * (NI * w + ii));
+        }
+    };
+    // What this wavefront loaded of tile t is in: rows that were not there hold
+    // nothing that counts, and a tile that some rows do not see in full is looked
+    // through for infinities and NaN.
+    auto loaded = [&](int t) {
+        uint8_t *Vs = kvs[t & 1][1];
+        if (ok != ~0ull) {
+#pragma unroll
+            for (int ii = 0; ii < NI; ii++) {
+                const int c = 64 * (NI * w + ii) + lane;
+                if (!((ok >> (c / CH)) & 1)) *(uint4 *)(Vs + 16 * c) = make_uint4(0, 0, 0, 0);
+            }
+        }
+        if (!tile_whole(tile_at(ps.tl, t, KT), KT, ps, p.window, p.n_first)) {
+            const bool odd = odd_chunks<E>(Vs, 64 * NI * w, NI);
+            if (lane == 0) ls.odd[t & 1][w] = odd;
+        }
+    };
+    if (t0 < t1) {
+        load_pages(t0);
+        wait_loads<0>();
+        load_tile(t0);
+        wait_loads<0>();
+        loaded(t0);
+    }
+    __syncthreads();
+    for (int t = t0; t < t1; t++) {
+        const Tile tile = tile_at(ps.tl, t, KT);
+        const uint64_t badc = bad;
+        const bool part = !tile_whole(tile, KT, ps, p.window, p.n_first);
+        const E *Ks = (const E *)kvs[t & 1][0], *Vs = (const E *)kvs[t & 1][1];
+        if (t + 1 < t1) load_tile(t + 1);
+        v4f s[4][RW];
+        if (work) {
+            scores<E, DP, RW, 4>(Q, Ks, s);
+            __builtin_amdgcn_sched_barrier(0);
+            if (part || badc) mask_scores<E, DP, RW, 4>(Q, s, tile.k0, tile.ke, badc, p.window, p.n_first);
+            softmax<E, DP, RW, 4>(Q, s);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if (part && (ls.odd[t & 1][0] | ls.odd[t & 1][1] | ls.odd[t & 1][2] | ls.odd[t & 1][3])) {
+            if (work) add_odd<E, DP, RW, 4>(Q, Vs, s);
+            __syncthreads();
+            clear_odd<E>(kvs[t & 1][1], 64 * NI * w, NI);
+            __syncthreads();
+        }
+        if (work) values<E, DP, RW, 4>(Q, Vs, s);
+        if (t + 1 < t1) {
+            wait_loads<0>();
+            loaded(t + 1);
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int rt = 0; rt < RW; rt++) {
+        const Row y = row_of(rt);
+        float l = row_sum(Q.l[rt]), m = Q.set[rt] ? -Q.mneg[rt][0] : -__builtin_inff(), f = 1.0f;
+        if (y.pos >= table) l = __builtin_nanf("");
+        if (!y.valid) continue;
+        if (!p.part) finish_stat(p, y.hd, m, l, f);
+        float *out = p.part ? p.part + y.pi * p.D : p.dst + y.tok * p.d_nb2 + y.hd * p.d_nb1;
+#pragma unroll
+        for (int dt = 0; dt < DP / 16; dt++) {
+            const int d = 16 * dt + 4 * g;
+            const v4f a = Q.o[rt][dt] * f;
+            if (d < p.D) __builtin_memcpy(out + d, &a, 16);
+        }
+        if (p.part && g == 0) {
+            p.stat[2 * y.pi] = m;
+            p.stat[2 * y.pi + 1] = l;
+        }
+    }
+}
+
+// ---- the splits' partials of a row -> dst, in the order of the splits
+
+// One wavefront a row (token, head): lane z holds split z's statistics, then the
+// lanes share the dims, 4 each, and the 64 / (D / 4) groups of lanes the splits.
+DEV void fap_join(const FapParams &p) {
+    const int lane = threadIdx.x & 63;
+    const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int h = (int)(id % p.H);
+    const int64_t bi = id / p.H;
+    const int b = (int)(bi / p.max_q), i = (int)(bi - (int64_t)b * p.max_q);
+    if (b >= p.B) return;
+    const PagedSeq sq = seq_of(p, b);
+    if (i >= sq.nq) return;
+    const int64_t tok = sq.q0 + i, row = tok * p.H + h;
+    const int nz = p.zs_sh + p.zs_own;
+    float m = -__builtin_inff(), l = 0.0f;
+    if (lane < nz) {
+        m = p.stat[2 * (row * nz + lane)];
+        l = p.stat[2 * (row * nz + lane) + 1];
+    }
+    float M = m;
+#pragma unroll
+    for (int o = 32; o; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+    const float wt = m > -__builtin_inff() ? __builtin_amdgcn_exp2f(m - M) : 0.0f;
+    float L = wave_sum(m > -__builtin_inff() ? l * wt : l), Mf = M, fin;  // l of a split without keys: 0, or NaN
+    finish_stat(p, h, Mf, L, fin);
+    const float f = wt * fin;
+    const uint64_t some = __ballot(f != 0.0f);
+    const float *part = p.part + row * nz * p.D;
+    float *out = p.dst + tok * p.d_nb2 + (int64_t)h * p.d_nb1;
+    for (int d = 4 * lane; d < p.D; d += 256) {
+        v4f a = {0, 0, 0, 0};
+        for (uint64_t s = some; s; s &= s - 1) {
+            const int z = __builtin_ctzll(s);
+            v4f x;
+            __builtin_memcpy(&x, part + (int64_t)z * p.D + d, 16);
+            a += x * __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), z));
+        }
+        if (L != L) a = v4f{L, L, L, L};
+        __builtin_memcpy(out + d, &a, 16);
+    }
+}
+
+extern "C" __global__ void __launch_bounds__(256) ghip_fap_join(FapParams p) { fap_join(p); }
+#define FAP_K(E, DP, RW)                                                                                              extern "C" __global__ void __launch_bounds__(256, 2) ghip_fap_few_##E##_##DP(FapParams p) { fap_few<E, DP>(p); }      extern "C" __global__ void __launch_bounds__(256, 2) ghip_fap_tile_##E##_##DP(FapParams p) { fap_tile<E, DP, RW>(p); }
+#define FAP_E(E) FAP_K(E, 64, 2) FAP_K(E, 96, 2) FAP_K(E, 128, 2) FAP_K(E, 256, 1)
+FAP_E(f16) FAP_E(bf16)

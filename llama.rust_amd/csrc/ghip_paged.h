@@ -48,3 +48,52 @@ PAGED_FN PagedKeys paged_keys(int64_t p0, int64_t p1, int window, int n_first) {
 PAGED_FN bool paged_seen(int64_t p, int64_t j, int window, int n_first) {
     return j <= p && (!window || j > p - window || j < n_first);
 }
+
+// n / d for any 32-bit n by a product (Granlund and Montgomery's division by an
+// invariant integer); paged_divisor works the factors out on the host.
+struct PagedDiv {
+    uint32_t mul, sh1, sh2;
+};
+static inline PagedDiv paged_divisor(uint32_t d) {
+    uint32_t l = 0;
+    while (l < 32 && (1ull << l) < d) l++;
+    PagedDiv r;
+    r.mul = (uint32_t)((((1ull << l) - d) << 32) / d + 1);
+    r.sh1 = l < 1 ? l : 1;
+    r.sh2 = l < 1 ? 0 : l - 1;
+    return r;
+}
+PAGED_FN uint32_t paged_div(uint32_t n, PagedDiv d) {
+#ifdef __HIPCC__
+    const uint32_t t = __umulhi(d.mul, n);
+#else
+    const uint32_t t = (uint32_t)(((uint64_t)d.mul * n) >> 32);
+#endif
+    return (t + ((n - t) >> d.sh1)) >> d.sh2;
+}
+
+// The tiles of `kt` keys that a block of rows at positions p0 .. p1 goes through
+// in [from, to) of the keys (a pass over the shared prefix: [0, n_shared), one
+// over what is a sequence's own: from n_shared on): na of them over [a0, a1),
+// which are the keys seen whatever the window, then those over [b0, b1).
+struct PagedTiles {
+    int a0, a1, b0, b1, na, n;
+};
+PAGED_FN PagedTiles paged_tiles(int64_t p0, int64_t p1, int window, int n_first, int from, int to, int kt) {
+    const PagedKeys k = paged_keys(p0, p1, window, n_first);
+    PagedTiles t;
+    t.a0 = from;
+    t.a1 = k.first < to ? (int)k.first : to;
+    if (t.a1 < t.a0) t.a1 = t.a0;
+    t.b0 = k.lo > from ? (k.lo < to ? (int)k.lo : to) : from;
+    t.b1 = k.hi < to ? (int)k.hi : to;
+    if (t.b1 < t.b0) t.b1 = t.b0;
+    t.na = (int)(((int64_t)t.a1 - t.a0 + kt - 1) / kt);
+    t.n = t.na + (int)(((int64_t)t.b1 - t.b0 + kt - 1) / kt);
+    return t;
+}
+// Split z of `nz` takes tiles [z c, z c + c) of n: even shares, but at least `least`.
+PAGED_FN int paged_share(int n, int nz, int least) {
+    const int c = (n + nz - 1) / nz;
+    return c < least ? least : c;
+}
