@@ -3390,24 +3390,40 @@ FapLayout fap_layout(FapParams &p) {
     // the most keys that one block of rows goes through outside the shared prefix
     int64_t keys = table - p.n_shared;
     if (p.window) keys = std::min(keys, (int64_t)p.window + p.max_q - 1 + p.n_first);
-    p.least = 4;
-    auto splits = [&](int64_t wgs, int64_t want, int64_t n) {
-        return (int)std::max<int64_t>(1, std::min<int64_t>({(want + wgs - 1) / wgs, n, 32}));
+    p.least = 1;
+    // Splits of the keys of `blocks` tile workgroups with n tiles each and `rows`
+    // rows: the fewest microseconds of  rounds x (start + tiles)  and of writing
+    // and reading the partials.  A workgroup starts in 8 us; a tile takes 2.0 us
+    // where a CU has one workgroup, 3.2 where it has two (512 in a round); the
+    // partials go at 4.8 TB/s.
+    auto tile_splits = [&](int64_t blocks, int64_t rows, int64_t n) {
+        int best = 1;
+        double least = 0;
+        for (int z = 1; z <= 32 && z <= std::max<int64_t>(1, n); z++) {
+            const int64_t wgs = blocks * z;
+            const double us = (double)((wgs + 511) / 512) * (8.0 + (double)((n + z - 1) / z) * (wgs <= 256 ? 2.0 : 3.2)) +
+                              (z > 1 || p.n_shared ? 8.0 * rows * z * p.D / 4.8e6 : 0.0);
+            if (z == 1 || us < least) {
+                best = z;
+                least = us;
+            }
+        }
+        return best;
     };
+    const int64_t rows = std::min((int64_t)p.T, (int64_t)p.B * p.max_q) * p.H;
     if (L.few) {
+        // 256 keys a workgroup at least, and about 1024 of them
         p.nb_own = p.B;
-        p.zs_own = splits((int64_t)p.nb_own * p.H_kv, env_int("GHIP_FAP_WGS", 1024), (keys + 127) / 128);
+        const int64_t wgs = (int64_t)p.nb_own * p.H_kv;
+        p.zs_own = (int)std::max<int64_t>(1, std::min<int64_t>({(1024 + wgs - 1) / wgs, (keys + 255) / 256, 32}));
     } else {
         p.nb_own = (int64_t)p.max_q * G <= L.rows ? p.B : (int)((int64_t)p.T * G / L.rows + p.B);
-        p.zs_own = splits((int64_t)p.nb_own * p.H_kv, env_int("GHIP_FAP_WGS", 1024) / 2, (keys + 255) / 256);
+        p.zs_own = tile_splits((int64_t)p.nb_own * p.H_kv, rows, (keys + 63) / 64);
     }
     p.nb_sh = p.zs_sh = p.wg_sh = 0;
     if (p.n_shared) {
-        const int64_t rows = std::min((int64_t)p.T, (int64_t)p.B * p.max_q) * G;
-        p.nb_sh = (int)((rows + L.rows - 1) / L.rows);
-        int64_t shk = p.n_shared;
-        if (p.window) shk = std::min(shk, (int64_t)p.n_first + p.window + table);
-        p.zs_sh = splits((int64_t)p.nb_sh * p.H_kv, env_int("GHIP_FAP_WGS", 1024) / 2, (shk + 255) / 256);
+        p.nb_sh = (int)((rows / p.H * G + L.rows - 1) / L.rows);
+        p.zs_sh = tile_splits((int64_t)p.nb_sh * p.H_kv, rows, (p.n_shared + 63) / 64);
         p.wg_sh = p.nb_sh * p.H_kv * p.zs_sh;
     }
     const int nz = p.zs_sh + p.zs_own;
@@ -3450,33 +3466,21 @@ ghip_status ghip_flash_attn_paged(ghip_context *ctx, const ghip_tensor *q, const
         p.kv = (const uint16_t *)((uintptr_t)p.q & ~(uintptr_t)15);
         p.kv_head = p.kv_row = p.kv_page = 0;
     }
-    auto expect = [&]() {
-        if (p.part) {
-            const size_t n = (size_t)p.T * p.H * (p.zs_sh + p.zs_own);
-            ctx->expect(p.part, n * p.D * 4, "partials");
-            ctx->expect(p.stat, n * 2 * 4, "statistics");
-        } else {
-            ctx->expect(p.dst, (size_t)(4 * ((p.T - 1) * p.d_nb2 + (p.H - 1) * p.d_nb1 + p.D)), "dst");
-        }
-    };
     char name[48];
     const char *ty = float_name(kv->type);
     const int64_t own = (int64_t)p.nb_own * p.H_kv * p.zs_own, joins = ((int64_t)p.B * p.max_q * p.H + 3) / 4;
     if (own + p.wg_sh > INT32_MAX || joins > INT32_MAX)
         return ctx->fail(GHIP_STATUS_BACKEND_ERROR, "flash_attn_paged: too many rows");
-    const int64_t tiles = p.wg_sh + (L.few ? 0 : own);
-    if (tiles) {
-        expect();
-        snprintf(name, sizeof name, "ghip_fap_tile_%s_%d", ty, L.DP);
-        st = ctx->launch(name, dim3((unsigned)tiles), dim3(256), 0, s, p);
-        if (st != GHIP_STATUS_SUCCESS) return st;
+    if (p.part) {
+        const size_t n = (size_t)p.T * p.H * (p.zs_sh + p.zs_own);
+        ctx->expect(p.part, n * p.D * 4, "partials");
+        ctx->expect(p.stat, n * 2 * 4, "statistics");
+    } else {
+        ctx->expect(p.dst, (size_t)(4 * ((p.T - 1) * p.d_nb2 + (p.H - 1) * p.d_nb1 + p.D)), "dst");
     }
-    if (L.few) {
-        expect();
-        snprintf(name, sizeof name, "ghip_fap_few_%s_%d", ty, L.DP);
-        st = ctx->launch(name, dim3((unsigned)own), dim3(256), 0, s, p);
-        if (st != GHIP_STATUS_SUCCESS) return st;
-    }
+    snprintf(name, sizeof name, "ghip_fap_%s_%s_%d", !L.few ? "tile" : p.wg_sh ? "both" : "few", ty, L.DP);
+    st = ctx->launch(name, dim3((unsigned)(own + p.wg_sh)), dim3(256), 0, s, p);
+    if (st != GHIP_STATUS_SUCCESS) return st;
     if (!p.part) return GHIP_STATUS_SUCCESS;
     ctx->expect(p.dst, (size_t)(4 * ((p.T - 1) * p.d_nb2 + (p.H - 1) * p.d_nb1 + p.D)), "dst");
     return ctx->launch("ghip_fap_join", dim3((unsigned)joins), dim3(256), 0, s, p);

@@ -42,8 +42,8 @@ template <> struct Frag<f16> {
     typedef __fp16 tr __attribute__((__vector_size__(8)));
     static constexpr int NQ = 2, NP = 2;
     static __device__ __forceinline__ v4f mfma(v8 a, v8 b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
-    static __device__ __forceinline__ v4 read_tr(const f16 *p) {
-        return __builtin_bit_cast(v4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) tr *)p));
+    static __device__ __forceinline__ v4 read_tr(uint32_t at) {
+        return __builtin_bit_cast(v4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) tr *)at));
     }
 };
 template <> struct Frag<bf16> {
@@ -52,8 +52,8 @@ template <> struct Frag<bf16> {
     typedef __bf16 v2 __attribute__((ext_vector_type(2)));
     static constexpr int NQ = 3, NP = 3;
     static __device__ __forceinline__ v4f mfma(v8 a, v8 b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
-    static __device__ __forceinline__ v4 read_tr(const bf16 *p) {
-        return __builtin_bit_cast(v4, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) v4 *)p));
+    static __device__ __forceinline__ v4 read_tr(uint32_t at) {
+        return __builtin_bit_cast(v4, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) v4 *)at));
     }
 };
 
@@ -65,8 +65,8 @@ DEV void split_pair(float x0, float x1, typename Frag<E>::v2 (&t)[N]) {
     for (int i = 0; i < N; i++) {
         t[i] = __builtin_convertvector(x, typename Frag<E>::v2);
         if (i + 1 < N) {
-            x[0] -= (float)t[i][0];
-            x[1] -= (float)t[i][1];
+            x[0] = fmaf((float)t[i][0], -1.0f, x[0]);
+            x[1] = fmaf((float)t[i][1], -1.0f, x[1]);
         }
     }
 }
@@ -95,6 +95,7 @@ struct FapParams {
     float *part, *stat;
 };
 
+#define DEV_M __device__ __forceinline__
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int FEW_ROWS = 16, TILE_ROWS = 128;
 
@@ -178,24 +179,60 @@ DEV void rows_load(Rows<E, DP, RW> &R, int rt, const float *qr, int D, float sca
     R.set[rt] = false;
 }
 
-// Scores of the NT 16-key tiles at Ks, less the reference maximum.
-template <typename E, int DP, int RW, int NT>
-DEV void scores(const Rows<E, DP, RW> &R, const E *Ks, v4f (&s)[NT][RW]) {
+// Fragment reads.  The swizzles touch the low bits of a chunk's number alone, so
+// a fragment's address is one lane's constant with the bits of kk (dt) flipped in,
+// the rest added: k_at / v_at give the constant, frag_at the address.
+template <int DP>
+DEV uint32_t k_at(uint32_t Ks) {
     constexpr int CH = DP / 8;
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    return Ks + 2 * n * DP + 16 * (CH == 8 ? g ^ ((n >> 1) & 7) : CH == 12 ? g ^ ((n >> 2) & 3) : g ^ n);
+}
+template <int DP>
+DEV uint32_t v_at(uint32_t Vs) {
+    constexpr int CH = DP / 8;
+    const int lane = threadIdx.x & 63, lj = lane & 15, r = 4 * (lane >> 4) + (lj >> 2), c = (lj & 3) >> 1;
+    return Vs + 2 * r * DP + 16 * v_swz<CH>(r, c) + 8 * (lj & 1);
+}
+template <int STEP, int MASK>
+DEV uint32_t frag_at(uint32_t at, int i) {
+    return (at ^ (STEP * (i & MASK))) + STEP * (i & ~MASK);
+}
+// K fragment of the MFMA: keys 16 t + (lane & 15), dims 32 kk + 8 (lane >> 4) ..
+template <typename E, int DP>
+DEV typename Frag<E>::v8 key_frag(uint32_t kat, int t, int kk) {
+    constexpr int CH = DP / 8;
+    const uint32_t at = frag_at<64, CH == 8 ? 1 : CH == 12 ? 0 : 3>(kat, kk) + 32 * t * DP;
+    return *(const __attribute__((address_space(3))) typename Frag<E>::v8 *)at;
+}
+// V^T: dims 16 dt + (lane & 15), in slot e key 32 u + 4 g + e, from slot 4 on 16
+// further (as the scores lie)
+template <typename E, int DP>
+DEV typename Frag<E>::v8 value_frag(uint32_t vat, int u, int dt) {
+    constexpr int CH = DP / 8;
+    const uint32_t at = frag_at<32, CH == 8 ? 3 : CH == 12 ? 1 : 7>(vat, dt) + 64 * u * DP;
+    const typename Frag<E>::v4 lo = Frag<E>::read_tr(at), hi = Frag<E>::read_tr(at + 32 * DP);
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+// Scores of the NT 16-key tiles at Ks, less the reference maximum.
+template <typename E, int DP, int RW, int NT>
+DEV void scores(const Rows<E, DP, RW> &R, uint32_t Ks, v4f (&s)[NT][RW]) {
+    constexpr int KK = DP / 32, N = NT * KK;
+    const uint32_t kat = k_at<DP>(Ks);
+    // fragments are read two ahead of the products that use them
+    typename Frag<E>::v8 a[3];
+    a[0] = key_frag<E, DP>(kat, 0, 0);
+    a[1] = key_frag<E, DP>(kat, 1 / KK, 1 % KK);
 #pragma unroll
-    for (int t = 0; t < NT; t++) {
+    for (int f = 0; f < N; f++) {
+        const int t = f / KK, kk = f % KK;
+        if (f + 2 < N) a[(f + 2) % 3] = key_frag<E, DP>(kat, (f + 2) / KK, (f + 2) % KK);
 #pragma unroll
-        for (int kk = 0; kk < DP / 32; kk++) {
-            const int r = 16 * t + n;
-            typename Frag<E>::v8 a;
-            __builtin_memcpy(&a, __builtin_assume_aligned(Ks + r * DP + 8 * k_swz<CH>(r, 4 * kk + g), 16), 16);
+        for (int i = Frag<E>::NQ - 1; i >= 0; i--)
 #pragma unroll
-            for (int i = Frag<E>::NQ - 1; i >= 0; i--)
-#pragma unroll
-                for (int rt = 0; rt < RW; rt++)
-                    s[t][rt] = Frag<E>::mfma(a, R.q[rt][kk][i], kk == 0 && i == Frag<E>::NQ - 1 ? R.mneg[rt] : s[t][rt]);
-        }
+            for (int rt = 0; rt < RW; rt++)
+                s[t][rt] = Frag<E>::mfma(a[f % 3], R.q[rt][kk][i], kk == 0 && i == Frag<E>::NQ - 1 ? R.mneg[rt] : s[t][rt]);
+        __builtin_amdgcn_sched_barrier(0);
     }
 }
 
@@ -267,21 +304,11 @@ DEV void softmax(Rows<E, DP, RW> &R, v4f (&s)[NT][RW]) {
     }
 }
 
-// fragment of V^T of the MFMA: dims 16 dt + (lane & 15), in slot e key 32 u + 4 g + e,
-// from slot 4 on 16 further (as the scores lie)
-template <typename E, int DP>
-DEV typename Frag<E>::v8 value_frag(const E *Vs, int u, int dt) {
-    constexpr int CH = DP / 8;
-    const int lane = threadIdx.x & 63, lj = lane & 15, g = lane >> 4;
-    const int r0 = 32 * u + 4 * g + (lj >> 2), c = 2 * dt + ((lj & 3) >> 1), h = 4 * (lj & 1);
-    const typename Frag<E>::v4 lo = Frag<E>::read_tr(Vs + r0 * DP + 8 * v_swz<CH>(r0, c) + h);
-    const typename Frag<E>::v4 hi = Frag<E>::read_tr(Vs + (r0 + 16) * DP + 8 * v_swz<CH>(r0 + 16, c) + h);
-    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-}
 // O^T += V^T P^T over NT 16-key tiles at Vs
 template <typename E, int DP, int RW, int NT>
-DEV void values(Rows<E, DP, RW> &R, const E *Vs, const v4f (&s)[NT][RW]) {
+DEV void values(Rows<E, DP, RW> &R, uint32_t Vs, const v4f (&s)[NT][RW]) {
     constexpr int NP = Frag<E>::NP;
+    const uint32_t vat = v_at<DP>(Vs);
     typename Frag<E>::v8 p[RW][NP];
 #pragma unroll
     for (int u = 0; u < NT / 2; u++) {
@@ -297,15 +324,19 @@ DEV void values(Rows<E, DP, RW> &R, const E *Vs, const v4f (&s)[NT][RW]) {
                     p[rt][i][2 * e + 1] = t[i][1];
                 }
             }
+        typename Frag<E>::v8 a[3];
+        a[0] = value_frag<E, DP>(vat, u, 0);
+        a[1] = value_frag<E, DP>(vat, u, 1);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int dt = 0; dt < DP / 16; dt++) {
-            const typename Frag<E>::v8 a = value_frag<E, DP>(Vs, u, dt);
+            if (dt + 2 < DP / 16) a[(dt + 2) % 3] = value_frag<E, DP>(vat, u, dt + 2);
 #pragma unroll
             for (int i = NP - 1; i >= 0; i--)
 #pragma unroll
-                for (int rt = 0; rt < RW; rt++) R.o[rt][dt] = Frag<E>::mfma(a, p[rt][i], R.o[rt][dt]);
+                for (int rt = 0; rt < RW; rt++) R.o[rt][dt] = Frag<E>::mfma(a[dt % 3], p[rt][i], R.o[rt][dt]);
+            __builtin_amdgcn_sched_barrier(0);
         }
-        __builtin_amdgcn_sched_barrier(0);
     }
 }
 
@@ -319,7 +350,8 @@ DEV bool odd_pair(uint32_t x) {
     return (x & LO) == LO || (x & HI) == HI;
 }
 template <typename E, int DP, int RW, int NT>
-DEV void add_odd(Rows<E, DP, RW> &R, const E *Vs, const v4f (&s)[NT][RW]) {
+DEV void add_odd(Rows<E, DP, RW> &R, uint32_t Vs, const v4f (&s)[NT][RW]) {
+    const uint32_t vat = v_at<DP>(Vs);
 #pragma unroll
     for (int u = 0; u < NT / 2; u++)
 #pragma unroll
@@ -329,7 +361,7 @@ DEV void add_odd(Rows<E, DP, RW> &R, const E *Vs, const v4f (&s)[NT][RW]) {
             for (int e = 0; e < 8; e++) p[e] = s[2 * u + e / 4][rt][e & 3] > 0.0f ? (E)1.0f : (E)0.0f;
 #pragma unroll
             for (int dt = 0; dt < DP / 16; dt++) {
-                const typename Frag<E>::v8 a = value_frag<E, DP>(Vs, u, dt);
+                const typename Frag<E>::v8 a = value_frag<E, DP>(vat, u, dt);
                 typename Frag<E>::v8 up, dn;
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
@@ -349,7 +381,8 @@ DEV void add_odd(Rows<E, DP, RW> &R, const E *Vs, const v4f (&s)[NT][RW]) {
             }
         }
 }
-// chunks from + 64 i + lane, i < n, of a tile: do they hold one?  / set to 0
+// chunks from + 64 i + lane, i < n, of a tile: do they hold one?  Chunks from, from
+// + step, .. below n: set to 0.
 template <typename E>
 DEV bool odd_chunks(const uint8_t *Vs, int from, int n) {
     bool odd = false;
@@ -361,11 +394,11 @@ DEV bool odd_chunks(const uint8_t *Vs, int from, int n) {
     return __ballot(odd) != 0;
 }
 template <typename E>
-DEV void clear_odd(uint8_t *Vs, int from, int n) {
+DEV void clear_odd(uint8_t *Vs, int from, int step, int n) {
     constexpr uint32_t LO = Frag<E>::NQ == 2 ? 0x7c00u : 0x7f80u, HI = LO << 16;
 #pragma unroll 1
-    for (int i = 0; i < n; i++) {
-        uint32_t *x = (uint32_t *)(Vs + 16 * (from + 64 * i + (threadIdx.x & 63)));
+    for (int i = from; i < n; i += step) {
+        uint32_t *x = (uint32_t *)(Vs + 16 * i);
 #pragma unroll
         for (int k = 0; k < 4; k++) {
             if ((x[k] & LO) == LO) x[k] &= 0xffff0000u;
@@ -419,19 +452,59 @@ DEV void stat_none(const FapParams &p, int64_t pi, bool nan) {
     p.stat[2 * pi + 1] = nan ? __builtin_nanf("") : 0.0f;
 }
 
+// Where the keys of a tile are: page numbers pg[] -> bytes into the cache of each
+// key's row, offs[] (a lane a key, once for all the lanes that load its row).
+// Keys past the tile's end or on no page: row 0 of page 0, which is not used.
+DEV void find_keys(const FapParams &p, const Tile &tl, int kt, const int32_t *pg, int64_t *offs, uint64_t &ok, uint64_t &bad) {
+    const int lane = threadIdx.x & 63;
+    const uint32_t j = tl.k0 + lane;
+    const bool in = lane < kt && (int)j < tl.ke;
+    const int page = in ? pg[lane] : 0;
+    const bool there = page >= 0 && page < p.n_pages;
+    ok = __ballot(in && there);
+    bad = __ballot(in && !there);
+    const uint32_t r = j - paged_div(j, p.by_page) * (uint32_t)p.page;
+    offs[lane] = in && there ? 2 * (page * p.kv_page + r * p.kv_row) : 0;
+}
+// The 16-byte pieces that a lane loads of a tile's rows: load ii of a wavefront
+// fills LDS chunks 64 (from + ii) + lane.  Chunks past the row's end (D < DP) take its last.
+template <int DP>
+struct RowLoads {
+    static constexpr int CH = DP / 8;
+    int at;
+    uint32_t last;
+    DEV_M RowLoads(int D, int from) : at(64 * from + (threadIdx.x & 63)), last(2 * D - 16) {}
+    DEV_M int row(int ii) const { return (at + 64 * ii) / CH; }
+    DEV_M uint32_t k_chunk(int ii) const {
+        const int r = row(ii);
+        return min((uint32_t)(16 * k_swz<CH>(r, (at + 64 * ii) - r * CH)), last);
+    }
+    DEV_M uint32_t v_chunk(int ii) const {
+        const int r = row(ii);
+        return min((uint32_t)(16 * v_swz<CH>(r, (at + 64 * ii) - r * CH)), last);
+    }
+};
+
 // ---- up to 16 rows a KV head: 4 wavefronts, each its own 32-key tiles
 
+template <int DP>
+struct FewLds {
+    uint8_t kvs[4][2][32 * DP * 2];  // each wavefront's K and V tile
+    int64_t offs[4][64];
+    int32_t te[4][2][64];
+    float ws[4][2][16];
+};
 template <typename E, int DP>
-DEV void fap_few(const FapParams &p) {
+DEV void fap_few(const FapParams &p, FewLds<DP> &lds) {
     constexpr int KT = 32, CH = DP / 8, NI = KT * CH / 64;  // loads of a K (or V) tile
-    constexpr int TB = KT * DP * 2;                         // bytes of one
-    __shared__ __attribute__((aligned(1024))) uint8_t kvs[4][2][TB];
-    __shared__ int32_t te[4][2][64];
-    __shared__ float ws[4][2][16];
+    auto &kvs = lds.kvs;
+    auto &offs = lds.offs;
+    auto &te = lds.te;
+    auto &ws = lds.ws;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
     const int G = p.H / p.H_kv;
     const int64_t table = (int64_t)p.per * p.page;
-    const int id = blockIdx.x, hk = id % p.H_kv, z = (id / p.H_kv) % p.zs_own, b = id / (p.H_kv * p.zs_own);
+    const int id = blockIdx.x - p.wg_sh, hk = id % p.H_kv, z = (id / p.H_kv) % p.zs_own, b = id / (p.H_kv * p.zs_own);
     const int32_t *row = p.seqs + (int64_t)b * p.seq_nb1;
     const PagedSeq sq = paged_seq(row[0], row[1], row[2], p.T, p.max_q);
     if (sq.nq == 0) return;
@@ -453,9 +526,7 @@ DEV void fap_few(const FapParams &p) {
     Rows<E, DP, 1> R;
     rows_load<E, DP, 1>(R, 0, p.q + tok * p.q_nb2 + hd * p.q_nb1, p.D, p.scale * kLog2e, valid);
     R.pos[0] = valid ? clip_pos(sq.pos0 + i, table) : -1;
-    const E *kvh = (const E *)p.kv + hk * p.kv_head;
-    E *Ks = (E *)kvs[w][0], *Vs = (E *)kvs[w][1];
-    const uint32_t ka = lds_addr(Ks), va = lds_addr(Vs);
+    const uint32_t ka = lds_addr(kvs[w][0]), va = lds_addr(kvs[w][1]);
 
     // page numbers of tile t's keys, a lane each
     auto load_pages = [&](int t) {
@@ -463,59 +534,37 @@ DEV void fap_few(const FapParams &p) {
         const int j = min(tl.k0 + lane, tl.ke - 1);
         load4(row + 3 + paged_div((uint32_t)j, p.by_page), lds_addr(te[w][t >> 2 & 1]));
     };
-    const E *at[NI];       // this lane's source of each load of the next tile
-    uint32_t ok = 0;       // its keys that are there
-    uint32_t bad = 0;      // those on no page
-    auto find_rows = [&](int t, uint32_t &okm, uint32_t &badm) {
-        const Tile tl = tile_at(ps.tl, t, KT);
-        const int32_t *pg = te[w][t >> 2 & 1];
-        const bool in = lane < KT && tl.k0 + lane < tl.ke;
-        const int my = in ? pg[lane] : 0;
-        const bool there = my >= 0 && my < p.n_pages;
-        okm = (uint32_t)__ballot(in && there);
-        badm = (uint32_t)__ballot(in && !there);
-#pragma unroll
-        for (int ii = 0; ii < NI; ii++) {
-            const int c = 64 * ii + lane, r = c / CH;
-            const uint32_t j = tl.k0 + r, page = pg[r];
-            const bool o = (okm >> r) & 1;
-            const int64_t off = o ? (int64_t)page * p.kv_page + (int64_t)(j - paged_div(j, p.by_page) * p.page) * p.kv_row : 0;
-            at[ii] = kvh + off;
-        }
-    };
+    const RowLoads<DP> rl(p.D, 0);
+    uint64_t ok = 0, bad = 0;  // the next tile's keys that are there, those on no page
+    auto find_rows = [&](int t) { find_keys(p, tile_at(ps.tl, t, KT), KT, te[w][t >> 2 & 1], offs[w], ok, bad); };
+    const uint8_t *kvh = (const uint8_t *)(p.kv + hk * p.kv_head);
     auto load_k = [&]() {
 #pragma unroll
-        for (int ii = 0; ii < NI; ii++) {
-            const int c = 64 * ii + lane, r = c / CH, x = k_swz<CH>(r, c % CH);
-            load16(at[ii] + (8 * x < p.D ? 8 * x : 0), ka + 1024 * ii);
-        }
+        for (int ii = 0; ii < NI; ii++) load16(kvh + offs[w][rl.row(ii)] + rl.k_chunk(ii), ka + 1024 * ii);
     };
     auto load_v = [&]() {
 #pragma unroll
-        for (int ii = 0; ii < NI; ii++) {
-            const int c = 64 * ii + lane, r = c / CH, x = v_swz<CH>(r, c % CH);
-            load16(at[ii] + p.D + (8 * x < p.D ? 8 * x : 0), va + 1024 * ii);
-        }
+        for (int ii = 0; ii < NI; ii++) load16(kvh + offs[w][rl.row(ii)] + 2 * p.D + rl.v_chunk(ii), va + 1024 * ii);
     };
     // in flight at the top of a step, oldest first: pages t + 4, K t, V t
     const int first = t0 + w;
     if (first < t1) {
         load_pages(first);
         wait_loads<0>();
-        find_rows(first, ok, bad);
+        find_rows(first);
         load_pages(first + 4);
         load_k();
         load_v();
     }
     for (int t = first; t < t1; t += 4) {
         const Tile tile = tile_at(ps.tl, t, KT);
-        const uint32_t okc = ok, badc = bad;
+        const uint64_t okc = ok, badc = bad;
         const bool more = t + 4 < t1;
         wait_loads<NI>();
         v4f s[2][1];
-        scores<E, DP, 1, 2>(R, Ks, s);
+        scores<E, DP, 1, 2>(R, ka, s);
         if (more) {
-            find_rows(t + 4, ok, bad);
+            find_rows(t + 4);
             wait_lds();
             load_pages(t + 8);
             load_k();
@@ -525,7 +574,7 @@ DEV void fap_few(const FapParams &p) {
         softmax<E, DP, 1, 2>(R, s);
         if (more) wait_loads<NI + 1>();
         else wait_loads<0>();
-        if (okc != 0xffffffffu) {
+        if (okc != 0xffffffffull) {
             // rows that were not there: no value of theirs may count
 #pragma unroll
             for (int ii = 0; ii < NI; ii++) {
@@ -535,10 +584,10 @@ DEV void fap_few(const FapParams &p) {
             wait_lds();
         }
         if (part && ps.p0 != ps.p1 && odd_chunks<E>(kvs[w][1], 0, NI)) {
-            add_odd<E, DP, 1, 2>(R, Vs, s);
-            clear_odd<E>(kvs[w][1], 0, NI);
+            add_odd<E, DP, 1, 2>(R, va, s);
+            clear_odd<E>(kvs[w][1], lane, 64, KT * CH);
         }
-        values<E, DP, 1, 2>(R, Vs, s);
+        values<E, DP, 1, 2>(R, va, s);
         if (more) {
             wait_lds();
             load_v();
@@ -623,13 +672,20 @@ DEV PagedSeq seq_of(const FapParams &p, int b) {
     return paged_seq(row[0], row[1], row[2], p.T, p.max_q);
 }
 
+template <int DP, int RW>
+struct TileLds {
+    uint8_t kvs[2][2][64 * DP * 2];  // this tile's K and V, the next one's
+    int64_t offs[4][64];
+    int32_t te[4][2][64];
+    RowList<64 * RW> ls;
+};
 template <typename E, int DP, int RW>
-DEV void fap_tile(const FapParams &p) {
+DEV void fap_tile(const FapParams &p, TileLds<DP, RW> &lds) {
     constexpr int KT = 64, R = 64 * RW, CH = DP / 8, NI = KT * CH / 256;  // loads of a K tile by each wavefront
-    constexpr int TB = KT * DP * 2;
-    __shared__ __attribute__((aligned(1024))) uint8_t kvs[2][2][TB];
-    __shared__ int32_t te[4][2][64];
-    __shared__ RowList<R> ls;
+    auto &kvs = lds.kvs;
+    auto &offs = lds.offs;
+    auto &te = lds.te;
+    auto &ls = lds.ls;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, g = lane >> 4;
     const int G = p.H / p.H_kv;
     const int64_t table = (int64_t)p.per * p.page;
@@ -754,7 +810,7 @@ DEV void fap_tile(const FapParams &p) {
         mine = mine || y.valid;
     }
     const bool work = __ballot(mine) != 0;  // a wavefront without rows only loads
-    const E *kvh = (const E *)p.kv + hk * p.kv_head;
+    const uint8_t *kvh = (const uint8_t *)(p.kv + hk * p.kv_head);
 
     auto load_pages = [&](int t) {
         const Tile tl = tile_at(ps.tl, min(t, t1 - 1), KT);
@@ -762,33 +818,16 @@ DEV void fap_tile(const FapParams &p) {
         load4(row + 3 + paged_div((uint32_t)j, p.by_page), lds_addr(te[w][t & 1]));
     };
     uint64_t ok = 0, bad = 0;  // keys of the next tile that are there, those on no page
+    const RowLoads<DP> rl(p.D, NI * w);
     auto load_tile = [&](int t) {
-        const Tile tl = tile_at(ps.tl, t, KT);
-        const int32_t *pg = te[w][t & 1];
-        const bool in = tl.k0 + lane < tl.ke;
-        const int my = in ? pg[lane] : 0;
-        const bool there = my >= 0 && my < p.n_pages;
-        ok = __ballot(in && there);
-        bad = __ballot(in && !there);
-        const uint32_t ka = lds_addr(kvs[t & 1][0]), va = lds_addr(kvs[t & 1][1]);
-        const E *at[NI];
-#pragma unroll
-        for (int ii = 0; ii < NI; ii++) {
-            const int r = (64 * (NI * w + ii) + lane) / CH;
-            const uint32_t j = tl.k0 + r, page = pg[r];
-            const bool o = (ok >> r) & 1;
-            at[ii] = kvh + (o ? (int64_t)page * p.kv_page + (int64_t)(j - paged_div(j, p.by_page) * p.page) * p.kv_row : 0);
-        }
+        find_keys(p, tile_at(ps.tl, t, KT), KT, te[w][t & 1], offs[w], ok, bad);
+        const uint32_t ka = lds_addr(kvs[t & 1][0]) + 1024 * NI * w, va = lds_addr(kvs[t & 1][1]) + 1024 * NI * w;
         load_pages(t + 1);
 #pragma unroll
         for (int ii = 0; ii < NI; ii++) {
-            const int c = 64 * (NI * w + ii) + lane, r = c / CH, x = k_swz<CH>(r, c % CH);
-            load16(at[ii] + (8 * x < p.D ? 8 * x : 0), ka + 1024 * (NI * w + ii));
-        }
-#pragma unroll
-        for (int ii = 0; ii < NI; ii++) {
-            const int c = 64 * (NI * w + ii) + lane, r = c / CH, x = v_swz<CH>(r, c % CH);
-            load16(at[ii] + p.D + (8 * x < p.D ? 8 * x : 0), va + 1024 * (NI * w + ii));
+            const uint8_t *row = kvh + offs[w][rl.row(ii)];
+            load16(row + rl.k_chunk(ii), ka + 1024 * ii);
+            load16(row + 2 * p.D + rl.v_chunk(ii), va + 1024 * ii);
         }
     };
     // What this wavefront loaded of tile t is in: rows that were not there hold
@@ -820,23 +859,34 @@ DEV void fap_tile(const FapParams &p) {
         const Tile tile = tile_at(ps.tl, t, KT);
         const uint64_t badc = bad;
         const bool part = !tile_whole(tile, KT, ps, p.window, p.n_first);
-        const E *Ks = (const E *)kvs[t & 1][0], *Vs = (const E *)kvs[t & 1][1];
+        const uint32_t Ks = lds_addr(kvs[t & 1][0]), Vs = lds_addr(kvs[t & 1][1]);
         if (t + 1 < t1) load_tile(t + 1);
-        v4f s[4][RW];
-        if (work) {
-            scores<E, DP, RW, 4>(Q, Ks, s);
-            __builtin_amdgcn_sched_barrier(0);
-            if (part || badc) mask_scores<E, DP, RW, 4>(Q, s, tile.k0, tile.ke, badc, p.window, p.n_first);
-            softmax<E, DP, RW, 4>(Q, s);
-            __builtin_amdgcn_sched_barrier(0);
+        const bool odd = part && (ls.odd[t & 1][0] | ls.odd[t & 1][1] | ls.odd[t & 1][2] | ls.odd[t & 1][3]);
+        // 32 keys at a time: their scores are fewer registers than 64 keys' (which
+        // then spill), and one half's products run under the other's softmax
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const uint32_t Kh = Ks + 64 * u * DP, Vh = Vs + 64 * u * DP;
+            v4f s[2][RW];
+            if (work) {
+                __builtin_amdgcn_s_setprio(1);
+                scores<E, DP, RW, 2>(Q, Kh, s);
+                __builtin_amdgcn_s_setprio(0);
+                if (part || badc) mask_scores<E, DP, RW, 2>(Q, s, tile.k0 + 32 * u, tile.ke, badc >> (32 * u), p.window, p.n_first);
+                softmax<E, DP, RW, 2>(Q, s);
+            }
+            if (odd) {
+                if (work) add_odd<E, DP, RW, 2>(Q, Vh, s);
+                __syncthreads();
+                clear_odd<E>(kvs[t & 1][1] + 64 * u * DP, tid, 256, 32 * CH);
+                __syncthreads();
+            }
+            if (work) {
+                __builtin_amdgcn_s_setprio(1);
+                values<E, DP, RW, 2>(Q, Vh, s);
+                __builtin_amdgcn_s_setprio(0);
+            }
         }
-        if (part && (ls.odd[t & 1][0] | ls.odd[t & 1][1] | ls.odd[t & 1][2] | ls.odd[t & 1][3])) {
-            if (work) add_odd<E, DP, RW, 4>(Q, Vs, s);
-            __syncthreads();
-            clear_odd<E>(kvs[t & 1][1], 64 * NI * w, NI);
-            __syncthreads();
-        }
-        if (work) values<E, DP, RW, 4>(Q, Vs, s);
         if (t + 1 < t1) {
             wait_loads<0>();
             loaded(t + 1);
@@ -866,8 +916,9 @@ DEV void fap_tile(const FapParams &p) {
 
 // ---- the splits' partials of a row -> dst, in the order of the splits
 
-// One wavefront a row (token, head): lane z holds split z's statistics, then the
-// lanes share the dims, 4 each, and the 64 / (D / 4) groups of lanes the splits.
+// One wavefront a row (token, head): lane z holds split z's statistics; then NG
+// groups of D / 4 lanes take 4 dims a lane of splits group, group + NG, .. (8 of
+// them in flight), and the groups are added in order.
 DEV void fap_join(const FapParams &p) {
     const int lane = threadIdx.x & 63;
     const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -878,7 +929,7 @@ DEV void fap_join(const FapParams &p) {
     const PagedSeq sq = seq_of(p, b);
     if (i >= sq.nq) return;
     const int64_t tok = sq.q0 + i, row = tok * p.H + h;
-    const int nz = p.zs_sh + p.zs_own;
+    const int nz = p.zs_sh + p.zs_own, LD = p.D / 4, NG = 64 / LD, grp = lane / LD;
     float m = -__builtin_inff(), l = 0.0f;
     if (lane < nz) {
         m = p.stat[2 * (row * nz + lane)];
@@ -891,23 +942,54 @@ DEV void fap_join(const FapParams &p) {
     float L = wave_sum(m > -__builtin_inff() ? l * wt : l), Mf = M, fin;  // l of a split without keys: 0, or NaN
     finish_stat(p, h, Mf, L, fin);
     const float f = wt * fin;
-    const uint64_t some = __ballot(f != 0.0f);
-    const float *part = p.part + row * nz * p.D;
-    float *out = p.dst + tok * p.d_nb2 + (int64_t)h * p.d_nb1;
-    for (int d = 4 * lane; d < p.D; d += 256) {
-        v4f a = {0, 0, 0, 0};
-        for (uint64_t s = some; s; s &= s - 1) {
-            const int z = __builtin_ctzll(s);
-            v4f x;
-            __builtin_memcpy(&x, part + (int64_t)z * p.D + d, 16);
-            a += x * __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), z));
+    const float *part = p.part + row * nz * p.D + 4 * (lane - grp * LD);
+    v4f a = {0, 0, 0, 0};
+    for (int z0 = 0; z0 < nz; z0 += 8 * NG) {
+        v4f x[8];
+        float w[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const int z = z0 + grp + k * NG;
+            w[k] = __shfl(f, min(z, 63), 64);
+            if (z >= nz || grp >= NG) w[k] = 0.0f;
+            x[k] = v4f{0, 0, 0, 0};
+            if (w[k] != 0.0f) __builtin_memcpy(&x[k], part + (int64_t)z * p.D, 16);
         }
-        if (L != L) a = v4f{L, L, L, L};
-        __builtin_memcpy(out + d, &a, 16);
+#pragma unroll
+        for (int k = 0; k < 8; k++) a += x[k] * w[k];
+    }
+    v4f sum = a;
+    for (int k = 1; k < NG; k++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) sum[e] += __shfl(a[e], (lane + k * LD) & 63, 64);
+    if (lane < LD) {
+        if (L != L) sum = v4f{L, L, L, L};
+        __builtin_memcpy(p.dst + tok * p.d_nb2 + (int64_t)h * p.d_nb1 + 4 * lane, &sum, 16);
     }
 }
 
 extern "C" __global__ void __launch_bounds__(256) ghip_fap_join(FapParams p) { fap_join(p); }
-#define FAP_K(E, DP, RW)                                                                                              extern "C" __global__ void __launch_bounds__(256, 2) ghip_fap_few_##E##_##DP(FapParams p) { fap_few<E, DP>(p); }      extern "C" __global__ void __launch_bounds__(256, 2) ghip_fap_tile_##E##_##DP(FapParams p) { fap_tile<E, DP, RW>(p); }
+
+// ghip_fap_both: the shared prefix on tiles and each sequence's own keys, for few
+// rows each, in one launch, so that the one's loads run under the other's products.
+template <int DP, int RW>
+union FapLds {
+    FewLds<DP> few;
+    TileLds<DP, RW> tile;
+};
+#define FAP_K(E, DP, RW)                                                                           \
+    extern "C" __global__ void __launch_bounds__(256, 2) ghip_fap_few_##E##_##DP(FapParams p) {    \
+        __shared__ __attribute__((aligned(1024))) uint8_t lds[sizeof(FewLds<DP>)];                 \
+        fap_few<E, DP>(p, *(FewLds<DP> *)lds);                                                     \
+    }                                                                                              \
+    extern "C" __global__ void __launch_bounds__(256, 2) ghip_fap_tile_##E##_##DP(FapParams p) {   \
+        __shared__ __attribute__((aligned(1024))) uint8_t lds[sizeof(TileLds<DP, RW>)];            \
+        fap_tile<E, DP, RW>(p, *(TileLds<DP, RW> *)lds);                                           \
+    }                                                                                              \
+    extern "C" __global__ void __launch_bounds__(256, 2) ghip_fap_both_##E##_##DP(FapParams p) {   \
+        __shared__ __attribute__((aligned(1024))) uint8_t lds[sizeof(FapLds<DP, RW>)];             \
+        if ((int)blockIdx.x < p.wg_sh) fap_tile<E, DP, RW>(p, *(TileLds<DP, RW> *)lds);            \
+        else fap_few<E, DP>(p, *(FewLds<DP> *)lds);                                                \
+    }
 #define FAP_E(E) FAP_K(E, 64, 2) FAP_K(E, 96, 2) FAP_K(E, 128, 2) FAP_K(E, 256, 1)
 FAP_E(f16) FAP_E(bf16)
