@@ -3006,10 +3006,11 @@ ghip_status ghip_quantize_chunk(ghip_context *ctx, int type, const float *src, v
 namespace {
 
 // Mirrors of the kernels' argument structs in ghip_rope.hip.
-struct RopeTab {
-    double rev[128];
+struct alignas(16) RopeTab {
+    uint64_t turn[128];
     uint8_t axis[128];
     float mscale;
+    int axes;
 };
 struct RopeParams {
     const void *x;
@@ -3058,7 +3059,7 @@ size_t byte_extent(const ghip_tensor *t, uint64_t e) {
 // Context extension mixes the frequency and the scaled one over the pairs whose
 // wavelength lies between n_ctx_orig / beta_fast and n_ctx_orig / beta_slow.
 // Returns the reason it is refused, or null.
-const char *rope_table(const ghip_rope_params &r, int64_t D, RopeTab &tab, int &P, int &axes) {
+const char *rope_table(const ghip_rope_params &r, int64_t D, bool factors, RopeTab &tab, int &P, int &axes) {
     const bool vision = r.mode == GHIP_ROPE_VISION;
     const bool multi = vision || r.mode == GHIP_ROPE_MROPE || r.mode == GHIP_ROPE_IMROPE;
     if (!multi && r.mode != GHIP_ROPE_NORM && r.mode != GHIP_ROPE_NEOX) return "mode must be one of GHIP_ROPE_*";
@@ -3111,10 +3112,14 @@ const char *rope_table(const ghip_rope_params &r, int64_t D, RopeTab &tab, int &
             const double mix = (1.0 - ramp) * r.ext_factor;
             scale = scale * (1.0 - mix) + mix;
         }
-        tab.rev[i] = (double)(f * scale / turn);
+        const long double t = f * scale / turn;
+        const double d = (double)t;
+        tab.turn[i] = (uint64_t)((t - std::floor(t)) * 0x1p64L);
+        if (factors) memcpy(&tab.turn[i], &d, 8);
         tab.axis[i] = (uint8_t)axis;
         f *= step;
     }
+    tab.axes = axes;
     tab.mscale = (float)r.attn_factor;
     if (r.ext_factor != 0.0) tab.mscale = (float)(r.attn_factor * (1.0 + 0.1 * std::log(1.0 / r.freq_scale)));
     return nullptr;
@@ -3130,19 +3135,21 @@ const char *rope_operands(const ghip_tensor *pos, const ghip_tensor *factors, in
     return nullptr;
 }
 
-// Units of 4 pairs where the pairs and what is not rotated divide into them
-// (loads need no alignment beyond the element's).  One head a thread while that
-// leaves too few threads to cover the loads' latency on 256 CUs (8 wavefronts
-// each), else four, which share their angles.
+// Units of 4 pairs -- of 8 for rows of 16-bit elements, whose loads are then 16
+// bytes too -- where the pairs and what is not rotated divide into them (loads
+// need no alignment beyond the element's).  One head a thread while that leaves
+// too few threads to cover the loads' latency on 256 CUs (4 wavefronts each),
+// else four, which share their angles (1500 tokens of 32 heads of 128, F32: 15.2
+// us with one head a thread, 13.2 with two, 12.8 with four).
 struct RopeShape {
     int vec, hn, U, UR, HG;
     unsigned grid;
 };
-bool rope_shape(int64_t T, int64_t H, int64_t D, int P, RopeShape &r) {
-    r.vec = P % 4 == 0 && D % 8 == 0 ? 4 : 1;
+bool rope_shape(int64_t T, int64_t H, int64_t D, int P, bool wide, RopeShape &r) {
+    r.vec = wide && P % 8 == 0 && D % 16 == 0 ? 8 : P % 4 == 0 && D % 8 == 0 ? 4 : 1;
     r.UR = P / r.vec;
     r.U = r.UR + (int)((D - 2 * P + 2 * r.vec - 1) / (2 * r.vec));
-    r.hn = T * ((H + 3) / 4) * r.U >= 256 * 8 * 64 ? 4 : 1;
+    r.hn = T * ((H + 3) / 4) * r.U >= 256 * 4 * 64 ? 4 : 1;
     r.HG = (int)((H + r.hn - 1) / r.hn);
     const int64_t n = T * r.HG * r.U;
     r.grid = (unsigned)((n + 255) / 256);
@@ -3169,7 +3176,7 @@ ghip_status ghip_rope(ghip_context *ctx, const ghip_tensor *x, const ghip_tensor
     if (D > INT32_MAX || H > INT32_MAX || T > INT32_MAX) return bad("dimension too large");
     RopeParams p;
     int axes;
-    if (const char *why = rope_table(*rope, D, p.tab, p.P, axes)) return bad(why);
+    if (const char *why = rope_table(*rope, D, factors != nullptr, p.tab, p.P, axes)) return bad(why);
     if (const char *why = rope_operands(pos, factors, T, p.P, axes)) return bad(why);
     if (T == 0 || H == 0) return GHIP_STATUS_SUCCESS;
     if (!x->data || !dst->data || !pos->data) return bad("null data");
@@ -3177,7 +3184,7 @@ ghip_status ghip_rope(ghip_context *ctx, const ghip_tensor *x, const ghip_tensor
     if (x->data == dst->data && (x->nb[1] != dst->nb[1] || x->nb[2] != dst->nb[2]))
         return bad("dst in the place of x must have its strides");
     RopeShape r;
-    if (!rope_shape(T, H, D, p.P, r)) return bad("x too large");
+    if (!rope_shape(T, H, D, p.P, x->type != GHIP_TYPE_F32, r)) return bad("x too large");
     hipStream_t s = (hipStream_t)stream;
     if (!ctx->set_device()) return ctx->fail(GHIP_STATUS_BACKEND_ERROR, "hipSetDevice failed");
     ghip_status st = ctx->begin(s);
@@ -3234,7 +3241,7 @@ ghip_status ghip_kv_append(ghip_context *ctx, const ghip_tensor *k, const ghip_t
     p.factors = nullptr;
     if (rope) {
         int axes;
-        if (const char *why = rope_table(*rope, D, p.tab, p.P, axes)) return bad(why);
+        if (const char *why = rope_table(*rope, D, factors != nullptr, p.tab, p.P, axes)) return bad(why);
         if (const char *why = rope_operands(pos, factors, T, p.P, axes)) return bad(why);
         p.pos = (const int32_t *)pos->data;
         p.pos_nb1 = (int64_t)(pos->nb[1] / 4);
@@ -3246,7 +3253,7 @@ ghip_status ghip_kv_append(ghip_context *ctx, const ghip_tensor *k, const ghip_t
     if (!k->data || !v->data || !slots->data || (!kv->data && kv->ne[3]) || (rope && !pos->data)) return bad("null data");
     if (kv->ne[3] && (overlaps(k, kv) || overlaps(v, kv))) return bad("k and v must lie apart from kv");
     RopeShape r;
-    if (!rope_shape(T, H, D, p.P, r)) return bad("k too large");
+    if (!rope_shape(T, H, D, p.P, false, r)) return bad("k too large");
     hipStream_t s = (hipStream_t)stream;
     if (!ctx->set_device()) return ctx->fail(GHIP_STATUS_BACKEND_ERROR, "hipSetDevice failed");
     ghip_status st = ctx->begin(s);

@@ -214,9 +214,10 @@ DEV typename Frag<E>::v8 value_frag(uint32_t vat, int u, int dt) {
     const typename Frag<E>::v4 lo = Frag<E>::read_tr(at), hi = Frag<E>::read_tr(at + 32 * DP);
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
-// Scores of the NT 16-key tiles at Ks, less the reference maximum.
-template <typename E, int DP, int RW, int NT>
-DEV void scores(const Rows<E, DP, RW> &R, uint32_t Ks, v4f (&s)[NT][RW]) {
+// Scores of the NT 16-key tiles at Ks, less the reference maximum.  between(f) is
+// called after the products of fragment f, for what is to go out under them.
+template <typename E, int DP, int RW, int NT, typename F>
+DEV void scores(const Rows<E, DP, RW> &R, uint32_t Ks, v4f (&s)[NT][RW], F between) {
     constexpr int KK = DP / 32, N = NT * KK;
     const uint32_t kat = k_at<DP>(Ks);
     // fragments are read two ahead of the products that use them
@@ -232,6 +233,7 @@ DEV void scores(const Rows<E, DP, RW> &R, uint32_t Ks, v4f (&s)[NT][RW]) {
 #pragma unroll
             for (int rt = 0; rt < RW; rt++)
                 s[t][rt] = Frag<E>::mfma(a[f % 3], R.q[rt][kk][i], kk == 0 && i == Frag<E>::NQ - 1 ? R.mneg[rt] : s[t][rt]);
+        between(f);
         __builtin_amdgcn_sched_barrier(0);
     }
 }
@@ -467,21 +469,33 @@ DEV void find_keys(const FapParams &p, const Tile &tl, int kt, const int32_t *pg
     offs[lane] = in && there ? 2 * (page * p.kv_page + r * p.kv_row) : 0;
 }
 // The 16-byte pieces that a lane loads of a tile's rows: load ii of a wavefront
-// fills LDS chunks 64 (from + ii) + lane.  Chunks past the row's end (D < DP) take its last.
+// fills LDS chunks 64 (from + ii) + lane.  Where 64 chunks are whole rows, the
+// load's part of a row's number is bits apart from the lane's, so its part of the
+// swizzle is flipped into the lane's.  Chunks past the row's end (D < DP) take its last.
 template <int DP>
 struct RowLoads {
     static constexpr int CH = DP / 8;
-    int at;
-    uint32_t last;
-    DEV_M RowLoads(int D, int from) : at(64 * from + (threadIdx.x & 63)), last(2 * D - 16) {}
-    DEV_M int row(int ii) const { return (at + 64 * ii) / CH; }
+    static constexpr bool WHOLE = 64 % CH == 0;
+    int from, row0;
+    uint32_t k0, v0, last;
+    DEV_M RowLoads(int D, int from_) : from(from_), last(2 * D - 16) {
+        const int lane = threadIdx.x & 63;
+        row0 = lane / CH;
+        k0 = 16 * k_swz<CH>(row0, lane % CH);
+        v0 = 16 * v_swz<CH>(row0, lane % CH);
+    }
+    DEV_M int row(int ii) const {
+        return WHOLE ? row0 + 64 / CH * (from + ii) : (64 * (from + ii) + (int)(threadIdx.x & 63)) / CH;
+    }
     DEV_M uint32_t k_chunk(int ii) const {
+        if (WHOLE) return min(k0 ^ (uint32_t)(16 * k_swz<CH>(64 / CH * (from + ii), 0)), last);
         const int r = row(ii);
-        return min((uint32_t)(16 * k_swz<CH>(r, (at + 64 * ii) - r * CH)), last);
+        return min((uint32_t)(16 * k_swz<CH>(r, (64 * (from + ii) + (int)(threadIdx.x & 63)) - r * CH)), last);
     }
     DEV_M uint32_t v_chunk(int ii) const {
+        if (WHOLE) return min(v0 ^ (uint32_t)(16 * v_swz<CH>(64 / CH * (from + ii), 0)), last);
         const int r = row(ii);
-        return min((uint32_t)(16 * v_swz<CH>(r, (at + 64 * ii) - r * CH)), last);
+        return min((uint32_t)(16 * v_swz<CH>(r, (64 * (from + ii) + (int)(threadIdx.x & 63)) - r * CH)), last);
     }
 };
 
@@ -562,7 +576,7 @@ DEV void fap_few(const FapParams &p, FewLds<DP> &lds) {
         const bool more = t + 4 < t1;
         wait_loads<NI>();
         v4f s[2][1];
-        scores<E, DP, 1, 2>(R, ka, s);
+        scores<E, DP, 1, 2>(R, ka, s, [](int) {});
         if (more) {
             find_rows(t + 4);
             wait_lds();
@@ -810,6 +824,19 @@ DEV void fap_tile(const FapParams &p, TileLds<DP, RW> &lds) {
         mine = mine || y.valid;
     }
     const bool work = __ballot(mine) != 0;  // a wavefront without rows only loads
+    int w0 = 0x7fffffff, w1 = -1;           // least and largest position of the wavefront's rows
+#pragma unroll
+    for (int rt = 0; rt < RW; rt++) {
+        if (Q.pos[rt] >= 0) w0 = min(w0, Q.pos[rt]);
+        w1 = max(w1, Q.pos[rt]);
+    }
+#pragma unroll
+    for (int o = 8; o; o >>= 1) {
+        w0 = min(w0, __shfl_xor(w0, o, 64));
+        w1 = max(w1, __shfl_xor(w1, o, 64));
+    }
+    w0 = __builtin_amdgcn_readfirstlane(w0);
+    w1 = __builtin_amdgcn_readfirstlane(w1);
     const uint8_t *kvh = (const uint8_t *)(p.kv + hk * p.kv_head);
 
     auto load_pages = [&](int t) {
@@ -817,18 +844,27 @@ DEV void fap_tile(const FapParams &p, TileLds<DP, RW> &lds) {
         const int j = min(tl.k0 + lane, tl.ke - 1);
         load4(row + 3 + paged_div((uint32_t)j, p.by_page), lds_addr(te[w][t & 1]));
     };
-    uint64_t ok = 0, bad = 0;  // keys of the next tile that are there, those on no page
+    // Three tiles are under way: t is computed, t + 1 loaded, and of t + 2 the rows
+    // are found (from pages that were loaded a step before), in the shadow of t's
+    // first products.
+    uint64_t ok = 0, bad = 0, ok2 = 0, bad2 = 0;  // keys of tiles t + 1, t + 2 that are there, those on no page
+    const uint8_t *at[NI];                        // this lane's rows of the tile found last
     const RowLoads<DP> rl(p.D, NI * w);
-    auto load_tile = [&](int t) {
-        find_keys(p, tile_at(ps.tl, t, KT), KT, te[w][t & 1], offs[w], ok, bad);
-        const uint32_t ka = lds_addr(kvs[t & 1][0]) + 1024 * NI * w, va = lds_addr(kvs[t & 1][1]) + 1024 * NI * w;
-        load_pages(t + 1);
+    auto find_tile = [&](int t) {
+        find_keys(p, tile_at(ps.tl, t, KT), KT, te[w][t & 1], offs[w], ok2, bad2);
 #pragma unroll
-        for (int ii = 0; ii < NI; ii++) {
-            const uint8_t *row = kvh + offs[w][rl.row(ii)];
-            load16(row + rl.k_chunk(ii), ka + 1024 * ii);
-            load16(row + 2 * p.D + rl.v_chunk(ii), va + 1024 * ii);
-        }
+        for (int ii = 0; ii < NI; ii++) at[ii] = kvh + offs[w][rl.row(ii)];
+    };
+    // load f of 2 NI of tile t: one goes out under each fragment's products (a tile's
+    // 8 at once keep the wavefronts from their products until the addresses are
+    // through: NOTE_US)
+    auto load_part = [&](int t, int f) {
+        const int ii = f >> 1, kv = f & 1;
+        load16(at[ii] + (kv ? 2 * p.D + rl.v_chunk(ii) : rl.k_chunk(ii)), lds_addr(kvs[t & 1][kv]) + 1024 * (NI * w + ii));
+    };
+    auto load_tile = [&](int t) {
+#pragma unroll
+        for (int f = 0; f < 2 * NI; f++) load_part(t, f);
     };
     // What this wavefront loaded of tile t is in: rows that were not there hold
     // nothing that counts, and a tile that some rows do not see in full is looked
@@ -849,8 +885,15 @@ DEV void fap_tile(const FapParams &p, TileLds<DP, RW> &lds) {
     };
     if (t0 < t1) {
         load_pages(t0);
+        load_pages(t0 + 1);
         wait_loads<0>();
+        find_tile(t0);
+        wait_lds();
+        load_pages(t0 + 2);
         load_tile(t0);
+        ok = ok2;
+        bad = bad2;
+        if (t0 + 1 < t1) find_tile(t0 + 1);
         wait_loads<0>();
         loaded(t0);
     }
@@ -860,34 +903,46 @@ DEV void fap_tile(const FapParams &p, TileLds<DP, RW> &lds) {
         const uint64_t badc = bad;
         const bool part = !tile_whole(tile, KT, ps, p.window, p.n_first);
         const uint32_t Ks = lds_addr(kvs[t & 1][0]), Vs = lds_addr(kvs[t & 1][1]);
-        if (t + 1 < t1) load_tile(t + 1);
+        const bool more = t + 1 < t1;
+        if (more) load_pages(t + 3);
         const bool odd = part && (ls.odd[t & 1][0] | ls.odd[t & 1][1] | ls.odd[t & 1][2] | ls.odd[t & 1][3]);
         // 32 keys at a time: their scores are fewer registers than 64 keys' (which
         // then spill), and one half's products run under the other's softmax
 #pragma unroll
         for (int u = 0; u < 2; u++) {
             const uint32_t Kh = Ks + 64 * u * DP, Vh = Vs + 64 * u * DP;
+            // what none of this wavefront's rows sees of an edge tile is passed over
+            const int h0 = tile.k0 + 32 * u, h1 = min(h0 + 32, tile.ke);
+            const bool need = work && (!part || (h0 < h1 && h0 <= w1 && (!p.window || h1 - 1 > w0 - p.window || h0 < p.n_first)));
             v4f s[2][RW];
-            if (work) {
+            if (need) {
                 __builtin_amdgcn_s_setprio(1);
-                scores<E, DP, RW, 2>(Q, Kh, s);
+                if (u == 0 && more) scores<E, DP, RW, 2>(Q, Kh, s, [&](int f) { load_part(t + 1, f); });
+                else scores<E, DP, RW, 2>(Q, Kh, s, [](int) {});
                 __builtin_amdgcn_s_setprio(0);
+            } else if (u == 0 && more) {
+                load_tile(t + 1);
+            }
+            if (need) {
                 if (part || badc) mask_scores<E, DP, RW, 2>(Q, s, tile.k0 + 32 * u, tile.ke, badc >> (32 * u), p.window, p.n_first);
                 softmax<E, DP, RW, 2>(Q, s);
             }
             if (odd) {
-                if (work) add_odd<E, DP, RW, 2>(Q, Vh, s);
+                if (need) add_odd<E, DP, RW, 2>(Q, Vh, s);
                 __syncthreads();
                 clear_odd<E>(kvs[t & 1][1] + 64 * u * DP, tid, 256, 32 * CH);
                 __syncthreads();
             }
-            if (work) {
+            if (need) {
                 __builtin_amdgcn_s_setprio(1);
                 values<E, DP, RW, 2>(Q, Vh, s);
                 __builtin_amdgcn_s_setprio(0);
             }
         }
-        if (t + 1 < t1) {
+        if (more) {
+            ok = ok2;
+            bad = bad2;
+            if (t + 2 < t1) find_tile(t + 2);
             wait_loads<0>();
             loaded(t + 1);
         }
