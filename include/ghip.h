@@ -346,6 +346,11 @@ ghip_status ghip_flash_attn_paged(ghip_context *ctx, const ghip_tensor *q, const
                                   const ghip_tensor *sinks, const ghip_paged_params *params, const ghip_tensor *dst,
                                   void *stream);
 
+/* Workspace bytes that such a call needs at most, whatever seqs holds (host
+ * arithmetic, as ghip_workspace_size). */
+ghip_status ghip_flash_attn_paged_workspace(const ghip_tensor *q, const ghip_tensor *kv, const ghip_tensor *seqs,
+                                            const ghip_paged_params *params, const ghip_tensor *dst, size_t *bytes);
+
 /* One node of a graph: the op, its sources in ggml order (MUL_MAT: src0,
  * src1; MUL_MAT_ID: as, b, ids; FLASH_ATTN_EXT: q, k, v, mask|NULL,
  * sinks|NULL; unused slots NULL) and its destination

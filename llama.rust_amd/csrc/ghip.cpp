@@ -3135,18 +3135,18 @@ const char *rope_operands(const ghip_tensor *pos, const ghip_tensor *factors, in
     return nullptr;
 }
 
-// Units of 4 pairs -- of 8 for rows of 16-bit elements, whose loads are then 16
-// bytes too -- where the pairs and what is not rotated divide into them (loads
-// need no alignment beyond the element's).  One head a thread while that leaves
-// too few threads to cover the loads' latency on 256 CUs (4 wavefronts each),
-// else four, which share their angles (1500 tokens of 32 heads of 128, F32: 15.2
-// us with one head a thread, 13.2 with two, 12.8 with four).
+// Units of 4 pairs where the pairs and what is not rotated divide into them (loads
+// need no alignment beyond the element's; units of 8 of 16-bit elements measured
+// slower, 9.2 against 8.2 us at 4900 x 16 x 80).  One head a thread while that
+// leaves too few threads to cover the loads' latency on 256 CUs (4 wavefronts
+// each), else four, which share their angles (1500 x 32 x 128 F32: 11.3 us with one
+// head a thread, 10.6 with two, 10.2 with four).
 struct RopeShape {
     int vec, hn, U, UR, HG;
     unsigned grid;
 };
-bool rope_shape(int64_t T, int64_t H, int64_t D, int P, bool wide, RopeShape &r) {
-    r.vec = wide && P % 8 == 0 && D % 16 == 0 ? 8 : P % 4 == 0 && D % 8 == 0 ? 4 : 1;
+bool rope_shape(int64_t T, int64_t H, int64_t D, int P, RopeShape &r) {
+    r.vec = P % 4 == 0 && D % 8 == 0 ? 4 : 1;
     r.UR = P / r.vec;
     r.U = r.UR + (int)((D - 2 * P + 2 * r.vec - 1) / (2 * r.vec));
     r.hn = T * ((H + 3) / 4) * r.U >= 256 * 4 * 64 ? 4 : 1;
@@ -3184,7 +3184,7 @@ ghip_status ghip_rope(ghip_context *ctx, const ghip_tensor *x, const ghip_tensor
     if (x->data == dst->data && (x->nb[1] != dst->nb[1] || x->nb[2] != dst->nb[2]))
         return bad("dst in the place of x must have its strides");
     RopeShape r;
-    if (!rope_shape(T, H, D, p.P, x->type != GHIP_TYPE_F32, r)) return bad("x too large");
+    if (!rope_shape(T, H, D, p.P, r)) return bad("x too large");
     hipStream_t s = (hipStream_t)stream;
     if (!ctx->set_device()) return ctx->fail(GHIP_STATUS_BACKEND_ERROR, "hipSetDevice failed");
     ghip_status st = ctx->begin(s);
@@ -3253,7 +3253,7 @@ ghip_status ghip_kv_append(ghip_context *ctx, const ghip_tensor *k, const ghip_t
     if (!k->data || !v->data || !slots->data || (!kv->data && kv->ne[3]) || (rope && !pos->data)) return bad("null data");
     if (kv->ne[3] && (overlaps(k, kv) || overlaps(v, kv))) return bad("k and v must lie apart from kv");
     RopeShape r;
-    if (!rope_shape(T, H, D, p.P, false, r)) return bad("k too large");
+    if (!rope_shape(T, H, D, p.P, r)) return bad("k too large");
     hipStream_t s = (hipStream_t)stream;
     if (!ctx->set_device()) return ctx->fail(GHIP_STATUS_BACKEND_ERROR, "hipSetDevice failed");
     ghip_status st = ctx->begin(s);
@@ -3309,7 +3309,8 @@ struct FapParams {
     float scale;
     int window, n_first, n_shared, max_q;
     PagedDiv by_page;
-    int nb_sh, zs_sh, nb_own, zs_own, wg_sh, least;
+    int nb_sh, zs_sh, nb_own, zs_own, wg_sh;
+    int join_ragged;
     float *part, *stat;
 };
 
@@ -3397,7 +3398,6 @@ FapLayout fap_layout(FapParams &p) {
     // the most keys that one block of rows goes through outside the shared prefix
     int64_t keys = table - p.n_shared;
     if (p.window) keys = std::min(keys, (int64_t)p.window + p.max_q - 1 + p.n_first);
-    p.least = 1;
     // Splits of the keys of `blocks` tile workgroups with n tiles each and `rows`
     // rows: the fewest microseconds of  rounds x (start + tiles)  and of writing
     // and reading the partials.  A workgroup starts in 8 us; a tile takes 2.0 us
@@ -3443,6 +3443,18 @@ FapLayout fap_layout(FapParams &p) {
 
 extern "C" {
 
+ghip_status ghip_flash_attn_paged_workspace(const ghip_tensor *q, const ghip_tensor *kv, const ghip_tensor *seqs,
+                                            const ghip_paged_params *params, const ghip_tensor *dst, size_t *bytes) {
+    if (!bytes) return GHIP_STATUS_BACKEND_ERROR;
+    *bytes = 0;
+    ghip_context tmp;
+    FapParams p;
+    ghip_status st;
+    if (!plan_fap(&tmp, q, kv, seqs, nullptr, dst, params, p, st)) return st;
+    if (p.max_q && p.H && p.B) *bytes = fap_layout(p).ws_bytes;
+    return GHIP_STATUS_SUCCESS;
+}
+
 ghip_status ghip_flash_attn_paged(ghip_context *ctx, const ghip_tensor *q, const ghip_tensor *kv, const ghip_tensor *seqs,
                                   const ghip_tensor *sinks, const ghip_paged_params *params, const ghip_tensor *dst,
                                   void *stream) {
@@ -3475,7 +3487,11 @@ ghip_status ghip_flash_attn_paged(ghip_context *ctx, const ghip_tensor *q, const
     }
     char name[48];
     const char *ty = float_name(kv->type);
-    const int64_t own = (int64_t)p.nb_own * p.H_kv * p.zs_own, joins = ((int64_t)p.B * p.max_q * p.H + 3) / 4;
+    const int64_t own = (int64_t)p.nb_own * p.H_kv * p.zs_own;
+    // a workgroup of the join for a row that no sequence has costs little, but
+    // B max_q can be many times T
+    p.join_ragged = p.max_q > 1 && (int64_t)p.B * p.max_q > 2 * (int64_t)p.T;
+    const int64_t joins = ((p.join_ragged ? (int64_t)p.T : (int64_t)p.B * p.max_q) * p.H + 3) / 4;
     if (own + p.wg_sh > INT32_MAX || joins > INT32_MAX)
         return ctx->fail(GHIP_STATUS_BACKEND_ERROR, "flash_attn_paged: too many rows");
     if (p.part) {

@@ -104,6 +104,7 @@ void *reg_proc_address(const ggml_hip_backend_reg *, const char *name) {
         {"ghip_rope", (void *)&ghip_rope},
         {"ghip_kv_append", (void *)&ghip_kv_append},
         {"ghip_flash_attn_paged", (void *)&ghip_flash_attn_paged},
+        {"ghip_flash_attn_paged_workspace", (void *)&ghip_flash_attn_paged_workspace},
         {"ghip_quantize_chunk", (void *)&ghip_quantize_chunk},
         {"ghip_graph_compute", (void *)&ghip_graph_compute},
         {"ghip_set_workspace", (void *)&ghip_set_workspace},

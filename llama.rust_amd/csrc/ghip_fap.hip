@@ -89,7 +89,8 @@ struct FapParams {
     PagedDiv by_page;
     // launch: the first wg_sh workgroups take the shared prefix (nb_sh blocks of
     // rows, zs_sh splits), the others each sequence's own keys (nb_own, zs_own)
-    int nb_sh, zs_sh, nb_own, zs_own, wg_sh, least;
+    int nb_sh, zs_sh, nb_own, zs_own, wg_sh;
+    int join_ragged;  // the join's workgroups go by all sequences' rows in a line, not by sequence and max_q
     // partials of row (token, head), split z (shared prefix first): part[.. + z][D]
     // and stat[.. + z][2] = (maximum, sum); null where zs_sh + zs_own == 1
     float *part, *stat;
@@ -151,27 +152,44 @@ struct Rows {
     bool set[RW];   // a key has been seen
 };
 
-template <typename E, int DP, int RW>
-DEV void rows_load(Rows<E, DP, RW> &R, int rt, const float *qr, int D, float scale, bool valid) {
-    const int g = (threadIdx.x & 63) >> 4;
+// A row's q: this lane's share as it lies (dims 32 kk + 8 (lane >> 4) ..), loaded
+// early; then, once it is in, as the terms of the fragments.
+template <int DP>
+struct RawRow {
+    float x[DP / 32][8];
+};
+template <int DP>
+DEV void raw_load(RawRow<DP> &r, const float *qr, int D, bool valid) {
 #pragma unroll
     for (int kk = 0; kk < DP / 32; kk++) {
-        const int d = 32 * kk + 8 * g;
-        float x[8];
+        const int d = 32 * kk + 8 * ((threadIdx.x & 63) >> 4);
 #pragma unroll
-        for (int e = 0; e < 8; e++) x[e] = 0.0f;
-        if (valid && d < D) __builtin_memcpy(x, qr + d, 32);
+        for (int e = 0; e < 8; e++) r.x[kk][e] = 0.0f;
+        if (valid && d < D) __builtin_memcpy(r.x[kk], qr + d, 32);
+    }
+}
+// (the compiler does not know of wait_loads: it waits here, where nothing else is in flight)
+template <int DP>
+DEV void raw_wait(RawRow<DP> &r) {
+#pragma unroll
+    for (int kk = 0; kk < DP / 32; kk++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) asm volatile("" : "+v"(r.x[kk][e]));
+}
+template <typename E, int DP, int RW>
+DEV void rows_start(Rows<E, DP, RW> &R, int rt, const RawRow<DP> &r, float scale) {
+#pragma unroll
+    for (int kk = 0; kk < DP / 32; kk++)
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             typename Frag<E>::v2 t[Frag<E>::NQ];
-            split_pair<E, Frag<E>::NQ>(x[2 * e] * scale, x[2 * e + 1] * scale, t);
+            split_pair<E, Frag<E>::NQ>(r.x[kk][2 * e] * scale, r.x[kk][2 * e + 1] * scale, t);
 #pragma unroll
             for (int i = 0; i < Frag<E>::NQ; i++) {
                 R.q[rt][kk][i][2 * e] = t[i][0];
                 R.q[rt][kk][i][2 * e + 1] = t[i][1];
             }
         }
-    }
 #pragma unroll
     for (int dt = 0; dt < DP / 16; dt++) R.o[rt][dt] = v4f{0, 0, 0, 0};
     R.mneg[rt] = v4f{0, 0, 0, 0};
@@ -527,7 +545,7 @@ DEV void fap_few(const FapParams &p, FewLds<DP> &lds) {
     ps.p0 = clip_pos(sq.pos0, table);
     ps.p1 = clip_pos(sq.pos0 + sq.nq - 1, table);
     ps.tl = paged_tiles(ps.p0, ps.p1, p.window, p.n_first, p.n_shared, (int)table, KT);
-    const int share = paged_share(ps.tl.n, p.zs_own, p.least);
+    const int share = paged_share(ps.tl.n, p.zs_own);
     const int t0 = (int)min((int64_t)z * share, (int64_t)ps.tl.n), t1 = min(ps.tl.n, t0 + share);
     const int i = n / G, hd = hk * G + n % G;
     const bool valid = n < sq.nq * G;
@@ -538,7 +556,8 @@ DEV void fap_few(const FapParams &p, FewLds<DP> &lds) {
         return;
     }
     Rows<E, DP, 1> R;
-    rows_load<E, DP, 1>(R, 0, p.q + tok * p.q_nb2 + hd * p.q_nb1, p.D, p.scale * kLog2e, valid);
+    RawRow<DP> raw;
+    raw_load<DP>(raw, p.q + tok * p.q_nb2 + hd * p.q_nb1, p.D, valid);
     R.pos[0] = valid ? clip_pos(sq.pos0 + i, table) : -1;
     const uint32_t ka = lds_addr(kvs[w][0]), va = lds_addr(kvs[w][1]);
 
@@ -562,14 +581,16 @@ DEV void fap_few(const FapParams &p, FewLds<DP> &lds) {
     };
     // in flight at the top of a step, oldest first: pages t + 4, K t, V t
     const int first = t0 + w;
+    if (first < t1) load_pages(first);
+    wait_loads<0>();
+    raw_wait<DP>(raw);
     if (first < t1) {
-        load_pages(first);
-        wait_loads<0>();
         find_rows(first);
         load_pages(first + 4);
         load_k();
         load_v();
     }
+    rows_start<E, DP, 1>(R, 0, raw, p.scale * kLog2e);
     for (int t = first; t < t1; t += 4) {
         const Tile tile = tile_at(ps.tl, t, KT);
         const uint64_t okc = ok, badc = bad;
@@ -788,7 +809,7 @@ DEV void fap_tile(const FapParams &p, TileLds<DP, RW> &lds) {
     ps.p0 = __builtin_amdgcn_readfirstlane(ps.p0);
     ps.p1 = __builtin_amdgcn_readfirstlane(ps.p1);
     ps.tl = paged_tiles(ps.p0, ps.p1, p.window, p.n_first, shared ? 0 : p.n_shared, shared ? p.n_shared : (int)table, KT);
-    const int share = paged_share(ps.tl.n, nz, p.least);
+    const int share = paged_share(ps.tl.n, nz);
     const int t0 = (int)min((int64_t)z * share, (int64_t)ps.tl.n), t1 = min(ps.tl.n, t0 + share);
     // this lane's rows
     struct Row {
@@ -815,11 +836,12 @@ DEV void fap_tile(const FapParams &p, TileLds<DP, RW> &lds) {
         return;
     }
     Rows<E, DP, RW> Q;
+    RawRow<DP> raw[RW];
     bool mine = false;
 #pragma unroll
     for (int rt = 0; rt < RW; rt++) {
         const Row y = row_of(rt);
-        rows_load<E, DP, RW>(Q, rt, p.q + y.tok * p.q_nb2 + y.hd * p.q_nb1, p.D, p.scale * kLog2e, y.valid);
+        raw_load<DP>(raw[rt], p.q + y.tok * p.q_nb2 + y.hd * p.q_nb1, p.D, y.valid);
         Q.pos[rt] = y.pos;
         mine = mine || y.valid;
     }
@@ -886,7 +908,11 @@ DEV void fap_tile(const FapParams &p, TileLds<DP, RW> &lds) {
     if (t0 < t1) {
         load_pages(t0);
         load_pages(t0 + 1);
-        wait_loads<0>();
+    }
+    wait_loads<0>();
+#pragma unroll
+    for (int rt = 0; rt < RW; rt++) raw_wait<DP>(raw[rt]);
+    if (t0 < t1) {
         find_tile(t0);
         wait_lds();
         load_pages(t0 + 2);
@@ -894,6 +920,10 @@ DEV void fap_tile(const FapParams &p, TileLds<DP, RW> &lds) {
         ok = ok2;
         bad = bad2;
         if (t0 + 1 < t1) find_tile(t0 + 1);
+    }
+#pragma unroll
+    for (int rt = 0; rt < RW; rt++) rows_start<E, DP, RW>(Q, rt, raw[rt], p.scale * kLog2e);
+    if (t0 < t1) {
         wait_loads<0>();
         loaded(t0);
     }
@@ -978,9 +1008,34 @@ DEV void fap_join(const FapParams &p) {
     const int lane = threadIdx.x & 63;
     const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     const int h = (int)(id % p.H);
-    const int64_t bi = id / p.H;
-    const int b = (int)(bi / p.max_q), i = (int)(bi - (int64_t)b * p.max_q);
-    if (b >= p.B) return;
+    const int64_t x = id / p.H;  // sequence b, row i as b max_q + i, or the row's number among all sequences' rows
+    int b, i;
+    if (!p.join_ragged) {
+        b = (int)(x / p.max_q);
+        i = (int)(x - (int64_t)b * p.max_q);
+        if (b >= p.B) return;
+    } else {
+        int64_t base = 0;
+        b = -1;
+        for (int b0 = 0; b0 < p.B && base <= x; b0 += 64) {
+            const int n = b0 + lane < p.B ? seq_of(p, b0 + lane).nq : 0;
+            int to = n;  // rows up to and with this lane's sequence
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const int y = __shfl_up(to, o, 64);
+                if (lane >= o) to += y;
+            }
+            const uint64_t here = __ballot(base + to - n <= x && x < base + to);
+            if (here) {
+                const int at = __builtin_ctzll(here);
+                b = b0 + at;
+                i = (int)(x - base - __builtin_amdgcn_readlane(to - n, at));
+                break;
+            }
+            base += __builtin_amdgcn_readlane(to, 63);
+        }
+        if (b < 0) return;
+    }
     const PagedSeq sq = seq_of(p, b);
     if (i >= sq.nq) return;
     const int64_t tok = sq.q0 + i, row = tok * p.H + h;

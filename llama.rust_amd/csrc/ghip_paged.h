@@ -92,8 +92,5 @@ PAGED_FN PagedTiles paged_tiles(int64_t p0, int64_t p1, int window, int n_first,
     t.n = t.na + (int)(((int64_t)t.b1 - t.b0 + kt - 1) / kt);
     return t;
 }
-// Split z of `nz` takes tiles [z c, z c + c) of n: even shares, but at least `least`.
-PAGED_FN int paged_share(int n, int nz, int least) {
-    const int c = (n + nz - 1) / nz;
-    return c < least ? least : c;
-}
+// Split z of `nz` takes tiles [z c, z c + c) of n.
+PAGED_FN int paged_share(int n, int nz) { return (int)(((int64_t)n + nz - 1) / nz); }

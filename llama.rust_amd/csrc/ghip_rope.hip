@@ -292,7 +292,5 @@ typedef float f32;
     APPEND_K(E, C, norm, true, 1, 1) APPEND_K(E, C, norm, true, 1, 4)                                            \
     APPEND_K(E, C, half, false, 4, 1) APPEND_K(E, C, half, false, 4, 4)                                          \
     APPEND_K(E, C, half, false, 1, 1) APPEND_K(E, C, half, false, 1, 4)
-#define ROPE_E8(E)                                                                                               \
-    ROPE_K(E, norm, true, 8, 1) ROPE_K(E, norm, true, 8, 4) ROPE_K(E, half, false, 8, 1) ROPE_K(E, half, false, 8, 4)
-ROPE_E(f32) ROPE_E(f16) ROPE_E(bf16) ROPE_E8(f16) ROPE_E8(bf16)
+ROPE_E(f32) ROPE_E(f16) ROPE_E(bf16)
 APPEND_E(f32, f16) APPEND_E(f32, bf16) APPEND_E(f16, f16) APPEND_E(bf16, bf16)

@@ -235,6 +235,8 @@ def lib():
         L.ghip_kv_append.argtypes = [V, V, V, V, V, V, R, V, V]
         L.ghip_flash_attn_paged.restype = C.c_int
         L.ghip_flash_attn_paged.argtypes = [V, V, V, V, V, C.POINTER(PagedParams), V, V]
+        L.ghip_flash_attn_paged_workspace.restype = C.c_int
+        L.ghip_flash_attn_paged_workspace.argtypes = [V, V, V, C.POINTER(PagedParams), V, C.POINTER(C.c_size_t)]
         _lib = L
     return _lib
 
@@ -417,6 +419,18 @@ class Backend:
         if st:
             self._check(st, "ghip_flash_attn_paged")
         return out
+
+    @staticmethod
+    def flash_attn_paged_workspace(q, kv, seqs, window=0, n_first=0, n_shared=0, max_q=None):
+        """Workspace bytes that flash_attn_paged needs at most for these shapes."""
+        pp = PagedParams(1.0, window, n_first, n_shared, q.shape[0] if max_q is None else max_q)
+        out, v = C.c_size_t(0), _view(q)
+        d = Tensor.from_buffer_copy(v)
+        d.data = (d.data or 0) + (1 << 60)  # any place apart from q: only compared
+        st = lib().ghip_flash_attn_paged_workspace(v, _view(kv), _view(seqs), C.byref(pp), bytes(d), C.byref(out))
+        if st:
+            raise GhipError(f"ghip_flash_attn_paged_workspace: status {st}")
+        return out.value
 
     # ---- graph
     def graph_compute(self, nodes):

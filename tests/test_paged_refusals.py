@@ -184,6 +184,10 @@ extern "C" void seq(int q0, int nq, int nkv, int T, int max_q, long long *o) {
     PagedSeq s = paged_seq(q0, nq, nkv, T, max_q); o[0] = s.q0; o[1] = s.nq; o[2] = s.pos0; }
 extern "C" void keys(long long p0, long long p1, int w, int f, long long *o) {
     PagedKeys k = paged_keys(p0, p1, w, f); o[0] = k.first; o[1] = k.lo; o[2] = k.hi; }
+extern "C" unsigned divide(unsigned n, unsigned d) { return paged_div(n, paged_divisor(d)); }
+extern "C" void tiles(long long p0, long long p1, int w, int f, int from, int to, int kt, int nz, int *o) {
+    PagedTiles t = paged_tiles(p0, p1, w, f, from, to, kt);
+    o[0] = t.a0; o[1] = t.a1; o[2] = t.b0; o[3] = t.b1; o[4] = t.na; o[5] = t.n; o[6] = paged_share(t.n, nz); }
 extern "C" int seen(long long p, long long j, int w, int f) { return paged_seen(p, j, w, f); }
 """
 
@@ -219,3 +223,25 @@ def test_index_arithmetic(tmp_path):
             assert some == any(L.seen(ll(p), ll(j), w, f) for p in range(p0, p1 + 1))
             assert some == (j < first or lo <= j < hi), (p0, p1, w, f, j)
         assert 0 <= first <= lo <= hi or hi == 0
+    L.divide.restype = C.c_uint
+    for d in [1, 2, 3, 7, 16, 24, 64, 100, 255, 256, 257, 641, 2 ** 16 + 1, 2 ** 30, 2 ** 31 - 1]:
+        for n in [0, 1, d - 1, d, d + 1, 3 * d - 1, 2 ** 31 - 1, 2 ** 32 - 1] + [rng.randrange(2 ** 32) for _ in range(200)]:
+            n %= 2 ** 32
+            assert L.divide(C.c_uint(n), C.c_uint(d)) == n // d, (n, d)
+    o7 = (C.c_int * 7)()
+    for _ in range(3000):
+        p0 = rng.randint(-20, 60)
+        p1 = p0 + rng.randint(0, 30)
+        w, f = rng.choice([0, 1, 7, 64]), rng.choice([0, 1, 9, 200])
+        fr = rng.choice([0, 0, 5, 40])
+        to, kt, nz = fr + rng.randint(0, 90), rng.choice([4, 8, 32]), rng.randint(1, 9)
+        L.tiles(ll(p0), ll(p1), w, f, fr, to, kt, nz, o7)
+        a0, a1, b0, b1, na, n, share = o7
+        keys = []  # as the kernels walk them: tile t, then its keys below the range's end
+        for t in range(n):
+            k0, ke = (a0 + t * kt, a1) if t < na else (b0 + (t - na) * kt, b1)
+            assert k0 < ke
+            keys += range(k0, min(k0 + kt, ke))
+        want = [j for j in range(fr, to) if any(L.seen(ll(p), ll(j), w, f) for p in range(p0, p1 + 1))]
+        assert keys == want, (p0, p1, w, f, fr, to, kt)
+        assert share * nz >= n
