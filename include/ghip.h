@@ -337,7 +337,8 @@ typedef struct ghip_paged_params {
  * with j > p - window or j < n_first.  A row that sees nothing gives 0; rows of
  * q that no sequence names are not written.  n_shared > 0 says that the first
  * n_shared keys of every sequence hold the same values: they are read through
- * the first sequence's pages, once for the batch.
+ * the first sequence's pages, once for the batch, or, where that costs more than
+ * it saves, through each sequence's own (both hold page numbers for them).
  * Pages of keys that no row sees are not looked at, and what the cache holds
  * there, NaN included, does not matter.  A row that sees a key on a page outside
  * [0, pages), or past its table row, gives NaN.  Rows past max_q are not

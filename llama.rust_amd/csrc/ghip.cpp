@@ -3395,43 +3395,65 @@ FapLayout fap_layout(FapParams &p) {
     L.few = (int64_t)p.max_q * G <= 16;
     L.rows = L.DP == 256 ? 64 : 128;
     const int64_t table = (int64_t)p.per * p.page;
-    // the most keys that one block of rows goes through outside the shared prefix
-    int64_t keys = table - p.n_shared;
-    if (p.window) keys = std::min(keys, (int64_t)p.window + p.max_q - 1 + p.n_first);
-    // Splits of the keys of `blocks` tile workgroups with n tiles each and `rows`
-    // rows: the fewest microseconds of  rounds x (start + tiles)  and of writing
-    // and reading the partials.  A workgroup starts in 8 us; a tile takes 2.0 us
-    // where a CU has one workgroup, 3.2 where it has two (512 in a round); the
-    // partials go at 4.8 TB/s.
-    auto tile_splits = [&](int64_t blocks, int64_t rows, int64_t n) {
-        int best = 1;
-        double least = 0;
-        for (int z = 1; z <= 32 && z <= std::max<int64_t>(1, n); z++) {
-            const int64_t wgs = blocks * z;
-            const double us = (double)((wgs + 511) / 512) * (8.0 + (double)((n + z - 1) / z) * (wgs <= 256 ? 2.0 : 3.2)) +
-                              (z > 1 || p.n_shared ? 8.0 * rows * z * p.D / 4.8e6 : 0.0);
-            if (z == 1 || us < least) {
-                best = z;
-                least = us;
-            }
+    const int64_t rows = std::min((int64_t)p.T, (int64_t)p.B * p.max_q);
+    const double wide = L.DP / 128.0, mem = 4.8e6;  // bytes a microsecond
+    // A way to take some keys: splits, and its microseconds.  (Lengths are on the
+    // device: the keys are the most that the table has room for.)
+    struct Way {
+        int z;
+        double us;
+    };
+    // partials written and read, and the launch that joins them
+    auto join = [&](int z) { return 5.0 + 8.0 * rows * p.H * z * p.D / mem; };
+    // Tiles: the splits with the least  rounds x (start + tiles)  + partials.  A
+    // workgroup starts in 8 us; a 64-key tile of 128 dims takes 2.0 us where a CU has
+    // one workgroup, 3.2 where it has two (512 in a round; 256 of 256 dims).
+    auto tiles = [&](int64_t blocks, int64_t keys, bool alone) {
+        const int64_t n = std::max<int64_t>(1, (keys + 63) / 64), slots = L.DP == 256 ? 256 : 512;
+        Way best{1, 0};
+        for (int z = 1; z <= 32 && z <= n; z++) {
+            const int64_t wgs = blocks * p.H_kv * z;
+            const double us = (double)((wgs + slots - 1) / slots) * (8.0 + (double)((n + z - 1) / z) * wide * (wgs <= 256 ? 2.0 : 3.2)) +
+                              (z > 1 || !alone ? join(z) : 0.0);
+            if (z == 1 || us < best.us) best = {z, us};
         }
         return best;
     };
-    const int64_t rows = std::min((int64_t)p.T, (int64_t)p.B * p.max_q) * p.H;
-    if (L.few) {
-        // 256 keys a workgroup at least, and about 1024 of them
-        p.nb_own = p.B;
-        const int64_t wgs = (int64_t)p.nb_own * p.H_kv;
-        p.zs_own = (int)std::max<int64_t>(1, std::min<int64_t>({(1024 + wgs - 1) / wgs, (keys + 255) / 256, 32}));
-    } else {
-        p.nb_own = (int64_t)p.max_q * G <= L.rows ? p.B : (int)((int64_t)p.T * G / L.rows + p.B);
-        p.zs_own = tile_splits((int64_t)p.nb_own * p.H_kv, rows, (keys + 63) / 64);
-    }
+    // Few rows: bound by memory, or by 512 workgroups at a time that start in 5 us and
+    // take 128 keys in 1.5; at least 256 keys a workgroup and about 1024 of them.
+    auto few = [&](int64_t keys, bool alone) {
+        const int64_t wgs = (int64_t)p.B * p.H_kv;
+        Way w;
+        w.z = (int)std::max<int64_t>(1, std::min<int64_t>({(1024 + wgs - 1) / wgs, (keys + 255) / 256, 32}));
+        const double steps = (double)((keys + 128 * w.z - 1) / (128 * w.z));
+        w.us = std::max((double)((wgs * w.z + 511) / 512) * (5.0 + steps * 1.5 * wide), 4.0 * wgs * keys * p.D / mem) +
+               (w.z > 1 || !alone ? join(w.z) : 0.0);
+        return w;
+    };
+    p.nb_own = L.few || (int64_t)p.max_q * G <= L.rows ? p.B : (int)((int64_t)p.T * G / L.rows + p.B);
+    auto own = [&](int64_t shared) {
+        // the most keys that one block of rows goes through outside the shared prefix
+        int64_t keys = table - shared;
+        if (p.window) keys = std::min(keys, (int64_t)p.window + p.max_q - 1 + p.n_first);
+        return L.few ? few(keys, !shared) : tiles(p.nb_own, keys, !shared);
+    };
+    // The shared prefix once for all, or each sequence's own pages: whichever is less
+    // (one launch and one join serve both parts).
+    const Way plain = own(0);
+    p.zs_own = plain.z;
     p.nb_sh = p.zs_sh = p.wg_sh = 0;
     if (p.n_shared) {
-        p.nb_sh = (int)((rows / p.H * G + L.rows - 1) / L.rows);
-        p.zs_sh = tile_splits((int64_t)p.nb_sh * p.H_kv, rows, (p.n_shared + 63) / 64);
-        p.wg_sh = p.nb_sh * p.H_kv * p.zs_sh;
+        const int64_t nb = (rows * G + L.rows - 1) / L.rows;
+        const Way sh = tiles(nb, p.n_shared, false), rest = own(p.n_shared);
+        const int forced = env_int("GHIP_FAP_SHARED", -1);
+        if (forced >= 0 ? forced != 0 : sh.us + rest.us - 13.0 < plain.us) {
+            p.zs_own = rest.z;
+            p.nb_sh = (int)nb;
+            p.zs_sh = sh.z;
+            p.wg_sh = p.nb_sh * p.H_kv * p.zs_sh;
+        } else {
+            p.n_shared = 0;
+        }
     }
     const int nz = p.zs_sh + p.zs_own;
     const size_t n = (size_t)p.T * p.H * nz;

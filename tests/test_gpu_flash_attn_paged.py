@@ -3,6 +3,7 @@ every element within attention_tol, and the whole within 2^-17 in 2-norm (17 bit
 of q and p are the least that a kernel holds; roundings of single elements do not
 all point one way)."""
 import math
+import os
 
 import pytest
 
@@ -52,6 +53,18 @@ def make(seqs, H, Hkv, D, ctype, page, n_shared=0, seed=0, spare=3, order=None):
     return q, kv, table
 
 
+def ways(n_shared):
+    """A shared prefix read once for all and read by each sequence: the sizes of
+    these tests would all take the latter by themselves."""
+    for how in ("1", "0") if n_shared else (None,):
+        if how is not None:
+            os.environ["GHIP_FAP_SHARED"] = how
+        try:
+            yield how
+        finally:
+            os.environ.pop("GHIP_FAP_SHARED", None)
+
+
 def compare(got, want, mag, wgt, D):
     got = got.double()
     named = ~torch.isnan(want)
@@ -68,9 +81,10 @@ def check(be, seqs, H, Hkv, D, ctype="f16", page=16, window=0, n_first=0, n_shar
     scale = 1 / math.sqrt(D)
     want, mag, wgt = P.attention(q, kv, table.tolist(), scale, sk, window, n_first)
     print(f"paged {seqs[:4]} H={H}/{Hkv} D={D} {ctype} page={page} window={window}+{n_first} shared={n_shared} sinks={sinks}", flush=True)
-    got = be.flash_attn_paged(q.cuda(), kv.cuda(), table.cuda(), scale=scale, sinks=sk.cuda() if sinks else None, window=window,
-                              n_first=n_first, n_shared=n_shared, max_q=max_q or max([a for a, _ in seqs] + [1]))
-    compare(got.cpu(), want, mag, wgt, D)
+    for how in ways(n_shared):
+        got = be.flash_attn_paged(q.cuda(), kv.cuda(), table.cuda(), scale=scale, sinks=sk.cuda() if sinks else None, window=window,
+                                  n_first=n_first, n_shared=n_shared, max_q=max_q or max([a for a, _ in seqs] + [1]))
+        compare(got.cpu(), want, mag, wgt, D)
 
 
 @pytest.mark.parametrize("ctype", ["f16", "bf16"])
@@ -161,8 +175,9 @@ def test_what_unseen_places_hold(be, nq, what):
             for i in range((m + 15) // 16):
                 if not seen[table[b, 3 + i].long()].any():
                     gone[b, 3 + i] = 10 ** 6
-        got = be.flash_attn_paged(q.cuda(), kv.cuda(), gone.cuda(), scale=0.125, window=window, n_first=n_first, n_shared=n_shared, max_q=nq)
-        compare(got.cpu(), want, mag, wgt, 64)
+        for how in ways(n_shared):
+            got = be.flash_attn_paged(q.cuda(), kv.cuda(), gone.cuda(), scale=0.125, window=window, n_first=n_first, n_shared=n_shared, max_q=nq)
+            compare(got.cpu(), want, mag, wgt, 64)
 
 
 def test_later_rows_do_not_reach_earlier_ones(be):
@@ -211,8 +226,9 @@ def test_large_scores(be):
 def test_equal_calls_give_equal_bits(be):
     for seqs, sh in (([(1, 5000), (1, 4990)], 4096), ([(40, 900), (3, 700)], 512), ([(1, 3000)], 0)):
         q, kv, table = make(seqs, 8, 2, 128, "bf16", 64, sh)
-        a = [be.flash_attn_paged(q.cuda(), kv.cuda(), table.cuda(), scale=0.1, n_shared=sh, max_q=max(n for n, _ in seqs)) for _ in range(4)]
-        assert all(torch.equal(a[0], x) for x in a[1:])
+        for how in ways(sh):
+            a = [be.flash_attn_paged(q.cuda(), kv.cuda(), table.cuda(), scale=0.1, n_shared=sh, max_q=max(n for n, _ in seqs)) for _ in range(4)]
+            assert all(torch.equal(a[0], x) for x in a[1:])
 
 
 def test_nothing_to_do(be):
@@ -262,22 +278,23 @@ def test_graph_replays_follow_the_table(be):
             q.copy_(torch.randn(q.shape, generator=g))
 
         call = lambda o: be.flash_attn_paged(q, kv, table, scale=0.125, n_shared=n_shared, max_q=nq, out=o)
-        fill(0)
-        s = torch.cuda.Stream()
-        s.wait_stream(torch.cuda.current_stream())
-        g = torch.cuda.CUDAGraph()
-        with torch.cuda.stream(s):
-            call(out)
-            torch.cuda.synchronize()
-            with torch.cuda.graph(g, stream=s):
+        for how in ways(n_shared):
+            fill(0)
+            s = torch.cuda.Stream()
+            s.wait_stream(torch.cuda.current_stream())
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.stream(s):
                 call(out)
-        for i in range(4):
-            fill(i)
-            torch.cuda.synchronize()
-            g.replay()
-            torch.cuda.synchronize()
-            assert torch.equal(out, call(torch.empty_like(out))), i
-            torch.cuda.synchronize()
+                torch.cuda.synchronize()
+                with torch.cuda.graph(g, stream=s):
+                    call(out)
+            for i in range(4):
+                fill(i)
+                torch.cuda.synchronize()
+                g.replay()
+                torch.cuda.synchronize()
+                assert torch.equal(out, call(torch.empty_like(out))), i
+                torch.cuda.synchronize()
 
 
 @pytest.mark.parametrize("nq,n_shared", [(1, 0), (30, 0), (1, 32), (30, 32)])
@@ -290,21 +307,38 @@ def test_bad_pages_give_nan(be, nq, n_shared):
     bad = table.clone()
     bad[0, 3 + 140 // 16] = kv.shape[0]
     bad[1, 3 + 96 // 16] = -1
-    got = be.flash_attn_paged(q.cuda(), kv.cuda(), bad.cuda(), scale=0.125, n_shared=n_shared, max_q=nq).cpu()
-    for b, first in ((0, 128), (1, 96), (2, 10 ** 6)):
-        for i in range(nq):
-            t, p = int(table[b, 0]) + i, seqs[b][1] - nq + i
-            if p >= first:
-                assert torch.isnan(got[t]).all(), (b, i)
-            else:
-                compare(got[t:t + 1], want[t:t + 1], mag[t:t + 1], wgt[t:t + 1], 64)
+    for how in ways(n_shared):
+        got = be.flash_attn_paged(q.cuda(), kv.cuda(), bad.cuda(), scale=0.125, n_shared=n_shared, max_q=nq).cpu()
+        for b, first in ((0, 128), (1, 96), (2, 10 ** 6)):
+            for i in range(nq):
+                t, p = int(table[b, 0]) + i, seqs[b][1] - nq + i
+                if p >= first:
+                    assert torch.isnan(got[t]).all(), (b, i)
+                else:
+                    compare(got[t:t + 1], want[t:t + 1], mag[t:t + 1], wgt[t:t + 1], 64)
     # lengths and rows that do not fit: past the table, before or past q
     odd = table.clone()
     odd[0, 2] = 16 * (table.shape[1] - 3) + 5
     odd[1, 0] = q.shape[0]
     odd[2, 0] = -1
-    out = torch.full(q.shape, 7.0).cuda()
-    be.flash_attn_paged(q.cuda(), kv.cuda(), odd.cuda(), scale=0.125, n_shared=n_shared, max_q=nq, out=out)
-    out = out.cpu()
-    assert torch.isnan(out[nq - 1]).all()
-    assert (out[nq:] == 7).all()
+    for how in ways(n_shared):
+        out = torch.full(q.shape, 7.0).cuda()
+        be.flash_attn_paged(q.cuda(), kv.cuda(), odd.cuda(), scale=0.125, n_shared=n_shared, max_q=nq, out=out)
+        out = out.cpu()
+        assert torch.isnan(out[nq - 1]).all()
+        assert (out[nq:] == 7).all()
+
+
+def test_shared_prefix_is_read_where_it_pays(be):
+    """Many sequences under a long prefix: the first sequence's pages are read (the
+    others' copies hold something else), few under a short one: each its own."""
+    for B, n_shared, once in ((40, 2048, True), (3, 32, False)):
+        seqs = [(1, n_shared + 20 + b) for b in range(B)]
+        q, kv, table = make(seqs, 8, 2, 128, "f16", 16)
+        want, _, _ = P.attention(q[:1], kv, table[:1].tolist(), 0.09)
+        first = be.flash_attn_paged(q.cuda(), kv.cuda(), table.cuda(), scale=0.09, n_shared=n_shared, max_q=1).cpu()
+        as_first = table.clone()
+        as_first[:, 3:3 + n_shared // 16] = table[0, 3:3 + n_shared // 16]
+        same = be.flash_attn_paged(q.cuda(), kv.cuda(), as_first.cuda(), scale=0.09, n_shared=n_shared, max_q=1).cpu()
+        assert ((first[:1].double() - want).abs() < 1e-4).all()
+        assert torch.equal(first, same) == once
