@@ -11,15 +11,27 @@
 // Both kernels walk the keys once with a running maximum and sum, on the matrix
 // cores (v_mfma_f32_16x16x32): S^T = K Q^T leaves a query row in 4 lanes (n, n +
 // 16, n + 32, n + 48), whose scores are the B operand of O^T += V^T P^T as they
-// are.  q is 32-bit and the output too, so q and p are split into NQ / NP terms
-// of the cache's type that add up to them (f16: 2 terms, 22 bits; bf16: 3 terms,
-// 24 bits), each a product of its own on the same K or V fragment; sums are 32-bit.
+// are.  q is 32-bit and the output too, so q and p are split into terms of the
+// cache's type that add up to them (f16: 2 terms, 22 bits; bf16: 3 terms, 24 bits),
+// each a product of its own on the same K or V fragment; sums are 32-bit.  With one
+// term fewer the error against 64 bits is 2e-6 (bf16, p: 2 terms; 2.5e-6 with 2
+// of q) where 32-bit arithmetic has 0.7e-6 and these terms 0.3e-6 to 0.5e-6.
 //
 //  * ghip_fap_few: up to 16 rows of a KV head (generation: the G = H / H_kv query
 //    heads that share it, times a few rows).  Bound by reading K and V once: each
 //    of the 4 wavefronts streams its own 32-key tiles and they meet at the end.
-//  * ghip_fap_tile: up to 128 rows; the 4 wavefronts hold 32 rows each and share
-//    64-key tiles.  Bound by the matrix cores and the softmax's vector work.
+//    24 sequences of 500 .. 16384 keys under a window of 4096, 32 / 8 heads of 128,
+//    bf16: 77 us for 365 MB, 4.7 TB/s, what a large copy reaches.
+//  * ghip_fap_tile: up to 128 rows (64 of more than 128 dims); the 4 wavefronts hold
+//    32 rows each and share 64-key tiles, so that a K or V fragment read from LDS
+//    serves 2 row tiles times the terms.  Bound by the matrix cores, the softmax's
+//    vector work and what of them two wavefronts a SIMD do not overlap (registers:
+//    q's terms and the output are 128 of 256): 1001 + 701 rows under a window of
+//    2048, 32 / 8 heads of 128, f16: 125 us, 0.49 PFLOP/s of the formula's, twice that of
+//    products.
+//  * ghip_fap_both: a prefix shared by the batch as tiles of all its rows, and each
+//    sequence's own keys for few rows, in one launch.
+//  * ghip_fap_join: the partials of keys split over workgroups, in their order.
 //
 // K and V go straight from memory into LDS, 16 bytes a lane.  A row's 16-byte
 // chunks are swapped about by its number so that the fragment reads meet no bank
@@ -40,7 +52,8 @@ template <> struct Frag<f16> {
     typedef _Float16 v4 __attribute__((ext_vector_type(4)));
     typedef _Float16 v2 __attribute__((ext_vector_type(2)));
     typedef __fp16 tr __attribute__((__vector_size__(8)));
-    static constexpr int NQ = 2, NP = 2;
+    static constexpr int NQ = 2, NP = 2;         // terms of q and of p
+    static constexpr uint32_t EXP = 0x7c00;      // exponent bits: all ones for infinities and NaN
     static __device__ __forceinline__ v4f mfma(v8 a, v8 b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ v4 read_tr(uint32_t at) {
         return __builtin_bit_cast(v4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) tr *)at));
@@ -51,6 +64,7 @@ template <> struct Frag<bf16> {
     typedef __bf16 v4 __attribute__((ext_vector_type(4)));
     typedef __bf16 v2 __attribute__((ext_vector_type(2)));
     static constexpr int NQ = 3, NP = 3;
+    static constexpr uint32_t EXP = 0x7f80;
     static __device__ __forceinline__ v4f mfma(v8 a, v8 b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ v4 read_tr(uint32_t at) {
         return __builtin_bit_cast(v4, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) v4 *)at));
@@ -98,7 +112,6 @@ struct FapParams {
 
 #define DEV_M __device__ __forceinline__
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int FEW_ROWS = 16, TILE_ROWS = 128;
 
 // LDS chunk (16 bytes) of a row of CH chunks that holds chunk c of row r.  Reads of
 // K take one chunk of 16 rows; reads of V 32 bytes of 8 rows at a time: both
@@ -366,7 +379,7 @@ DEV void values(Rows<E, DP, RW> &R, uint32_t Vs, const v4f (&s)[NT][RW]) {
 // p with flags; the values themselves are then set to 0 in the tile.
 template <typename E>
 DEV bool odd_pair(uint32_t x) {
-    constexpr uint32_t LO = Frag<E>::NQ == 2 ? 0x7c00u : 0x7f80u, HI = LO << 16;
+    constexpr uint32_t LO = Frag<E>::EXP, HI = LO << 16;
     return (x & LO) == LO || (x & HI) == HI;
 }
 template <typename E, int DP, int RW, int NT>
@@ -415,7 +428,7 @@ DEV bool odd_chunks(const uint8_t *Vs, int from, int n) {
 }
 template <typename E>
 DEV void clear_odd(uint8_t *Vs, int from, int step, int n) {
-    constexpr uint32_t LO = Frag<E>::NQ == 2 ? 0x7c00u : 0x7f80u, HI = LO << 16;
+    constexpr uint32_t LO = Frag<E>::EXP, HI = LO << 16;
 #pragma unroll 1
     for (int i = from; i < n; i += step) {
         uint32_t *x = (uint32_t *)(Vs + 16 * i);
@@ -427,13 +440,10 @@ DEV void clear_odd(uint8_t *Vs, int from, int step, int n) {
     }
 }
 
-// One pass of a workgroup: which rows, which keys.
+// A workgroup's keys.
 struct Pass {
-    const int32_t *row;  // table row of its pages
-    int hk, z, share;    // KV head, split, tiles of a split
-    int p0, p1;          // least and largest position of its rows
+    int p0, p1;  // least and largest position of its rows
     PagedTiles tl;
-    int zi;              // where its partials go
 };
 DEV int clip_pos(int64_t p, int64_t table) { return (int)(p < -1 ? -1 : p > table ? table : p); }
 
@@ -541,7 +551,6 @@ DEV void fap_few(const FapParams &p, FewLds<DP> &lds) {
     const PagedSeq sq = paged_seq(row[0], row[1], row[2], p.T, p.max_q);
     if (sq.nq == 0) return;
     Pass ps;
-    ps.row = row;
     ps.p0 = clip_pos(sq.pos0, table);
     ps.p1 = clip_pos(sq.pos0 + sq.nq - 1, table);
     ps.tl = paged_tiles(ps.p0, ps.p1, p.window, p.n_first, p.n_shared, (int)table, KT);
@@ -866,9 +875,9 @@ DEV void fap_tile(const FapParams &p, TileLds<DP, RW> &lds) {
         const int j = min(tl.k0 + lane, tl.ke - 1);
         load4(row + 3 + paged_div((uint32_t)j, p.by_page), lds_addr(te[w][t & 1]));
     };
-    // Three tiles are under way: t is computed, t + 1 loaded, and of t + 2 the rows
-    // are found (from pages that were loaded a step before), in the shadow of t's
-    // first products.
+    // Three tiles are under way: t is computed, t + 1 loaded, and at the step's end,
+    // where it would wait for those loads, the rows of t + 2 are found (from pages
+    // that were loaded a step before).
     uint64_t ok = 0, bad = 0, ok2 = 0, bad2 = 0;  // keys of tiles t + 1, t + 2 that are there, those on no page
     const uint8_t *at[NI];                        // this lane's rows of the tile found last
     const RowLoads<DP> rl(p.D, NI * w);
@@ -877,9 +886,8 @@ DEV void fap_tile(const FapParams &p, TileLds<DP, RW> &lds) {
 #pragma unroll
         for (int ii = 0; ii < NI; ii++) at[ii] = kvh + offs[w][rl.row(ii)];
     };
-    // load f of 2 NI of tile t: one goes out under each fragment's products (a tile's
-    // 8 at once keep the wavefronts from their products until the addresses are
-    // through: NOTE_US)
+    // load f of 2 NI of tile t: one goes out under each fragment's products (bf16 125
+    // us, and 130 with all of them at the step's start; f16 the same)
     auto load_part = [&](int t, int f) {
         const int ii = f >> 1, kv = f & 1;
         load16(at[ii] + (kv ? 2 * p.D + rl.v_chunk(ii) : rl.k_chunk(ii)), lds_addr(kvs[t & 1][kv]) + 1024 * (NI * w + ii));
@@ -936,8 +944,7 @@ DEV void fap_tile(const FapParams &p, TileLds<DP, RW> &lds) {
         const bool more = t + 1 < t1;
         if (more) load_pages(t + 3);
         const bool odd = part && (ls.odd[t & 1][0] | ls.odd[t & 1][1] | ls.odd[t & 1][2] | ls.odd[t & 1][3]);
-        // 32 keys at a time: their scores are fewer registers than 64 keys' (which
-        // then spill), and one half's products run under the other's softmax
+        // 32 keys at a time: the scores of 64 are 16 registers more, which then spill
 #pragma unroll
         for (int u = 0; u < 2; u++) {
             const uint32_t Kh = Ks + 64 * u * DP, Vh = Vs + 64 * u * DP;
