@@ -3420,11 +3420,12 @@ FapLayout fap_layout(FapParams &p) {
         return best;
     };
     // Few rows: bound by memory, or by 512 workgroups at a time that start in 5 us and
-    // take 128 keys in 1.5; at least 256 keys a workgroup and about 1024 of them.
+    // take 128 keys in 1.5; at least 256 keys a workgroup and about 1024 of them, and
+    // no splits up to 512 keys (15 rows of 4 heads over 258 keys: 11.9 us in two, 9.7).
     auto few = [&](int64_t keys, bool alone) {
         const int64_t wgs = (int64_t)p.B * p.H_kv;
         Way w;
-        w.z = (int)std::max<int64_t>(1, std::min<int64_t>({(1024 + wgs - 1) / wgs, (keys + 255) / 256, 32}));
+        w.z = keys <= 512 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>({(1024 + wgs - 1) / wgs, (keys + 255) / 256, 32}));
         const double steps = (double)((keys + 128 * w.z - 1) / (128 * w.z));
         w.us = std::max((double)((wgs * w.z + 511) / 512) * (5.0 + steps * 1.5 * wide), 4.0 * wgs * keys * p.D / mem) +
                (w.z > 1 || !alone ? join(w.z) : 0.0);

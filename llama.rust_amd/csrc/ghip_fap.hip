@@ -275,16 +275,25 @@ DEV void scores(const Rows<E, DP, RW> &R, uint32_t Ks, v4f (&s)[NT][RW], F betwe
 template <typename E, int DP, int RW, int NT>
 DEV void mask_scores(const Rows<E, DP, RW> &R, v4f (&s)[NT][RW], int k0, int ke, uint64_t bad, int window, int n_first) {
     const int at = k0 + 4 * ((threadIdx.x & 63) >> 4);
+    // seen(c, lo, hi): is this lane's key c in sight of a row?
+    auto cut = [&](auto seen) {
 #pragma unroll
-    for (int rt = 0; rt < RW; rt++) {
-        const int hi = min(R.pos[rt], ke - 1) - at, lo = window ? R.pos[rt] - window - at : -0x7fffffff, first = n_first - at;
+        for (int rt = 0; rt < RW; rt++) {
+            const int hi = min(R.pos[rt], ke - 1) - at, lo = R.pos[rt] - window - at;
 #pragma unroll
-        for (int t = 0; t < NT; t++)
+            for (int t = 0; t < NT; t++)
 #pragma unroll
-            for (int v = 0; v < 4; v++) {
-                const int c = 16 * t + v;
-                if (!(c <= hi && (c > lo || c < first))) s[t][rt][v] = -__builtin_inff();
-            }
+                for (int v = 0; v < 4; v++)
+                    if (!seen(16 * t + v, lo, hi)) s[t][rt][v] = -__builtin_inff();
+        }
+    };
+    if (!window || ke <= n_first) {
+        cut([](int c, int, int hi) { return c <= hi; });
+    } else if (k0 >= n_first) {  // lo < c <= hi in one comparison
+        cut([](int c, int lo, int hi) { return (uint32_t)(c - 1 - lo) < (uint32_t)(max(hi, lo) - lo); });
+    } else {
+        const int first = n_first - at;
+        cut([=](int c, int lo, int hi) { return c <= hi && (c > lo || c < first); });
     }
     if (bad) {
         const uint64_t mine = bad >> (4 * ((threadIdx.x & 63) >> 4));
