@@ -3388,12 +3388,11 @@ struct FapLayout {
     int DP, rows;
     size_t ws_bytes;
 };
-FapLayout fap_layout(FapParams &p) {
+FapLayout fap_layout(FapParams &p, bool bf16) {
     FapLayout L;
     const int G = p.H / p.H_kv;
     L.DP = p.D <= 64 ? 64 : p.D <= 96 ? 96 : p.D <= 128 ? 128 : 256;
     L.few = (int64_t)p.max_q * G <= 16;
-    L.rows = L.DP == 256 ? 64 : 128;
     const int64_t table = (int64_t)p.per * p.page;
     const int64_t rows = std::min((int64_t)p.T, (int64_t)p.B * p.max_q);
     const double wide = L.DP / 128.0, mem = 4.8e6;  // bytes a microsecond
@@ -3405,15 +3404,17 @@ FapLayout fap_layout(FapParams &p) {
     };
     // partials written and read, and the launch that joins them
     auto join = [&](int z) { return 5.0 + 8.0 * rows * p.H * z * p.D / mem; };
-    // Tiles: the splits with the least  rounds x (start + tiles)  + partials.  A
-    // workgroup starts in 8 us; a 64-key tile of 128 dims takes 2.0 us where a CU has
-    // one workgroup, 3.2 where it has two (512 in a round; 256 of 256 dims).
-    auto tiles = [&](int64_t blocks, int64_t keys, bool alone) {
+    // Tiles of R rows: the splits with the least  rounds x (start + tiles)  +
+    // partials.  A workgroup starts in 8 us (64 rows: 7); a 64-key tile of 128 dims takes
+    // 2.0 us (1.4) where a CU has one workgroup, 3.2 (2.2) where it has two (512 in a
+    // round; 256 of 256 dims).
+    auto tiles = [&](int R, int64_t blocks, int64_t keys, bool alone) {
         const int64_t n = std::max<int64_t>(1, (keys + 63) / 64), slots = L.DP == 256 ? 256 : 512;
+        const double start = R == 64 ? 7.0 : 8.0, one = (R == 64 ? 1.4 : 2.0) * wide, two = (R == 64 ? 2.2 : 3.2) * wide;
         Way best{1, 0};
         for (int z = 1; z <= 32 && z <= n; z++) {
             const int64_t wgs = blocks * p.H_kv * z;
-            const double us = (double)((wgs + slots - 1) / slots) * (8.0 + (double)((n + z - 1) / z) * wide * (wgs <= 256 ? 2.0 : 3.2)) +
+            const double us = (double)((wgs + slots - 1) / slots) * (start + (double)((n + z - 1) / z) * (wgs <= 256 ? one : two)) +
                               (z > 1 || !alone ? join(z) : 0.0);
             if (z == 1 || us < best.us) best = {z, us};
         }
@@ -3431,31 +3432,46 @@ FapLayout fap_layout(FapParams &p) {
                (w.z > 1 || !alone ? join(w.z) : 0.0);
         return w;
     };
-    p.nb_own = L.few || (int64_t)p.max_q * G <= L.rows ? p.B : (int)((int64_t)p.T * G / L.rows + p.B);
-    auto own = [&](int64_t shared) {
+    auto own_blocks = [&](int R) { return L.few || (int64_t)p.max_q * G <= R ? p.B : (int)((int64_t)p.T * G / R + p.B); };
+    auto own = [&](int R, int64_t shared) {
         // the most keys that one block of rows goes through outside the shared prefix
         int64_t keys = table - shared;
         if (p.window) keys = std::min(keys, (int64_t)p.window + p.max_q - 1 + p.n_first);
-        return L.few ? few(keys, !shared) : tiles(p.nb_own, keys, !shared);
+        return L.few ? few(keys, !shared) : tiles(R, own_blocks(R), keys, !shared);
     };
-    // The shared prefix once for all, or each sequence's own pages: whichever is less
-    // (one launch and one join serve both parts).
-    const Way plain = own(0);
-    p.zs_own = plain.z;
-    p.nb_sh = p.zs_sh = p.wg_sh = 0;
-    if (p.n_shared) {
-        const int64_t nb = (rows * G + L.rows - 1) / L.rows;
-        const Way sh = tiles(nb, p.n_shared, false), rest = own(p.n_shared);
-        const int forced = env_int("GHIP_FAP_SHARED", -1);
-        if (forced >= 0 ? forced != 0 : sh.us + rest.us - 13.0 < plain.us) {
-            p.zs_own = rest.z;
+    // 128 rows a workgroup read each K and V fragment for twice the products; 64 rows
+    // are twice the workgroups, and all that fits the registers of 256 dims, or of
+    // bf16's terms at 128 (12 turns under 4001 keys 123 us with 128 rows, 112 with 64; 19
+    // sequences of 27 .. 111 rows, window 230 + 130, f16: 33 and 23; 1702
+    // rows over 2048 keys, f16: 123 and 160).  And the shared prefix once for all, or
+    // each sequence's own pages (one launch and one join serve both parts).
+    const int forced = env_int("GHIP_FAP_SHARED", -1), forced_rows = env_int("GHIP_FAP_ROWS", 0);
+    const int64_t n_shared = p.n_shared;
+    double least = -1.0;
+    for (int R = 64; R <= 128; R += 64) {
+        const bool wider = L.DP == 256 || (L.DP == 128 && bf16);  // 64 rows only
+        if (wider ? R == 128 : forced_rows && R != forced_rows && (forced_rows == 64 || forced_rows == 128)) continue;
+        const Way plain = own(R, 0);
+        if ((!n_shared || forced <= 0) && (least < 0.0 || plain.us < least)) {
+            least = plain.us;
+            L.rows = R;
+            p.n_shared = p.nb_sh = p.zs_sh = 0;
+            p.zs_own = plain.z;
+        }
+        if (!n_shared || forced == 0) continue;
+        const int64_t nb = (rows * G + R - 1) / R;
+        const Way sh = tiles(R, nb, n_shared, false), rest = own(R, n_shared);
+        if (least < 0.0 || sh.us + rest.us - 13.0 < least) {
+            least = sh.us + rest.us - 13.0;
+            L.rows = R;
+            p.n_shared = (int)n_shared;
             p.nb_sh = (int)nb;
             p.zs_sh = sh.z;
-            p.wg_sh = p.nb_sh * p.H_kv * p.zs_sh;
-        } else {
-            p.n_shared = 0;
+            p.zs_own = rest.z;
         }
     }
+    p.nb_own = own_blocks(L.rows);
+    p.wg_sh = p.nb_sh * p.H_kv * p.zs_sh;
     const int nz = p.zs_sh + p.zs_own;
     const size_t n = (size_t)p.T * p.H * nz;
     L.ws_bytes = nz > 1 ? n * (p.D + 2) * sizeof(float) : 0;
@@ -3474,7 +3490,7 @@ ghip_status ghip_flash_attn_paged_workspace(const ghip_tensor *q, const ghip_ten
     FapParams p;
     ghip_status st;
     if (!plan_fap(&tmp, q, kv, seqs, nullptr, dst, params, p, st)) return st;
-    if (p.max_q && p.H && p.B) *bytes = fap_layout(p).ws_bytes;
+    if (p.max_q && p.H && p.B) *bytes = fap_layout(p, kv->type == GHIP_TYPE_BF16).ws_bytes;
     return GHIP_STATUS_SUCCESS;
 }
 
@@ -3492,7 +3508,7 @@ ghip_status ghip_flash_attn_paged(ghip_context *ctx, const ghip_tensor *q, const
     st = ctx->begin(s);
     if (st != GHIP_STATUS_SUCCESS) return st;
     ctx->allow(dst->data, byte_extent(dst, 4), "dst");
-    const FapLayout L = fap_layout(p);
+    const FapLayout L = fap_layout(p, kv->type == GHIP_TYPE_BF16);
     p.part = p.stat = nullptr;
     if (L.ws_bytes) {
         void *ws = nullptr;
@@ -3524,7 +3540,8 @@ ghip_status ghip_flash_attn_paged(ghip_context *ctx, const ghip_tensor *q, const
     } else {
         ctx->expect(p.dst, (size_t)(4 * ((p.T - 1) * p.d_nb2 + (p.H - 1) * p.d_nb1 + p.D)), "dst");
     }
-    snprintf(name, sizeof name, "ghip_fap_%s_%s_%d", !L.few ? "tile" : p.wg_sh ? "both" : "few", ty, L.DP);
+    if (L.few && !p.wg_sh) snprintf(name, sizeof name, "ghip_fap_few_%s_%d", ty, L.DP);
+    else snprintf(name, sizeof name, "ghip_fap_%s%d_%s_%d", L.few ? "both" : "tile", L.rows, ty, L.DP);
     st = ctx->launch(name, dim3((unsigned)(own + p.wg_sh)), dim3(256), 0, s, p);
     if (st != GHIP_STATUS_SUCCESS) return st;
     if (!p.part) return GHIP_STATUS_SUCCESS;

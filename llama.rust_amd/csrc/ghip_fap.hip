@@ -1103,19 +1103,25 @@ union FapLds {
     FewLds<DP> few;
     TileLds<DP, RW> tile;
 };
-#define FAP_K(E, DP, RW)                                                                           \
-    extern "C" __global__ void __launch_bounds__(256, 2) ghip_fap_few_##E##_##DP(FapParams p) {    \
-        __shared__ __attribute__((aligned(1024))) uint8_t lds[sizeof(FewLds<DP>)];                 \
-        fap_few<E, DP>(p, *(FewLds<DP> *)lds);                                                     \
-    }                                                                                              \
-    extern "C" __global__ void __launch_bounds__(256, 2) ghip_fap_tile_##E##_##DP(FapParams p) {   \
-        __shared__ __attribute__((aligned(1024))) uint8_t lds[sizeof(TileLds<DP, RW>)];            \
-        fap_tile<E, DP, RW>(p, *(TileLds<DP, RW> *)lds);                                           \
-    }                                                                                              \
-    extern "C" __global__ void __launch_bounds__(256, 2) ghip_fap_both_##E##_##DP(FapParams p) {   \
-        __shared__ __attribute__((aligned(1024))) uint8_t lds[sizeof(FapLds<DP, RW>)];             \
-        if ((int)blockIdx.x < p.wg_sh) fap_tile<E, DP, RW>(p, *(TileLds<DP, RW> *)lds);            \
-        else fap_few<E, DP>(p, *(FewLds<DP> *)lds);                                                \
+#define FAP_FEW(E, DP)                                                                                   \
+    extern "C" __global__ void __launch_bounds__(256, 2) ghip_fap_few_##E##_##DP(FapParams p) {          \
+        __shared__ __attribute__((aligned(1024))) uint8_t lds[sizeof(FewLds<DP>)];                       \
+        fap_few<E, DP>(p, *(FewLds<DP> *)lds);                                                           \
     }
-#define FAP_E(E) FAP_K(E, 64, 2) FAP_K(E, 96, 2) FAP_K(E, 128, 2) FAP_K(E, 256, 1)
+// (R: rows of a workgroup, 64 RW)
+#define FAP_TILE(E, DP, RW, R)                                                                           \
+    extern "C" __global__ void __launch_bounds__(256, 2) ghip_fap_tile##R##_##E##_##DP(FapParams p) {    \
+        __shared__ __attribute__((aligned(1024))) uint8_t lds[sizeof(TileLds<DP, RW>)];                  \
+        fap_tile<E, DP, RW>(p, *(TileLds<DP, RW> *)lds);                                                 \
+    }                                                                                                    \
+    extern "C" __global__ void __launch_bounds__(256, 2) ghip_fap_both##R##_##E##_##DP(FapParams p) {    \
+        __shared__ __attribute__((aligned(1024))) uint8_t lds[sizeof(FapLds<DP, RW>)];                   \
+        if ((int)blockIdx.x < p.wg_sh) fap_tile<E, DP, RW>(p, *(TileLds<DP, RW> *)lds);                  \
+        else fap_few<E, DP>(p, *(FewLds<DP> *)lds);                                                      \
+    }
+#define FAP_E(E)                                                                                         \
+    FAP_FEW(E, 64) FAP_FEW(E, 96) FAP_FEW(E, 128) FAP_FEW(E, 256)                                        \
+    FAP_TILE(E, 64, 1, 64) FAP_TILE(E, 96, 1, 64) FAP_TILE(E, 128, 1, 64) FAP_TILE(E, 256, 1, 64)        \
+    FAP_TILE(E, 64, 2, 128) FAP_TILE(E, 96, 2, 128)
 FAP_E(f16) FAP_E(bf16)
+FAP_TILE(f16, 128, 2, 128)

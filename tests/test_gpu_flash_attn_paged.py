@@ -54,15 +54,18 @@ def make(seqs, H, Hkv, D, ctype, page, n_shared=0, seed=0, spare=3, order=None):
 
 
 def ways(n_shared):
-    """A shared prefix read once for all and read by each sequence: the sizes of
-    these tests would all take the latter by themselves."""
-    for how in ("1", "0") if n_shared else (None,):
-        if how is not None:
-            os.environ["GHIP_FAP_SHARED"] = how
-        try:
-            yield how
-        finally:
-            os.environ.pop("GHIP_FAP_SHARED", None)
+    """A shared prefix read once for all and read by each sequence, tiles of 64 rows
+    and of 128: the sizes of these tests would take one of each by themselves."""
+    for shared in ("1", "0") if n_shared else (None,):
+        for rows in ("64", "128"):
+            os.environ["GHIP_FAP_ROWS"] = rows
+            if shared is not None:
+                os.environ["GHIP_FAP_SHARED"] = shared
+            try:
+                yield shared, rows
+            finally:
+                os.environ.pop("GHIP_FAP_SHARED", None)
+                os.environ.pop("GHIP_FAP_ROWS", None)
 
 
 def compare(got, want, mag, wgt, D):
@@ -187,9 +190,10 @@ def test_later_rows_do_not_reach_earlier_ones(be):
         want, mag, wgt = P.attention(q, kv, table.tolist(), 0.125)
         for j in (80, 100):
             kv[table[0, 3 + j // 16].long(), j % 16, :, 64:] = what
-        got = be.flash_attn_paged(q.cuda(), kv.cuda(), table.cuda(), scale=0.125, max_q=50).cpu()
-        compare(got[:10], want[:10], mag[:10], wgt[:10], 64)
-        assert not torch.isfinite(got[10:]).any()
+        for how in ways(0):
+            got = be.flash_attn_paged(q.cuda(), kv.cuda(), table.cuda(), scale=0.125, max_q=50).cpu()
+            compare(got[:10], want[:10], mag[:10], wgt[:10], 64)
+            assert not torch.isfinite(got[10:]).any()
 
 
 @pytest.mark.parametrize("nq", [1, 40])
@@ -219,8 +223,9 @@ def test_large_scores(be):
         for j in range(500):
             kv[table[0, 3 + j // 16].long(), j % 16, :, :64] *= 0.01 * j
         want, mag, wgt = P.attention(q, kv, table.tolist(), 0.125)
-        got = be.flash_attn_paged(q.cuda(), kv.cuda(), table.cuda(), scale=0.125, max_q=nq).cpu().double()
-        assert ((got - want).abs() <= P.attention_tol(mag, wgt, 64)).all()
+        for how in ways(0):
+            got = be.flash_attn_paged(q.cuda(), kv.cuda(), table.cuda(), scale=0.125, max_q=nq).cpu().double()
+            assert ((got - want).abs() <= P.attention_tol(mag, wgt, 64)).all()
 
 
 def test_equal_calls_give_equal_bits(be):
