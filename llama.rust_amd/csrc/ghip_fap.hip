@@ -128,10 +128,10 @@ DEV int v_swz(int r, int c) {
 DEV uint32_t lds_addr(const void *p) { return (uint32_t)(uintptr_t)(lds_void *)p; }
 // 16 / 4 bytes a lane from memory to LDS at `to` (wave-uniform) + lane's place
 DEV void load16(const void *from, uint32_t to) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory", "m0");
 }
 DEV void load4(const void *from, uint32_t to) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(to), "v"(from) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(to), "v"(from) : "memory", "m0");
 }
 template <int N>
 DEV void wait_loads() {
@@ -735,6 +735,7 @@ struct TileLds {
 template <typename E, int DP, int RW>
 DEV void fap_tile(const FapParams &p, TileLds<DP, RW> &lds) {
     constexpr int KT = 64, R = 64 * RW, CH = DP / 8, NI = KT * CH / 256;  // loads of a K tile by each wavefront
+    static_assert(KT * CH % 256 == 0 && 2 * NI == DP / 16, "the wavefronts load alike, one load under each of a half's fragments");
     auto &kvs = lds.kvs;
     auto &offs = lds.offs;
     auto &te = lds.te;
