@@ -3405,39 +3405,47 @@ FapLayout fap_layout(FapParams &p, bool bf16) {
     // partials written and read, and the launch that joins them
     auto join = [&](int z) { return 5.0 + 8.0 * rows * p.H * z * p.D / mem; };
     // Tiles of R rows: the splits with the least  rounds x (start + tiles)  +
-    // partials.  A workgroup starts in 8 us (64 rows: 7); a 64-key tile of 128 dims takes
-    // 2.0 us (1.4) where a CU has one workgroup, 3.2 (2.2) where it has two (512 in a
-    // round; 256 of 256 dims).
-    auto tiles = [&](int R, int64_t blocks, int64_t keys, bool alone) {
+    // partials, with 256 workgroups in a round (one a CU) or 512 (two; not of 256
+    // dims).  Measured, us, one a CU and two: a 64-key tile of 64 / 96 / 128 / 256 dims
+    // with 64 rows 1.5 1.6 1.8 2.6 and 1.8 2.1 2.5 -, with 128 rows 2.0 2.3 2.7 - and
+    // 2.6 3.3 3.9 -, bf16 a quarter more; start 7 7 10 16 and 9 10 13 -, 10 11 14 - and
+    // 13 14 20 -.  The lines below go through these.
+    auto tiles = [&](int R, double blocks, int64_t keys, bool alone) {
         const int64_t n = std::max<int64_t>(1, (keys + 63) / 64), slots = L.DP == 256 ? 256 : 512;
-        const double start = R == 64 ? 7.0 : 8.0, one = (R == 64 ? 1.4 : 2.0) * wide, two = (R == 64 ? 2.2 : 3.2) * wide;
+        const double terms = bf16 ? 1.25 : 1.0;
+        const double start[2] = {R == 64 ? 4.0 + 6.0 * wide : 5.0 + 9.0 * wide, R == 64 ? 5.0 + 8.0 * wide : 6.0 + 14.0 * wide};
+        const double tile[2] = {terms * (R == 64 ? 1.2 + 0.6 * wide : 1.35 + 1.3 * wide),
+                                terms * (R == 64 ? 1.0 + 1.5 * wide : 1.25 + 2.7 * wide)};
         Way best{1, 0};
         for (int z = 1; z <= 32 && z <= n; z++) {
-            const int64_t wgs = blocks * p.H_kv * z;
-            const double us = (double)((wgs + slots - 1) / slots) * (start + (double)((n + z - 1) / z) * (wgs <= 256 ? one : two)) +
+            const double wgs = blocks * p.H_kv * z;
+            const int two = wgs > 256 && slots == 512;
+            const double us = std::max(1.0, std::ceil(wgs / slots - 0.1)) * (start[two] + (double)((n + z - 1) / z) * tile[two]) +
                               (z > 1 || !alone ? join(z) : 0.0);
             if (z == 1 || us < best.us) best = {z, us};
         }
         return best;
     };
-    // Few rows: bound by memory, or by 512 workgroups at a time that start in 5 us and
-    // take 128 keys in 1.5; at least 256 keys a workgroup and about 1024 of them, and
+    // Few rows: bound by memory, or by 512 workgroups at a time that start in 6 us and
+    // take 128 keys in 2 (of 128 dims); at least 256 keys a workgroup and about 1024 of them, and
     // no splits up to 512 keys (15 rows of 4 heads over 258 keys: 11.9 us in two, 9.7).
     auto few = [&](int64_t keys, bool alone) {
         const int64_t wgs = (int64_t)p.B * p.H_kv;
         Way w;
         w.z = keys <= 512 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>({(1024 + wgs - 1) / wgs, (keys + 255) / 256, 32}));
         const double steps = (double)((keys + 128 * w.z - 1) / (128 * w.z));
-        w.us = std::max((double)((wgs * w.z + 511) / 512) * (5.0 + steps * 1.5 * wide), 4.0 * wgs * keys * p.D / mem) +
+        w.us = std::max((double)((wgs * w.z + 511) / 512) * (6.0 + steps * (1.2 + 0.8 * wide)), 4.0 * wgs * keys * p.D / mem) +
                (w.z > 1 || !alone ? join(w.z) : 0.0);
         return w;
     };
     auto own_blocks = [&](int R) { return L.few || (int64_t)p.max_q * G <= R ? p.B : (int)((int64_t)p.T * G / R + p.B); };
+    // (about: half of the sequences' last blocks are half empty)
+    auto own_about = [&](int R) { return own_blocks(R) - ((int64_t)p.max_q * G <= R ? 0.0 : 0.5 * p.B); };
     auto own = [&](int R, int64_t shared) {
         // the most keys that one block of rows goes through outside the shared prefix
         int64_t keys = table - shared;
         if (p.window) keys = std::min(keys, (int64_t)p.window + p.max_q - 1 + p.n_first);
-        return L.few ? few(keys, !shared) : tiles(R, own_blocks(R), keys, !shared);
+        return L.few ? few(keys, !shared) : tiles(R, own_about(R), keys, !shared);
     };
     // 128 rows a workgroup read each K and V fragment for twice the products; 64 rows
     // are twice the workgroups, and all that fits the registers of 256 dims, or of
@@ -3460,7 +3468,12 @@ FapLayout fap_layout(FapParams &p, bool bf16) {
         }
         if (!n_shared || forced == 0) continue;
         const int64_t nb = (rows * G + R - 1) / R;
-        const Way sh = tiles(R, nb, n_shared, false), rest = own(R, n_shared);
+        // beside the own keys of few rows, many products count more than many workgroups:
+        // 128 rows from two 64-row tiles on for each of the 512 that run at a time (64 rows
+        // over 8192 keys, 8 tiles: 50 us, with 64 a workgroup 56; 46 rows of 8 / 2 heads of 64
+        // over 4451 keys, 0.8 tiles: 17 and 15)
+        if (R == 64 && L.few && !wider && !forced_rows && nb * p.H_kv * ((n_shared + 63) / 64) >= 1024) continue;
+        const Way sh = tiles(R, (double)nb, n_shared, false), rest = own(R, n_shared);
         if (least < 0.0 || sh.us + rest.us - 13.0 < least) {
             least = sh.us + rest.us - 13.0;
             L.rows = R;
