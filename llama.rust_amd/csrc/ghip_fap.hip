@@ -22,13 +22,12 @@
 //    of the 4 wavefronts streams its own 32-key tiles and they meet at the end.
 //    24 sequences of 500 .. 16384 keys under a window of 4096, 32 / 8 heads of 128,
 //    bf16: 77 us for 365 MB, 4.7 TB/s, what a large copy reaches.
-//  * ghip_fap_tile: up to 128 rows (64 of more than 128 dims); the 4 wavefronts hold
-//    32 rows each and share 64-key tiles, so that a K or V fragment read from LDS
-//    serves 2 row tiles times the terms.  Bound by the matrix cores, the softmax's
-//    vector work and what of them two wavefronts a SIMD do not overlap (registers:
-//    q's terms and the output are 128 of 256): 1001 + 701 rows under a window of
-//    2048, 32 / 8 heads of 128, f16: 125 us, 0.49 PFLOP/s of the formula's, twice that of
-//    products.
+//  * ghip_fap_tile: 128 or 64 rows; the 4 wavefronts hold 32 or 16 rows each and share
+//    64-key tiles, so that a K or V fragment read from LDS serves one or two row
+//    tiles times the terms.  Bound by the matrix cores, the softmax's vector work and
+//    what of them two wavefronts a SIMD do not overlap (registers: q's terms and the
+//    output are 128 of 256): 1001 + 701 rows under a window of 2048, 32 / 8 heads of 128,
+//    f16, 128 rows: 125 us, 0.49 PFLOP/s of the formula's, twice that of products.
 //  * ghip_fap_both: a prefix shared by the batch as tiles of all its rows, and each
 //    sequence's own keys for few rows, in one launch.
 //  * ghip_fap_join: the partials of keys split over workgroups, in their order.
@@ -896,8 +895,9 @@ DEV void fap_tile(const FapParams &p, TileLds<DP, RW> &lds) {
 #pragma unroll
         for (int ii = 0; ii < NI; ii++) at[ii] = kvh + offs[w][rl.row(ii)];
     };
-    // load f of 2 NI of tile t: one goes out under each fragment's products (bf16 125
-    // us, and 130 with all of them at the step's start; f16 the same)
+    // load f of 2 NI of tile t: one goes out under each fragment's products (bf16, 12
+    // turns under 4001 keys, 128 rows: 125 us, and 130 with all of them at the step's
+    // start; f16 the same)
     auto load_part = [&](int t, int f) {
         const int ii = f >> 1, kv = f & 1;
         load16(at[ii] + (kv ? 2 * p.D + rl.v_chunk(ii) : rl.k_chunk(ii)), lds_addr(kvs[t & 1][kv]) + 1024 * (NI * w + ii));
