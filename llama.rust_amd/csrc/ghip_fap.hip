@@ -754,7 +754,7 @@ DEV void fap_tile(const FapParams &p, TileLds<DP, RW> &lds) {
         const int nx = (r0 + R - 1) / G - x0 + 1;
         for (int k = tid; k < nx; k += 256) ls.tok[k] = -1;
         __syncthreads();
-        if (p.max_q == 1) {  // one row a sequence: sequence x0 + k
+        if (p.max_q == 1 && p.B <= p.T) {  // at most one row a sequence, and blocks for all of them: sequence x0 + k
             for (int k = tid; k < nx && x0 + k < p.B; k += 256) {
                 const PagedSeq sq = seq_of(p, x0 + k);
                 ls.tok[k] = sq.nq ? sq.q0 : -1;
