@@ -51,3 +51,18 @@ def test_many_idle_slots(be):
     slots = [(1 if b in (3, 255, 256, 290, 511, 599) else 0, 70 + b % 3) for b in range(600)]
     check(be, slots, 8, 1, 64, "f16", 64)
     check(be, slots, 8, 1, 64, "f16", 64, window=20, n_first=3)
+
+
+@pytest.mark.parametrize("rows", [1, 3])
+@pytest.mark.parametrize("live", [(1, 6), (35, 40)])
+def test_idle_first_slots_hold_nothing(be, live, rows):
+    """The prefix is read through the pages of a slot that has rows: those of idle ones
+    before it are gone, or past the cache."""
+    n_shared = 96
+    slots = [(rows if live[0] <= b < live[1] else 0, n_shared + 5 + b % 7) for b in range(40)]
+    for what in (-1, 0, 10 ** 9):
+        def change(table):
+            for b in range(40):
+                if not live[0] <= b < live[1]:
+                    table[b, :3], table[b, 3:] = 0, what
+        check(be, slots, 16, 4, 64, "f16", n_shared, change)
