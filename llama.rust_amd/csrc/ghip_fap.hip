@@ -52,6 +52,14 @@ template <> struct Frag<f16> {
     typedef _Float16 v2 __attribute__((ext_vector_type(2)));
     typedef __fp16 tr __attribute__((__vector_size__(8)));
     static constexpr int NQ = 2, NP = 2;         // terms of q and of p
+    // Where p is held: 2^HOME at a tile's largest key when the reference moves, below
+    // 2^TOP from then on (moves are 8 apart: with 3 the rescaling of o made 1702 rows
+    // over 2048 keys 138 us, now 123).  Terms of f16 end at 2^-24 however many they
+    // are, so a p of 2^-5 has 20 bits and smaller ones have less: the reference follows
+    // tiles down whose largest p is below 2^LOW, and where it moves, a tile's keys from
+    // 2^REST on take a pass before those below.
+    static constexpr float HOME = 8.0f, TOP = 15.9f, LOW = -2.0f, REST = -5.0f;
+    static constexpr bool FOLLOW = true;
     static constexpr uint32_t EXP = 0x7c00;      // exponent bits: all ones for infinities and NaN
     static __device__ __forceinline__ v4f mfma(v8 a, v8 b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ v4 read_tr(uint32_t at) {
@@ -63,6 +71,8 @@ template <> struct Frag<bf16> {
     typedef __bf16 v4 __attribute__((ext_vector_type(4)));
     typedef __bf16 v2 __attribute__((ext_vector_type(2)));
     static constexpr int NQ = 3, NP = 3;
+    static constexpr float HOME = 0.0f, TOP = 8.0f, LOW = 0.0f, REST = 0.0f;  // (32 bits' range: no need to follow)
+    static constexpr bool FOLLOW = false;
     static constexpr uint32_t EXP = 0x7f80;
     static __device__ __forceinline__ v4f mfma(v8 a, v8 b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ v4 read_tr(uint32_t at) {
@@ -158,10 +168,10 @@ struct Rows {
     typedef Frag<E> F;
     typename F::v8 q[RW][DP / 32][F::NQ];
     v4f o[RW][DP / 16];
-    v4f mneg[RW];   // minus the reference maximum (log2 units) four times: the scores' start; 0 while unset
+    v4f mneg[RW];   // minus the reference (log2 units) four times: the scores' start; 0 while unset
     float l[RW];    // this lane's share of the sum
     int pos[RW];    // position of this lane's row; -1: there is none, or it sees nothing
-    bool set[RW];   // a key has been seen
+    float from[RW]; // scores below this move the reference: infinity until a key has been seen
 };
 
 // A row's q: this lane's share as it lies (dims 32 kk + 8 (lane >> 4) ..), loaded
@@ -206,7 +216,7 @@ DEV void rows_start(Rows<E, DP, RW> &R, int rt, const RawRow<DP> &r, float scale
     for (int dt = 0; dt < DP / 16; dt++) R.o[rt][dt] = v4f{0, 0, 0, 0};
     R.mneg[rt] = v4f{0, 0, 0, 0};
     R.l[rt] = 0.0f;
-    R.set[rt] = false;
+    R.from[rt] = R.pos[rt] < 0 ? -__builtin_inff() : __builtin_inff();
 }
 
 // Fragment reads.  The swizzles touch the low bits of a chunk's number alone, so
@@ -308,31 +318,120 @@ DEV void mask_scores(const Rows<E, DP, RW> &R, v4f (&s)[NT][RW], int k0, int ke,
     }
 }
 
-// Scores -> probabilities.  The reference maximum moves only when a score passes
-// it by more than 8 (so p <= 256) or on a row's first key; o and l are rescaled
-// only then.
+// Row tile rt's keys from 2^REST on: their part of O^T += V^T P^T and of the row's
+// sum, after which they are gone from the scores.  (Called hardly ever, and straight
+// through: in a loop the compiler copies all of o.)
 template <typename E, int DP, int RW, int NT>
-DEV void softmax(Rows<E, DP, RW> &R, v4f (&s)[NT][RW]) {
+DEV void top_keys(Rows<E, DP, RW> &R, int rt, uint32_t Vs, v4f (&s)[NT][RW]) {
+    constexpr int NP = Frag<E>::NP;
+    const uint32_t vat = v_at<DP>(Vs);
 #pragma unroll
-    for (int rt = 0; rt < RW; rt++) {
-        float mx = -__builtin_inff();
+    for (int u = 0; u < NT / 2; u++) {
+        typename Frag<E>::v8 p[NP];
 #pragma unroll
-        for (int t = 0; t < NT; t++)
+        for (int e = 0; e < 4; e++) {
+            float x[2];
 #pragma unroll
-            for (int v = 0; v < 4; v++) mx = fmaxf(mx, s[t][rt][v]);
-        if (__ballot(mx > 8.0f || !R.set[rt])) {
-            mx = row_max(mx);
-            if (mx > 8.0f || (!R.set[rt] && mx > -__builtin_inff())) {
-                const float alpha = R.set[rt] ? __builtin_amdgcn_exp2f(-mx) : 1.0f;
-                R.set[rt] = true;
-                R.mneg[rt] -= mx;
-                R.l[rt] *= alpha;
+            for (int k = 0; k < 2; k++) {
+                const int v = 2 * (e & 1) + k;
+                const float y = s[2 * u + e / 2][rt][v];
+                const bool top = !(y < Frag<E>::REST);
+                x[k] = top ? __builtin_amdgcn_exp2f(y) : 0.0f;
+                s[2 * u + e / 2][rt][v] = top ? -__builtin_inff() : y;
+                R.l[rt] += x[k];
+            }
+            typename Frag<E>::v2 t[NP];
+            split_pair<E, NP>(x[0], x[1], t);
 #pragma unroll
-                for (int dt = 0; dt < DP / 16; dt++) R.o[rt][dt] *= alpha;
-#pragma unroll
-                for (int t = 0; t < NT; t++) s[t][rt] -= mx;
+            for (int i = 0; i < NP; i++) {
+                p[i][2 * e] = t[i][0];
+                p[i][2 * e + 1] = t[i][1];
             }
         }
+#pragma unroll
+        for (int dt = 0; dt < DP / 16; dt++) {
+            const typename Frag<E>::v8 a = value_frag<E, DP>(vat, u, dt);
+#pragma unroll
+            for (int i = NP - 1; i >= 0; i--) R.o[rt][dt] = Frag<E>::mfma(a, p[i], R.o[rt][dt]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+}
+
+// Row tile rt's largest score against its reference.  That moves on the row's first
+// key, when a p would pass 2^TOP, and, where it follows, when all of a row's p in the
+// tile are below 2^LOW; the tile's largest is then 2^HOME, and o and l are rescaled
+// (followed: by powers of two, as it may come often).  Followed down, o and l stay below
+// 2^107: the reference is at most 2^90 below what l has.  Returns whether it moved and
+// left keys below 2^REST.
+template <typename E, int DP, int RW, int NT>
+DEV bool find_reference(Rows<E, DP, RW> &R, int rt, v4f (&s)[NT][RW]) {
+    typedef Frag<E> F;
+    constexpr float INF = __builtin_inff();
+    float mx = -INF;
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int v = 0; v < 4; v++) mx = fmaxf(mx, s[t][rt][v]);
+    if (!__ballot(mx < R.from[rt] || mx > F::TOP)) return false;
+    mx = row_max(mx);
+    const bool set = R.from[rt] < INF;
+    float shift = mx - F::HOME;
+    bool move = mx > F::TOP || (!set && mx > -INF), low = false;
+    if constexpr (F::FOLLOW) {
+        const bool down = set && mx < F::LOW && mx > -INF;
+        if (__builtin_expect(__ballot(down) != 0, 0)) {
+            const float least = (float)__builtin_amdgcn_frexp_expf(row_max(R.l[rt])) - 90.0f;
+            if (down) shift = fmaxf(shift, least);
+        }
+        shift = __builtin_rintf(shift);
+        move = move || down;
+    }
+    if (__ballot(move && set)) {  // (o and l are 0 before a row's first key)
+        const float alpha = move && set ? __builtin_amdgcn_exp2f(-shift) : 1.0f;
+        R.l[rt] *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < DP / 16; dt++) R.o[rt][dt] *= alpha;
+    }
+    if (move) {
+        R.from[rt] = F::FOLLOW ? F::LOW : -INF;
+        R.mneg[rt] -= shift;
+#pragma unroll
+        for (int t = 0; t < NT; t++) s[t][rt] -= shift;
+        if constexpr (F::FOLLOW) {
+            // a score in (-inf, 2^REST): bits past those of REST, before those of -inf
+            constexpr uint32_t REST = __builtin_bit_cast(uint32_t, F::REST) + 1;
+            uint32_t mn = ~0u;
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int v = 0; v < 4; v++) mn = min(mn, __float_as_uint(s[t][rt][v]) - REST);
+            low = mn < 0xff800000u - REST && mx - shift > F::LOW;  // (else the reference went as far as it may)
+        }
+    }
+    return F::FOLLOW && __ballot(low);
+}
+
+// Scores -> probabilities, 2^(s - reference).  values_in(): is the tile's V in, and has
+// it no infinities that some rows do not see?  (f16, a first key whose own value is 0,
+// 299 others of e^-12 its weight: 2.2e-4 of the output in error with p of 1 at the
+// largest key and no following, at e^-18 8.6e-2; with it, but without the pass for the
+// top keys, 1.5e-5 at e^-18.)
+template <typename E, int DP, int RW, int NT, typename F>
+DEV void softmax(Rows<E, DP, RW> &R, v4f (&s)[NT][RW], uint32_t Vs, F values_in) {
+    bool low = false;
+#pragma unroll
+    for (int rt = 0; rt < RW; rt++) low |= find_reference<E, DP, RW, NT>(R, rt, s);
+    if constexpr (Frag<E>::FOLLOW)
+        if (__builtin_expect(low, 0) && values_in()) {
+#pragma unroll
+            for (int rt = 0; rt < RW; rt++) {
+                top_keys<E, DP, RW, NT>(R, rt, Vs, s);
+                find_reference<E, DP, RW, NT>(R, rt, s);
+            }
+        }
+#pragma unroll
+    for (int rt = 0; rt < RW; rt++) {
         float sum = 0.0f;
 #pragma unroll
         for (int t = 0; t < NT; t++)
@@ -623,19 +722,22 @@ DEV void fap_few(const FapParams &p, FewLds<DP> &lds) {
         }
         const bool part = !tile_whole(tile, KT, ps, p.window, p.n_first);
         if (part || badc) mask_scores<E, DP, 1, 2>(R, s, tile.k0, tile.ke, badc, p.window, p.n_first);
-        softmax<E, DP, 1, 2>(R, s);
-        if (more) wait_loads<NI + 1>();
-        else wait_loads<0>();
-        if (okc != 0xffffffffull) {
-            // rows that were not there: no value of theirs may count
+        auto values_in = [&]() {
+            if (more) wait_loads<NI + 1>();
+            else wait_loads<0>();
+            if (okc != 0xffffffffull) {
+                // rows that were not there: no value of theirs may count
 #pragma unroll
-            for (int ii = 0; ii < NI; ii++) {
-                const int c = 64 * ii + lane;
-                if (!((okc >> (c / CH)) & 1)) *(uint4 *)(kvs[w][1] + 16 * c) = make_uint4(0, 0, 0, 0);
+                for (int ii = 0; ii < NI; ii++) {
+                    const int c = 64 * ii + lane;
+                    if (!((okc >> (c / CH)) & 1)) *(uint4 *)(kvs[w][1] + 16 * c) = make_uint4(0, 0, 0, 0);
+                }
+                wait_lds();
             }
-            wait_lds();
-        }
-        if (part && ps.p0 != ps.p1 && odd_chunks<E>(kvs[w][1], 0, NI)) {
+            return !(part && ps.p0 != ps.p1 && odd_chunks<E>(kvs[w][1], 0, NI));
+        };
+        softmax<E, DP, 1, 2>(R, s, va, values_in);
+        if (!values_in()) {
             add_odd<E, DP, 1, 2>(R, va, s);
             clear_odd<E>(kvs[w][1], lane, 64, KT * CH);
         }
@@ -647,7 +749,7 @@ DEV void fap_few(const FapParams &p, FewLds<DP> &lds) {
     }
     // the 4 wavefronts' rows: everyone takes the common maximum, then thread
     // (dims, row) adds the four
-    const float l = row_sum(R.l[0]), m = R.set[0] ? -R.mneg[0][0] : -__builtin_inff();
+    const float l = row_sum(R.l[0]), m = R.from[0] < __builtin_inff() ? -R.mneg[0][0] : -__builtin_inff();
     if (g == 0) {
         ws[w][0][n] = m;
         ws[w][1][n] = l;
@@ -983,7 +1085,7 @@ DEV void fap_tile(const FapParams &p, TileLds<DP, RW> &lds) {
             }
             if (need) {
                 if (part || badc) mask_scores<E, DP, RW, 2>(Q, s, tile.k0 + 32 * u, tile.ke, badc >> (32 * u), p.window, p.n_first);
-                softmax<E, DP, RW, 2>(Q, s);
+                softmax<E, DP, RW, 2>(Q, s, Vh, [&]() { return !odd; });
             }
             if (odd) {
                 if (need) add_odd<E, DP, RW, 2>(Q, Vh, s);
@@ -1009,7 +1111,7 @@ DEV void fap_tile(const FapParams &p, TileLds<DP, RW> &lds) {
 #pragma unroll
     for (int rt = 0; rt < RW; rt++) {
         const Row y = row_of(rt);
-        float l = row_sum(Q.l[rt]), m = Q.set[rt] ? -Q.mneg[rt][0] : -__builtin_inff(), f = 1.0f;
+        float l = row_sum(Q.l[rt]), m = Q.from[rt] < __builtin_inff() ? -Q.mneg[rt][0] : -__builtin_inff(), f = 1.0f;
         if (y.pos >= table) l = __builtin_nanf("");
         if (!y.valid) continue;
         if (!p.part) finish_stat(p, y.hd, m, l, f);
