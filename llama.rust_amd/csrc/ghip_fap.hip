@@ -12,8 +12,8 @@
 // cores (v_mfma_f32_16x16x32): S^T = K Q^T leaves a query row in 4 lanes (n, n +
 // 16, n + 32, n + 48), whose scores are the B operand of O^T += V^T P^T as they
 // are.  q is 32-bit and the output too, so q and p are split into terms of the
-// cache's type that add up to them (f16: 2 terms, 22 bits; bf16: 3 terms, 24 bits),
-// each a product of its own on the same K or V fragment; sums are 32-bit.  With one
+// cache's type that add up to them (f16: 2 terms, 22 bits of what is first brought into
+// its range; bf16: 3 terms, 24 bits), each a product of its own on the same K or V fragment; sums are 32-bit.  With one
 // term fewer the error against 64 bits is 2e-6 (bf16, p: 2 terms; 2.5e-6 with 2
 // of q) where 32-bit arithmetic has 0.7e-6 and these terms 0.3e-6 to 0.5e-6.
 //
@@ -60,6 +60,12 @@ template <> struct Frag<f16> {
     // 2^REST on take a pass before those below.
     static constexpr float HOME = 8.0f, TOP = 15.9f, LOW = -2.0f, REST = -5.0f;
     static constexpr bool FOLLOW = true;
+    // A row's q is held 2^k times, its largest from 2^14 to 2^15, and the scores lose that
+    // again: small elements against large keys keep their bits, and none overflows (q of
+    // 1e-2 against keys of 100: error 1.0e-5 without, 2.2e-7; one more operation a score,
+    // 1702 rows over 2048 keys 125 -> 128 us).
+    static constexpr bool SCALED = true;
+    typedef float ref;
     static constexpr uint32_t EXP = 0x7c00;      // exponent bits: all ones for infinities and NaN
     static __device__ __forceinline__ v4f mfma(v8 a, v8 b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ v4 read_tr(uint32_t at) {
@@ -72,7 +78,8 @@ template <> struct Frag<bf16> {
     typedef __bf16 v2 __attribute__((ext_vector_type(2)));
     static constexpr int NQ = 3, NP = 3;
     static constexpr float HOME = 0.0f, TOP = 8.0f, LOW = 0.0f, REST = 0.0f;  // (32 bits' range: no need to follow)
-    static constexpr bool FOLLOW = false;
+    static constexpr bool FOLLOW = false, SCALED = false;
+    typedef v4f ref;
     static constexpr uint32_t EXP = 0x7f80;
     static __device__ __forceinline__ v4f mfma(v8 a, v8 b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ v4 read_tr(uint32_t at) {
@@ -168,7 +175,10 @@ struct Rows {
     typedef Frag<E> F;
     typename F::v8 q[RW][DP / 32][F::NQ];
     v4f o[RW][DP / 16];
-    v4f mneg[RW];   // minus the reference (log2 units) four times: the scores' start; 0 while unset
+    // minus the reference (log2 units), 0 while unset; where q is not scaled four times,
+    // as the products start with it
+    typename F::ref mneg[RW];
+    float unit[RW]; // what a score counts, 2^-k
     float l[RW];    // this lane's share of the sum
     int pos[RW];    // position of this lane's row; -1: there is none, or it sees nothing
     float from[RW]; // scores below this move the reference: infinity until a key has been seen
@@ -176,6 +186,9 @@ struct Rows {
 
 // A row's q: this lane's share as it lies (dims 32 kk + 8 (lane >> 4) ..), loaded
 // early; then, once it is in, as the terms of the fragments.
+// (row_ref: the reference itself)
+DEV float row_ref(float mneg) { return -mneg; }
+DEV float row_ref(v4f mneg) { return -mneg[0]; }
 template <int DP>
 struct RawRow {
     float x[DP / 32][8];
@@ -200,12 +213,28 @@ DEV void raw_wait(RawRow<DP> &r) {
 }
 template <typename E, int DP, int RW>
 DEV void rows_start(Rows<E, DP, RW> &R, int rt, const RawRow<DP> &r, float scale) {
+    int k = 0;
+    if constexpr (Frag<E>::SCALED) {
+        float mx = 0.0f;
+#pragma unroll
+        for (int kk = 0; kk < DP / 32; kk++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(r.x[kk][e] * scale));
+        mx = row_max(mx);
+        if (mx > 0.0f && mx < __builtin_inff()) k = min(15 - __builtin_amdgcn_frexp_expf(mx), 100);
+    }
+    R.unit[rt] = __builtin_amdgcn_ldexpf(1.0f, -k);
 #pragma unroll
     for (int kk = 0; kk < DP / 32; kk++)
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             typename Frag<E>::v2 t[Frag<E>::NQ];
-            split_pair<E, Frag<E>::NQ>(r.x[kk][2 * e] * scale, r.x[kk][2 * e + 1] * scale, t);
+            float x0 = r.x[kk][2 * e] * scale, x1 = r.x[kk][2 * e + 1] * scale;
+            if constexpr (Frag<E>::SCALED) {
+                x0 = __builtin_amdgcn_ldexpf(x0, k);
+                x1 = __builtin_amdgcn_ldexpf(x1, k);
+            }
+            split_pair<E, Frag<E>::NQ>(x0, x1, t);
 #pragma unroll
             for (int i = 0; i < Frag<E>::NQ; i++) {
                 R.q[rt][kk][i][2 * e] = t[i][0];
@@ -214,7 +243,7 @@ DEV void rows_start(Rows<E, DP, RW> &R, int rt, const RawRow<DP> &r, float scale
         }
 #pragma unroll
     for (int dt = 0; dt < DP / 16; dt++) R.o[rt][dt] = v4f{0, 0, 0, 0};
-    R.mneg[rt] = v4f{0, 0, 0, 0};
+    R.mneg[rt] = typename Frag<E>::ref{};
     R.l[rt] = 0.0f;
     R.from[rt] = R.pos[rt] < 0 ? -__builtin_inff() : __builtin_inff();
 }
@@ -254,8 +283,14 @@ DEV typename Frag<E>::v8 value_frag(uint32_t vat, int u, int dt) {
     const typename Frag<E>::v4 lo = Frag<E>::read_tr(at), hi = Frag<E>::read_tr(at + 32 * DP);
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
-// Scores of the NT 16-key tiles at Ks, less the reference maximum.  between(f) is
-// called after the products of fragment f, for what is to go out under them.
+// Scores of the NT 16-key tiles at Ks, less the reference (where q is scaled: as they
+// are, in its units; softmax() takes both off).  between(f) is called after the products of
+// fragment f, for what is to go out under them.
+template <typename E>
+DEV v4f start(typename Frag<E>::ref mneg) {
+    if constexpr (Frag<E>::SCALED) return v4f{0, 0, 0, 0};
+    else return mneg;
+}
 template <typename E, int DP, int RW, int NT, typename F>
 DEV void scores(const Rows<E, DP, RW> &R, uint32_t Ks, v4f (&s)[NT][RW], F between) {
     constexpr int KK = DP / 32, N = NT * KK;
@@ -272,7 +307,7 @@ DEV void scores(const Rows<E, DP, RW> &R, uint32_t Ks, v4f (&s)[NT][RW], F betwe
         for (int i = Frag<E>::NQ - 1; i >= 0; i--)
 #pragma unroll
             for (int rt = 0; rt < RW; rt++)
-                s[t][rt] = Frag<E>::mfma(a[f % 3], R.q[rt][kk][i], kk == 0 && i == Frag<E>::NQ - 1 ? R.mneg[rt] : s[t][rt]);
+                s[t][rt] = Frag<E>::mfma(a[f % 3], R.q[rt][kk][i], kk > 0 || i < Frag<E>::NQ - 1 ? s[t][rt] : start<E>(R.mneg[rt]));
         between(f);
         __builtin_amdgcn_sched_barrier(0);
     }
@@ -415,11 +450,18 @@ DEV bool find_reference(Rows<E, DP, RW> &R, int rt, v4f (&s)[NT][RW]) {
 // Scores -> probabilities, 2^(s - reference).  values_in(): is the tile's V in, and has
 // it no infinities that some rows do not see?  (f16, a first key whose own value is 0,
 // 299 others of e^-12 its weight: 2.2e-4 of the output in error with p of 1 at the
-// largest key and no following, at e^-18 8.6e-2; with it, but without the pass for the
-// top keys, 1.5e-5 at e^-18.)
+// largest key and no following, at e^-18 8.6e-2; as it is 9e-7 and 1.6e-6; without the
+// pass for the top keys 1.5e-5 at e^-18.)
 template <typename E, int DP, int RW, int NT, typename F>
 DEV void softmax(Rows<E, DP, RW> &R, v4f (&s)[NT][RW], uint32_t Vs, F values_in) {
     bool low = false;
+    if constexpr (Frag<E>::SCALED)
+#pragma unroll
+        for (int rt = 0; rt < RW; rt++)
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int v = 0; v < 4; v++) s[t][rt][v] = fmaf(s[t][rt][v], R.unit[rt], R.mneg[rt]);
 #pragma unroll
     for (int rt = 0; rt < RW; rt++) low |= find_reference<E, DP, RW, NT>(R, rt, s);
     if constexpr (Frag<E>::FOLLOW)
@@ -749,7 +791,7 @@ DEV void fap_few(const FapParams &p, FewLds<DP> &lds) {
     }
     // the 4 wavefronts' rows: everyone takes the common maximum, then thread
     // (dims, row) adds the four
-    const float l = row_sum(R.l[0]), m = R.from[0] < __builtin_inff() ? -R.mneg[0][0] : -__builtin_inff();
+    const float l = row_sum(R.l[0]), m = R.from[0] < __builtin_inff() ? row_ref(R.mneg[0]) : -__builtin_inff();
     if (g == 0) {
         ws[w][0][n] = m;
         ws[w][1][n] = l;
@@ -1111,7 +1153,7 @@ DEV void fap_tile(const FapParams &p, TileLds<DP, RW> &lds) {
 #pragma unroll
     for (int rt = 0; rt < RW; rt++) {
         const Row y = row_of(rt);
-        float l = row_sum(Q.l[rt]), m = Q.from[rt] < __builtin_inff() ? -Q.mneg[rt][0] : -__builtin_inff(), f = 1.0f;
+        float l = row_sum(Q.l[rt]), m = Q.from[rt] < __builtin_inff() ? row_ref(Q.mneg[rt]) : -__builtin_inff(), f = 1.0f;
         if (y.pos >= table) l = __builtin_nanf("");
         if (!y.valid) continue;
         if (!p.part) finish_stat(p, y.hd, m, l, f);

@@ -77,3 +77,30 @@ def test_weight_that_moves_down_and_up(be):
             if at > 1:
                 rows[:, D:] = 0
         check(be, q, kv, table, D ** -0.5, gap=76)
+
+
+@pytest.mark.parametrize("ctype", ["f16", "bf16"])
+@pytest.mark.parametrize("nq", [1, 40])
+@pytest.mark.parametrize("of_q,of_k", [(0.1, 10.0), (1e-2, 100.0), (1e-4, 1e4), (1e-30, 1.0), (1e6, 1e-6), (3e4, 1e-4)])
+def test_sizes_of_q(be, of_q, of_k, nq, ctype):
+    q, kv, table = make([(nq, 300)], 4, 2, 64, ctype, 16)
+    kv[..., :64] *= of_k
+    check(be, q * of_q, kv, table, 0.125)
+
+
+@pytest.mark.parametrize("ctype", ["f16", "bf16"])
+@pytest.mark.parametrize("nq", [1, 40])
+def test_channels_of_different_size(be, nq, ctype):
+    """Strong channels of q against weak ones of the keys, each adding as much to a score."""
+    for D in (64, 128, 256):
+        q, kv, table = make([(nq, 300)], 4, 2, D, ctype, 16)
+        size = 10.0 ** torch.linspace(-2, 2, D)
+        kv[..., :D] = (kv[..., :D].float() / size).to(kv.dtype)
+        check(be, q * size, kv, table, D ** -0.5)
+
+
+@pytest.mark.parametrize("ctype", ["f16", "bf16"])
+def test_rows_of_different_size(be, ctype):
+    for nq in (3, 40):
+        q, kv, table = make([(nq, 300)], 4, 2, 128, ctype, 16)
+        check(be, q * 10.0 ** -(torch.arange(nq * 4).view(nq, 4, 1) % 7), kv, table, 128 ** -0.5)
