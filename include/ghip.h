@@ -344,7 +344,9 @@ typedef struct ghip_paged_params {
  * Pages of keys that no row sees are not looked at, and what the cache holds
  * there, NaN included, does not matter.  A row that sees a key on a page outside
  * [0, pages), or past its table row, gives NaN.  Rows past max_q are not
- * computed. */
+ * computed.  Infinities and NaN of q and of what a row sees come out as 32-bit
+ * arithmetic has them: a key scoring -inf has no weight, an infinite value makes its
+ * element of the output infinite, neither reaches rows that do not see it. */
 ghip_status ghip_flash_attn_paged(ghip_context *ctx, const ghip_tensor *q, const ghip_tensor *kv, const ghip_tensor *seqs,
                                   const ghip_tensor *sinks, const ghip_paged_params *params, const ghip_tensor *dst,
                                   void *stream);

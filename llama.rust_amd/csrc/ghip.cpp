@@ -3559,7 +3559,8 @@ ghip_status ghip_flash_attn_paged(ghip_context *ctx, const ghip_tensor *q, const
     if (st != GHIP_STATUS_SUCCESS) return st;
     if (!p.part) return GHIP_STATUS_SUCCESS;
     ctx->expect(p.dst, (size_t)(4 * ((p.T - 1) * p.d_nb2 + (p.H - 1) * p.d_nb1 + p.D)), "dst");
-    return ctx->launch("ghip_fap_join", dim3((unsigned)joins), dim3(256), 0, s, p);
+    snprintf(name, sizeof name, "ghip_fap_join_%s", ty);
+    return ctx->launch(name, dim3((unsigned)joins), dim3(256), 0, s, p);
 }
 
 }  // extern "C"

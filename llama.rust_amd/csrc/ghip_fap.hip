@@ -66,7 +66,6 @@ template <> struct Frag<f16> {
     // 1702 rows over 2048 keys 125 -> 128 us).
     static constexpr bool SCALED = true;
     typedef float ref;
-    static constexpr uint32_t EXP = 0x7c00;      // exponent bits: all ones for infinities and NaN
     static __device__ __forceinline__ v4f mfma(v8 a, v8 b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ v4 read_tr(uint32_t at) {
         return __builtin_bit_cast(v4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) tr *)at));
@@ -80,7 +79,6 @@ template <> struct Frag<bf16> {
     static constexpr float HOME = 0.0f, TOP = 8.0f, LOW = 0.0f, REST = 0.0f;  // (32 bits' range: no need to follow)
     static constexpr bool FOLLOW = false, SCALED = false;
     typedef v4f ref;
-    static constexpr uint32_t EXP = 0x7f80;
     static __device__ __forceinline__ v4f mfma(v8 a, v8 b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ v4 read_tr(uint32_t at) {
         return __builtin_bit_cast(v4, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) v4 *)at));
@@ -447,8 +445,7 @@ DEV bool find_reference(Rows<E, DP, RW> &R, int rt, v4f (&s)[NT][RW]) {
     return F::FOLLOW && __ballot(low);
 }
 
-// Scores -> probabilities, 2^(s - reference).  values_in(): is the tile's V in, and has
-// it no infinities that some rows do not see?  (f16, a first key whose own value is 0,
+// Scores -> probabilities, 2^(s - reference).  values_in() waits for the tile's V.  (f16, a first key whose own value is 0,
 // 299 others of e^-12 its weight: 2.2e-4 of the output in error with p of 1 at the
 // largest key and no following, at e^-18 8.6e-2; as it is 9e-7 and 1.6e-6; without the
 // pass for the top keys 1.5e-5 at e^-18.)
@@ -465,7 +462,8 @@ DEV void softmax(Rows<E, DP, RW> &R, v4f (&s)[NT][RW], uint32_t Vs, F values_in)
 #pragma unroll
     for (int rt = 0; rt < RW; rt++) low |= find_reference<E, DP, RW, NT>(R, rt, s);
     if constexpr (Frag<E>::FOLLOW)
-        if (__builtin_expect(low, 0) && values_in()) {
+        if (__builtin_expect(low, 0)) {
+            values_in();
 #pragma unroll
             for (int rt = 0; rt < RW; rt++) {
                 top_keys<E, DP, RW, NT>(R, rt, Vs, s);
@@ -522,73 +520,6 @@ DEV void values(Rows<E, DP, RW> &R, uint32_t Vs, const v4f (&s)[NT][RW]) {
     }
 }
 
-// Infinities and NaN among the values of a tile that some rows do not see in
-// full: there a product with p = 0 would be NaN.  Each output whose row has such
-// a value with p > 0 takes an infinity of that sign (NaN: both) from products of
-// p with flags; the values themselves are then set to 0 in the tile.
-template <typename E>
-DEV bool odd_pair(uint32_t x) {
-    constexpr uint32_t LO = Frag<E>::EXP, HI = LO << 16;
-    return (x & LO) == LO || (x & HI) == HI;
-}
-template <typename E, int DP, int RW, int NT>
-DEV void add_odd(Rows<E, DP, RW> &R, uint32_t Vs, const v4f (&s)[NT][RW]) {
-    const uint32_t vat = v_at<DP>(Vs);
-#pragma unroll
-    for (int u = 0; u < NT / 2; u++)
-#pragma unroll
-        for (int rt = 0; rt < RW; rt++) {
-            typename Frag<E>::v8 p;
-#pragma unroll
-            for (int e = 0; e < 8; e++) p[e] = s[2 * u + e / 4][rt][e & 3] > 0.0f ? (E)1.0f : (E)0.0f;
-#pragma unroll
-            for (int dt = 0; dt < DP / 16; dt++) {
-                const typename Frag<E>::v8 a = value_frag<E, DP>(vat, u, dt);
-                typename Frag<E>::v8 up, dn;
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const float x = (float)a[e];
-                    const bool odd = !(fabsf(x) < __builtin_inff());
-                    up[e] = odd && !(x < 0.0f) ? (E)1.0f : (E)0.0f;
-                    dn[e] = odd && !(x > 0.0f) ? (E)1.0f : (E)0.0f;
-                }
-                const v4f zero = {0, 0, 0, 0};
-                const v4f nu = Frag<E>::mfma(up, p, zero), nd = Frag<E>::mfma(dn, p, zero);
-#pragma unroll
-                for (int v = 0; v < 4; v++) {
-                    if (nu[v] > 0.0f) R.o[rt][dt][v] += __builtin_inff();
-                    if (nd[v] > 0.0f) R.o[rt][dt][v] -= __builtin_inff();
-                }
-                __builtin_amdgcn_sched_barrier(0);
-            }
-        }
-}
-// chunks from + 64 i + lane, i < n, of a tile: do they hold one?  Chunks from, from
-// + step, .. below n: set to 0.
-template <typename E>
-DEV bool odd_chunks(const uint8_t *Vs, int from, int n) {
-    bool odd = false;
-#pragma unroll 1
-    for (int i = 0; i < n; i++) {
-        const uint4 x = *(const uint4 *)(Vs + 16 * (from + 64 * i + (threadIdx.x & 63)));
-        odd = odd || odd_pair<E>(x.x) || odd_pair<E>(x.y) || odd_pair<E>(x.z) || odd_pair<E>(x.w);
-    }
-    return __ballot(odd) != 0;
-}
-template <typename E>
-DEV void clear_odd(uint8_t *Vs, int from, int step, int n) {
-    constexpr uint32_t LO = Frag<E>::EXP, HI = LO << 16;
-#pragma unroll 1
-    for (int i = from; i < n; i += step) {
-        uint32_t *x = (uint32_t *)(Vs + 16 * i);
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            if ((x[k] & LO) == LO) x[k] &= 0xffff0000u;
-            if ((x[k] & HI) == HI) x[k] &= 0x0000ffffu;
-        }
-    }
-}
-
 // A workgroup's keys.
 struct Pass {
     int p0, p1;  // least and largest position of its rows
@@ -629,6 +560,98 @@ DEV void finish_stat(const FapParams &p, int h, float &m, float &l, float &f) {
 DEV void stat_none(const FapParams &p, int64_t pi, bool nan) {
     p.stat[2 * pi] = -__builtin_inff();
     p.stat[2 * pi + 1] = nan ? __builtin_nanf("") : 0.0f;
+}
+
+// An infinity in the cache: the terms of q and p make NaN of it (its product with a
+// term that is 0, or below it), and so does p = 0 of a row that does not see its key.
+// So a row whose result is not finite is computed again here, as the formula says, in
+// 32 bits and with the keys that it sees alone: a lane a key for the scores, first their
+// maximum, then p and its products with the values, lane l the dims 4 l ... A wavefront
+// a row, and hardly ever one: 12 us for 64 keys (512 rows of 32 heads over 2048 keys that
+// all see an infinite value: 3.4 ms, 60 us where it is finite); it ends at a score
+// of NaN (94 us).
+template <typename E>
+DEV v4f row_again(const FapParams &p, const int32_t *table, int64_t tok, int h, int64_t pos) {
+    const int lane = threadIdx.x & 63;
+    const float *q = p.q + tok * p.q_nb2 + h * p.q_nb1;
+    const uint16_t *kv = p.kv + h / (p.H / p.H_kv) * p.kv_head;
+    const PagedKeys ks = paged_keys(pos, pos, p.window, p.n_first);
+    const float nan = __builtin_nanf("");
+    const v4f none = {nan, nan, nan, nan};
+    float m = p.sinks ? p.sinks[h] * kLog2e : -__builtin_inff(), l = 0.0f;
+    v4f o = {0, 0, 0, 0};
+    for (int pass = 0; pass < 2; pass++) {
+        if (pass) {
+            if (m == -__builtin_inff()) m = 0.0f;  // nothing has weight
+            if (p.sinks) l = __builtin_amdgcn_exp2f(p.sinks[h] * kLog2e - m);
+        }
+        for (int64_t j0 = 0; j0 < ks.hi; j0 += 64) {
+            if (j0 >= ks.first && j0 + 64 <= ks.lo) {  // to the window
+                j0 = (ks.lo & ~(int64_t)63) - 64;
+                continue;
+            }
+            const int64_t j = j0 + lane;
+            const bool seen = j < ks.first || (j >= ks.lo && j < ks.hi);
+            const uint32_t i = paged_div(seen ? (uint32_t)j : 0, p.by_page);
+            const int32_t page = seen ? table[i] : 0;
+            if (__ballot(page < 0 || page >= p.n_pages)) return none;
+            const uint16_t *at = kv + page * p.kv_page + (seen ? (uint32_t)j - i * (uint32_t)p.page : 0) * p.kv_row;
+            float s = 0.0f;
+#pragma unroll 2
+            for (int d = 0; d < p.D; d += 8) {
+                const uint4 x = *(const uint4 *)(at + d);
+                const E *k = (const E *)&x;
+#pragma unroll
+                for (int e = 0; e < 8; e++) s = fmaf(q[d + e], (float)k[e], s);
+            }
+            s = seen ? s * (p.scale * kLog2e) : -__builtin_inff();
+            if (__ballot(!(s < __builtin_inff()))) return none;
+            if (!pass) {
+#pragma unroll
+                for (int t = 32; t; t >>= 1) s = fmaxf(s, __shfl_xor(s, t, 64));
+                m = fmaxf(m, s);
+                continue;
+            }
+            const float w = __builtin_amdgcn_exp2f(s - m);
+            l += wave_sum(w);
+            const float f = seen ? w : -1.0f;
+            for (int k0 = 0; k0 < 64; k0 += 8) {
+                uint2 x[8];
+#pragma unroll
+                for (int k = 0; k < 8; k++)
+                    x[k] = *(const uint2 *)(__shfl((unsigned long long)(at + p.D), k0 + k, 64) + 2 * min(4 * lane, p.D - 4));
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    const float y = __shfl(f, k0 + k, 64);
+                    const E *e = (const E *)&x[k];
+#pragma unroll
+                    for (int c = 0; c < 4; c++) o[c] = y < 0.0f ? o[c] : fmaf(y, (float)e[c], o[c]);
+                }
+            }
+        }
+    }
+    return l == 0.0f ? v4f{0, 0, 0, 0} : o / l;
+}
+// infinite or NaN?
+DEV bool odd(v4f x) {
+    const float y = x[0] * 0.0f + x[1] * 0.0f + x[2] * 0.0f + x[3] * 0.0f;
+    return y != y;
+}
+// The rows of a row tile (lanes n, n + 16, .. hold row n) that have to be computed
+// again; mine(d): are dims d .. d + 3 this wavefront's to store?
+template <typename E, typename F>
+DEV void rows_again(const FapParams &p, const int32_t *table, bool again, int64_t tok, int h, int pos, F mine) {
+    const int lane = threadIdx.x & 63;
+    uint64_t b = __ballot(again);
+    b |= b >> 32;
+    b |= b >> 16;
+    for (uint32_t rows = b & 0xffff; rows; rows &= rows - 1) {
+        const int n = __builtin_ctz(rows);
+        const int64_t t = __builtin_amdgcn_readlane((int)tok, n);
+        const int hd = __builtin_amdgcn_readlane(h, n);
+        const v4f o = row_again<E>(p, table, t, hd, __builtin_amdgcn_readlane(pos, n));
+        if (4 * lane < p.D && mine(4 * lane)) __builtin_memcpy(p.dst + t * p.d_nb2 + hd * p.d_nb1 + 4 * lane, &o, 16);
+    }
 }
 
 // Where the keys of a tile are: page numbers pg[] -> bytes into the cache of each
@@ -776,13 +799,9 @@ DEV void fap_few(const FapParams &p, FewLds<DP> &lds) {
                 }
                 wait_lds();
             }
-            return !(part && ps.p0 != ps.p1 && odd_chunks<E>(kvs[w][1], 0, NI));
         };
         softmax<E, DP, 1, 2>(R, s, va, values_in);
-        if (!values_in()) {
-            add_odd<E, DP, 1, 2>(R, va, s);
-            clear_odd<E>(kvs[w][1], lane, 64, KT * CH);
-        }
+        values_in();
         values<E, DP, 1, 2>(R, va, s);
         if (more) {
             wait_lds();
@@ -815,6 +834,7 @@ DEV void fap_few(const FapParams &p, FewLds<DP> &lds) {
     float fin = 1.0f, Mf = M, Lf = L;
     if (direct) finish_stat(p, hd, Mf, Lf, fin);
     // lanes of row n: wavefront w and lane group g take dims 16 w + 4 g + 64 k
+    bool again = false;
     if (valid) {
         float *out = direct ? p.dst + tok * p.d_nb2 + hd * p.d_nb1 : p.part + pi * p.D;
         for (int d = 16 * w + 4 * g; d < p.D; d += 64) {
@@ -823,12 +843,15 @@ DEV void fap_few(const FapParams &p, FewLds<DP> &lds) {
             for (int u = 0; u < 4; u++) a += *(v4f *)&os[(u * 16 + n) * (DP + 4) + d];
             a *= fin;
             __builtin_memcpy(out + d, &a, 16);
+            again = again || odd(a);
         }
         if (!direct && w == 0 && g == 0) {
             p.stat[2 * pi] = M;
             p.stat[2 * pi + 1] = L;
         }
     }
+    // (each wavefront the dims that it stores)
+    if (direct) rows_again<E>(p, row + 3, again && R.pos[0] < table, tok, hd, R.pos[0], [&](int d) { return (d >> 4 & 3) == w; });
 }
 
 // ---- up to 64 RW rows: 4 wavefronts of 16 RW rows, 64-key tiles for all
@@ -839,7 +862,6 @@ template <int R>
 struct RowList {
     int tok[R + 1], pos[R + 1];
     int sums[4], found[2];
-    int odd[2][4];  // by the tile's parity and the wavefront that loaded the part
 };
 // exclusive sum of v over the 256 threads; total: that of all
 template <int R>
@@ -1062,8 +1084,7 @@ DEV void fap_tile(const FapParams &p, TileLds<DP, RW> &lds) {
         for (int f = 0; f < 2 * NI; f++) load_part(t, f);
     };
     // What this wavefront loaded of tile t is in: rows that were not there hold
-    // nothing that counts, and a tile that some rows do not see in full is looked
-    // through for infinities and NaN.
+    // nothing that counts.
     auto loaded = [&](int t) {
         uint8_t *Vs = kvs[t & 1][1];
         if (ok != ~0ull) {
@@ -1072,10 +1093,6 @@ DEV void fap_tile(const FapParams &p, TileLds<DP, RW> &lds) {
                 const int c = 64 * (NI * w + ii) + lane;
                 if (!((ok >> (c / CH)) & 1)) *(uint4 *)(Vs + 16 * c) = make_uint4(0, 0, 0, 0);
             }
-        }
-        if (!tile_whole(tile_at(ps.tl, t, KT), KT, ps, p.window, p.n_first)) {
-            const bool odd = odd_chunks<E>(Vs, 64 * NI * w, NI);
-            if (lane == 0) ls.odd[t & 1][w] = odd;
         }
     };
     if (t0 < t1) {
@@ -1108,7 +1125,6 @@ DEV void fap_tile(const FapParams &p, TileLds<DP, RW> &lds) {
         const uint32_t Ks = lds_addr(kvs[t & 1][0]), Vs = lds_addr(kvs[t & 1][1]);
         const bool more = t + 1 < t1;
         if (more) load_pages(t + 3);
-        const bool odd = part && (ls.odd[t & 1][0] | ls.odd[t & 1][1] | ls.odd[t & 1][2] | ls.odd[t & 1][3]);
         // 32 keys at a time: the scores of 64 are 16 registers more, which then spill
 #pragma unroll
         for (int u = 0; u < 2; u++) {
@@ -1127,13 +1143,7 @@ DEV void fap_tile(const FapParams &p, TileLds<DP, RW> &lds) {
             }
             if (need) {
                 if (part || badc) mask_scores<E, DP, RW, 2>(Q, s, tile.k0 + 32 * u, tile.ke, badc >> (32 * u), p.window, p.n_first);
-                softmax<E, DP, RW, 2>(Q, s, Vh, [&]() { return !odd; });
-            }
-            if (odd) {
-                if (need) add_odd<E, DP, RW, 2>(Q, Vh, s);
-                __syncthreads();
-                clear_odd<E>(kvs[t & 1][1] + 64 * u * DP, tid, 256, 32 * CH);
-                __syncthreads();
+                softmax<E, DP, RW, 2>(Q, s, Vh, []() {});
             }
             if (need) {
                 __builtin_amdgcn_s_setprio(1);
@@ -1153,21 +1163,25 @@ DEV void fap_tile(const FapParams &p, TileLds<DP, RW> &lds) {
 #pragma unroll
     for (int rt = 0; rt < RW; rt++) {
         const Row y = row_of(rt);
+        bool again = false;
         float l = row_sum(Q.l[rt]), m = Q.from[rt] < __builtin_inff() ? row_ref(Q.mneg[rt]) : -__builtin_inff(), f = 1.0f;
         if (y.pos >= table) l = __builtin_nanf("");
-        if (!y.valid) continue;
-        if (!p.part) finish_stat(p, y.hd, m, l, f);
-        float *out = p.part ? p.part + y.pi * p.D : p.dst + y.tok * p.d_nb2 + y.hd * p.d_nb1;
+        if (y.valid) {
+            if (!p.part) finish_stat(p, y.hd, m, l, f);
+            float *out = p.part ? p.part + y.pi * p.D : p.dst + y.tok * p.d_nb2 + y.hd * p.d_nb1;
 #pragma unroll
-        for (int dt = 0; dt < DP / 16; dt++) {
-            const int d = 16 * dt + 4 * g;
-            const v4f a = Q.o[rt][dt] * f;
-            if (d < p.D) __builtin_memcpy(out + d, &a, 16);
+            for (int dt = 0; dt < DP / 16; dt++) {
+                const int d = 16 * dt + 4 * g;
+                const v4f a = Q.o[rt][dt] * f;
+                if (d < p.D) __builtin_memcpy(out + d, &a, 16);
+                again = again || (d < p.D && odd(a));
+            }
+            if (p.part && g == 0) {
+                p.stat[2 * y.pi] = m;
+                p.stat[2 * y.pi + 1] = l;
+            }
         }
-        if (p.part && g == 0) {
-            p.stat[2 * y.pi] = m;
-            p.stat[2 * y.pi + 1] = l;
-        }
+        if (!p.part) rows_again<E>(p, row + 3, again && y.pos < table, y.tok, y.hd, y.pos, [](int) { return true; });
     }
 }
 
@@ -1176,6 +1190,7 @@ DEV void fap_tile(const FapParams &p, TileLds<DP, RW> &lds) {
 // One wavefront a row (token, head): lane z holds split z's statistics; then NG
 // groups of D / 4 lanes take 4 dims a lane of splits group, group + NG, .. (8 of
 // them in flight), and the groups are added in order.
+template <typename E>
 DEV void fap_join(const FapParams &p) {
     const int lane = threadIdx.x & 63;
     const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -1244,13 +1259,15 @@ DEV void fap_join(const FapParams &p) {
     for (int k = 1; k < NG; k++)
 #pragma unroll
         for (int e = 0; e < 4; e++) sum[e] += __shfl(a[e], (lane + k * LD) & 63, 64);
-    if (lane < LD) {
-        if (L != L) sum = v4f{L, L, L, L};
-        __builtin_memcpy(p.dst + tok * p.d_nb2 + (int64_t)h * p.d_nb1 + 4 * lane, &sum, 16);
-    }
+    if (lane < LD && L != L) sum = v4f{L, L, L, L};
+    const int64_t pos = sq.pos0 + i;
+    if (__ballot(lane < LD && odd(sum)) && pos >= 0 && pos < (int64_t)p.per * p.page)
+        sum = row_again<E>(p, p.seqs + (int64_t)b * p.seq_nb1 + 3, tok, h, pos);
+    if (lane < LD) __builtin_memcpy(p.dst + tok * p.d_nb2 + (int64_t)h * p.d_nb1 + 4 * lane, &sum, 16);
 }
 
-extern "C" __global__ void __launch_bounds__(256) ghip_fap_join(FapParams p) { fap_join(p); }
+extern "C" __global__ void __launch_bounds__(256) ghip_fap_join_f16(FapParams p) { fap_join<f16>(p); }
+extern "C" __global__ void __launch_bounds__(256) ghip_fap_join_bf16(FapParams p) { fap_join<bf16>(p); }
 
 // ghip_fap_both: the shared prefix on tiles and each sequence's own keys, for few
 // rows each, in one launch, so that the one's loads run under the other's products.
