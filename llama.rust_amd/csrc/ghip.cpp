@@ -3378,6 +3378,9 @@ bool plan_fap(ghip_context *ctx, const ghip_tensor *q, const ghip_tensor *kv, co
     p.n_shared = B > 1 ? pp->n_shared : 0;
     p.by_page = paged_divisor((uint32_t)page);
     p.max_q = (int)std::min<int64_t>(pp->max_q, T);
+    // no pages: whatever a row sees is missing, as past a table without room, and
+    // there is no row to read in its place
+    if (p.n_pages == 0) p.per = p.n_shared = 0;
     st = GHIP_STATUS_SUCCESS;
     return true;
 }
@@ -3530,12 +3533,6 @@ ghip_status ghip_flash_attn_paged(ghip_context *ctx, const ghip_tensor *q, const
         const size_t n = (size_t)p.T * p.H * (p.zs_sh + p.zs_own);
         p.part = (float *)ws;
         p.stat = p.part + n * p.D;
-    }
-    // no pages: keys that rows see are all missing; what is read in their place
-    // (and not used) is q's first row, which is as long as a cache row
-    if (p.n_pages == 0) {
-        p.kv = (const uint16_t *)((uintptr_t)p.q & ~(uintptr_t)15);
-        p.kv_head = p.kv_row = p.kv_page = 0;
     }
     char name[48];
     const char *ty = float_name(kv->type);

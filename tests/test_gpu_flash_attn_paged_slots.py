@@ -66,3 +66,20 @@ def test_idle_first_slots_hold_nothing(be, live, rows):
                 if not live[0] <= b < live[1]:
                     table[b, :3], table[b, 3:] = 0, what
         check(be, slots, 16, 4, 64, "f16", n_shared, change)
+
+
+@pytest.mark.parametrize("rows", [1, 9, 70])
+def test_cache_without_pages(be, rows):
+    """Nothing is read in the place of missing pages (q lies at no multiple of 16 bytes):
+    rows that see a key are NaN, those before the first one 0."""
+    be.set_workspace(None)
+    for n_shared in (0, 20):
+        flat = torch.randn(2 * rows * 4 * 64 + 3, device="cuda")
+        q = flat[3:].view(2 * rows, 4, 64)
+        kv = torch.empty((0, 16, 2, 128), dtype=torch.float16, device="cuda")
+        seqs = torch.tensor([[0, rows, rows, 0, 1], [rows, rows, rows // 2, 5, -1]], dtype=torch.int32, device="cuda")
+        for sinks in (None, torch.zeros(4, device="cuda")):
+            got = be.flash_attn_paged(q, kv, seqs, sinks=sinks, n_shared=n_shared, max_q=rows).cpu()
+            torch.cuda.synchronize()
+            first = rows + rows - rows // 2
+            assert torch.isnan(got[:rows]).all() and torch.isnan(got[first:]).all() and (got[rows:first] == 0).all()
