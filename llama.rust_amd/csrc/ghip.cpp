@@ -3179,7 +3179,7 @@ ghip_status ghip_rope(ghip_context *ctx, const ghip_tensor *x, const ghip_tensor
     if (const char *why = rope_table(*rope, D, factors != nullptr, p.tab, p.P, axes)) return bad(why);
     if (const char *why = rope_operands(pos, factors, T, p.P, axes)) return bad(why);
     if (T == 0 || H == 0) return GHIP_STATUS_SUCCESS;
-    if (!x->data || !dst->data || !pos->data) return bad("null data");
+    if (!x->data || !dst->data || !pos->data || (factors && !factors->data)) return bad("null data");
     if (x->data != dst->data && overlaps(x, dst)) return bad("dst must be x itself or lie apart from it");
     if (x->data == dst->data && (x->nb[1] != dst->nb[1] || x->nb[2] != dst->nb[2]))
         return bad("dst in the place of x must have its strides");
@@ -3250,7 +3250,8 @@ ghip_status ghip_kv_append(ghip_context *ctx, const ghip_tensor *k, const ghip_t
         return bad("pos and factors need a rotation");
     }
     if (T == 0 || H == 0) return GHIP_STATUS_SUCCESS;
-    if (!k->data || !v->data || !slots->data || (!kv->data && kv->ne[3]) || (rope && !pos->data)) return bad("null data");
+    if (!k->data || !v->data || !slots->data || (!kv->data && kv->ne[3]) || (rope && !pos->data) || (factors && !factors->data))
+        return bad("null data");
     if (kv->ne[3] && (overlaps(k, kv) || overlaps(v, kv))) return bad("k and v must lie apart from kv");
     RopeShape r;
     if (!rope_shape(T, H, D, p.P, r)) return bad("k too large");
@@ -3347,7 +3348,7 @@ bool plan_fap(ghip_context *ctx, const ghip_tensor *q, const ghip_tensor *kv, co
     if (pp->n_shared < 0 || pp->n_shared > per * page) return bad("n_shared must be 0 .. the keys of a table row");
     if (pp->max_q < 0) return bad("max_q must not be negative");
     if (T && H && B) {
-        if (!q->data || !d->data || !seqs->data || (!kv->data && kv->ne[3])) return bad("null data");
+        if (!q->data || !d->data || !seqs->data || (!kv->data && kv->ne[3]) || (sinks && !sinks->data)) return bad("null data");
         if (overlaps(q, d)) return bad("dst must lie apart from q");
     }
     p.q = (const float *)q->data;

@@ -245,3 +245,12 @@ def test_index_arithmetic(tmp_path):
         want = [j for j in range(fr, to) if any(L.seen(ll(p), ll(j), w, f) for p in range(p0, p1 + 1))]
         assert keys == want, (p0, p1, w, f, fr, to, kt)
         assert share * nz >= n
+
+
+def test_null_data_is_refused(ctx):
+    """A tensor that is given has data: without it factors and sinks would be left out
+    (and the rotation's table read as another one)."""
+    import ghip
+    for st, msg in (run_rope(ctx, factors=T(ghip.F32, [32], None)), run_append(ctx, factors=T(ghip.F32, [32], None)),
+                    run_paged(ctx, sinks=T(ghip.F32, [8], None))):
+        assert st != 0 and "null data" in msg, msg
