@@ -299,7 +299,7 @@ typedef struct ghip_rope_params {
 
 /* dst = x rotated.
  *   x, dst:  F32 | F16 | BF16 [D, H, T], the same type (nb0 == the element, any
- *            other strides); dst may be x itself
+ *            other strides); dst may be x itself, or apart from all that is read
  *   pos:     I32 [T] or, with several axes, I32 [T, axes] (nb0 == 4)
  *   factors: F32 [pairs] or NULL
  * Angles are formed in 64 bits and outputs rounded once.  */
@@ -312,7 +312,7 @@ ghip_status ghip_rope(ghip_context *ctx, const ghip_tensor *x, const ghip_tensor
  *   slots: I64 [T]; a negative slot (padding) or one outside the cache writes
  *          nothing.  Slots of one call must differ.
  *   kv:    F16 | BF16 [2 D, H_kv, page, pages] (nb0 == 2)
- * k and v must not overlap kv. */
+ * None of the others may overlap kv. */
 ghip_status ghip_kv_append(ghip_context *ctx, const ghip_tensor *k, const ghip_tensor *v, const ghip_tensor *slots,
                            const ghip_tensor *pos, const ghip_tensor *factors, const ghip_rope_params *rope,
                            const ghip_tensor *kv, void *stream);
@@ -327,7 +327,7 @@ typedef struct ghip_paged_params {
 
 /* dst = attention of a batch of sequences over a paged cache.
  *   q, dst: F32 [D, H, T] (nb0 == 4), D a multiple of 8 up to 256, H % H_kv == 0;
- *           dst apart from q
+ *           dst apart from all that is read
  *   kv:     F16 | BF16 [2 D, H_kv, page, pages], data and strides multiples of 16 bytes
  *   seqs:   I32 [3 + per, B] (nb0 == 4): for each sequence its first row in q, its
  *           number of rows nq, its number of keys nkv (those of its rows among

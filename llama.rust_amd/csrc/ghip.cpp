@@ -3183,6 +3183,7 @@ ghip_status ghip_rope(ghip_context *ctx, const ghip_tensor *x, const ghip_tensor
     if (x->data != dst->data && overlaps(x, dst)) return bad("dst must be x itself or lie apart from it");
     if (x->data == dst->data && (x->nb[1] != dst->nb[1] || x->nb[2] != dst->nb[2]))
         return bad("dst in the place of x must have its strides");
+    if (overlaps(dst, pos) || overlaps(dst, factors)) return bad("dst must lie apart from pos and factors");
     RopeShape r;
     if (!rope_shape(T, H, D, p.P, r)) return bad("x too large");
     hipStream_t s = (hipStream_t)stream;
@@ -3253,6 +3254,8 @@ ghip_status ghip_kv_append(ghip_context *ctx, const ghip_tensor *k, const ghip_t
     if (!k->data || !v->data || !slots->data || (!kv->data && kv->ne[3]) || (rope && !pos->data) || (factors && !factors->data))
         return bad("null data");
     if (kv->ne[3] && (overlaps(k, kv) || overlaps(v, kv))) return bad("k and v must lie apart from kv");
+    if (kv->ne[3] && (overlaps(slots, kv) || overlaps(pos, kv) || overlaps(factors, kv)))
+        return bad("slots, pos and factors must lie apart from kv");
     RopeShape r;
     if (!rope_shape(T, H, D, p.P, r)) return bad("k too large");
     hipStream_t s = (hipStream_t)stream;
@@ -3350,6 +3353,8 @@ bool plan_fap(ghip_context *ctx, const ghip_tensor *q, const ghip_tensor *kv, co
     if (T && H && B) {
         if (!q->data || !d->data || !seqs->data || (!kv->data && kv->ne[3]) || (sinks && !sinks->data)) return bad("null data");
         if (overlaps(q, d)) return bad("dst must lie apart from q");
+        if ((kv->ne[3] && overlaps(kv, d)) || overlaps(seqs, d) || overlaps(sinks, d))
+            return bad("dst must lie apart from kv, seqs and sinks");
     }
     p.q = (const float *)q->data;
     p.q_nb1 = (int64_t)(q->nb[1] / 4);

@@ -254,3 +254,16 @@ def test_null_data_is_refused(ctx):
     for st, msg in (run_rope(ctx, factors=T(ghip.F32, [32], None)), run_append(ctx, factors=T(ghip.F32, [32], None)),
                     run_paged(ctx, sinks=T(ghip.F32, [8], None))):
         assert st != 0 and "null data" in msg, msg
+
+
+def test_outputs_lie_apart_from_what_is_read(ctx):
+    import ghip
+    for want, (st, msg) in [
+            ("kv", run_paged(ctx, dst=T(ghip.F32, [64, 8, 9], A[1] + 64))), ("seqs", run_paged(ctx, dst=T(ghip.F32, [64, 8, 9], A[2] - 64))),
+            ("sinks", run_paged(ctx, sinks=T(ghip.F32, [8], A[3] + 4096))), ("pos", run_rope(ctx, pos=T(ghip.I32, [9], A[1] + 8))),
+            ("factors", run_rope(ctx, factors=T(ghip.F32, [32], A[1] + 8))), ("slots", run_append(ctx, slots=T(ghip.I64, [9], A[3] + 8))),
+            ("pos", run_append(ctx, pos=T(ghip.I32, [9], A[3] + 8))), ("factors", run_append(ctx, factors=T(ghip.F32, [32], A[3] + 8)))]:
+        assert st != 0 and "apart" in msg and want in msg, (want, msg)
+    # an empty cache lies nowhere
+    st, msg = run_paged(ctx, pages=0, dst=T(ghip.F32, [64, 8, 9], A[1]))
+    assert st == 0, msg
