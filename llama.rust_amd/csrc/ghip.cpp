@@ -3040,10 +3040,15 @@ struct AppendParams {
 
 bool float_type(int t) { return t == GHIP_TYPE_F32 || t == GHIP_TYPE_F16 || t == GHIP_TYPE_BF16; }
 const char *float_name(int t) { return t == GHIP_TYPE_F32 ? "f32" : t == GHIP_TYPE_F16 ? "f16" : "bf16"; }
-// rows of elements, strides in whole elements
-bool elem_rows(const ghip_tensor *t, uint64_t e) {
-    return t->nb[0] == e && t->nb[1] % e == 0 && t->nb[2] % e == 0 && t->nb[3] % e == 0;
+// A stride counts where there is more than one element to step over.
+bool packed(const ghip_tensor *t, uint64_t e) { return t->ne[0] <= 1 || t->nb[0] == e; }
+bool in_steps(const ghip_tensor *t, int from, uint64_t of) {
+    for (int d = from; d < 4; d++)
+        if (t->ne[d] > 1 && t->nb[d] % of) return false;
+    return true;
 }
+// rows of elements, strides in whole elements
+bool elem_rows(const ghip_tensor *t, uint64_t e) { return packed(t, e) && in_steps(t, 1, e); }
 size_t byte_extent(const ghip_tensor *t, uint64_t e) {
     uint64_t n = e;
     for (int d = 0; d < 4; d++) {
@@ -3127,10 +3132,10 @@ const char *rope_table(const ghip_rope_params &r, int64_t D, bool factors, RopeT
 
 // positions and frequency factors of T tokens; the reason they are refused, or null
 const char *rope_operands(const ghip_tensor *pos, const ghip_tensor *factors, int64_t T, int P, int axes) {
-    if (!pos || pos->type != GHIP_TYPE_I32 || pos->nb[0] != 4 || pos->nb[1] % 4) return "pos must be I32 rows";
+    if (!pos || pos->type != GHIP_TYPE_I32 || !elem_rows(pos, 4)) return "pos must be I32 rows";
     if (pos->ne[0] < T) return "pos has fewer positions than there are tokens";
     if (axes > 1 && pos->ne[1] < axes) return "pos needs a row for each axis";
-    if (factors && (factors->type != GHIP_TYPE_F32 || factors->nb[0] != 4 || factors->ne[0] < P))
+    if (factors && (factors->type != GHIP_TYPE_F32 || !packed(factors, 4) || factors->ne[0] < P))
         return "factors must be F32, one for each pair";
     return nullptr;
 }
@@ -3181,7 +3186,7 @@ ghip_status ghip_rope(ghip_context *ctx, const ghip_tensor *x, const ghip_tensor
     if (T == 0 || H == 0) return GHIP_STATUS_SUCCESS;
     if (!x->data || !dst->data || !pos->data || (factors && !factors->data)) return bad("null data");
     if (x->data != dst->data && overlaps(x, dst)) return bad("dst must be x itself or lie apart from it");
-    if (x->data == dst->data && (x->nb[1] != dst->nb[1] || x->nb[2] != dst->nb[2]))
+    if (x->data == dst->data && ((H > 1 && x->nb[1] != dst->nb[1]) || (T > 1 && x->nb[2] != dst->nb[2])))
         return bad("dst in the place of x must have its strides");
     if (overlaps(dst, pos) || overlaps(dst, factors)) return bad("dst must lie apart from pos and factors");
     RopeShape r;
@@ -3234,7 +3239,7 @@ ghip_status ghip_kv_append(ghip_context *ctx, const ghip_tensor *k, const ghip_t
     if (!elem_rows(kv, 2) || kv->ne[0] != 2 * D || kv->ne[1] != H || kv->ne[2] < 1 || kv->ne[3] < 0)
         return bad("kv must be [2 D, H_kv, page, pages]");
     if (kv->ne[2] > INT32_MAX || kv->ne[3] > INT32_MAX) return bad("dimension too large");
-    if (slots->type != GHIP_TYPE_I64 || slots->nb[0] != 8 || slots->ne[0] < T) return bad("slots must be I64, one for each token");
+    if (slots->type != GHIP_TYPE_I64 || !packed(slots, 8) || slots->ne[0] < T) return bad("slots must be I64, one for each token");
     AppendParams p;
     p.P = 0;
     p.pos = nullptr;
@@ -3331,21 +3336,21 @@ bool plan_fap(ghip_context *ctx, const ghip_tensor *q, const ghip_tensor *kv, co
     if (q->ne[3] != 1) return bad("q must be [D, H, T]");
     if (D < 8 || D > 256 || D % 8) return bad("head size must be a multiple of 8, 8..256");
     if (kv->type != GHIP_TYPE_F16 && kv->type != GHIP_TYPE_BF16) return bad("kv must be F16 or BF16");
-    if (kv->nb[0] != 2 || kv->ne[0] != 2 * D || kv->ne[1] < 1 || kv->ne[2] < 1 || kv->ne[3] < 0)
+    if (!packed(kv, 2) || kv->ne[0] != 2 * D || kv->ne[1] < 1 || kv->ne[2] < 1 || kv->ne[3] < 0)
         return bad("kv must be [2 D, H_kv, page, pages]");
-    if (kv->nb[1] % 16 || kv->nb[2] % 16 || kv->nb[3] % 16 || (uintptr_t)kv->data % 16)
+    if (!in_steps(kv, 1, 16) || (uintptr_t)kv->data % 16)
         return bad("kv and its strides must be multiples of 16 bytes");
     const int64_t H_kv = kv->ne[1], page = kv->ne[2];
     if (H % H_kv) return bad("H % H_kv != 0");
     // the kernels count rows in 32 bits, 256 sequences of them at a time
     if (H > 65535 || T >= (1 << 23) || T * H >= (1ll << 29) || page > INT32_MAX || kv->ne[3] > INT32_MAX)
         return bad("dimension too large");
-    if (seqs->type != GHIP_TYPE_I32 || seqs->nb[0] != 4 || seqs->nb[1] % 4 || seqs->ne[0] < 3 || seqs->ne[1] < 0 ||
+    if (seqs->type != GHIP_TYPE_I32 || !elem_rows(seqs, 4) || seqs->ne[0] < 3 || seqs->ne[1] < 0 ||
         seqs->ne[2] != 1 || seqs->ne[3] != 1)
         return bad("seqs must be I32 [3 + pages of a sequence, sequences]");
     const int64_t per = seqs->ne[0] - 3, B = seqs->ne[1];
     if (per * page >= (1ll << 30) || B >= (1 << 23)) return bad("dimension too large");
-    if (sinks && (sinks->type != GHIP_TYPE_F32 || sinks->nb[0] != 4 || sinks->ne[0] < H)) return bad("sinks must be F32 [H]");
+    if (sinks && (sinks->type != GHIP_TYPE_F32 || !packed(sinks, 4) || sinks->ne[0] < H)) return bad("sinks must be F32 [H]");
     if (!std::isfinite(pp->scale)) return bad("scale must be finite");
     if (pp->window < 0 || pp->n_first < 0) return bad("window and n_first must not be negative");
     if (pp->n_shared < 0 || pp->n_shared > per * page) return bad("n_shared must be 0 .. the keys of a table row");

@@ -235,3 +235,22 @@ def test_streams_and_graph(be):
         be.kv_append(x, x, slots, kv2, pos=pos, rope=r)
         torch.cuda.synchronize()
         assert torch.equal(out, eager) and torch.equal(kv, kv2), i
+
+
+def test_one_token_of_strided_tables(be):
+    """Positions by axis as a column, a slot out of a longer table: the strides of axes
+    of one element do not count."""
+    import ghip
+    r = ghip.Rope(64, ghip.ROPE_MROPE, sections=(8, 8, 16, 0))
+    x = torch.randn((1, 4, 64), device="cuda")
+    pos = torch.tensor([[7, 3, 900, 1]], dtype=torch.int32, device="cuda").t()
+    slots = torch.arange(8, device="cuda")[3:4]
+    wide = torch.arange(64, device="cuda").view(8, 8)[3:4, ::4][:, :1].t()[0]
+    kv, kv2 = (torch.zeros((2, 8, 4, 128), dtype=torch.float16, device="cuda") for _ in range(2))
+    assert torch.equal(be.rope(x, pos, r), be.rope(x, pos.contiguous(), r))
+    be.kv_append(x, x, wide, kv, pos=pos, rope=r)
+    be.kv_append(x, x, torch.full_like(slots, 24) % 16, kv2, pos=pos.contiguous(), rope=r)
+    torch.cuda.synchronize()
+    assert not kv.any() and int(wide[0]) == 24  # (past the 16 slots of this cache)
+    be.kv_append(x, x, torch.arange(32, device="cuda")[8:16:8], kv, pos=pos, rope=r)
+    assert torch.equal(kv, kv2) and kv2.any()

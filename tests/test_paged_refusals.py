@@ -267,3 +267,28 @@ def test_outputs_lie_apart_from_what_is_read(ctx):
     # an empty cache lies nowhere
     st, msg = run_paged(ctx, pages=0, dst=T(ghip.F32, [64, 8, 9], A[1]))
     assert st == 0, msg
+
+
+def test_strides_of_axes_of_one_element_do_not_count(ctx):
+    """What is never stepped over may have any stride: one token of a batch's slots, one
+    head of several, one page, positions of one token by axis."""
+    import ghip
+    odd = 4 * 7 + 1
+    one = lambda ty, ne, e, data: T(ty, ne, data, nb=[e if n > 1 else odd for n in (list(ne) + [1] * 4)[:4]])
+    for st, msg in (
+            run_rope(ctx, N=1, H=1, x=T(0, [64, 1, 1], A[0], nb=[4, odd, odd, odd]), dst=T(0, [64, 1, 1], A[0], nb=[4, 256, 256, 256])),
+            run_rope(ctx, N=1, pos=T(ghip.I32, [1], A[2], nb=[32, odd, odd, odd])),
+            run_rope(ctx, N=1, mode=8, sections=(8, 8, 8, 8), pos=T(ghip.I32, [1, 4], A[2], nb=[16, 4, 16, 16])),
+            run_rope(ctx, D=2, n_dims=2, factors=one(ghip.F32, [1], 4, A[3])),
+            run_append(ctx, N=1, slots=one(ghip.I64, [1], 8, A[2]), kv=T(1, [128, 2, 16, 1], A[3], nb=[2, 256, 512, odd])),
+            run_append(ctx, D=1, rope=False, pos=None, k=T(0, [1, 2, 9], A[0], nb=[odd, 4, 8, 72]), v=T(0, [1, 2, 9], A[1], nb=[odd, 4, 8, 72])),
+            run_paged(ctx, H=1, Hkv=1, sinks=one(ghip.F32, [1], 4, A[4]), kv=T(1, [128, 1, 16, 50], A[1], nb=[2, odd, 256, 4096])),
+            run_paged(ctx, page=1, pages=1, kv=T(1, [128, 2, 1, 1], A[1], nb=[2, 256, odd, odd])),
+            run_paged(ctx, B=1, N=1, H=2, q=T(0, [64, 2, 1], A[0], nb=[4, 256, odd, odd]), dst=T(0, [64, 2, 1], A[3], nb=[4, 256, odd, odd]),
+                      seqs=T(ghip.I32, [10, 1], A[2], nb=[4, odd, odd, odd]))):
+        assert st == 0, msg
+    # where they are stepped over they do
+    for want, (st, msg) in (("I32", run_rope(ctx, N=2, pos=T(ghip.I32, [2], A[2], nb=[32, 64, 64, 64]))),
+                            ("I64", run_append(ctx, N=2, slots=T(ghip.I64, [2], A[2], nb=[32, 64, 64, 64]))),
+                            ("16 bytes", run_paged(ctx, kv=T(1, [128, 2, 16, 50], A[1], nb=[2, 256, 512, 8196])))):
+        assert st != 0 and want in msg, msg
