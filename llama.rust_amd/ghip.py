@@ -64,11 +64,26 @@ class PagedParams(C.Structure):
                 ("max_q", C.c_int32)]
 
 
+_PAGED = struct.Struct("=fiiii").pack
+assert struct.calcsize("=fiiii") == C.sizeof(PagedParams)
+
+
+def paged_params(scale, window, n_first, n_shared, max_q):
+    """The bytes of a PagedParams (whose fields take an int's low 32 bits)."""
+    try:
+        return _PAGED(scale, window, n_first, n_shared, max_q)
+    except (struct.error, OverflowError):
+        raise GhipError("scale must be a float, window, n_first, n_shared and max_q whole numbers of 32 bits") from None
+
+
 class Rope:
     """A rotation of head rows by their positions, made once for a model."""
 
     def __init__(self, n_dims, mode=ROPE_NEOX, freq_base=10000.0, freq_scale=1.0, sections=(0, 0, 0, 0), ext_factor=0.0,
                  attn_factor=1.0, beta_fast=32.0, beta_slow=1.0, n_ctx_orig=0):
+        for v in (n_dims, mode, n_ctx_orig, *sections):
+            if not -2 ** 31 <= v < 2 ** 31:
+                raise GhipError("n_dims, mode, sections and n_ctx_orig must be whole numbers of 32 bits")
         self.params = RopeParams(n_dims, mode, (C.c_int32 * 4)(*sections), freq_base, freq_scale, ext_factor,
                                  attn_factor, beta_fast, beta_slow, n_ctx_orig)
         self._ref = C.byref(self.params)
@@ -229,14 +244,14 @@ def lib():
         L.ghip_flash_attn_ext.argtypes = [C.c_void_p, P, P, P, P, P, P, C.c_void_p]
         R = C.POINTER(RopeParams)
         L.ghip_rope.restype = C.c_int
-        V = C.c_void_p  # a ghip_tensor by reference, or its bytes (_view)
+        V = C.c_void_p  # a struct by reference, or its bytes (_view, paged_params)
         L.ghip_rope.argtypes = [V, V, V, V, R, V, V]
         L.ghip_kv_append.restype = C.c_int
         L.ghip_kv_append.argtypes = [V, V, V, V, V, V, R, V, V]
         L.ghip_flash_attn_paged.restype = C.c_int
-        L.ghip_flash_attn_paged.argtypes = [V, V, V, V, V, C.POINTER(PagedParams), V, V]
+        L.ghip_flash_attn_paged.argtypes = [V, V, V, V, V, V, V, V]
         L.ghip_flash_attn_paged_workspace.restype = C.c_int
-        L.ghip_flash_attn_paged_workspace.argtypes = [V, V, V, C.POINTER(PagedParams), V, C.POINTER(C.c_size_t)]
+        L.ghip_flash_attn_paged_workspace.argtypes = [V, V, V, V, V, C.POINTER(C.c_size_t)]
         _lib = L
     return _lib
 
@@ -413,8 +428,8 @@ class Backend:
         f32.  max_q: the most rows of a sequence (T where None) -> [T, H, D] f32."""
         if out is None:
             out = torch.empty_like(q)
-        pp = PagedParams(scale, window, n_first, n_shared, q.shape[0] if max_q is None else max_q)
-        st = lib().ghip_flash_attn_paged(self._ctx, _view(q), _view(kv), _view(seqs), _view(sinks), C.byref(pp), _view(out),
+        pp = paged_params(scale, window, n_first, n_shared, q.shape[0] if max_q is None else max_q)
+        st = lib().ghip_flash_attn_paged(self._ctx, _view(q), _view(kv), _view(seqs), _view(sinks), pp, _view(out),
                                          _raw_stream(self.device))
         if st:
             self._check(st, "ghip_flash_attn_paged")
@@ -423,11 +438,11 @@ class Backend:
     @staticmethod
     def flash_attn_paged_workspace(q, kv, seqs, window=0, n_first=0, n_shared=0, max_q=None):
         """Workspace bytes that flash_attn_paged needs at most for these shapes."""
-        pp = PagedParams(1.0, window, n_first, n_shared, q.shape[0] if max_q is None else max_q)
+        pp = paged_params(1.0, window, n_first, n_shared, q.shape[0] if max_q is None else max_q)
         out, v = C.c_size_t(0), _view(q)
         d = Tensor.from_buffer_copy(v)
         d.data = (d.data or 0) + (1 << 60)  # any place apart from q: only compared
-        st = lib().ghip_flash_attn_paged_workspace(v, _view(kv), _view(seqs), C.byref(pp), bytes(d), C.byref(out))
+        st = lib().ghip_flash_attn_paged_workspace(v, _view(kv), _view(seqs), pp, bytes(d), C.byref(out))
         if st:
             raise GhipError(f"ghip_flash_attn_paged_workspace: status {st}")
         return out.value

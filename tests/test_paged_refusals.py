@@ -292,3 +292,16 @@ def test_strides_of_axes_of_one_element_do_not_count(ctx):
                             ("I64", run_append(ctx, N=2, slots=T(ghip.I64, [2], A[2], nb=[32, 64, 64, 64]))),
                             ("16 bytes", run_paged(ctx, kv=T(1, [128, 2, 16, 50], A[1], nb=[2, 256, 512, 8196])))):
         assert st != 0 and want in msg, msg
+
+
+def test_binding_refuses_numbers_that_do_not_fit():
+    """A window or a size past 32 bits would be taken for its low bits."""
+    pytest.importorskip("torch")
+    import ghip
+    for kw in (dict(scale=1e39), dict(window=2 ** 32 + 5), dict(n_first=2 ** 31), dict(n_shared=-2 ** 31 - 1), dict(max_q=2 ** 40), dict(window=1.5)):
+        with pytest.raises(ghip.GhipError, match="32 bits"):
+            ghip.paged_params(**{**dict(scale=1.0, window=0, n_first=0, n_shared=0, max_q=1), **kw})
+    for kw in (dict(n_dims=2 ** 32 + 64), dict(n_dims=64, mode=2 ** 32), dict(n_dims=64, sections=(2 ** 33, 0, 0, 0)), dict(n_dims=64, n_ctx_orig=2 ** 31)):
+        with pytest.raises(ghip.GhipError, match="32 bits"):
+            ghip.Rope(**kw)
+    assert bytes(ghip.PagedParams(0.5, 7, 4, 3, 2)) == ghip.paged_params(0.5, 7, 4, 3, 2)
