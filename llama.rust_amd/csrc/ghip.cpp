@@ -3440,15 +3440,16 @@ FapLayout fap_layout(FapParams &p, bool bf16) {
         }
         return best;
     };
-    // Few rows: bound by memory, or by 512 workgroups at a time that start in 6 us and
-    // take 128 keys in 2 (of 128 dims); at least 256 keys a workgroup and about 1024 of them, and
-    // no splits up to 512 keys (15 rows of 4 heads over 258 keys: 11.9 us in two, 9.7).
+    // Few rows: bound by memory, or by 512 workgroups at a time (256 of 256 dims, one a CU)
+    // that start in 6 us and take 128 keys in 2 (of 128 dims); about 256 keys a workgroup or
+    // more, up to about 1024 workgroups, and no splits up to 512 keys (15 rows of 4 heads
+    // over 258 keys: 11.9 us in two, 9.7).
     auto few = [&](int64_t keys, bool alone) {
-        const int64_t wgs = (int64_t)p.B * p.H_kv;
+        const int64_t wgs = (int64_t)p.B * p.H_kv, slots = L.DP == 256 ? 256 : 512;
         Way w;
         w.z = keys <= 512 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>({(1024 + wgs - 1) / wgs, (keys + 255) / 256, 32}));
         const double steps = (double)((keys + 128 * w.z - 1) / (128 * w.z));
-        w.us = std::max((double)((wgs * w.z + 511) / 512) * (6.0 + steps * (1.2 + 0.8 * wide)), 4.0 * wgs * keys * p.D / mem) +
+        w.us = std::max((double)((wgs * w.z + slots - 1) / slots) * (6.0 + steps * (1.2 + 0.8 * wide)), 4.0 * wgs * keys * p.D / mem) +
                (w.z > 1 || !alone ? join(w.z) : 0.0);
         return w;
     };
