@@ -3553,7 +3553,8 @@ ghip_status ghip_flash_attn_paged(ghip_context *ctx, const ghip_tensor *q, const
     // B max_q can be many times T
     p.join_ragged = p.max_q > 1 && (int64_t)p.B * p.max_q > 2 * (int64_t)p.T;
     const int64_t joins = ((p.join_ragged ? (int64_t)p.T : (int64_t)p.B * p.max_q) * p.H + 3) / 4;
-    if (own + p.wg_sh > INT32_MAX || joins > INT32_MAX)
+    const int64_t most = ((1ll << 32) - 1) / 256;  // workgroups of 256 threads in a launch
+    if (own + p.wg_sh > most || (p.part && joins > most))
         return ctx->fail(GHIP_STATUS_BACKEND_ERROR, "flash_attn_paged: too many rows");
     if (p.part) {
         const size_t n = (size_t)p.T * p.H * (p.zs_sh + p.zs_own);
