@@ -310,6 +310,6 @@ def test_binding_refuses_numbers_that_do_not_fit():
 def test_more_workgroups_than_a_launch_takes_are_refused(ctx, monkeypatch):
     """A launch has fewer than 2^32 threads: refused before anything runs, not by the join."""
     monkeypatch.setenv("GHIP_FAP_SHARED", "1")
-    for N, ok in ((1 << 20, True), (1 << 22, False)):
+    for N, ok in ((1 << 19, True), (1 << 20, False), (1 << 22, False)):
         st, msg = run_paged(ctx, D=8, H=32, Hkv=8, N=N, B=2, n_shared=16, max_q=N)
         assert (st == 0) == ok and (ok or "too many rows" in msg), msg
