@@ -457,27 +457,22 @@ DEV bool find_reference(Rows<E, DP, RW> &R, int rt, v4f (&s)[NT][RW]) {
 // pass for the top keys 1.5e-5 at e^-18.)
 template <typename E, int DP, int RW, int NT, typename F>
 DEV void softmax(Rows<E, DP, RW> &R, v4f (&s)[NT][RW], uint32_t Vs, F values_in) {
-    bool low = false;
-    if constexpr (Frag<E>::SCALED)
+    // (one row tile after the other: the next one's products end under this one's work; all
+    // references first measured 39.7 for 38.6 us, 3 prompts of 16 heads of 64)
 #pragma unroll
-        for (int rt = 0; rt < RW; rt++)
+    for (int rt = 0; rt < RW; rt++) {
+        if constexpr (Frag<E>::SCALED)
 #pragma unroll
             for (int t = 0; t < NT; t++)
 #pragma unroll
                 for (int v = 0; v < 4; v++) s[t][rt][v] = fmaf(s[t][rt][v], R.unit[rt], R.mneg[rt]);
-#pragma unroll
-    for (int rt = 0; rt < RW; rt++) low |= find_reference<E, DP, RW, NT>(R, rt, s);
-    if constexpr (Frag<E>::FOLLOW)
-        if (__builtin_expect(low, 0)) {
-            values_in();
-#pragma unroll
-            for (int rt = 0; rt < RW; rt++) {
+        const bool low = find_reference<E, DP, RW, NT>(R, rt, s);
+        if constexpr (Frag<E>::FOLLOW)
+            if (__builtin_expect(low, 0)) {
+                values_in();
                 top_keys<E, DP, RW, NT>(R, rt, Vs, s);
                 find_reference<E, DP, RW, NT>(R, rt, s);
             }
-        }
-#pragma unroll
-    for (int rt = 0; rt < RW; rt++) {
         float sum = 0.0f;
 #pragma unroll
         for (int t = 0; t < NT; t++)
