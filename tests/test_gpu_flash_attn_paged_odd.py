@@ -79,3 +79,31 @@ def test_keys(be, nq, H, Hkv, D, ctype):
         at(1, 20)[:, 1], at(1, 20)[:, 2] = -INF, INF
         at(2, 60)[:, 3] = NAN
     expect(be, [(nq, 200), (nq, 90), (nq, 70)], H, Hkv, D, ctype, both)
+
+
+# sizes where several rows at different positions share a workgroup of up to 16
+
+@pytest.mark.parametrize("nq", [2, 3, 4])
+@pytest.mark.parametrize("what", [INF, NAN])
+def test_few_rows_and_what_they_do_not_see(be, nq, what):
+    import test_gpu_flash_attn_paged as A
+    A.test_what_unseen_places_hold(be, nq, what)
+
+
+@pytest.mark.parametrize("n_shared", [0, 32])
+@pytest.mark.parametrize("nq", [3, 8])
+def test_few_rows_and_missing_pages(be, nq, n_shared):
+    import test_gpu_flash_attn_paged as A
+    A.test_bad_pages_give_nan(be, nq, n_shared)
+
+
+@pytest.mark.parametrize("ctype", ["f16", "bf16"])
+@pytest.mark.parametrize("H,Hkv,D,nq", [(4, 2, 64, 8), (3, 1, 96, 5), (8, 2, 128, 4), (2, 2, 256, 16), (1, 1, 8, 3)])
+def test_few_rows_and_later_values(be, H, Hkv, D, nq, ctype):
+    """Values of the last keys, which only some of the rows see."""
+    def put(at, q):
+        for i, x in enumerate((INF, -INF, NAN)):
+            at(0, 100 - nq + 1 + i % (nq - 1))[:, D + i] = x
+            at(1, 200 - 1 - i % nq)[:, D + 3 + i] = x
+    expect(be, [(nq, 100), (nq, 200)], H, Hkv, D, ctype, put)
+    expect(be, [(nq, 100), (nq, 200)], H, Hkv, D, ctype, put, window=50, n_first=3)

@@ -254,3 +254,40 @@ def test_one_token_of_strided_tables(be):
     assert not kv.any() and int(wide[0]) == 24  # (past the 16 slots of this cache)
     be.kv_append(x, x, torch.arange(32, device="cuda")[8:16:8], kv, pos=pos, rope=r)
     assert torch.equal(kv, kv2) and kv2.any()
+
+
+@pytest.mark.parametrize("dtype,ctype", [("f32", "f16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("T,Hkv,D,page", [(9, 2, 80, 16), (600, 4, 128, 24), (5, 3, 36, 1)])
+def test_append_of_patches(be, T, Hkv, D, page, dtype, ctype):
+    append(be, T, Hkv, D, D // 2, "vision", dtype, ctype, page, T // page + 3)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("D", [64, 80, 36])
+def test_rows_at_odd_elements(be, D, dtype):
+    """16-bit rows whose addresses are no multiples of 4 bytes, read and written by vectors."""
+    import ghip
+    g = torch.Generator().manual_seed(7)
+    w = torch.randn((300, 6, D + 3), generator=g).to(TYPES[dtype])
+    pos = _positions(300, 1, 70, g)
+    r = ghip.Rope(D, ghip.ROPE_NEOX)
+    for T, at in ((3, 1), (300, 3)):
+        x = w[:T, :, at:at + D]
+        want, mag = P.rope(x, pos[:, :T], "neox", D, 10000.0)
+        out = torch.full((T, 6, D + 5), 7.0, dtype=TYPES[dtype], device="cuda")
+        be.rope(w.cuda()[:T, :, at:at + D], pos[0, :T].cuda(), r, out=out[:, :, 3:3 + D])
+        got = out.cpu()
+        assert ((got[:, :, 3:3 + D].double() - want).abs() <= _tol(want, mag, TYPES[dtype])).all()
+        got[:, :, 3:3 + D] = 7.0
+        assert (got == 7.0).all()
+
+
+@pytest.mark.parametrize("fast,slow", [(8.0, 0.25), (64.0, 4.0), (1.0, 1.0)])
+def test_context_extension_between_other_wavelengths(be, fast, slow):
+    import ghip
+    g = torch.Generator().manual_seed(5)
+    x, pos = torch.randn((20, 3, 128), generator=g), _positions(20, 1, 30000, g)
+    want, mag = P.rope(x, pos, "neox", 128, 1e4, scale=0.25, ext=1.0, n_ctx=8192, fast=fast, slow=slow)
+    r = ghip.Rope(128, ghip.ROPE_NEOX, freq_scale=0.25, ext_factor=1.0, n_ctx_orig=8192, beta_fast=fast, beta_slow=slow)
+    got = be.rope(x.cuda(), pos[0].cuda(), r).cpu()
+    assert ((got.double() - want).abs() <= _tol(want, mag, torch.float32)).all()
