@@ -1194,7 +1194,7 @@ DEV void fap_tile(const FapParams &p, TileLds<DP, RW> &lds) {
 template <typename E>
 DEV void fap_join(const FapParams &p) {
     const int lane = threadIdx.x & 63;
-    const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int64_t id = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int h = (int)(id % p.H);
     const int64_t x = id / p.H;  // sequence b, row i as b max_q + i, or the row's number among all sequences' rows
     int b, i;
