@@ -337,10 +337,10 @@ typedef struct ghip_paged_params {
  * with j > p - window or j < n_first.  A row that sees nothing gives 0; rows of
  * q that no sequence names are not written, and no row is named by two.  n_shared
  * > 0 says that the first n_shared keys of every sequence that has rows hold the
- * same values: they are read through the pages of the first such sequence, once
- * for the batch, or, where that costs more than it saves, through each sequence's
- * own (all hold page numbers for them).  A sequence without rows (nq 0: an idle
- * slot) may hold anything else.
+ * same values (of a shorter one: as many as it has).  They are read through the
+ * pages of the first such sequence that has all of them, once for the batch, or,
+ * where that costs more than it saves, through each sequence's own.  A sequence
+ * without rows (nq 0: an idle slot) may hold anything.
  * Pages of keys that no row sees are not looked at, and what the cache holds
  * there, NaN included, does not matter.  A row that sees a key on a page outside
  * [0, pages), or past its table row, gives NaN.  Rows past max_q are not

@@ -890,15 +890,25 @@ DEV PagedSeq seq_of(const FapParams &p, int b) {
     const int32_t *row = p.seqs + (int64_t)b * p.seq_nb1;
     return paged_seq(row[0], row[1], row[2], p.T, p.max_q);
 }
-// the first sequence that has rows (idle ones need not hold the prefix's pages); 0: none has
-DEV int first_live(const FapParams &p) {
-    if (seq_of(p, 0).nq) return 0;
+// The sequence whose pages hold the shared prefix: the first one with rows (idle ones
+// may hold anything) and all of its keys, else the one with the most of them.
+DEV int prefix_of(const FapParams &p) {
+    if (seq_of(p, 0).nq && p.seqs[2] >= p.n_shared) return 0;
     const int lane = threadIdx.x & 63;
-    for (int b0 = 0; b0 < p.B; b0 += 64) {
-        const uint64_t live = __ballot(b0 + lane < p.B && seq_of(p, b0 + lane).nq);
-        if (live) return b0 + __builtin_ctzll(live);
+    int best = 0, most = -1;
+    for (int b0 = 0; b0 < p.B && most < p.n_shared; b0 += 64) {
+        int n = -1;
+        if (b0 + lane < p.B && seq_of(p, b0 + lane).nq) n = min(p.seqs[(b0 + lane) * p.seq_nb1 + 2], p.n_shared);
+        int mx = n;
+#pragma unroll
+        for (int o = 32; o; o >>= 1) mx = max(mx, __shfl_xor(mx, o, 64));
+        mx = __builtin_amdgcn_readfirstlane(mx);
+        if (mx > most) {
+            most = mx;
+            best = b0 + __builtin_ctzll(__ballot(n == mx));
+        }
     }
-    return 0;
+    return best;
 }
 
 template <int DP, int RW>
@@ -922,11 +932,11 @@ DEV void fap_tile(const FapParams &p, TileLds<DP, RW> &lds) {
     const bool shared = (int)blockIdx.x < p.wg_sh;
     const int id = shared ? blockIdx.x : blockIdx.x - p.wg_sh, nz = shared ? p.zs_sh : p.zs_own;
     const int hk = id % p.H_kv, z = (id / p.H_kv) % nz, blk = id / (p.H_kv * nz);
-    const int32_t *row;  // the pages: for the shared prefix those of the first sequence with rows
+    const int32_t *row;  // the pages: for the shared prefix those of the sequence that prefix_of finds
     int x0, r0;  // first token of the list, first row of the block (rows of token x0 + k: G (x0 + k) ..)
     if (shared) {
         // tokens x0 .. of all sequences in order
-        row = p.seqs + first_live(p) * p.seq_nb1;
+        row = p.seqs + prefix_of(p) * p.seq_nb1;
         r0 = blk * R;
         x0 = r0 / G;
         const int nx = (r0 + R - 1) / G - x0 + 1;

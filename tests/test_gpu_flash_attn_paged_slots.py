@@ -83,3 +83,16 @@ def test_cache_without_pages(be, rows):
             torch.cuda.synchronize()
             first = rows + rows - rows // 2
             assert torch.isnan(got[:rows]).all() and torch.isnan(got[first:]).all() and (got[rows:first] == 0).all()
+
+
+@pytest.mark.parametrize("rows", [1, 3])
+def test_first_sequence_ends_inside_the_prefix(be, rows):
+    """A sequence that is shorter than the prefix holds pages for its own keys alone: the
+    prefix is read through one that has all of it."""
+    def zeros(table):  # (what a table that is cleared at first holds there)
+        table[:, 3:][table[:, 3:] < 0] = 0
+
+    for change in (None, zeros):
+        check(be, [(rows, 30), (rows, 100), (rows, 150), (rows, 97)], 16, 4, 64, "f16", 96, change)
+        check(be, [(0, 200), (rows, 30)] + [(rows, 100 + b) for b in range(80)], 8, 2, 64, "bf16", 96, change)
+        check(be, [(rows, 30), (rows, 64), (rows, 95)], 16, 4, 64, "f16", 96, change)
