@@ -341,6 +341,8 @@ typedef struct ghip_paged_params {
  * pages of the first such sequence that has all of them, once for the batch, or,
  * where that costs more than it saves, through each sequence's own.  A sequence
  * without rows (nq 0: an idle slot) may hold anything.
+ * How keys are split and whether a prefix is read once goes by what a table row has
+ * room for: a row much wider than the keys costs up to a fifth of the time.
  * Pages of keys that no row sees are not looked at, and what the cache holds
  * there, NaN included, does not matter.  A row that sees a key on a page outside
  * [0, pages), or past its table row, gives NaN.  Rows past max_q are not

@@ -8,14 +8,16 @@
 // Key j is row j % page of page table[j / page]; a row that sees a key whose
 // page does not exist gives NaN.
 //
-// Both kernels walk the keys once with a running maximum and sum, on the matrix
+// Both kernels walk the keys once with a running reference and sum, on the matrix
 // cores (v_mfma_f32_16x16x32): S^T = K Q^T leaves a query row in 4 lanes (n, n +
 // 16, n + 32, n + 48), whose scores are the B operand of O^T += V^T P^T as they
 // are.  q is 32-bit and the output too, so q and p are split into terms of the
-// cache's type that add up to them (f16: 2 terms, 22 bits of what is first brought into
-// its range; bf16: 3 terms, 24 bits), each a product of its own on the same K or V fragment; sums are 32-bit.  With one
-// term fewer the error against 64 bits is 2e-6 (bf16, p: 2 terms; 2.5e-6 with 2
-// of q) where 32-bit arithmetic has 0.7e-6 and these terms 0.3e-6 to 0.5e-6.
+// cache's type that add up to them (bf16: 3 terms, 24 bits; f16: 2 terms, 22 bits of
+// what is brought into its range first, a row's q by a power of two, p by where the
+// reference is), each a product of its own on the same K or V fragment; sums are
+// 32-bit.  With one term fewer the error against 64 bits is 2e-6 (bf16, p: 2 terms;
+// 2.5e-6 with 2 of q) where 32-bit arithmetic has 0.7e-6 and these terms 0.3e-6 to
+// 0.5e-6.
 //
 //  * ghip_fap_few: up to 16 rows of a KV head (generation: the G = H / H_kv query
 //    heads that share it, times a few rows).  Bound by reading K and V once: each
@@ -53,17 +55,17 @@ template <> struct Frag<f16> {
     typedef __fp16 tr __attribute__((__vector_size__(8)));
     static constexpr int NQ = 2, NP = 2;         // terms of q and of p
     // Where p is held: 2^HOME at a tile's largest key when the reference moves, below
-    // 2^TOP from then on (moves are 8 apart: with 3 the rescaling of o made 1702 rows
-    // over 2048 keys 138 us, now 123).  Terms of f16 end at 2^-24 however many they
-    // are, so a p of 2^-5 has 20 bits and smaller ones have less: the reference follows
-    // tiles down whose largest p is below 2^LOW, and where it moves, a tile's keys from
-    // 2^REST on take a pass before those below.
+    // 2^TOP from then on (8 apart: with 3 the rescaling of o makes 1702 rows over 2048
+    // keys 132 us instead of 125).  Terms of f16 end at 2^-24 however many they are, so a p
+    // of 2^-5 has 20 bits and smaller ones have less: the reference follows tiles down
+    // whose largest p is below 2^LOW, and where it moves, a tile's keys from 2^REST on take
+    // a pass before those below (one: behind two such gaps in one tile bits are lost).
     static constexpr float HOME = 8.0f, TOP = 15.9f, LOW = -2.0f, REST = -5.0f;
     static constexpr bool FOLLOW = true;
     // A row's q is held 2^k times, its largest from 2^14 to 2^15, and the scores lose that
     // again: small elements against large keys keep their bits, and none overflows (q of
     // 1e-2 against keys of 100: error 1.0e-5 without, 2.2e-7; one more operation a score,
-    // 1702 rows over 2048 keys 125 -> 128 us).
+    // 1702 rows over 2048 keys 122 us without, 125).
     static constexpr bool SCALED = true;
     typedef float ref;
     static __device__ __forceinline__ v4f mfma(v8 a, v8 b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
@@ -178,8 +180,8 @@ struct Rows {
     typename F::ref mneg[RW];
     float unit[RW]; // what a score counts, 2^-k
     // four registers of 0, where they are to spare: a constant is written out for every
-    // product (3 prompts of 16 heads of 64 42.8 us, 39.6; 128 rows of 128 dims, which then
-    // spill one, 124 and 127)
+    // product (3 of 43 us, 3 prompts of 16 heads of 64; 128 rows of 128 dims would spill one
+    // register for it, 3 of 127 us)
     v4f zero;
     DEV_M v4f start(int rt) const {
         if constexpr (!F::SCALED) return mneg[rt];
@@ -569,8 +571,8 @@ DEV void stat_none(const FapParams &p, int64_t pi, bool nan) {
 // 32 bits and with the keys that it sees alone: a lane a key for the scores, first their
 // maximum, then p and its products with the values, lane l the dims 4 l ... A wavefront
 // a row, and hardly ever one: 12 us for 64 keys (512 rows of 32 heads over 2048 keys that
-// all see an infinite value: 3.4 ms, 60 us where it is finite); it ends at a score
-// of NaN (94 us).
+// all see an infinite value: 2.6 ms, 58 us where it is finite); it ends at a score of
+// NaN (77 us).
 template <typename E>
 DEV v4f row_again(const FapParams &p, const int32_t *table, int64_t tok, int h, int64_t pos) {
     const int lane = threadIdx.x & 63;
