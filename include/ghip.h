@@ -81,6 +81,11 @@ enum {
     GHIP_TYPE_NVFP4 = 40,
     GHIP_TYPE_Q1_0 = 41,
     GHIP_TYPE_Q2_0 = 42,
+    /* codes of a quantized KV cache and the scales of their blocks: this backend's own
+     * ids, ggml has none for them */
+    GHIP_TYPE_E4M3 = 256,
+    GHIP_TYPE_E2M1 = 257, /* two to a byte, the first in the low bits */
+    GHIP_TYPE_E8M0 = 258, /* 2^(byte - 127); 255: NaN */
 };
 
 /* The ops of the hot path (GgmlOp::MulMat / MulMatId / FlashAttnExt,
@@ -316,6 +321,35 @@ ghip_status ghip_rope(ghip_context *ctx, const ghip_tensor *x, const ghip_tensor
 ghip_status ghip_kv_append(ghip_context *ctx, const ghip_tensor *k, const ghip_tensor *v, const ghip_tensor *slots,
                            const ghip_tensor *pos, const ghip_tensor *factors, const ghip_rope_params *rope,
                            const ghip_tensor *kv, void *stream);
+
+/* ---- A quantized KV cache: the paged cache in 8 or 4 bits an element, as two tensors,
+ *   kv:      E4M3 | E2M1 [2 D, H_kv, page, pages] (nb0 == 1; nb1 .. nb3 in bytes), D a
+ *            multiple of 16 up to 256, data and strides multiples of 16 bytes
+ *   scales:  E8M0 [2 S, H_kv, page, pages] (nb0 == 1), data and strides multiples of 2 S
+ * For each slot and KV head scales hold a byte for every 32 elements of the key, in S
+ * bytes, then of the value; S is D / 32 rounded up to 1, 2, 4 or 8.  An element is
+ * its code times 2^(byte - 127); below 2^-126 it may count as 0.  A block with byte 255 is NaN.
+ *
+ * Writing a block takes the least power of two from 2^-100 on that brings its largest
+ * element to at most 448 (E4M3) or 7 (E2M1: what is over 6 becomes 6) and rounds each
+ * element once, to the nearest code, ties to the even one.  A block with an infinity or
+ * NaN is NaN.  Scale bytes that D leaves over are written as of a block of zeros, 27. */
+
+/* ghip_kv_append into a quantized cache: the same tokens, slots and rotation; k, v:
+ * F32 | F16 | BF16, the same type, [D, H_kv, T].  The rotation is formed in 64 bits, so that
+ * a code is its rounding, not that of a value in 32 bits.  None of the others may overlap kv
+ * or scales, nor may these overlap. */
+ghip_status ghip_kv_append_mx(ghip_context *ctx, const ghip_tensor *k, const ghip_tensor *v, const ghip_tensor *slots,
+                              const ghip_tensor *pos, const ghip_tensor *factors, const ghip_rope_params *rope,
+                              const ghip_tensor *kv, const ghip_tensor *scales, void *stream);
+
+/* Rows of a quantized cache as floats:
+ *   slots: I64 [T]; for a negative slot (padding) or one outside the cache nothing
+ *          is written
+ *   dst:   F32 | F16 | BF16 [2 D, H_kv, T] (nb0 == the element): token t's key, then its
+ *          value; each element rounded once (F32, and E2M1 to BF16: not at all) */
+ghip_status ghip_kv_read_mx(ghip_context *ctx, const ghip_tensor *kv, const ghip_tensor *scales, const ghip_tensor *slots,
+                            const ghip_tensor *dst, void *stream);
 
 typedef struct ghip_paged_params {
     float scale;      /* of q . k */

@@ -21,7 +21,7 @@
 
 namespace {
 
-const char *const kModules[] = {"ghip_quant.hsaco", "ghip_kq.hsaco", "ghip_gemv.hsaco", "ghip_wquant.hsaco", "ghip_gemm.hsaco", "ghip_fa.hsaco", "ghip_moe.hsaco", "ghip_skinny.hsaco", "ghip_iq.hsaco", "ghip_dense.hsaco", "ghip_rope.hsaco", "ghip_fap.hsaco"};
+const char *const kModules[] = {"ghip_quant.hsaco", "ghip_kq.hsaco", "ghip_gemv.hsaco", "ghip_wquant.hsaco", "ghip_gemm.hsaco", "ghip_fa.hsaco", "ghip_moe.hsaco", "ghip_skinny.hsaco", "ghip_iq.hsaco", "ghip_dense.hsaco", "ghip_rope.hsaco", "ghip_fap.hsaco", "ghip_kvq.hsaco"};
 
 struct TypeInfo {
     int blck;
@@ -60,6 +60,9 @@ TypeInfo type_info(int t) {
     case GHIP_TYPE_NVFP4: return {64, 36};
     case GHIP_TYPE_Q1_0: return {128, 18};
     case GHIP_TYPE_Q2_0: return {64, 18};
+    case GHIP_TYPE_E4M3: return {1, 1};
+    case GHIP_TYPE_E2M1: return {2, 1};
+    case GHIP_TYPE_E8M0: return {1, 1};
     default: return {0, 0};
     }
 }
@@ -3293,6 +3296,210 @@ ghip_status ghip_kv_append(ghip_context *ctx, const ghip_tensor *k, const ghip_t
     snprintf(name, sizeof name, "ghip_append_%s_%s_%s_v%d_h%d", float_name(k->type), float_name(kv->type),
              rope && rope->mode != GHIP_ROPE_NORM ? "half" : "norm", r.vec, r.hn);
     return ctx->launch(name, dim3(r.grid), dim3(256), 0, s, p);
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------ a quantized KV cache
+
+namespace {
+
+// Mirrors of the kernels' argument structs in ghip_kvq.hip.
+struct MxRows {
+    uint8_t *kv, *sc;
+    int64_t kv_head, kv_row, kv_page, sc_head, sc_row, sc_page;
+    int64_t n_slots;
+    uint32_t page;
+    int small;
+    PagedDiv by_page;
+};
+struct AppendMxParams {
+    const void *k, *v;
+    int64_t k_nb1, k_nb2, v_nb1, v_nb2;
+    MxRows to;
+    const int64_t *slots;
+    const int32_t *pos;
+    int64_t pos_nb1;
+    const float *factors;
+    int T, H, D, P;
+    int S, HG;
+    RopeTab tab;
+};
+struct ReadMxParams {
+    MxRows from;
+    const int64_t *slots;
+    void *dst;
+    int64_t d_nb1, d_nb2;
+    int T, H, D, S;
+    int U;
+    uint32_t step;
+};
+
+bool mx_type(int t) { return t == GHIP_TYPE_E4M3 || t == GHIP_TYPE_E2M1; }
+int mx_bits(const ghip_tensor *kv) { return kv->type == GHIP_TYPE_E4M3 ? 8 : 4; }
+// scale bytes of a key (or value) of D elements
+int mx_scale_bytes(int64_t D) { return D <= 32 ? 1 : D <= 64 ? 2 : D <= 128 ? 4 : 8; }
+// A quantized cache of heads of D elements: the reason it is refused, or null.
+const char *mx_cache(const ghip_tensor *kv, const ghip_tensor *sc, int64_t D) {
+    if (!mx_type(kv->type)) return "kv must be E4M3 or E2M1";
+    if (D < 16 || D > 256 || D % 16) return "head size must be a multiple of 16, 16..256";
+    if (!packed(kv, 1) || kv->ne[0] != 2 * D || kv->ne[1] < 1 || kv->ne[2] < 1 || kv->ne[3] < 0)
+        return "kv must be [2 D, H_kv, page, pages]";
+    if (kv->ne[1] > INT32_MAX || kv->ne[2] > INT32_MAX || kv->ne[3] > INT32_MAX) return "dimension too large";
+    if (!in_steps(kv, 1, 16) || (uintptr_t)kv->data % 16) return "kv and its strides must be multiples of 16 bytes";
+    const int S = mx_scale_bytes(D);
+    if (sc->type != GHIP_TYPE_E8M0) return "scales must be E8M0";
+    if (!packed(sc, 1) || sc->ne[0] != 2 * S || sc->ne[1] != kv->ne[1] || sc->ne[2] != kv->ne[2] || sc->ne[3] != kv->ne[3])
+        return "scales must be [2 S, H_kv, page, pages], S = 1, 2, 4 or 8 for heads of up to 32, 64, 128 or 256";
+    if (!in_steps(sc, 1, 2 * S) || (uintptr_t)sc->data % (2 * S)) return "scales and their strides must be multiples of 2 S bytes";
+    if (kv->ne[3] && (!kv->data || !sc->data)) return "null data";
+    return nullptr;
+}
+MxRows mx_rows(const ghip_tensor *kv, const ghip_tensor *sc) {
+    MxRows m;
+    m.kv = (uint8_t *)kv->data;
+    m.sc = (uint8_t *)sc->data;
+    m.kv_head = (int64_t)kv->nb[1];
+    m.kv_row = (int64_t)kv->nb[2];
+    m.kv_page = (int64_t)kv->nb[3];
+    m.sc_head = (int64_t)sc->nb[1];
+    m.sc_row = (int64_t)sc->nb[2];
+    m.sc_page = (int64_t)sc->nb[3];
+    m.n_slots = kv->ne[2] * kv->ne[3];
+    m.page = m.kv_page == m.kv_row * kv->ne[2] && m.sc_page == m.sc_row * kv->ne[2] ? 0 : (uint32_t)kv->ne[2];
+    m.small = m.n_slots <= UINT32_MAX;
+    m.by_page = paged_divisor((uint32_t)kv->ne[2]);
+    return m;
+}
+
+}  // namespace
+
+extern "C" {
+
+ghip_status ghip_kv_append_mx(ghip_context *ctx, const ghip_tensor *k, const ghip_tensor *v, const ghip_tensor *slots,
+                              const ghip_tensor *pos, const ghip_tensor *factors, const ghip_rope_params *rope,
+                              const ghip_tensor *kv, const ghip_tensor *scales, void *stream) {
+    if (!ctx) return GHIP_STATUS_BACKEND_ERROR;
+    std::lock_guard<std::mutex> lock(ctx->mu);
+    auto bad = [&](const char *why) { return ctx->fail(GHIP_STATUS_BACKEND_ERROR, "kv_append_mx: %s", why); };
+    if (!k || !v || !slots || !kv || !scales) return bad("null operand");
+    if (!float_type(k->type) || v->type != k->type) return bad("k and v must be F32, F16 or BF16, of one type");
+    const uint64_t e = type_info(k->type).bytes;
+    if (!elem_rows(k, e) || !elem_rows(v, e)) return bad("k and v must be rows of elements");
+    for (int d = 0; d < 4; d++)
+        if (k->ne[d] != v->ne[d] || k->ne[d] < 0) return bad("k and v must have the same shape");
+    if (k->ne[3] != 1) return bad("k and v must be [D, H_kv, T]");
+    const int64_t D = k->ne[0], H = k->ne[1], T = k->ne[2];
+    if (const char *why = mx_cache(kv, scales, D)) return bad(why);
+    if (kv->ne[1] != H) return bad("kv must be [2 D, H_kv, page, pages]");
+    if (T > INT32_MAX) return bad("dimension too large");
+    if (slots->type != GHIP_TYPE_I64 || !packed(slots, 8) || slots->ne[0] < T) return bad("slots must be I64, one for each token");
+    AppendMxParams p;
+    p.P = 0;
+    p.pos = nullptr;
+    p.pos_nb1 = 0;
+    p.factors = nullptr;
+    if (rope) {
+        int axes;
+        if (const char *why = rope_table(*rope, D, factors != nullptr, p.tab, p.P, axes)) return bad(why);
+        if (const char *why = rope_operands(pos, factors, T, p.P, axes)) return bad(why);
+        p.pos = (const int32_t *)pos->data;
+        p.pos_nb1 = (int64_t)(pos->nb[1] / 4);
+        p.factors = factors ? (const float *)factors->data : nullptr;
+    } else if (pos || factors) {
+        return bad("pos and factors need a rotation");
+    }
+    if (T == 0) return GHIP_STATUS_SUCCESS;
+    if (!k->data || !v->data || !slots->data || (rope && !pos->data) || (factors && !factors->data)) return bad("null data");
+    if (kv->ne[3]) {
+        for (const ghip_tensor *t : {k, v, slots, pos, factors})
+            if (overlaps(t, kv) || overlaps(t, scales)) return bad("k, v, slots, pos and factors must lie apart from kv and scales");
+        if (overlaps(kv, scales)) return bad("kv and scales must lie apart");
+    }
+    p.S = mx_scale_bytes(D);
+    // Four heads a thread share their angles, where that leaves enough threads to cover the
+    // loads' latency.
+    const int hn = T * ((H + 3) / 4) * 4 * p.S >= 256 * 4 * 64 ? 4 : 1;
+    p.HG = (int)((H + hn - 1) / hn);
+    const int64_t n = T * p.HG * 4 * p.S;
+    if (n >= (1ll << 32) - 256) return bad("k too large");
+    hipStream_t s = (hipStream_t)stream;
+    if (!ctx->set_device()) return ctx->fail(GHIP_STATUS_BACKEND_ERROR, "hipSetDevice failed");
+    ghip_status st = ctx->begin(s);
+    if (st != GHIP_STATUS_SUCCESS) return st;
+    p.k = k->data;
+    p.v = v->data;
+    p.k_nb1 = (int64_t)(k->nb[1] / e);
+    p.k_nb2 = (int64_t)(k->nb[2] / e);
+    p.v_nb1 = (int64_t)(v->nb[1] / e);
+    p.v_nb2 = (int64_t)(v->nb[2] / e);
+    p.to = mx_rows(kv, scales);
+    p.slots = (const int64_t *)slots->data;
+    p.T = (int)T;
+    p.H = (int)H;
+    p.D = (int)D;
+    uintptr_t lo, hi;
+    byte_span(kv, lo, hi);
+    ctx->allow(kv->data, hi - lo, "kv");
+    byte_span(scales, lo, hi);
+    ctx->allow(scales->data, hi - lo, "scales");
+    if (p.to.n_slots) {
+        const MxRows &m = p.to;
+        ctx->expect(m.kv, (size_t)((kv->ne[3] - 1) * m.kv_page + (kv->ne[2] - 1) * m.kv_row + (H - 1) * m.kv_head + 2 * D * mx_bits(kv) / 8), "kv");
+        ctx->expect(m.sc, (size_t)((kv->ne[3] - 1) * m.sc_page + (kv->ne[2] - 1) * m.sc_row + (H - 1) * m.sc_head + 2 * p.S), "scales");
+    }
+    const char *mode = !rope || rope->mode == GHIP_ROPE_NORM ? "norm" : p.P % 8 ? "odd" : "half";
+    char name[64];
+    snprintf(name, sizeof name, "ghip_append_mx%d_%s_%s_h%d", mx_bits(kv), float_name(k->type), mode, hn);
+    return ctx->launch(name, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, p);
+}
+
+ghip_status ghip_kv_read_mx(ghip_context *ctx, const ghip_tensor *kv, const ghip_tensor *scales, const ghip_tensor *slots,
+                            const ghip_tensor *dst, void *stream) {
+    if (!ctx) return GHIP_STATUS_BACKEND_ERROR;
+    std::lock_guard<std::mutex> lock(ctx->mu);
+    auto bad = [&](const char *why) { return ctx->fail(GHIP_STATUS_BACKEND_ERROR, "kv_read_mx: %s", why); };
+    if (!kv || !scales || !slots || !dst) return bad("null operand");
+    if (!float_type(dst->type)) return bad("dst must be F32, F16 or BF16");
+    const uint64_t e = type_info(dst->type).bytes;
+    if (!elem_rows(dst, e)) return bad("dst must be rows of elements");
+    for (int d = 0; d < 4; d++)
+        if (dst->ne[d] < 0) return bad("dst must be [2 D, H_kv, T]");
+    const int64_t D = dst->ne[0] / 2, H = dst->ne[1], T = dst->ne[2];
+    if (dst->ne[0] % 2 || dst->ne[3] != 1) return bad("dst must be [2 D, H_kv, T]");
+    if (const char *why = mx_cache(kv, scales, D)) return bad(why);
+    if (kv->ne[1] != H) return bad("kv must be [2 D, H_kv, page, pages]");
+    if (T > INT32_MAX || T * H > INT32_MAX) return bad("dimension too large");
+    if (slots->type != GHIP_TYPE_I64 || !packed(slots, 8) || slots->ne[0] < T) return bad("slots must be I64, one for each token");
+    if (T == 0 || kv->ne[3] == 0) return GHIP_STATUS_SUCCESS;
+    if (!slots->data || !dst->data) return bad("null data");
+    if (overlaps(kv, dst) || overlaps(scales, dst) || overlaps(slots, dst)) return bad("dst must lie apart from kv, scales and slots");
+    ReadMxParams p;
+    p.U = (int)(2 * D * (int64_t)e / 16);
+    const int64_t rows = T * H;
+    // Four rows a thread, all their loads in flight, where that leaves enough threads.
+    const int rn = rows * p.U >= 4 * 256 * 8 * 64 ? 4 : 1;
+    p.step = (uint32_t)((rows + rn - 1) / rn);
+    const int64_t n = (int64_t)p.step * p.U;
+    if (n >= (1ll << 32) - 256) return bad("dst too large");
+    hipStream_t s = (hipStream_t)stream;
+    if (!ctx->set_device()) return ctx->fail(GHIP_STATUS_BACKEND_ERROR, "hipSetDevice failed");
+    ghip_status st = ctx->begin(s);
+    if (st != GHIP_STATUS_SUCCESS) return st;
+    p.from = mx_rows(kv, scales);
+    p.slots = (const int64_t *)slots->data;
+    p.dst = dst->data;
+    p.d_nb1 = (int64_t)(dst->nb[1] / e);
+    p.d_nb2 = (int64_t)(dst->nb[2] / e);
+    p.T = (int)T;
+    p.H = (int)H;
+    p.D = (int)D;
+    p.S = mx_scale_bytes(D);
+    ctx->allow(dst->data, byte_extent(dst, e), "dst");
+    ctx->expect(p.dst, (size_t)(((T - 1) * p.d_nb2 + (H - 1) * p.d_nb1 + 2 * D) * (int64_t)e), "dst");
+    char name[64];
+    snprintf(name, sizeof name, "ghip_read_mx%d_%s_r%d", mx_bits(kv), float_name(dst->type), rn);
+    return ctx->launch(name, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, p);
 }
 
 }  // extern "C"

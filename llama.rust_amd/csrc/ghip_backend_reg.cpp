@@ -103,6 +103,8 @@ void *reg_proc_address(const ggml_hip_backend_reg *, const char *name) {
         {"ghip_flash_attn_ext", (void *)&ghip_flash_attn_ext},
         {"ghip_rope", (void *)&ghip_rope},
         {"ghip_kv_append", (void *)&ghip_kv_append},
+        {"ghip_kv_append_mx", (void *)&ghip_kv_append_mx},
+        {"ghip_kv_read_mx", (void *)&ghip_kv_read_mx},
         {"ghip_flash_attn_paged", (void *)&ghip_flash_attn_paged},
         {"ghip_flash_attn_paged_workspace", (void *)&ghip_flash_attn_paged_workspace},
         {"ghip_quantize_chunk", (void *)&ghip_quantize_chunk},

@@ -21,6 +21,7 @@ Q1_0, Q2_0 = 41, 42
 BF16 = 30
 I64 = 27
 IQ2_XXS, IQ2_XS, IQ3_XXS, IQ1_S, IQ3_S, IQ2_S, IQ1_M = 16, 17, 18, 19, 21, 22, 29
+E4M3, E2M1, E8M0 = 256, 257, 258
 ROPE_NORM, ROPE_NEOX, ROPE_MROPE, ROPE_VISION, ROPE_IMROPE = 0, 2, 8, 24, 40
 OP_MUL_MAT, OP_MUL_MAT_ID, OP_FLASH_ATTN_EXT = 1, 2, 3
 BLOCK = {Q4_0: (32, 18), Q5_0: (32, 22), Q8_0: (32, 34), Q4_K: (256, 144), Q5_K: (256, 176), Q6_K: (256, 210),
@@ -195,6 +196,41 @@ def _view(t):
     raise GhipError(f"tensors of {n} dimensions are not supported")
 
 
+# the dtypes of a quantized cache: its codes (two 4-bit ones to a byte) and their scales
+_CODES = {torch.float8_e4m3fn: (E4M3, 1), torch.uint8: (E2M1, 2)}
+_SCALES = frozenset((torch.uint8, torch.float8_e8m0fnu))
+
+
+def _view_mx(kv, scales):
+    """The bytes of describe() of a quantized cache's codes and scales."""
+    ty = _CODES.get(kv.dtype)
+    if ty is None:
+        raise GhipError(f"dtype {kv.dtype} not supported beside scales (codes are float8_e4m3fn, or uint8 of two 4-bit ones)")
+    if scales.dtype not in _SCALES:
+        raise GhipError("scales must be uint8 or float8_e8m0fnu")
+    if not kv.is_cuda or not scales.is_cuda:
+        raise GhipError("tensors must be on the GPU")
+    if kv.dim() != 4 or scales.dim() != 4:
+        raise GhipError("kv must be [pages, page, H_kv, 2 D] (4 bits: D bytes) and scales [pages, page, H_kv, 2 S]")
+    (a3, a2, a1, a0), (s3, s2, s1, s0) = kv.shape, kv.stride()
+    (b3, b2, b1, b0), (t3, t2, t1, t0) = scales.shape, scales.stride()
+    return (_PACK(ty[0], ty[1] * a0, a1, a2, a3, s0, s1, s2, s3, kv.data_ptr()),
+            _PACK(E8M0, b0, b1, b2, b3, t0, t1, t2, t3, scales.data_ptr()))
+
+
+def mx_cache(pages, page, n_kv, head, bits=8, device="cuda"):
+    """An empty quantized KV cache -> (codes, scales) for kv_append, kv_read and
+    flash_attn_paged."""
+    if bits not in (4, 8):
+        raise GhipError("a quantized cache has 4 or 8 bits")
+    S = 1
+    while 32 * S < head:
+        S *= 2
+    kv = torch.zeros((pages, page, n_kv, 2 * head * bits // 8), dtype=torch.uint8, device=device)
+    return (kv.view(torch.float8_e4m3fn) if bits == 8 else kv,
+            torch.full((pages, page, n_kv, 2 * S), 27, dtype=torch.uint8, device=device))
+
+
 _lib = None
 
 
@@ -248,6 +284,10 @@ def lib():
         L.ghip_rope.argtypes = [V, V, V, V, R, V, V]
         L.ghip_kv_append.restype = C.c_int
         L.ghip_kv_append.argtypes = [V, V, V, V, V, V, R, V, V]
+        L.ghip_kv_append_mx.restype = C.c_int
+        L.ghip_kv_append_mx.argtypes = [V, V, V, V, V, V, R, V, V, V]
+        L.ghip_kv_read_mx.restype = C.c_int
+        L.ghip_kv_read_mx.argtypes = [V, V, V, V, V, V]
         L.ghip_flash_attn_paged.restype = C.c_int
         L.ghip_flash_attn_paged.argtypes = [V, V, V, V, V, V, V, V]
         L.ghip_flash_attn_paged_workspace.restype = C.c_int
@@ -413,14 +453,36 @@ class Backend:
             self._check(st, "ghip_rope")
         return out
 
-    def kv_append(self, k, v, slots, kv, pos=None, rope=None, factors=None):
+    def kv_append(self, k, v, slots, kv, pos=None, rope=None, factors=None, scales=None):
         """Write k / v [T, H_kv, D] (f32 or kv's type) into rows `slots` [T] int64
-        (negative: skipped) of kv [pages, page, H_kv, 2 D], k rotated by `rope`."""
+        (negative: skipped) of kv [pages, page, H_kv, 2 D], k rotated by `rope`.
+        With scales [pages, page, H_kv, 2 S] uint8 the cache is a quantized one (mx_cache):
+        kv float8_e4m3fn, or uint8 [pages, page, H_kv, D] of 4-bit codes; k / v f32, f16 or bf16."""
+        if scales is not None:
+            codes, sc = _view_mx(kv, scales)
+            st = lib().ghip_kv_append_mx(self._ctx, _view(k), _view(v), _view(slots), _view(pos), _view(factors),
+                                         rope._ref if rope is not None else None, codes, sc, _raw_stream(self.device))
+            if st:
+                self._check(st, "ghip_kv_append_mx")
+            return kv
         st = lib().ghip_kv_append(self._ctx, _view(k), _view(v), _view(slots), _view(pos), _view(factors),
                                   rope._ref if rope is not None else None, _view(kv), _raw_stream(self.device))
         if st:
             self._check(st, "ghip_kv_append")
         return kv
+
+    def kv_read(self, kv, slots, scales, out=None, dtype=torch.float32):
+        """Rows `slots` [T] int64 of a quantized cache (mx_cache) as [T, H_kv, 2 D] f32 /
+        f16 / bf16: key, then value.  Rows of negative slots are left as they are in
+        `out`, 0 where there is none."""
+        codes, sc = _view_mx(kv, scales)
+        if out is None:
+            out = torch.zeros((slots.shape[0], kv.shape[2], kv.shape[3] * (2 if kv.dtype == torch.uint8 else 1)), dtype=dtype,
+                              device=kv.device)
+        st = lib().ghip_kv_read_mx(self._ctx, codes, sc, _view(slots), _view(out), _raw_stream(self.device))
+        if st:
+            self._check(st, "ghip_kv_read_mx")
+        return out
 
     def flash_attn_paged(self, q, kv, seqs, scale=1.0, sinks=None, window=0, n_first=0, n_shared=0, max_q=None, out=None):
         """q [T, H, D] f32 over kv [pages, page, H_kv, 2 D] f16 / bf16; seqs

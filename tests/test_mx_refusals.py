@@ -1,0 +1,138 @@
+"""What the calls on a quantized KV cache refuse, and that what they accept stores
+inside its buffers, on a context without a device."""
+import ctypes as C
+
+import pytest
+
+from test_paged_refusals import A, T, ctx, ref, rope_params  # noqa: F401
+
+
+def codes(ty, ne, data, nb=None):
+    """a tensor of codes: strides in bytes"""
+    import ghip
+    row = ne[0] * (1 if ty == ghip.E4M3 else 0.5)
+    return T(ty, ne, data, 1, nb or [1, int(row), int(row * ne[1]), int(row * ne[1] * ne[2])])
+
+
+def scales_of(D, Hkv, page, pages, data, nb=None):
+    import ghip
+    S = 1 if D <= 32 else 2 if D <= 64 else 4 if D <= 128 else 8
+    return T(ghip.E8M0, [2 * S, Hkv, page, pages], data, 1, nb)
+
+
+def run_append(ctx, D=64, Hkv=2, N=9, kty=0, vty=None, cty=256, page=16, pages=5, slots=None, kv=None, sc=None, v=None, k=None, rope=True,
+               pos=True, factors=None, **kw):
+    import ghip
+    k = T(kty, [D, Hkv, N], A[0]) if k is None else k
+    v = T(kty if vty is None else vty, [D, Hkv, N], A[1]) if v is None else v
+    slots = T(ghip.I64, [N], A[2]) if slots is None else slots
+    kv = codes(cty, [2 * D, Hkv, page, pages], A[3]) if kv is None else kv
+    sc = scales_of(D, Hkv, page, pages, A[5]) if sc is None else sc
+    p = T(ghip.I32, [N], A[4]) if pos is True else pos
+    kw.setdefault("n_dims", min(64, D))
+    r = rope_params(**kw) if rope else None
+    st = ghip.lib().ghip_kv_append_mx(ctx, ref(k), ref(v), ref(slots), ref(p), ref(factors), ref(r), ref(kv), ref(sc), None)
+    return st, ghip.lib().ghip_last_error(ctx).decode()
+
+
+def run_read(ctx, D=64, Hkv=2, N=9, oty=0, cty=256, page=16, pages=5, slots=None, kv=None, sc=None, dst=None):
+    import ghip
+    slots = T(ghip.I64, [N], A[2]) if slots is None else slots
+    kv = codes(cty, [2 * D, Hkv, page, pages], A[3]) if kv is None else kv
+    sc = scales_of(D, Hkv, page, pages, A[5]) if sc is None else sc
+    dst = T(oty, [2 * D, Hkv, N], A[0]) if dst is None else dst
+    st = ghip.lib().ghip_kv_read_mx(ctx, ref(kv), ref(sc), ref(slots), ref(dst), None)
+    return st, ghip.lib().ghip_last_error(ctx).decode()
+
+
+# what is wrong with a cache, whatever the call
+def wrong_caches():
+    import ghip
+    e4, e2 = ghip.E4M3, ghip.E2M1
+    return [
+        ("E4M3 or E2M1", dict(cty=ghip.F16)), ("multiple of 16", dict(D=24)), ("multiple of 16", dict(D=272)), ("multiple of 16", dict(D=8)),
+        ("2 D", dict(kv=codes(e4, [64, 2, 16, 5], A[3]))), ("2 D", dict(kv=codes(e4, [128, 3, 16, 5], A[3]), sc=scales_of(64, 3, 16, 5, A[5]))),
+        ("2 D", dict(kv=codes(e4, [128, 2, 16, 5], A[3], [2, 256, 512, 8192]))),
+        ("16 bytes", dict(kv=codes(e4, [128, 2, 16, 5], A[3] + 8))), ("16 bytes", dict(kv=codes(e4, [128, 2, 16, 5], A[3], [1, 136, 272, 4352]))),
+        ("16 bytes", dict(kv=codes(e2, [128, 2, 16, 5], A[3], [1, 72, 144, 2304]))),
+        ("scales must be E8M0", dict(sc=T(ghip.F32, [4, 2, 16, 5], A[5]))),
+        ("S = 1, 2, 4 or 8", dict(sc=scales_of(128, 2, 16, 5, A[5]))), ("S = 1, 2, 4 or 8", dict(sc=scales_of(64, 2, 16, 4, A[5]))),
+        ("S = 1, 2, 4 or 8", dict(sc=scales_of(64, 2, 8, 5, A[5]))), ("S = 1, 2, 4 or 8", dict(sc=scales_of(64, 1, 16, 5, A[5]))),
+        ("S = 1, 2, 4 or 8", dict(sc=scales_of(64, 2, 16, 5, A[5], [2, 8, 16, 256]))),
+        ("2 S bytes", dict(sc=scales_of(64, 2, 16, 5, A[5] + 2))), ("2 S bytes", dict(sc=scales_of(64, 2, 16, 5, A[5], [1, 6, 12, 192]))),
+        ("null data", dict(kv=codes(e4, [128, 2, 16, 5], None))), ("null data", dict(sc=scales_of(64, 2, 16, 5, None)))]
+
+
+def test_append(ctx):
+    import ghip
+    for N in (0, 1, 9, 8192):
+        for kty in (0, 1, 30):
+            for cty in (ghip.E4M3, ghip.E2M1):
+                for D, page, pages in ((64, 1, 4), (128, 24, 600), (80, 16, 0), (16, 16, 3), (256, 64, 3)):
+                    st, msg = run_append(ctx, N=N, kty=kty, cty=cty, D=D, page=page, pages=pages)
+                    assert st == 0, msg
+    st, msg = run_append(ctx, rope=False, pos=None)
+    assert st == 0, msg
+    st, msg = run_append(ctx, kv=codes(256, [128, 2, 16, 5], A[3], nb=[1, 160, 640, 16384]), sc=scales_of(64, 2, 16, 5, A[5], [1, 4, 12, 256]))
+    assert st == 0, msg
+    for want, kw in wrong_caches() + [
+            ("of one type", dict(kty=ghip.I32)), ("of one type", dict(vty=1)), ("same shape", dict(v=T(0, [64, 2, 8], A[1]))),
+            ("[D, H_kv, T]", dict(k=T(0, [64, 2, 9, 2], A[0]), v=T(0, [64, 2, 9, 2], A[1]))),
+            ("rows of elements", dict(k=T(0, [64, 2, 9], A[0], nb=[8, 512, 1024, 9216]))),
+            ("I64", dict(slots=T(ghip.I32, [9], A[2]))), ("I64", dict(slots=T(ghip.I64, [8], A[2]))),
+            ("need a rotation", dict(rope=False)), ("n_dims", dict(n_dims=128)), ("pos", dict(pos=None)),
+            ("null data", dict(slots=T(ghip.I64, [9], None))), ("null data", dict(pos=T(ghip.I32, [9], None))),
+            ("lie apart", dict(kv=codes(256, [128, 2, 16, 5], A[0] + 64))), ("lie apart", dict(sc=scales_of(64, 2, 16, 5, A[2] + 64))),
+            ("lie apart", dict(sc=scales_of(64, 2, 16, 5, A[3] + 4096))), ("lie apart", dict(kv=codes(256, [128, 2, 16, 5], A[4]))),
+            ("factors", dict(factors=T(ghip.F32, [9], A[6]))), ("null data", dict(factors=T(ghip.F32, [32], None)))]:
+        st, msg = run_append(ctx, **kw)
+        assert st != 0 and want in msg, (want, kw, msg)
+    L, none = ghip.lib(), None
+    for i in range(9):
+        args = [ref(T(0, [64, 2, 9], A[0])), ref(T(0, [64, 2, 9], A[1])), ref(T(ghip.I64, [9], A[2])), none, none, none,
+                ref(codes(256, [128, 2, 16, 5], A[3])), ref(scales_of(64, 2, 16, 5, A[5]))]
+        if i < 8 and args[i] is not None:
+            args[i] = None
+            assert L.ghip_kv_append_mx(ctx, *args, None) != 0
+    assert L.ghip_kv_append_mx(None, *args, None) != 0
+
+
+def test_read(ctx):
+    import ghip
+    for N in (0, 1, 9, 20000):
+        for oty in (0, 1, 30):
+            for cty in (ghip.E4M3, ghip.E2M1):
+                for D, page, pages in ((64, 1, 4), (128, 24, 600), (80, 16, 0), (16, 16, 3), (256, 64, 3)):
+                    st, msg = run_read(ctx, N=N, oty=oty, cty=cty, D=D, page=page, pages=pages)
+                    assert st == 0, msg
+    st, msg = run_read(ctx, dst=T(0, [128, 2, 9], A[0], nb=[4, 540, 2000, 18000]))
+    assert st == 0, msg
+    for want, kw in wrong_caches() + [
+            ("dst must be F32", dict(oty=ghip.I32)), ("rows of elements", dict(dst=T(0, [128, 2, 9], A[0], nb=[8, 1024, 2048, 20480]))),
+            ("[2 D, H_kv, T]", dict(dst=T(0, [128, 2, 9, 2], A[0]))), ("[2 D, H_kv", dict(dst=T(0, [128, 3, 9], A[0]))),
+            ("I64", dict(slots=T(ghip.I32, [9], A[2]))), ("I64", dict(slots=T(ghip.I64, [8], A[2]))),
+            ("null data", dict(dst=T(0, [128, 2, 9], None))), ("null data", dict(slots=T(ghip.I64, [9], None))),
+            ("lie apart", dict(dst=T(0, [128, 2, 9], A[3] + 256))), ("lie apart", dict(dst=T(0, [128, 2, 9], A[5]))),
+            ("lie apart", dict(dst=T(0, [128, 2, 9], A[2])))]:
+        st, msg = run_read(ctx, **kw)
+        assert st != 0 and want in msg, (want, kw, msg)
+    L = ghip.lib()
+    args = [ref(codes(256, [128, 2, 16, 5], A[3])), ref(scales_of(64, 2, 16, 5, A[5])), ref(T(ghip.I64, [9], A[2])), ref(T(0, [128, 2, 9], A[0]))]
+    for i in range(4):
+        assert L.ghip_kv_read_mx(ctx, *[None if j == i else a for j, a in enumerate(args)], None) != 0
+    assert L.ghip_kv_read_mx(None, *args, None) != 0
+
+
+def test_binding_refuses():
+    """Codes and scales of other dtypes or shapes, before any call."""
+    import ghip
+    torch = pytest.importorskip("torch")
+    kv, sc = ghip.mx_cache(3, 16, 2, 64, 8, device="cpu")
+    assert kv.shape == (3, 16, 2, 128) and kv.dtype == torch.float8_e4m3fn and sc.shape == (3, 16, 2, 4) and (sc == 27).all()
+    kv4, sc4 = ghip.mx_cache(3, 16, 2, 80, 4, device="cpu")
+    assert kv4.shape == (3, 16, 2, 80) and kv4.dtype == torch.uint8 and sc4.shape == (3, 16, 2, 8)
+    for a, b, why in ((kv.float(), sc, "not supported"), (kv, sc.float(), "scales"), (kv, sc, "GPU")):
+        with pytest.raises(ghip.GhipError, match=why):
+            ghip._view_mx(a, b)
+    with pytest.raises(ghip.GhipError, match="4 or 8"):
+        ghip.mx_cache(3, 16, 2, 64, 6, device="cpu")
