@@ -21,7 +21,7 @@
 
 namespace {
 
-const char *const kModules[] = {"ghip_quant.hsaco", "ghip_kq.hsaco", "ghip_gemv.hsaco", "ghip_wquant.hsaco", "ghip_gemm.hsaco", "ghip_fa.hsaco", "ghip_moe.hsaco", "ghip_skinny.hsaco", "ghip_iq.hsaco", "ghip_dense.hsaco", "ghip_rope.hsaco", "ghip_fap.hsaco", "ghip_kvq.hsaco"};
+const char *const kModules[] = {"ghip_quant.hsaco", "ghip_kq.hsaco", "ghip_gemv.hsaco", "ghip_wquant.hsaco", "ghip_gemm.hsaco", "ghip_fa.hsaco", "ghip_moe.hsaco", "ghip_skinny.hsaco", "ghip_iq.hsaco", "ghip_dense.hsaco", "ghip_rope.hsaco", "ghip_fap.hsaco", "ghip_kvq.hsaco", "ghip_fapq.hsaco"};
 
 struct TypeInfo {
     int blck;
@@ -3512,7 +3512,7 @@ namespace {
 struct FapParams {
     const float *q;
     int64_t q_nb1, q_nb2;
-    const uint16_t *kv;
+    const void *kv;
     int64_t kv_head, kv_row, kv_page;
     int n_pages, page;
     const int32_t *seqs;
@@ -3529,11 +3529,18 @@ struct FapParams {
     int join_ragged;
     float *part, *stat;
 };
+// ... and of FapMxParams in ghip_fapq.hip: kv's strides in bytes, the scales
+struct FapMxParams : FapParams {
+    const uint8_t *sc;
+    int64_t sc_head, sc_row, sc_page;
+    int S;
+};
 
-bool plan_fap(ghip_context *ctx, const ghip_tensor *q, const ghip_tensor *kv, const ghip_tensor *seqs,
-              const ghip_tensor *sinks, const ghip_tensor *d, const ghip_paged_params *pp, FapParams &p, ghip_status &st) {
+// sc: a quantized cache's scales, else null
+bool plan_fap(ghip_context *ctx, const char *call, const ghip_tensor *q, const ghip_tensor *kv, const ghip_tensor *sc, const ghip_tensor *seqs,
+              const ghip_tensor *sinks, const ghip_tensor *d, const ghip_paged_params *pp, FapMxParams &p, ghip_status &st) {
     st = GHIP_STATUS_BACKEND_ERROR;
-    auto bad = [&](const char *why) { st = ctx->fail(GHIP_STATUS_BACKEND_ERROR, "flash_attn_paged: %s", why); return false; };
+    auto bad = [&](const char *why) { st = ctx->fail(GHIP_STATUS_BACKEND_ERROR, "%s: %s", call, why); return false; };
     if (!q || !kv || !seqs || !d || !pp) return bad("null operand");
     if (q->type != GHIP_TYPE_F32 || !elem_rows(q, 4) || d->type != GHIP_TYPE_F32 || !elem_rows(d, 4))
         return bad("q and dst must be F32 rows");
@@ -3541,12 +3548,16 @@ bool plan_fap(ghip_context *ctx, const ghip_tensor *q, const ghip_tensor *kv, co
         if (q->ne[i] != d->ne[i] || q->ne[i] < 0) return bad("dst must have the shape of q");
     const int64_t D = q->ne[0], H = q->ne[1], T = q->ne[2];
     if (q->ne[3] != 1) return bad("q must be [D, H, T]");
-    if (D < 8 || D > 256 || D % 8) return bad("head size must be a multiple of 8, 8..256");
-    if (kv->type != GHIP_TYPE_F16 && kv->type != GHIP_TYPE_BF16) return bad("kv must be F16 or BF16");
-    if (!packed(kv, 2) || kv->ne[0] != 2 * D || kv->ne[1] < 1 || kv->ne[2] < 1 || kv->ne[3] < 0)
-        return bad("kv must be [2 D, H_kv, page, pages]");
-    if (!in_steps(kv, 1, 16) || (uintptr_t)kv->data % 16)
-        return bad("kv and its strides must be multiples of 16 bytes");
+    if (sc) {
+        if (const char *why = mx_cache(kv, sc, D)) return bad(why);
+    } else {
+        if (D < 8 || D > 256 || D % 8) return bad("head size must be a multiple of 8, 8..256");
+        if (kv->type != GHIP_TYPE_F16 && kv->type != GHIP_TYPE_BF16) return bad("kv must be F16 or BF16");
+        if (!packed(kv, 2) || kv->ne[0] != 2 * D || kv->ne[1] < 1 || kv->ne[2] < 1 || kv->ne[3] < 0)
+            return bad("kv must be [2 D, H_kv, page, pages]");
+        if (!in_steps(kv, 1, 16) || (uintptr_t)kv->data % 16)
+            return bad("kv and its strides must be multiples of 16 bytes");
+    }
     const int64_t H_kv = kv->ne[1], page = kv->ne[2];
     if (H % H_kv) return bad("H % H_kv != 0");
     // the kernels count rows in 32 bits, 256 sequences of them at a time
@@ -3567,14 +3578,23 @@ bool plan_fap(ghip_context *ctx, const ghip_tensor *q, const ghip_tensor *kv, co
         if (overlaps(q, d)) return bad("dst must lie apart from q");
         if ((kv->ne[3] && overlaps(kv, d)) || overlaps(seqs, d) || overlaps(sinks, d))
             return bad("dst must lie apart from kv, seqs and sinks");
+        if (sc && kv->ne[3] && overlaps(sc, d)) return bad("dst must lie apart from scales");
     }
     p.q = (const float *)q->data;
     p.q_nb1 = (int64_t)(q->nb[1] / 4);
     p.q_nb2 = (int64_t)(q->nb[2] / 4);
-    p.kv = (const uint16_t *)kv->data;
-    p.kv_head = (int64_t)(kv->nb[1] / 2);
-    p.kv_row = (int64_t)(kv->nb[2] / 2);
-    p.kv_page = (int64_t)(kv->nb[3] / 2);
+    const uint64_t unit = sc ? 1 : 2;
+    p.kv = kv->data;
+    p.kv_head = (int64_t)(kv->nb[1] / unit);
+    p.kv_row = (int64_t)(kv->nb[2] / unit);
+    p.kv_page = (int64_t)(kv->nb[3] / unit);
+    if (sc) {
+        p.sc = (const uint8_t *)sc->data;
+        p.sc_head = (int64_t)sc->nb[1];
+        p.sc_row = (int64_t)sc->nb[2];
+        p.sc_page = (int64_t)sc->nb[3];
+        p.S = mx_scale_bytes(D);
+    }
     p.n_pages = (int)kv->ne[3];
     p.page = (int)page;
     p.seqs = (const int32_t *)seqs->data;
@@ -3722,9 +3742,9 @@ ghip_status ghip_flash_attn_paged_workspace(const ghip_tensor *q, const ghip_ten
     if (!bytes) return GHIP_STATUS_BACKEND_ERROR;
     *bytes = 0;
     ghip_context tmp;
-    FapParams p;
+    FapMxParams p;
     ghip_status st;
-    if (!plan_fap(&tmp, q, kv, seqs, nullptr, dst, params, p, st)) return st;
+    if (!plan_fap(&tmp, "flash_attn_paged", q, kv, nullptr, seqs, nullptr, dst, params, p, st)) return st;
     if (p.max_q && p.H && p.B) *bytes = fap_layout(p, kv->type == GHIP_TYPE_BF16).ws_bytes;
     return GHIP_STATUS_SUCCESS;
 }
@@ -3734,9 +3754,9 @@ ghip_status ghip_flash_attn_paged(ghip_context *ctx, const ghip_tensor *q, const
                                   void *stream) {
     if (!ctx) return GHIP_STATUS_BACKEND_ERROR;
     std::lock_guard<std::mutex> lock(ctx->mu);
-    FapParams p;
+    FapMxParams p;
     ghip_status st;
-    if (!plan_fap(ctx, q, kv, seqs, sinks, dst, params, p, st)) return st;
+    if (!plan_fap(ctx, "flash_attn_paged", q, kv, nullptr, seqs, sinks, dst, params, p, st)) return st;
     if (p.max_q == 0 || p.H == 0 || p.B == 0) return GHIP_STATUS_SUCCESS;
     hipStream_t s = (hipStream_t)stream;
     if (!ctx->set_device()) return ctx->fail(GHIP_STATUS_BACKEND_ERROR, "hipSetDevice failed");
@@ -3772,12 +3792,48 @@ ghip_status ghip_flash_attn_paged(ghip_context *ctx, const ghip_tensor *q, const
     }
     if (L.few && !p.wg_sh) snprintf(name, sizeof name, "ghip_fap_few_%s_%d", ty, L.DP);
     else snprintf(name, sizeof name, "ghip_fap_%s%d_%s_%d", L.few ? "both" : "tile", L.rows, ty, L.DP);
-    st = ctx->launch(name, dim3((unsigned)(own + p.wg_sh)), dim3(256), 0, s, p);
+    const FapParams a = p;
+    st = ctx->launch(name, dim3((unsigned)(own + p.wg_sh)), dim3(256), 0, s, a);
     if (st != GHIP_STATUS_SUCCESS) return st;
     if (!p.part) return GHIP_STATUS_SUCCESS;
     ctx->expect(p.dst, (size_t)(4 * ((p.T - 1) * p.d_nb2 + (p.H - 1) * p.d_nb1 + p.D)), "dst");
     snprintf(name, sizeof name, "ghip_fap_join_%s", ty);
-    return ctx->launch(name, dim3((unsigned)joins), dim3(256), 0, s, p);
+    return ctx->launch(name, dim3((unsigned)joins), dim3(256), 0, s, a);
+}
+
+ghip_status ghip_flash_attn_paged_mx_workspace(const ghip_tensor *q, const ghip_tensor *kv, const ghip_tensor *scales,
+                                               const ghip_tensor *seqs, const ghip_paged_params *params, const ghip_tensor *dst,
+                                               size_t *bytes) {
+    if (!bytes) return GHIP_STATUS_BACKEND_ERROR;
+    *bytes = 0;
+    if (!scales) return GHIP_STATUS_BACKEND_ERROR;
+    ghip_context tmp;
+    FapMxParams p;
+    ghip_status st;
+    if (!plan_fap(&tmp, "flash_attn_paged_mx", q, kv, scales, seqs, nullptr, dst, params, p, st)) return st;
+    return GHIP_STATUS_SUCCESS;
+}
+
+ghip_status ghip_flash_attn_paged_mx(ghip_context *ctx, const ghip_tensor *q, const ghip_tensor *kv, const ghip_tensor *scales,
+                                     const ghip_tensor *seqs, const ghip_tensor *sinks, const ghip_paged_params *params,
+                                     const ghip_tensor *dst, void *stream) {
+    if (!ctx) return GHIP_STATUS_BACKEND_ERROR;
+    std::lock_guard<std::mutex> lock(ctx->mu);
+    if (!scales) return ctx->fail(GHIP_STATUS_BACKEND_ERROR, "flash_attn_paged_mx: null operand");
+    FapMxParams p;
+    ghip_status st;
+    if (!plan_fap(ctx, "flash_attn_paged_mx", q, kv, scales, seqs, sinks, dst, params, p, st)) return st;
+    if (p.max_q == 0 || p.H == 0 || p.B == 0) return GHIP_STATUS_SUCCESS;
+    hipStream_t s = (hipStream_t)stream;
+    if (!ctx->set_device()) return ctx->fail(GHIP_STATUS_BACKEND_ERROR, "hipSetDevice failed");
+    st = ctx->begin(s);
+    if (st != GHIP_STATUS_SUCCESS) return st;
+    ctx->allow(dst->data, byte_extent(dst, 4), "dst");
+    const int64_t wgs = std::min<int64_t>(((int64_t)p.B * p.max_q * p.H + 3) / 4, 1 << 20);
+    ctx->expect(p.dst, (size_t)(4 * ((p.T - 1) * p.d_nb2 + (p.H - 1) * p.d_nb1 + p.D)), "dst");
+    char name[48];
+    snprintf(name, sizeof name, "ghip_fapq_rows_%d", mx_bits(kv));
+    return ctx->launch(name, dim3((unsigned)wgs), dim3(256), 0, s, p);
 }
 
 }  // extern "C"

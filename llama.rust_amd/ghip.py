@@ -290,6 +290,10 @@ def lib():
         L.ghip_kv_read_mx.argtypes = [V, V, V, V, V, V]
         L.ghip_flash_attn_paged.restype = C.c_int
         L.ghip_flash_attn_paged.argtypes = [V, V, V, V, V, V, V, V]
+        L.ghip_flash_attn_paged_mx.restype = C.c_int
+        L.ghip_flash_attn_paged_mx.argtypes = [V, V, V, V, V, V, V, V, V]
+        L.ghip_flash_attn_paged_mx_workspace.restype = C.c_int
+        L.ghip_flash_attn_paged_mx_workspace.argtypes = [V, V, V, V, V, V, C.POINTER(C.c_size_t)]
         L.ghip_flash_attn_paged_workspace.restype = C.c_int
         L.ghip_flash_attn_paged_workspace.argtypes = [V, V, V, V, V, C.POINTER(C.c_size_t)]
         _lib = L
@@ -484,13 +488,21 @@ class Backend:
             self._check(st, "ghip_kv_read_mx")
         return out
 
-    def flash_attn_paged(self, q, kv, seqs, scale=1.0, sinks=None, window=0, n_first=0, n_shared=0, max_q=None, out=None):
-        """q [T, H, D] f32 over kv [pages, page, H_kv, 2 D] f16 / bf16; seqs
-        [B, 3 + per] int32 rows (first row in q, rows, keys, pages ..); sinks [H]
-        f32.  max_q: the most rows of a sequence (T where None) -> [T, H, D] f32."""
+    def flash_attn_paged(self, q, kv, seqs, scale=1.0, sinks=None, window=0, n_first=0, n_shared=0, max_q=None, out=None, scales=None):
+        """q [T, H, D] f32 over kv [pages, page, H_kv, 2 D] f16 / bf16, or with scales over a
+        quantized cache (mx_cache); seqs [B, 3 + per] int32 rows (first row in q, rows, keys,
+        pages ..); sinks [H] f32.  max_q: the most rows of a sequence (T where None) ->
+        [T, H, D] f32."""
         if out is None:
             out = torch.empty_like(q)
         pp = paged_params(scale, window, n_first, n_shared, q.shape[0] if max_q is None else max_q)
+        if scales is not None:
+            codes, sc = _view_mx(kv, scales)
+            st = lib().ghip_flash_attn_paged_mx(self._ctx, _view(q), codes, sc, _view(seqs), _view(sinks), pp, _view(out),
+                                                _raw_stream(self.device))
+            if st:
+                self._check(st, "ghip_flash_attn_paged_mx")
+            return out
         st = lib().ghip_flash_attn_paged(self._ctx, _view(q), _view(kv), _view(seqs), _view(sinks), pp, _view(out),
                                          _raw_stream(self.device))
         if st:
@@ -498,13 +510,16 @@ class Backend:
         return out
 
     @staticmethod
-    def flash_attn_paged_workspace(q, kv, seqs, window=0, n_first=0, n_shared=0, max_q=None):
+    def flash_attn_paged_workspace(q, kv, seqs, window=0, n_first=0, n_shared=0, max_q=None, scales=None):
         """Workspace bytes that flash_attn_paged needs at most for these shapes."""
         pp = paged_params(1.0, window, n_first, n_shared, q.shape[0] if max_q is None else max_q)
         out, v = C.c_size_t(0), _view(q)
         d = Tensor.from_buffer_copy(v)
         d.data = (d.data or 0) + (1 << 60)  # any place apart from q: only compared
-        st = lib().ghip_flash_attn_paged_workspace(v, _view(kv), _view(seqs), pp, bytes(d), C.byref(out))
+        if scales is not None:
+            st = lib().ghip_flash_attn_paged_mx_workspace(v, *_view_mx(kv, scales), _view(seqs), pp, bytes(d), C.byref(out))
+        else:
+            st = lib().ghip_flash_attn_paged_workspace(v, _view(kv), _view(seqs), pp, bytes(d), C.byref(out))
         if st:
             raise GhipError(f"ghip_flash_attn_paged_workspace: status {st}")
         return out.value

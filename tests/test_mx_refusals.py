@@ -136,3 +136,61 @@ def test_binding_refuses():
             ghip._view_mx(a, b)
     with pytest.raises(ghip.GhipError, match="4 or 8"):
         ghip.mx_cache(3, 16, 2, 64, 6, device="cpu")
+
+
+def run_paged(ctx, D=64, H=8, Hkv=2, N=9, B=3, per=7, cty=256, page=16, pages=5, q=None, kv=None, sc=None, seqs=None, sinks=None, dst=None, scale=0.1,
+              window=0, n_first=0, n_shared=0, max_q=3, workspace=False):
+    import ghip
+    q = T(0, [D, H, N], A[0]) if q is None else q
+    kv = codes(cty, [2 * D, Hkv, page, pages], A[3]) if kv is None else kv
+    sc = scales_of(D, Hkv, page, pages, A[5]) if sc is None else sc
+    seqs = T(ghip.I32, [3 + per, B], A[2]) if seqs is None else seqs
+    dst = T(0, [D, H, N], A[6]) if dst is None else dst
+    pp = ghip.PagedParams(scale, window, n_first, n_shared, max_q)
+    if workspace:
+        n = C.c_size_t()
+        return ghip.lib().ghip_flash_attn_paged_mx_workspace(ref(q), ref(kv), ref(sc), ref(seqs), C.byref(pp), ref(dst), C.byref(n)), n.value
+    st = ghip.lib().ghip_flash_attn_paged_mx(ctx, ref(q), ref(kv), ref(sc), ref(seqs), ref(sinks), C.byref(pp), ref(dst), None)
+    return st, ghip.lib().ghip_last_error(ctx).decode()
+
+
+def test_paged_stores_inside_its_buffers(ctx):
+    import random
+    import ghip
+    rng = random.Random(5)
+    for _ in range(300):
+        Hkv = rng.choice([1, 2, 4, 8])
+        N = rng.choice([1, 3, 40, 700, 5000])
+        kw = dict(D=rng.choice([16, 64, 80, 96, 112, 128, 256]), Hkv=Hkv, H=Hkv * rng.choice([1, 3, 4, 8, 16, 40]), N=N, B=rng.choice([1, 2, 64, 300]),
+                  per=rng.choice([1, 9, 1000]), cty=rng.choice([ghip.E4M3, ghip.E2M1]), page=rng.choice([1, 24, 64, 256]), pages=rng.choice([0, 1, 9000]),
+                  window=rng.choice([0, 1, 4096]), n_first=rng.choice([0, 4]), n_shared=rng.choice([0, 1]), max_q=rng.choice([0, 1, 5, 60, 5000]))
+        st, msg = run_paged(ctx, **kw)
+        assert st == 0, msg
+        assert run_paged(ctx, workspace=True, **kw)[0] == 0
+
+
+def test_paged_refuses(ctx):
+    import ghip
+    wrong = [(want, kw) for want, kw in wrong_caches() if not ("sc" in kw and "kv" in kw)]
+    for want, kw in wrong + [
+            ("H_kv", dict(H=9)), ("F32 rows", dict(q=T(1, [64, 8, 9], A[0]))), ("shape", dict(dst=T(0, [64, 8, 8], A[6]))),
+            ("seqs", dict(seqs=T(ghip.I64, [10, 3], A[2]))), ("seqs", dict(seqs=T(ghip.I32, [2, 3], A[2]))), ("sinks", dict(sinks=T(0, [7], A[4]))),
+            ("scale", dict(scale=float("nan"))), ("window", dict(window=-1)), ("n_first", dict(n_first=-1)), ("n_shared", dict(n_shared=-1)),
+            ("n_shared", dict(n_shared=113)), ("max_q", dict(max_q=-1)), ("apart", dict(dst=T(0, [64, 8, 9], A[0] + 4096))),
+            ("apart from kv", dict(dst=T(0, [64, 8, 9], A[3] + 4096))), ("apart from scales", dict(dst=T(0, [64, 8, 9], A[5] + 256))),
+            ("null data", dict(seqs=T(ghip.I32, [10, 3], None))), ("null data", dict(sinks=T(0, [8], None)))]:
+        st, msg = run_paged(ctx, **kw)
+        assert st != 0 and want in msg, (want, kw, msg)
+        if "sinks" not in kw:
+            assert run_paged(ctx, workspace=True, **kw)[0] != 0
+    L = ghip.lib()
+    pp = ghip.PagedParams(1.0, 0, 0, 0, 3)
+    args = [ref(T(0, [64, 8, 9], A[0])), ref(codes(256, [128, 2, 16, 5], A[3])), ref(scales_of(64, 2, 16, 5, A[5])), ref(T(ghip.I32, [10, 3], A[2])), None,
+            C.byref(pp), ref(T(0, [64, 8, 9], A[6]))]
+    for i in range(7):
+        if args[i] is not None:
+            assert L.ghip_flash_attn_paged_mx(ctx, *[None if j == i else a for j, a in enumerate(args)], None) != 0
+    assert L.ghip_flash_attn_paged_mx(None, *args, None) != 0
+    # the cache of the other call
+    st = L.ghip_flash_attn_paged(ctx, args[0], args[1], args[3], None, args[5], args[6], None)
+    assert st != 0 and "F16 or BF16" in L.ghip_last_error(ctx).decode()
