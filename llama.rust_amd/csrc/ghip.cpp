@@ -3629,10 +3629,13 @@ struct FapLayout {
     int DP, rows;
     size_t ws_bytes;
 };
-FapLayout fap_layout(FapParams &p, bool bf16) {
+FapLayout fap_layout(FapParams &p, int type) {
     FapLayout L;
     const int G = p.H / p.H_kv;
-    L.DP = p.D <= 64 ? 64 : p.D <= 96 ? 96 : p.D <= 128 ? 128 : 256;
+    const bool mx = mx_type(type), bf16 = type != GHIP_TYPE_F16;  // (codes are computed with as bfloat16)
+    L.DP = p.D <= 64 ? 64 : p.D <= 96 && !mx ? 96 : p.D <= 128 ? 128 : 256;
+    // bytes of a head's key and value
+    const double key_bytes = !mx ? 4.0 * p.D : type == GHIP_TYPE_E4M3 ? 2.0 * p.D + 2 * mx_scale_bytes(p.D) : p.D + 2.0 * mx_scale_bytes(p.D);
     L.few = (int64_t)p.max_q * G <= 16;
     const int64_t table = (int64_t)p.per * p.page;
     const int64_t rows = std::min((int64_t)p.T, (int64_t)p.B * p.max_q);
@@ -3676,7 +3679,7 @@ FapLayout fap_layout(FapParams &p, bool bf16) {
         Way w;
         w.z = keys <= 512 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>({(1024 + wgs - 1) / wgs, (keys + 255) / 256, 32}));
         const double steps = (double)((keys + 128 * w.z - 1) / (128 * w.z));
-        w.us = std::max((double)((wgs * w.z + slots - 1) / slots) * (6.0 + steps * (1.2 + 0.8 * wide)), 4.0 * wgs * keys * p.D / mem) +
+        w.us = std::max((double)((wgs * w.z + slots - 1) / slots) * (6.0 + steps * (1.2 + 0.8 * wide)), key_bytes * wgs * keys / mem) +
                (w.z > 1 || !alone ? join(w.z) : 0.0);
         return w;
     };
@@ -3733,37 +3736,27 @@ FapLayout fap_layout(FapParams &p, bool bf16) {
     return L;
 }
 
-}  // namespace
-
-extern "C" {
-
-ghip_status ghip_flash_attn_paged_workspace(const ghip_tensor *q, const ghip_tensor *kv, const ghip_tensor *seqs,
-                                            const ghip_paged_params *params, const ghip_tensor *dst, size_t *bytes) {
-    if (!bytes) return GHIP_STATUS_BACKEND_ERROR;
-    *bytes = 0;
+// Both kinds of cache: sc null, or the scales of a quantized one.
+ghip_status fap_workspace(const char *call, const ghip_tensor *q, const ghip_tensor *kv, const ghip_tensor *sc, const ghip_tensor *seqs,
+                          const ghip_paged_params *params, const ghip_tensor *dst, size_t *bytes) {
     ghip_context tmp;
     FapMxParams p;
     ghip_status st;
-    if (!plan_fap(&tmp, "flash_attn_paged", q, kv, nullptr, seqs, nullptr, dst, params, p, st)) return st;
-    if (p.max_q && p.H && p.B) *bytes = fap_layout(p, kv->type == GHIP_TYPE_BF16).ws_bytes;
+    if (!plan_fap(&tmp, call, q, kv, sc, seqs, nullptr, dst, params, p, st)) return st;
+    if (p.max_q && p.H && p.B) *bytes = fap_layout(p, kv->type).ws_bytes;
     return GHIP_STATUS_SUCCESS;
 }
-
-ghip_status ghip_flash_attn_paged(ghip_context *ctx, const ghip_tensor *q, const ghip_tensor *kv, const ghip_tensor *seqs,
-                                  const ghip_tensor *sinks, const ghip_paged_params *params, const ghip_tensor *dst,
-                                  void *stream) {
-    if (!ctx) return GHIP_STATUS_BACKEND_ERROR;
-    std::lock_guard<std::mutex> lock(ctx->mu);
+ghip_status fap_run(ghip_context *ctx, const char *call, const ghip_tensor *q, const ghip_tensor *kv, const ghip_tensor *sc,
+                    const ghip_tensor *seqs, const ghip_tensor *sinks, const ghip_paged_params *params, const ghip_tensor *dst, hipStream_t s) {
     FapMxParams p;
     ghip_status st;
-    if (!plan_fap(ctx, "flash_attn_paged", q, kv, nullptr, seqs, sinks, dst, params, p, st)) return st;
+    if (!plan_fap(ctx, call, q, kv, sc, seqs, sinks, dst, params, p, st)) return st;
     if (p.max_q == 0 || p.H == 0 || p.B == 0) return GHIP_STATUS_SUCCESS;
-    hipStream_t s = (hipStream_t)stream;
     if (!ctx->set_device()) return ctx->fail(GHIP_STATUS_BACKEND_ERROR, "hipSetDevice failed");
     st = ctx->begin(s);
     if (st != GHIP_STATUS_SUCCESS) return st;
     ctx->allow(dst->data, byte_extent(dst, 4), "dst");
-    const FapLayout L = fap_layout(p, kv->type == GHIP_TYPE_BF16);
+    const FapLayout L = fap_layout(p, kv->type);
     p.part = p.stat = nullptr;
     if (L.ws_bytes) {
         void *ws = nullptr;
@@ -3773,8 +3766,6 @@ ghip_status ghip_flash_attn_paged(ghip_context *ctx, const ghip_tensor *q, const
         p.part = (float *)ws;
         p.stat = p.part + n * p.D;
     }
-    char name[48];
-    const char *ty = float_name(kv->type);
     const int64_t own = (int64_t)p.nb_own * p.H_kv * p.zs_own;
     // a workgroup of the join for a row that no sequence has costs little, but
     // B max_q can be many times T
@@ -3782,7 +3773,7 @@ ghip_status ghip_flash_attn_paged(ghip_context *ctx, const ghip_tensor *q, const
     const int64_t joins = ((p.join_ragged ? (int64_t)p.T : (int64_t)p.B * p.max_q) * p.H + 3) / 4;
     const int64_t most = ((1ll << 32) - 1) / 256;  // workgroups of 256 threads in a launch
     if (own + p.wg_sh > most || (p.part && joins > most))
-        return ctx->fail(GHIP_STATUS_BACKEND_ERROR, "flash_attn_paged: too many rows");
+        return ctx->fail(GHIP_STATUS_BACKEND_ERROR, "%s: too many rows", call);
     if (p.part) {
         const size_t n = (size_t)p.T * p.H * (p.zs_sh + p.zs_own);
         ctx->expect(p.part, n * p.D * 4, "partials");
@@ -3790,15 +3781,39 @@ ghip_status ghip_flash_attn_paged(ghip_context *ctx, const ghip_tensor *q, const
     } else {
         ctx->expect(p.dst, (size_t)(4 * ((p.T - 1) * p.d_nb2 + (p.H - 1) * p.d_nb1 + p.D)), "dst");
     }
-    if (L.few && !p.wg_sh) snprintf(name, sizeof name, "ghip_fap_few_%s_%d", ty, L.DP);
-    else snprintf(name, sizeof name, "ghip_fap_%s%d_%s_%d", L.few ? "both" : "tile", L.rows, ty, L.DP);
-    const FapParams a = p;
-    st = ctx->launch(name, dim3((unsigned)(own + p.wg_sh)), dim3(256), 0, s, a);
-    if (st != GHIP_STATUS_SUCCESS) return st;
-    if (!p.part) return GHIP_STATUS_SUCCESS;
+    // ghip_fap_few_f16_128, ghip_fapq_both64_8_128
+    const char *set = sc ? "fapq" : "fap", *ty = !sc ? float_name(kv->type) : mx_bits(kv) == 8 ? "8" : "4";
+    char name[48];
+    if (L.few && !p.wg_sh) snprintf(name, sizeof name, "ghip_%s_few_%s_%d", set, ty, L.DP);
+    else snprintf(name, sizeof name, "ghip_%s_%s%d_%s_%d", set, L.few ? "both" : "tile", L.rows, ty, L.DP);
+    auto launch = [&](int64_t wgs) {
+        if (sc) return ctx->launch(name, dim3((unsigned)wgs), dim3(256), 0, s, p);
+        return ctx->launch(name, dim3((unsigned)wgs), dim3(256), 0, s, (FapParams)p);
+    };
+    st = launch(own + p.wg_sh);
+    if (st != GHIP_STATUS_SUCCESS || !p.part) return st;
     ctx->expect(p.dst, (size_t)(4 * ((p.T - 1) * p.d_nb2 + (p.H - 1) * p.d_nb1 + p.D)), "dst");
-    snprintf(name, sizeof name, "ghip_fap_join_%s", ty);
-    return ctx->launch(name, dim3((unsigned)joins), dim3(256), 0, s, a);
+    snprintf(name, sizeof name, "ghip_%s_join_%s", set, ty);
+    return launch(joins);
+}
+
+}  // namespace
+
+extern "C" {
+
+ghip_status ghip_flash_attn_paged_workspace(const ghip_tensor *q, const ghip_tensor *kv, const ghip_tensor *seqs,
+                                            const ghip_paged_params *params, const ghip_tensor *dst, size_t *bytes) {
+    if (!bytes) return GHIP_STATUS_BACKEND_ERROR;
+    *bytes = 0;
+    return fap_workspace("flash_attn_paged", q, kv, nullptr, seqs, params, dst, bytes);
+}
+
+ghip_status ghip_flash_attn_paged(ghip_context *ctx, const ghip_tensor *q, const ghip_tensor *kv, const ghip_tensor *seqs,
+                                  const ghip_tensor *sinks, const ghip_paged_params *params, const ghip_tensor *dst,
+                                  void *stream) {
+    if (!ctx) return GHIP_STATUS_BACKEND_ERROR;
+    std::lock_guard<std::mutex> lock(ctx->mu);
+    return fap_run(ctx, "flash_attn_paged", q, kv, nullptr, seqs, sinks, params, dst, (hipStream_t)stream);
 }
 
 ghip_status ghip_flash_attn_paged_mx_workspace(const ghip_tensor *q, const ghip_tensor *kv, const ghip_tensor *scales,
@@ -3807,11 +3822,7 @@ ghip_status ghip_flash_attn_paged_mx_workspace(const ghip_tensor *q, const ghip_
     if (!bytes) return GHIP_STATUS_BACKEND_ERROR;
     *bytes = 0;
     if (!scales) return GHIP_STATUS_BACKEND_ERROR;
-    ghip_context tmp;
-    FapMxParams p;
-    ghip_status st;
-    if (!plan_fap(&tmp, "flash_attn_paged_mx", q, kv, scales, seqs, nullptr, dst, params, p, st)) return st;
-    return GHIP_STATUS_SUCCESS;
+    return fap_workspace("flash_attn_paged_mx", q, kv, scales, seqs, params, dst, bytes);
 }
 
 ghip_status ghip_flash_attn_paged_mx(ghip_context *ctx, const ghip_tensor *q, const ghip_tensor *kv, const ghip_tensor *scales,
@@ -3820,20 +3831,7 @@ ghip_status ghip_flash_attn_paged_mx(ghip_context *ctx, const ghip_tensor *q, co
     if (!ctx) return GHIP_STATUS_BACKEND_ERROR;
     std::lock_guard<std::mutex> lock(ctx->mu);
     if (!scales) return ctx->fail(GHIP_STATUS_BACKEND_ERROR, "flash_attn_paged_mx: null operand");
-    FapMxParams p;
-    ghip_status st;
-    if (!plan_fap(ctx, "flash_attn_paged_mx", q, kv, scales, seqs, sinks, dst, params, p, st)) return st;
-    if (p.max_q == 0 || p.H == 0 || p.B == 0) return GHIP_STATUS_SUCCESS;
-    hipStream_t s = (hipStream_t)stream;
-    if (!ctx->set_device()) return ctx->fail(GHIP_STATUS_BACKEND_ERROR, "hipSetDevice failed");
-    st = ctx->begin(s);
-    if (st != GHIP_STATUS_SUCCESS) return st;
-    ctx->allow(dst->data, byte_extent(dst, 4), "dst");
-    const int64_t wgs = std::min<int64_t>(((int64_t)p.B * p.max_q * p.H + 3) / 4, 1 << 20);
-    ctx->expect(p.dst, (size_t)(4 * ((p.T - 1) * p.d_nb2 + (p.H - 1) * p.d_nb1 + p.D)), "dst");
-    char name[48];
-    snprintf(name, sizeof name, "ghip_fapq_rows_%d", mx_bits(kv));
-    return ctx->launch(name, dim3((unsigned)wgs), dim3(256), 0, s, p);
+    return fap_run(ctx, "flash_attn_paged_mx", q, kv, scales, seqs, sinks, params, dst, (hipStream_t)stream);
 }
 
 }  // extern "C"

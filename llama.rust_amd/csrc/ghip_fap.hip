@@ -272,50 +272,8 @@ DEV void fap_few(const FapParams &p, FewLds<DP> &lds) {
             load_v();
         }
     }
-    // the 4 wavefronts' rows: everyone takes the common maximum, then thread
-    // (dims, row) adds the four
-    const float l = row_sum(R.l[0]), m = R.from[0] < __builtin_inff() ? row_ref(R.mneg[0]) : -__builtin_inff();
-    if (g == 0) {
-        ws[w][0][n] = m;
-        ws[w][1][n] = l;
-    }
-    __syncthreads();
-    float M = -__builtin_inff(), L = 0.0f;
-#pragma unroll
-    for (int u = 0; u < 4; u++) M = fmaxf(M, ws[u][0][n]);
-#pragma unroll
-    for (int u = 0; u < 4; u++) L += M > -__builtin_inff() ? ws[u][1][n] * __builtin_amdgcn_exp2f(ws[u][0][n] - M) : ws[u][1][n];
-    if (valid && R.pos[0] >= table) L = __builtin_nanf("");
-    const float f = M > -__builtin_inff() ? __builtin_amdgcn_exp2f(m - M) : 1.0f;
-    float *os = (float *)&kvs[0][0][0];  // [4][16][DP + 4]
     static_assert(sizeof(kvs) >= 4 * 16 * (DP + 4) * 4, "the wavefronts' rows fit the tiles");
-    if (n < sq.nq * G) {
-#pragma unroll
-        for (int dt = 0; dt < DP / 16; dt++) *(v4f *)&os[(w * 16 + n) * (DP + 4) + 16 * dt + 4 * g] = R.o[0][dt] * f;
-    }
-    __syncthreads();
-    const bool direct = !p.part;
-    float fin = 1.0f, Mf = M, Lf = L;
-    if (direct) finish_stat(p, hd, Mf, Lf, fin);
-    // lanes of row n: wavefront w and lane group g take dims 16 w + 4 g + 64 k
-    bool again = false;
-    if (valid) {
-        float *out = direct ? p.dst + tok * p.d_nb2 + hd * p.d_nb1 : p.part + pi * p.D;
-        for (int d = 16 * w + 4 * g; d < p.D; d += 64) {
-            v4f a = {0, 0, 0, 0};
-#pragma unroll
-            for (int u = 0; u < 4; u++) a += *(v4f *)&os[(u * 16 + n) * (DP + 4) + d];
-            a *= fin;
-            __builtin_memcpy(out + d, &a, 16);
-            again = again || odd(a);
-        }
-        if (!direct && w == 0 && g == 0) {
-            p.stat[2 * pi] = M;
-            p.stat[2 * pi + 1] = L;
-        }
-    }
-    // (each wavefront the dims that it stores)
-    if (direct) rows_again<Again<E>>(p, row + 3, again && R.pos[0] < table, tok, hd, R.pos[0], [&](int d) { return (d >> 4 & 3) == w; });
+    few_join<Again<E>, E, DP>(p, R, (float *)&kvs[0][0][0], ws, sq.nq * G, valid, table, tok, hd, pi, row + 3);
 }
 
 // How a tile of a cache of 16-bit elements comes into LDS: straight from memory.

@@ -498,9 +498,10 @@ struct Tile {
     int k0, ke;
 };
 DEV Tile tile_at(const PagedTiles &tl, int t, int kt) {
+    const int a0 = tl.a0, a1 = tl.a1, b0 = tl.b0, b1 = tl.b1, na = tl.na;  // (or the choice is between their addresses, in memory)
     Tile r;
-    r.k0 = t < tl.na ? tl.a0 + t * kt : tl.b0 + (t - tl.na) * kt;
-    r.ke = t < tl.na ? tl.a1 : tl.b1;
+    r.k0 = t < na ? a0 + t * kt : b0 + (t - na) * kt;
+    r.ke = t < na ? a1 : b1;
     return r;
 }
 DEV bool tile_whole(const Tile &tile, int kt, const Pass &ps, int window, int n_first) {
@@ -549,6 +550,57 @@ DEV void rows_again(const FapParams &p, const int32_t *table, bool again, int64_
         const v4f o = A::row(p, table, t, hd, __builtin_amdgcn_readlane(pos, n));
         if (4 * lane < p.D && mine(4 * lane)) __builtin_memcpy(p.dst + t * p.d_nb2 + hd * p.d_nb1 + 4 * lane, &o, 16);
     }
+}
+
+// ---- up to 16 rows a KV head, each wavefront over keys of its own
+
+// The 4 wavefronts' rows: everyone takes the common maximum, then thread (dims, row) adds
+// the four.  os: [4][16][DP + 4]; rows: how many there are; of this lane's row n = lane & 15:
+// is there one, its token, head and place among the partials.
+template <typename A, typename E, int DP>
+DEV void few_join(const FapParams &p, Rows<E, DP, 1> &R, float *os, float (&ws)[4][2][16], int rows, bool valid, int64_t table, int64_t tok, int hd,
+                  int64_t pi, const int32_t *pages) {
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
+    const float l = row_sum(R.l[0]), m = R.from[0] < __builtin_inff() ? row_ref(R.mneg[0]) : -__builtin_inff();
+    if (g == 0) {
+        ws[w][0][n] = m;
+        ws[w][1][n] = l;
+    }
+    __syncthreads();
+    float M = -__builtin_inff(), L = 0.0f;
+#pragma unroll
+    for (int u = 0; u < 4; u++) M = fmaxf(M, ws[u][0][n]);
+#pragma unroll
+    for (int u = 0; u < 4; u++) L += M > -__builtin_inff() ? ws[u][1][n] * __builtin_amdgcn_exp2f(ws[u][0][n] - M) : ws[u][1][n];
+    if (valid && R.pos[0] >= table) L = __builtin_nanf("");
+    const float f = M > -__builtin_inff() ? __builtin_amdgcn_exp2f(m - M) : 1.0f;
+    if (n < rows) {
+#pragma unroll
+        for (int dt = 0; dt < DP / 16; dt++) *(v4f *)&os[(w * 16 + n) * (DP + 4) + 16 * dt + 4 * g] = R.o[0][dt] * f;
+    }
+    __syncthreads();
+    const bool direct = !p.part;
+    float fin = 1.0f, Mf = M, Lf = L;
+    if (direct) finish_stat(p, hd, Mf, Lf, fin);
+    // lanes of row n: wavefront w and lane group g take dims 16 w + 4 g + 64 k
+    bool again = false;
+    if (valid) {
+        float *out = direct ? p.dst + tok * p.d_nb2 + hd * p.d_nb1 : p.part + pi * p.D;
+        for (int d = 16 * w + 4 * g; d < p.D; d += 64) {
+            v4f a = {0, 0, 0, 0};
+#pragma unroll
+            for (int u = 0; u < 4; u++) a += *(v4f *)&os[(u * 16 + n) * (DP + 4) + d];
+            a *= fin;
+            __builtin_memcpy(out + d, &a, 16);
+            again = again || odd(a);
+        }
+        if (!direct && w == 0 && g == 0) {
+            p.stat[2 * pi] = M;
+            p.stat[2 * pi + 1] = L;
+        }
+    }
+    // (each wavefront the dims that it stores)
+    if (direct) rows_again<A>(p, pages, again && R.pos[0] < table, tok, hd, R.pos[0], [&](int d) { return (d >> 4 & 3) == w; });
 }
 
 // ---- up to 64 RW rows: 4 wavefronts of 16 RW rows, 64-key tiles for all
