@@ -3533,7 +3533,7 @@ struct FapParams {
 struct FapMxParams : FapParams {
     const uint8_t *sc;
     int64_t sc_head, sc_row, sc_page;
-    int S;
+    int S, together, wgs, least;
 };
 
 // sc: a quantized cache's scales, else null
@@ -3636,7 +3636,9 @@ FapLayout fap_layout(FapParams &p, int type) {
     L.DP = p.D <= 64 ? 64 : p.D <= 96 && !mx ? 96 : p.D <= 128 ? 128 : 256;
     // bytes of a head's key and value
     const double key_bytes = !mx ? 4.0 * p.D : type == GHIP_TYPE_E4M3 ? 2.0 * p.D + 2 * mx_scale_bytes(p.D) : p.D + 2.0 * mx_scale_bytes(p.D);
-    L.few = (int64_t)p.max_q * G <= 16;
+    // (of a quantized cache up to 32 rows, if there is no prefix to share: a tile of 64 would be empty
+    // by half)
+    L.few = (int64_t)p.max_q * G <= (mx && L.DP <= 128 && !p.n_shared ? 32 : 16);
     const int64_t table = (int64_t)p.per * p.page;
     const int64_t rows = std::min((int64_t)p.T, (int64_t)p.B * p.max_q);
     const double wide = L.DP / 128.0, mem = 4.8e6;  // bytes a microsecond
@@ -3678,6 +3680,8 @@ FapLayout fap_layout(FapParams &p, int type) {
         const int64_t wgs = (int64_t)p.B * p.H_kv, slots = L.DP == 256 ? 256 : 512;
         Way w;
         w.z = keys <= 512 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>({(1024 + wgs - 1) / wgs, (keys + 255) / 256, 32}));
+        // (a quantized cache by itself: splits by length, up to four times an even share for the longest)
+        if (mx && alone) w.z = keys <= 256 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>({(4 * 768 + wgs - 1) / wgs, (keys + 127) / 128, 32}));
         const double steps = (double)((keys + 128 * w.z - 1) / (128 * w.z));
         w.us = std::max((double)((wgs * w.z + slots - 1) / slots) * (6.0 + steps * (1.2 + 0.8 * wide)), key_bytes * wgs * keys / mem) +
                (w.z > 1 || !alone ? join(w.z) : 0.0);
@@ -3766,7 +3770,26 @@ ghip_status fap_run(ghip_context *ctx, const char *call, const ghip_tensor *q, c
         p.part = (float *)ws;
         p.stat = p.part + n * p.D;
     }
-    const int64_t own = (int64_t)p.nb_own * p.H_kv * p.zs_own;
+    int64_t own = (int64_t)p.nb_own * p.H_kv * p.zs_own;
+    p.together = p.wgs = p.least = 0;
+    const int few_rows = (int)std::min<int64_t>((int64_t)p.max_q * (p.H / p.H_kv), 1 << 20);
+    if (sc && L.few) {
+        // Splits: the sequences' tiles shared out over as many workgroups as run at a time (a CU holds 4 of
+        // 64 dims, 3 of 128, 1 or 2 of 256, 2 of more than 16 rows; a multiple of 8 for each head), or twice as
+        // many .. until there are three for each sequence; of 4 tiles, one a wavefront, at least.
+        int64_t parts = (int64_t)p.B * p.zs_own;
+        if (p.zs_own > 1 && !p.wg_sh) {
+            const int64_t slots = 256 * (few_rows > 16 ? 2 : L.DP == 64 ? 4 : L.DP == 128 ? 3 : few_rows <= 4 ? 2 : 1);
+            const int64_t round = std::max<int64_t>(8, slots / p.H_kv / 8 * 8);
+            parts = p.wgs = (int)(std::max<int64_t>(1, (3 * (int64_t)p.B + round - 1) / round) * round);
+            p.least = 4;
+        }
+        // The heads of the same keys follow one another on one XCD (workgroups go to the 8 XCDs in
+        // turn), whose cache then has the keys' scales once: where the parts divide into eights, or nearly so.
+        const int64_t even = (parts + 7) / 8 * 8;
+        p.together = 8 * even <= 9 * parts;
+        own = (p.together ? even : parts) * p.H_kv;
+    }
     // a workgroup of the join for a row that no sequence has costs little, but
     // B max_q can be many times T
     p.join_ragged = p.max_q > 1 && (int64_t)p.B * p.max_q > 2 * (int64_t)p.T;
@@ -3784,7 +3807,8 @@ ghip_status fap_run(ghip_context *ctx, const char *call, const ghip_tensor *q, c
     // ghip_fap_few_f16_128, ghip_fapq_both64_8_128
     const char *set = sc ? "fapq" : "fap", *ty = !sc ? float_name(kv->type) : mx_bits(kv) == 8 ? "8" : "4";
     char name[48];
-    if (L.few && !p.wg_sh) snprintf(name, sizeof name, "ghip_%s_few_%s_%d", set, ty, L.DP);
+    if (L.few && !p.wg_sh && sc) snprintf(name, sizeof name, "ghip_fapq_few%d_%s_%d", few_rows <= 4 ? 4 : few_rows <= 8 ? 8 : few_rows <= 16 ? 16 : 32, ty, L.DP);
+    else if (L.few && !p.wg_sh) snprintf(name, sizeof name, "ghip_fap_few_%s_%d", ty, L.DP);
     else snprintf(name, sizeof name, "ghip_%s_%s%d_%s_%d", set, L.few ? "both" : "tile", L.rows, ty, L.DP);
     auto launch = [&](int64_t wgs) {
         if (sc) return ctx->launch(name, dim3((unsigned)wgs), dim3(256), 0, s, p);

@@ -273,7 +273,7 @@ DEV void fap_few(const FapParams &p, FewLds<DP> &lds) {
         }
     }
     static_assert(sizeof(kvs) >= 4 * 16 * (DP + 4) * 4, "the wavefronts' rows fit the tiles");
-    few_join<Again<E>, E, DP>(p, R, (float *)&kvs[0][0][0], ws, sq.nq * G, valid, table, tok, hd, pi, row + 3);
+    few_join<Again<E>, E, DP, 1>(p, R, 0, (float *)&kvs[0][0][0], ws, sq.nq * G, valid, table, tok, hd, pi, row + 3);
 }
 
 // How a tile of a cache of 16-bit elements comes into LDS: straight from memory.

@@ -554,14 +554,14 @@ DEV void rows_again(const FapParams &p, const int32_t *table, bool again, int64_
 
 // ---- up to 16 rows a KV head, each wavefront over keys of its own
 
-// The 4 wavefronts' rows: everyone takes the common maximum, then thread (dims, row) adds
-// the four.  os: [4][16][DP + 4]; rows: how many there are; of this lane's row n = lane & 15:
+// The 4 wavefronts' rows of row tile rt: everyone takes the common maximum, then thread (dims, row)
+// adds the four.  os: [4][16][DP + 4]; rows: how many there are; of this lane's row n = lane & 15:
 // is there one, its token, head and place among the partials.
-template <typename A, typename E, int DP>
-DEV void few_join(const FapParams &p, Rows<E, DP, 1> &R, float *os, float (&ws)[4][2][16], int rows, bool valid, int64_t table, int64_t tok, int hd,
-                  int64_t pi, const int32_t *pages) {
+template <typename A, typename E, int DP, int RW>
+DEV void few_join(const FapParams &p, Rows<E, DP, RW> &R, int rt, float *os, float (&ws)[4][2][16], int rows, bool valid, int64_t table, int64_t tok,
+                  int hd, int64_t pi, const int32_t *pages) {
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
-    const float l = row_sum(R.l[0]), m = R.from[0] < __builtin_inff() ? row_ref(R.mneg[0]) : -__builtin_inff();
+    const float l = row_sum(R.l[rt]), m = R.from[rt] < __builtin_inff() ? row_ref(R.mneg[rt]) : -__builtin_inff();
     if (g == 0) {
         ws[w][0][n] = m;
         ws[w][1][n] = l;
@@ -572,11 +572,11 @@ DEV void few_join(const FapParams &p, Rows<E, DP, 1> &R, float *os, float (&ws)[
     for (int u = 0; u < 4; u++) M = fmaxf(M, ws[u][0][n]);
 #pragma unroll
     for (int u = 0; u < 4; u++) L += M > -__builtin_inff() ? ws[u][1][n] * __builtin_amdgcn_exp2f(ws[u][0][n] - M) : ws[u][1][n];
-    if (valid && R.pos[0] >= table) L = __builtin_nanf("");
+    if (valid && R.pos[rt] >= table) L = __builtin_nanf("");
     const float f = M > -__builtin_inff() ? __builtin_amdgcn_exp2f(m - M) : 1.0f;
     if (n < rows) {
 #pragma unroll
-        for (int dt = 0; dt < DP / 16; dt++) *(v4f *)&os[(w * 16 + n) * (DP + 4) + 16 * dt + 4 * g] = R.o[0][dt] * f;
+        for (int dt = 0; dt < DP / 16; dt++) *(v4f *)&os[(w * 16 + n) * (DP + 4) + 16 * dt + 4 * g] = R.o[rt][dt] * f;
     }
     __syncthreads();
     const bool direct = !p.part;
@@ -600,7 +600,7 @@ DEV void few_join(const FapParams &p, Rows<E, DP, 1> &R, float *os, float (&ws)[
         }
     }
     // (each wavefront the dims that it stores)
-    if (direct) rows_again<A>(p, pages, again && R.pos[0] < table, tok, hd, R.pos[0], [&](int d) { return (d >> 4 & 3) == w; });
+    if (direct) rows_again<A>(p, pages, again && R.pos[rt] < table, tok, hd, R.pos[rt], [&](int d) { return (d >> 4 & 3) == w; });
 }
 
 // ---- up to 64 RW rows: 4 wavefronts of 16 RW rows, 64-key tiles for all

@@ -7,7 +7,10 @@
 struct FapMxParams : FapParams {
     const uint8_t *sc;
     int64_t sc_head, sc_row, sc_page;
-    int S;  // scale bytes of a key
+    int S;         // scale bytes of a key
+    int together;  // few rows: the heads of the same keys follow one another on one XCD
+    int wgs;       // ... workgroups of a head, which share out the sequences' tiles; 0: zs_own a sequence
+    int least;     // ... tiles of a workgroup at least
 };
 
 // One row of q, a wavefront: as the formula says, in 32 bits, a lane a key for the
@@ -104,10 +107,11 @@ struct Alone {
 
 // Where the keys of a tile are, a lane a key (its page: pg): bytes into the codes and the
 // scales of its row.  Keys past the tile's end or on no page: row 0 of page 0, which is not used.
-DEV void find_keys_mx(const FapMxParams &p, const Tile &tl, int kt, int pg, int64_t *offs, int64_t *soffs, uint64_t &ok, uint64_t &bad) {
+DEV void find_keys_mx(const FapMxParams &p, const Tile &tl, int kt, int pg, int64_t *offs, int64_t *soffs, uint64_t &ok, uint64_t &bad,
+                      bool any = true) {
     const int lane = threadIdx.x & 63;
     const uint32_t j = tl.k0 + lane;
-    const bool in = lane < kt && (int)j < tl.ke;
+    const bool in = any && lane < kt && (int)j < tl.ke;
     const bool there = in && pg >= 0 && pg < p.n_pages;
     ok = __ballot(there);
     bad = __ballot(in && !there);
@@ -117,61 +121,261 @@ DEV void find_keys_mx(const FapMxParams &p, const Tile &tl, int kt, int pg, int6
         soffs[lane] = there ? pg * p.sc_page + r * p.sc_row : 0;
     }
 }
+// Words and bytes of the cache.  The address has been through LDS, and of that the compiler cannot
+// tell that it is not LDS itself: said to be global memory, or the loads count as LDS's too
+// and each wait for LDS waits for memory (24 sequences of 500 .. 16384 keys: 118 us).
+typedef const __attribute__((address_space(1))) uint8_t *in_memory;
 template <int W>
 DEV void load_words(uint32_t (&w)[W], const uint8_t *from) {
-    __builtin_memcpy(w, from, 4 * W);
+    typedef uint32_t words __attribute__((ext_vector_type(W)));
+    const words x = *(const __attribute__((address_space(1))) words *)from;
+#pragma unroll
+    for (int i = 0; i < W; i++) w[i] = x[i];
+}
+DEV uint32_t load_byte(const uint8_t *from) { return *(in_memory)from; }
+
+// ---- up to 16 RW rows a KV head: 4 wavefronts, each its own tiles of KT keys
+
+// 64 keys a tile are twice the bytes in flight and half the work of finding them; of 8-bit codes
+// they are too many registers for three wavefronts a SIMD.
+constexpr int few_keys(int bits, int DP) { return DP == 256 || bits == 8 ? 32 : 64; }
+
+// Which part of the keys a workgroup takes: split z (of `of`) of sequence b, its tiles [t0, t1).
+// With p.wgs the sequences' tiles are shared out over that many workgroups, each sequence having
+// as many splits as its tiles are worth: of splits alike for all, the longest sequence's are the last to
+// end (24 sequences of 500 .. 16384 keys: 108 us).
+struct Part {
+    int b, z, of, t0, t1;
+};
+template <int KT>
+DEV bool find_part(const FapMxParams &p, int no, Part &w) {
+    const int lane = threadIdx.x & 63;
+    const int64_t table = (int64_t)p.per * p.page;
+    // a sequence's tiles; one at least, whose workgroup says that the rows see nothing
+    auto tiles_of = [&](int b) {
+        const PagedSeq sq = seq_of(p, b);
+        if (sq.nq == 0) return 0;
+        return max(1, paged_tiles(clip_pos(sq.pos0, table), clip_pos(sq.pos0 + sq.nq - 1, table), p.window, p.n_first, p.n_shared, (int)table, KT).n);
+    };
+    if (!p.wgs) {
+        w.b = no / p.zs_own;
+        w.z = no - w.b * p.zs_own;
+        w.of = p.zs_own;
+        if (w.b >= p.B) return false;
+        const int n = tiles_of(w.b), share = paged_share(n, w.of);
+        w.t0 = (int)min((int64_t)w.z * share, (int64_t)n);
+        w.t1 = min(n, w.t0 + share);
+        return n > 0;
+    }
+    int64_t total = 0;
+    int live = 0;
+    const int first = lane < p.B ? tiles_of(lane) : 0;
+    for (int b0 = 0; b0 < p.B; b0 += 64) {
+        int n = b0 == 0 ? first : b0 + lane < p.B ? tiles_of(b0 + lane) : 0;
+        live += __popcll(__ballot(n > 0));
+#pragma unroll
+        for (int o = 32; o; o >>= 1) n += __shfl_xor(n, o, 64);
+        total += n;
+    }
+    // The fewest tiles a part that need no more parts than there are workgroups: with total / (wgs - live)
+    // they never do; up to 64 sequences the least is looked for.
+    const int64_t room = max(p.wgs - live, 1);
+    int64_t each = max((total + room - 1) / room, (int64_t)p.least);
+    if (p.B <= 64) {
+        int lo = max((int)((total + p.wgs - 1) / p.wgs), p.least), hi = (int)each;
+        while (lo < hi) {
+            const int mid = (lo + hi) / 2;
+            int parts = (first + mid - 1) / mid;
+#pragma unroll
+            for (int o = 32; o; o >>= 1) parts += __shfl_xor(parts, o, 64);
+            if (parts <= p.wgs) hi = mid;
+            else lo = mid + 1;
+        }
+        each = hi;
+    }
+    int base = 0;
+    for (int b0 = 0; b0 < p.B && base <= no; b0 += 64) {
+        const int n = b0 == 0 ? first : b0 + lane < p.B ? tiles_of(b0 + lane) : 0;
+        const int parts = (int)min((n + each - 1) / each, (int64_t)p.zs_own);
+        int to = parts;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int y = __shfl_up(to, o, 64);
+            if (lane >= o) to += y;
+        }
+        const uint64_t here = __ballot(base + to - parts <= no && no < base + to);
+        if (here) {
+            const int at = __builtin_ctzll(here), tiles = __builtin_amdgcn_readlane(n, at);
+            w.b = b0 + at;
+            w.of = __builtin_amdgcn_readlane(parts, at);
+            w.z = no - base - __builtin_amdgcn_readlane(to - parts, at);
+            const int share = paged_share(tiles, w.of);
+            w.t0 = (int)min((int64_t)w.z * share, (int64_t)tiles);
+            w.t1 = min(tiles, w.t0 + share);
+            return true;
+        }
+        base += __builtin_amdgcn_readlane(to, 63);
+    }
+    return false;
 }
 
-// ---- up to 16 rows a KV head: 4 wavefronts, each its own 32-key tiles
+// The products have 16 columns for rows.  Where there are 16 / CG rows at most, the columns are CG
+// groups of them: group j has term j of q and of p, and one product does what takes three (CG 4; its
+// fourth group is not used) or two of three (CG 2: the third term in a product of its own, group 1).
+// A score is then the sum over the groups, taken pair by pair so that all have the same bits.
+template <int CG>
+DEV float all_groups(float x) {
+    if (CG > 1) x += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x128, 0xf, 0xf, true));  // the lane 8 on, of 16
+    if (CG > 2) x += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x124, 0xf, 0xf, true));  // 4 on
+    return x;
+}
+// products for the three terms
+template <int CG>
+constexpr int few_products() { return CG == 4 ? 1 : CG == 2 ? 2 : 3; }
+// x's term for this lane's group in each product; j1, j2: 1 in the groups that leave the first term
+// (and the second) to others, else 0
+template <int CG>
+DEV void group_terms(v2f x, float j1, float j2, Frag<bf16>::v2 (&t)[few_products<CG>()]) {
+    typedef Frag<bf16>::v2 v2;
+    if constexpr (CG == 1) {
+        split_pair<bf16, 3>(x[0], x[1], t);
+    } else {
+        v2 y = __builtin_convertvector(x, v2);
+#pragma unroll
+        for (int k = 0; k < 2; k++) x[k] = fmaf((float)y[k], -j1, x[k]);
+        y = __builtin_convertvector(x, v2);
+        if (CG == 2) t[0] = y;
+#pragma unroll
+        for (int k = 0; k < 2; k++) x[k] = CG == 2 ? fmaf((float)y[k], -1.0f, x[k]) * j1 : fmaf((float)y[k], -j2, x[k]);
+        t[few_products<CG>() - 1] = __builtin_convertvector(x, v2);
+    }
+}
+// O^T += V^T P^T over 32 keys at Vs, p a group's terms
+template <int DP, int CG>
+DEV void group_values(v4f (&o)[DP / 16], uint32_t Vs, const v4f &s0, const v4f &s1, float j1, float j2) {
+    typedef Frag<bf16> F;
+    constexpr int NM = few_products<CG>();
+    const uint32_t vat = v_at<DP>(Vs);
+    F::v8 p[NM];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const v4f &s = e < 2 ? s0 : s1;
+        F::v2 t[NM];
+        group_terms<CG>(v2f{s[2 * (e & 1)], s[2 * (e & 1) + 1]}, j1, j2, t);
+#pragma unroll
+        for (int i = 0; i < NM; i++) {
+            p[i][2 * e] = t[i][0];
+            p[i][2 * e + 1] = t[i][1];
+        }
+    }
+    F::v8 a[3];
+    a[0] = value_frag<bf16, DP>(vat, 0, 0);
+    a[1] = value_frag<bf16, DP>(vat, 0, 1);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int dt = 0; dt < DP / 16; dt++) {
+        if (dt + 2 < DP / 16) a[(dt + 2) % 3] = value_frag<bf16, DP>(vat, 0, dt + 2);
+#pragma unroll
+        for (int i = NM - 1; i >= 0; i--) o[dt] = F::mfma(a[dt % 3], p[i], o[dt]);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
 
-template <int DP>
+// A tile's rows (a key's codes, then its value's) as they lie, 16-byte chunk c of row r at place raw_swz of CH:
+// reads of one chunk of 16 rows then touch each bank once.
+template <int CH>
+DEV int raw_swz(int r, int c) {
+    return CH == 4 ? c ^ ((r >> 2) & 3) : CH == 8 ? c ^ ((r >> 1) & 7) : c ^ (r & 15);
+}
+template <int BITS, int DP, int CG, int RW>
 struct FewqLds {
-    uint8_t v[4 * 64 * (DP + 4)];  // each wavefront's values as bfloat16 [32][DP]; at the end their rows
-    int64_t offs[4][2][32];
+    uint8_t v[4][64 * DP + (CG == 1 ? 256 : 0)];         // each wavefront's rows as they lie, then 32 values as bfloat16; at the end its sums
+    uint8_t q[RW][DP / 32][few_products<CG>()][1024];    // the fragments of q, the same for all wavefronts
+    int64_t offs[4][2][few_keys(BITS, DP)];
+    uint8_t sc[4][few_keys(BITS, DP)][DP / 16];  // a tile's scales: a row of 2 S bytes for each key
     float ws[4][2][16];
 };
-template <int BITS, int DP>
-DEV void fapq_few(const FapMxParams &p, FewqLds<DP> &lds) {
+template <int BITS, int DP, int CG, int RW>
+DEV void fapq_few(const FapMxParams &p, FewqLds<BITS, DP, CG, RW> &lds) {
+    static_assert(RW == 1 || CG == 1, "more than 16 rows have no columns to spare");
     // A lane's codes of a key: NU units of EL elements, unit g + 4 i; fragment kk of the products takes 8 of
     // them, and so does q's.
-    constexpr int KT = 32, CH = DP / 8, EL = BITS == 4 && DP >= 128 ? 32 : 16, NU = DP / EL / 4, FU = EL / 8, WK = EL * BITS / 32;
-    // ... of the values: unit lane % U of keys lane / U + (64 / U) ii
-    constexpr int U = DP / 16, NV = KT * U / 64, WV = BITS / 2;
+    constexpr int KT = few_keys(BITS, DP), NT = KT / 16, CH = DP / 8, EL = BITS == 4 && DP >= 128 ? 32 : 16, NU = DP / EL / 4, FU = EL / 8,
+                  WK = EL * BITS / 32;
+    // ... of the values: unit lane % U of keys lane / U + (64 / U) ii, NVH loads for 32 keys
+    constexpr int U = DP / 16, NV = KT * U / 64, NVH = U / 2, WV = BITS / 2;
+    constexpr int SB = DP / 16;  // bytes of a key's and its value's scales (of up to 32 dims: half of that)
+    constexpr int NM = few_products<CG>(), ROWS = 16 / CG;
     auto &offs = lds.offs;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
     const int G = p.H / p.H_kv;
     const int64_t table = (int64_t)p.per * p.page;
-    const int id = blockIdx.x - p.wg_sh, hk = id % p.H_kv, z = (id / p.H_kv) % p.zs_own, b = id / (p.H_kv * p.zs_own);
-    const int32_t *row = p.seqs + (int64_t)b * p.seq_nb1;
+    const int id = blockIdx.x - p.wg_sh, k = p.together ? id >> 3 : id, hk = k % p.H_kv;
+    Part part;
+    if (!find_part<KT>(p, p.together ? (k / p.H_kv) * 8 + (id & 7) : k / p.H_kv, part)) return;
+    const int32_t *row = p.seqs + (int64_t)part.b * p.seq_nb1;
     const PagedSeq sq = paged_seq(row[0], row[1], row[2], p.T, p.max_q);
-    if (sq.nq == 0) return;
     Pass ps;
     ps.p0 = clip_pos(sq.pos0, table);
     ps.p1 = clip_pos(sq.pos0 + sq.nq - 1, table);
     ps.tl = paged_tiles(ps.p0, ps.p1, p.window, p.n_first, p.n_shared, (int)table, KT);
-    const int share = paged_share(ps.tl.n, p.zs_own);
-    const int t0 = (int)min((int64_t)z * share, (int64_t)ps.tl.n), t1 = min(ps.tl.n, t0 + share);
-    const int i = n / G, hd = hk * G + n % G;
-    const bool valid = n < sq.nq * G;
-    const int64_t tok = sq.q0 + (valid ? i : 0);
-    const int64_t pi = (tok * p.H + hd) * (p.zs_sh + p.zs_own) + p.zs_sh + z;
-    if (t0 >= t1 && p.part) {  // nothing in this split
-        if (valid && w == 0 && g == 0) stat_none(p, pi, sq.pos0 + i >= table);
-        return;
-    }
-    Rows<bf16, DP, 1> R;
-    R.pos[0] = valid ? clip_pos(sq.pos0 + i, table) : -1;
-    RawRow<DP> raw;
-    const float *qr = p.q + tok * p.q_nb2 + hd * p.q_nb1;
+    const int t0 = part.t0, t1 = min(part.t1, ps.tl.n);
+    // this lane's row of row tile rt
+    const int j = n / ROWS;
+    struct Row {
+        int hd, i;
+        bool there, valid;  // is there one; does the lane stand for it
+        int64_t tok, pi;
+    };
+    auto row_of = [&](int rt) {
+        Row y;
+        const int r = 16 * rt + n % ROWS;
+        y.i = r / G;
+        y.hd = hk * G + r % G;
+        y.there = r < sq.nq * G;
+        y.valid = y.there && j == 0;
+        y.tok = sq.q0 + (y.there ? y.i : 0);
+        y.pi = (y.tok * p.H + y.hd) * (p.zs_sh + p.zs_own) + p.zs_sh + part.z;
+        return y;
+    };
+    Rows<bf16, DP, RW> R;  // (its q: in LDS)
 #pragma unroll
-    for (int kk = 0; kk < DP / 32; kk++) {
-        const int d = EL * (g + 4 * (kk / FU)) + 8 * (kk % FU);
+    for (int rt = 0; rt < RW; rt++) {
+        const Row y = row_of(rt);
+        if (part.z == part.of - 1 && y.valid)  // no more splits of this sequence
+            for (int z = part.of + 4 * w + g; z < p.zs_own; z += 16) stat_none(p, y.pi - part.z + z, sq.pos0 + y.i >= table);
+        if (t0 >= t1 && p.part && y.valid && w == 0 && g == 0) stat_none(p, y.pi, sq.pos0 + y.i >= table);
+        R.pos[rt] = y.there ? clip_pos(sq.pos0 + y.i, table) : -1;
+        R.mneg[rt] = v4f{0, 0, 0, 0};
+        R.l[rt] = 0.0f;
+        R.from[rt] = R.pos[rt] < 0 ? -__builtin_inff() : __builtin_inff();
 #pragma unroll
-        for (int e = 0; e < 8; e++) raw.x[kk][e] = 0.0f;
-        if (valid && d < p.D) __builtin_memcpy(raw.x[kk], qr + d, 32);
+        for (int dt = 0; dt < DP / 16; dt++) R.o[rt][dt] = v4f{0, 0, 0, 0};
     }
+    if (t0 >= t1 && p.part) return;  // nothing in this split
+    const float j1 = j >= 1, j2 = j >= 2;
+    for (int f = w; f < RW * DP / 32; f += 4) {
+        const int rt = f / (DP / 32), kk = f % (DP / 32), d = EL * (g + 4 * (kk / FU)) + 8 * (kk % FU);
+        const Row y = row_of(rt);
+        float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (y.there && d < p.D && j < 3) __builtin_memcpy(x, p.q + y.tok * p.q_nb2 + y.hd * p.q_nb1 + d, 32);
+        Frag<bf16>::v8 terms[NM];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            Frag<bf16>::v2 t[NM];
+            group_terms<CG>(v2f{x[2 * e], x[2 * e + 1]} * (p.scale * kLog2e), j1, j2, t);
+#pragma unroll
+            for (int m = 0; m < NM; m++) {
+                terms[m][2 * e] = t[m][0];
+                terms[m][2 * e + 1] = t[m][1];
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < NM; m++) *(Frag<bf16>::v8 *)&lds.q[rt][kk][m][16 * lane] = terms[m];
+    }
+    __syncthreads();
     const uint8_t *kvh = (const uint8_t *)p.kv + hk * p.kv_head, *sch = p.sc + hk * p.sc_head;
-    uint8_t *Vs = lds.v + w * (64 * DP);
+    uint8_t *Vs = lds.v[w];
     const uint32_t va = lds_addr(Vs);
 
     auto load_page = [&](int t) {  // page number of a key of tile t, a lane each
@@ -180,75 +384,154 @@ DEV void fapq_few(const FapMxParams &p, FewqLds<DP> &lds) {
     };
     uint64_t ok = 0, bad = 0;  // the next tile's keys that are there, those on no page
     const int units = (p.D + EL - 1) / EL, uv = min(lane % U, p.D / 16 - 1);
-    uint32_t kw[2][NU][WK], ks[2][NU], vw[NV][WV], vs[NV];
-    auto load_k = [&]() {
+    // A tile is loaded as whole rows, 16 bytes a lane and a row's bytes in neighbouring lanes (loads of the
+    // fragments' own places, 64 bytes of a line each, were twice the requests: 64 sequences of
+    // 8192 keys in 4 bits 162 us), and goes through LDS to the lanes that need it.
+    constexpr int RCH = DP * BITS / 64, RS = 16 * RCH, KPI = 64 / RCH, NLD = KT / KPI;
+    uint32_t st[NLD][4], sc[SB / 4];  // (sc: a lane a key)
+    const int chunk = 16 * min(lane % RCH, p.D * BITS / 64 - 1);
+    auto load_tile = [&]() {
 #pragma unroll
-        for (int t = 0; t < 2; t++) {
-            const uint8_t *at = kvh + offs[w][0][16 * t + n], *sat = sch + offs[w][1][16 * t + n];
-#pragma unroll
-            for (int u = 0; u < NU; u++) {
-                const int un = min(g + 4 * u, units - 1);
-                load_words(kw[t][u], at + un * (EL * BITS / 8));
-                ks[t][u] = sat[un * EL / 32];
-            }
+        for (int ii = 0; ii < NLD; ii++) {
+            load_words(st[ii], kvh + offs[w][0][lane / RCH + KPI * ii] + chunk);
+            if (ii & 1) __builtin_amdgcn_sched_barrier(0);
+        }
+        const uint8_t *at = sch + offs[w][1][lane % KT];
+        if constexpr (DP == 64) {
+            typedef const __attribute__((address_space(1))) uint16_t *halves;
+            sc[0] = *(halves)at | (uint32_t)*(halves)(at + (p.S & 2)) << 16;
+        } else {
+            load_words(sc, at);
         }
     };
-    auto load_v = [&]() {
-#pragma unroll
-        for (int ii = 0; ii < NV; ii++) {
-            const int key = lane / U + 64 / U * ii;
-            load_words(vw[ii], kvh + offs[w][0][key] + (p.D + 16 * uv) * BITS / 8);
-            vs[ii] = sch[offs[w][1][key] + p.S + uv / 2];
-        }
-    };
+    // (a later load's row differs in bits of its own, and so does its swizzle)
+    const int rkey = lane / RCH, rto = rkey * RS + 16 * raw_swz<RCH>(rkey, lane % RCH);
+    // the scales go through LDS, from where each lane reads the byte that it needs
+    const int vkey = lane / U, vto = 2 * vkey * DP + 16 * v_swz<CH>(vkey, 2 * (lane % U));  // of load 0: a later one's row differs in bits of its own
+    const uint8_t *scw = &lds.sc[w][0][0];
+    const int vat = p.D * BITS / 8 + uv * 2 * BITS, vfrom = vkey * RS + 16 * raw_swz<RCH>(vkey, vat / 16) + vat % 16;
     const int first = t0 + w;
     int pg = 0;
     if (first < t1) {
         find_keys_mx(p, tile_at(ps.tl, first, KT), KT, load_page(first), offs[w][0], offs[w][1], ok, bad);
         pg = load_page(first + 4);
-        load_k();
-        load_v();
+        load_tile();
     }
-    rows_start<bf16, DP, 1>(R, 0, raw, p.scale * kLog2e);
     for (int t = first; t < t1; t += 4) {
         const Tile tile = tile_at(ps.tl, t, KT);
         const uint64_t okc = ok, badc = bad;
-        const bool more = t + 4 < t1;
-        v4f s[2][1];
 #pragma unroll
-        for (int kk = 0; kk < DP / 32; kk++)
+        for (int ii = 0; ii < NLD; ii++)
+            __builtin_memcpy(Vs + (rto ^ (16 * raw_swz<RCH>(KPI * ii, 0))) + KPI * ii * RS, st[ii], 16);
+        if (KT == 64 || lane < KT) __builtin_memcpy(lds.sc[w][lane % KT], sc, SB);
+        // The next tile's loads, after the last one too (then all of one row): with branches around them the
+        // compiler cannot count them and waits for all.
+        find_keys_mx(p, tile_at(ps.tl, t + 4, KT), KT, pg, offs[w][0], offs[w][1], ok, bad, t + 4 < t1);
+        pg = load_page(t + 8);
+        load_tile();
+        __builtin_amdgcn_sched_barrier(0);
+        const uint8_t *kscale[NU], *kraw[NU], *vscale = scw + vkey * SB + p.S + uv / 2;
 #pragma unroll
-            for (int x = 0; x < 2; x++) {
-                const mx_bf8 a = mx_eight<BITS>(&kw[x][kk / FU][kk % FU * (BITS / 4)], mx_scale(ks[x][kk / FU]));
+        for (int u = 0; u < NU; u++) {
+            const int un = min(g + 4 * u, units - 1), at = un * (EL * BITS / 8);
+            kscale[u] = scw + n * SB + un * EL / 32;
+            kraw[u] = Vs + n * RS + 16 * raw_swz<RCH>(n, at / 16) + at % 16;
+        }
+        // (the reference: in one group)
+        v4f start[RW];
 #pragma unroll
-                for (int j = Frag<bf16>::NQ - 1; j >= 0; j--)
-                    s[x][0] = Frag<bf16>::mfma(a, R.q[0][kk][j], kk > 0 || j < Frag<bf16>::NQ - 1 ? s[x][0] : R.start(0));
+        for (int rt = 0; rt < RW; rt++) {
+            const float ref = CG == 1 || j == 0 ? R.mneg[rt][0] : 0.0f;
+            start[rt] = CG == 1 ? R.mneg[rt] : v4f{ref, ref, ref, ref};
+        }
+        v4f s[NT][RW];
+#pragma unroll
+        for (int u = 0; u < NU; u++) {
+            float f[NT];
+            uint32_t kw[NT][WK];
+#pragma unroll
+            for (int x = 0; x < NT; x++) {
+                f[x] = mx_scale(kscale[u][16 * x * SB]);
+                __builtin_memcpy(kw[x], kraw[u] + 16 * x * RS, 4 * WK);
             }
-        if (more) {
-            find_keys_mx(p, tile_at(ps.tl, t + 4, KT), KT, pg, offs[w][0], offs[w][1], ok, bad);
-            pg = load_page(t + 8);
-            load_k();
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        const bool part = !tile_whole(tile, KT, ps, p.window, p.n_first);
-        if (part || badc) mask_scores<bf16, DP, 1, 2>(R, s, tile.k0, tile.ke, badc, p.window, p.n_first);
-        softmax<bf16, DP, 1, 2>(R, s, va, []() {});
 #pragma unroll
-        for (int ii = 0; ii < NV; ii++) {
-            const int key = lane / U + 64 / U * ii;
-            const float f = mx_scale(vs[ii]);
-            mx_bf8 lo = mx_eight<BITS>(&vw[ii][0], f), hi = mx_eight<BITS>(&vw[ii][WV / 2], f);
-            // rows that were not there: no value of theirs may count
-            if (!((okc >> key) & 1)) lo = hi = mx_bf8{};
-            mx_bf8 *to = (mx_bf8 *)(Vs + 2 * key * DP + 16 * v_swz<CH>(key, 2 * (lane % U)));
-            to[0] = lo;
-            to[1] = hi;
+            for (int e = 0; e < FU; e++) {
+                const int kk = u * FU + e;
+                Frag<bf16>::v8 q[RW][NM];
+#pragma unroll
+                for (int rt = 0; rt < RW; rt++)
+#pragma unroll
+                    for (int m = 0; m < NM; m++) q[rt][m] = *(const Frag<bf16>::v8 *)&lds.q[rt][kk][m][16 * lane];
+#pragma unroll
+                for (int x = 0; x < NT; x++) {
+                    const mx_bf8 a = mx_eight<BITS>(&kw[x][e * (BITS / 4)], f[x]);
+#pragma unroll
+                    for (int m = NM - 1; m >= 0; m--)
+#pragma unroll
+                        for (int rt = 0; rt < RW; rt++)
+                            s[x][rt] = Frag<bf16>::mfma(a, q[rt][m], kk > 0 || m < NM - 1 ? s[x][rt] : start[rt]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
         }
-        if (more) load_v();
+        uint32_t vw[NV][WV];
+#pragma unroll
+        for (int ii = 0; ii < NV; ii++)
+            __builtin_memcpy(vw[ii], Vs + (vfrom ^ (16 * raw_swz<RCH>(64 / U * ii, 0))) + 64 / U * ii * RS, 4 * WV);
         __builtin_amdgcn_sched_barrier(0);
-        values<bf16, DP, 1, 2>(R, va, s);
+        if constexpr (CG > 1)
+#pragma unroll
+            for (int x = 0; x < NT; x++)
+#pragma unroll
+                for (int v = 0; v < 4; v++) s[x][0][v] = all_groups<CG>(s[x][0][v]);
+        if (badc || !tile_whole(tile, KT, ps, p.window, p.n_first)) mask_scores<bf16, DP, RW, NT>(R, s, tile.k0, tile.ke, badc, p.window, p.n_first);
+        softmax<bf16, DP, RW, NT>(R, s, va, []() {});
+        // 32 values at a time through LDS
+#pragma unroll
+        for (int h = 0; h < KT / 32; h++) {
+#pragma unroll
+            for (int ii = h * NVH; ii < (h + 1) * NVH; ii++) {
+                const float f = mx_scale(vscale[64 / U * ii * SB]);
+                mx_bf8 *to = (mx_bf8 *)(Vs + (vto ^ (16 * v_swz<CH>(64 / U * ii, 0))) + 64 / U * (ii - h * NVH) * 2 * DP);
+                to[0] = mx_eight<BITS>(&vw[ii][0], f);
+                to[1] = mx_eight<BITS>(&vw[ii][WV / 2], f);
+            }
+            // rows that were not there: no value of theirs may count
+            if (const uint32_t miss = ~(uint32_t)(okc >> (32 * h))) {
+                int l = lane;
+                asm volatile("" : "+v"(l));  // (or what follows is worked out before the loop, into registers that the loop needs)
+                for (int c = l; c < 32 * CH; c += 64)
+                    if ((miss >> (c / CH)) & 1) *(uint4 *)(Vs + 16 * c) = make_uint4(0, 0, 0, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            uint32_t at = va;
+            asm volatile("" : "+v"(at));  // (the fragments' addresses likewise)
+            if constexpr (CG > 1) {
+                group_values<DP, CG>(R.o[0], at, s[2 * h][0], s[2 * h + 1][0], j1, j2);
+            } else {
+                v4f y[2][RW];
+#pragma unroll
+                for (int rt = 0; rt < RW; rt++) {
+                    y[0][rt] = s[2 * h][rt];
+                    y[1][rt] = s[2 * h + 1][rt];
+                }
+                values<bf16, DP, RW, 2>(R, at, y);
+            }
+        }
     }
-    few_join<Alone<BITS>, bf16, DP>(p, R, (float *)lds.v, lds.ws, sq.nq * G, valid, table, tok, hd, pi, row + 3);
+    if constexpr (CG > 1) {
+#pragma unroll
+        for (int dt = 0; dt < DP / 16; dt++)
+#pragma unroll
+            for (int v = 0; v < 4; v++) R.o[0][dt][v] = all_groups<CG>(CG == 4 && j == 3 ? 0.0f : R.o[0][dt][v]);
+    }
+    static_assert(sizeof(lds.v) >= ((3 * 16 + 16 / CG - 1) * (DP + 4) + DP) * 4, "the wavefronts' rows fit their values");
+#pragma unroll
+    for (int rt = 0; rt < RW; rt++) {
+        const Row y = row_of(rt);
+        if (rt) __syncthreads();  // (the sums of the row tile before have been read)
+        few_join<Alone<BITS>, bf16, DP, RW>(p, R, rt, (float *)lds.v, lds.ws, sq.nq * G - 16 * rt, y.valid, table, y.tok, y.hd, y.pi, row + 3);
+    }
 }
 
 // How a tile comes into LDS: its codes go into registers, 16 elements a lane (load ii of wavefront
@@ -298,10 +581,10 @@ struct Decoded {
         DEV_M void load_part(int t, int f) {
             if (f < NL) {
                 load_words(kw[f], at[f]);
-                ks[f] = *sat[f];
+                ks[f] = load_byte(sat[f]);
             } else if (f < 2 * NL) {
                 load_words(vw[f - NL], at[f - NL] + p.D * BITS / 8);
-                vs[f - NL] = sat[f - NL][p.S];
+                vs[f - NL] = load_byte(sat[f - NL] + p.S);
             }
         }
         DEV_M void load_tile(int t) {
@@ -332,26 +615,28 @@ extern "C" __global__ void __launch_bounds__(256) ghip_fapq_join_4(FapMxParams p
 
 template <int BITS, int DP, int RW>
 union FapqLds {
-    FewqLds<DP> few;
+    FewqLds<BITS, DP, 1, 1> few;
     TileLds<Decoded<BITS>, DP, RW> tile;
 };
-#define FAPQ_FEW(B, DP, WG)                                                                            \
-    extern "C" __global__ void __launch_bounds__(256, WG) ghip_fapq_few_##B##_##DP(FapMxParams p) {    \
-        __shared__ __attribute__((aligned(1024))) uint8_t lds[sizeof(FewqLds<DP>)];                   \
-        fapq_few<B, DP>(p, *(FewqLds<DP> *)lds);                                                      \
+// (ROWS: up to how many, 16 RW / CG; WG: workgroups a CU)
+#define FAPQ_FEW(B, DP, CG, RW, ROWS, WG)                                                                          \
+    extern "C" __global__ void __launch_bounds__(256, WG) ghip_fapq_few##ROWS##_##B##_##DP(FapMxParams p) {        \
+        __shared__ __attribute__((aligned(1024))) uint8_t lds[sizeof(FewqLds<B, DP, CG, RW>)];                       \
+        fapq_few<B, DP, CG, RW>(p, *(FewqLds<B, DP, CG, RW> *)lds);                                              \
     }
+#define FAPQ_FEWS(B, DP, WG) FAPQ_FEW(B, DP, 4, 1, 4, WG) FAPQ_FEW(B, DP, 2, 1, 8, WG) FAPQ_FEW(B, DP, 1, 1, 16, WG)
 // (R: rows of a workgroup, 64 RW)
-#define FAPQ_TILE(B, DP, RW, R)                                                                                                 \
-    extern "C" __global__ void __launch_bounds__(256, 2) ghip_fapq_tile##R##_##B##_##DP(FapMxParams p) {                         \
-        __shared__ __attribute__((aligned(1024))) uint8_t lds[sizeof(TileLds<Decoded<B>, DP, RW>)];                              \
-        fap_tile<Decoded<B>, bf16, DP, RW>(p, *(TileLds<Decoded<B>, DP, RW> *)lds);                                              \
-    }                                                                                                                           \
-    extern "C" __global__ void __launch_bounds__(256, 2) ghip_fapq_both##R##_##B##_##DP(FapMxParams p) {                         \
-        __shared__ __attribute__((aligned(1024))) uint8_t lds[sizeof(FapqLds<B, DP, RW>)];                                       \
-        if ((int)blockIdx.x < p.wg_sh) fap_tile<Decoded<B>, bf16, DP, RW>(p, *(TileLds<Decoded<B>, DP, RW> *)lds);               \
-        else fapq_few<B, DP>(p, *(FewqLds<DP> *)lds);                                                                            \
+#define FAPQ_TILE(B, DP, RW, R)                                                                                    \
+    extern "C" __global__ void __launch_bounds__(256, 2) ghip_fapq_tile##R##_##B##_##DP(FapMxParams p) {            \
+        __shared__ __attribute__((aligned(1024))) uint8_t lds[sizeof(TileLds<Decoded<B>, DP, RW>)];                 \
+        fap_tile<Decoded<B>, bf16, DP, RW>(p, *(TileLds<Decoded<B>, DP, RW> *)lds);                                 \
+    }                                                                                                              \
+    extern "C" __global__ void __launch_bounds__(256, 2) ghip_fapq_both##R##_##B##_##DP(FapMxParams p) {            \
+        __shared__ __attribute__((aligned(1024))) uint8_t lds[sizeof(FapqLds<B, DP, RW>)];                          \
+        if ((int)blockIdx.x < p.wg_sh) fap_tile<Decoded<B>, bf16, DP, RW>(p, *(TileLds<Decoded<B>, DP, RW> *)lds);  \
+        else fapq_few<B, DP, 1, 1>(p, *(FewqLds<B, DP, 1, 1> *)lds);                                                      \
     }
-#define FAPQ_B(B)                                                                                                \
-    FAPQ_FEW(B, 64, 2) FAPQ_FEW(B, 128, 2) FAPQ_FEW(B, 256, 1)                                                          \
+#define FAPQ_B(B)                                                                                                  \
+    FAPQ_FEWS(B, 64, 3) FAPQ_FEW(B, 64, 1, 2, 32, 2) FAPQ_FEWS(B, 128, 3) FAPQ_FEW(B, 128, 1, 2, 32, 2) FAPQ_FEWS(B, 256, 1)                                                  \
     FAPQ_TILE(B, 64, 1, 64) FAPQ_TILE(B, 128, 1, 64) FAPQ_TILE(B, 256, 1, 64) FAPQ_TILE(B, 64, 2, 128)
 FAPQ_B(8) FAPQ_B(4)
