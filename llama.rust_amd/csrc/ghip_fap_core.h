@@ -288,6 +288,18 @@ DEV void scores(const Rows<E, DP, RW> &R, uint32_t Ks, v4f (&s)[NT][RW], F betwe
 // 16 t + v with limits less k0 + 4 g.
 template <typename E, int DP, int RW, int NT>
 DEV void mask_scores(const Rows<E, DP, RW> &R, v4f (&s)[NT][RW], int k0, int ke, uint64_t bad, int window, int n_first) {
+    // (first: what a key on no page was scored with may be minus infinity too)
+    if (bad) {
+        const uint64_t mine = bad >> (4 * ((threadIdx.x & 63) >> 4));
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int v = 0; v < 4; v++)
+                if ((mine >> (16 * t + v)) & 1) {
+#pragma unroll
+                    for (int rt = 0; rt < RW; rt++) s[t][rt][v] = __builtin_nanf("");
+                }
+    }
     const int at = k0 + 4 * ((threadIdx.x & 63) >> 4);
     // seen(c, lo, hi): is this lane's key c in sight of a row?
     auto cut = [&](auto seen) {
@@ -308,18 +320,6 @@ DEV void mask_scores(const Rows<E, DP, RW> &R, v4f (&s)[NT][RW], int k0, int ke,
     } else {
         const int first = n_first - at;
         cut([=](int c, int lo, int hi) { return c <= hi && (c > lo || c < first); });
-    }
-    if (bad) {
-        const uint64_t mine = bad >> (4 * ((threadIdx.x & 63) >> 4));
-#pragma unroll
-        for (int t = 0; t < NT; t++)
-#pragma unroll
-            for (int v = 0; v < 4; v++)
-                if ((mine >> (16 * t + v)) & 1) {
-#pragma unroll
-                    for (int rt = 0; rt < RW; rt++)
-                        if (s[t][rt][v] > -__builtin_inff()) s[t][rt][v] = __builtin_nanf("");
-                }
     }
 }
 

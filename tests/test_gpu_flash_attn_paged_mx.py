@@ -441,3 +441,22 @@ def test_workspace_of_the_caller(be, bits):
             own.flash_attn_paged(q, kv, seqs, scale=0.09, scales=sc, **kw)
         torch.cuda.synchronize()
         own.close()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", 8, 4])
+def test_bad_page_beside_keys_that_overflow(be, dtype):
+    """A row that sees a key on no page is NaN whatever the cache holds elsewhere: keys of the first page's first
+    row whose product with the row's q is minus infinity."""
+    for nq in (1, 3, 40):
+        for Hkv in (1, 2):
+            q = torch.ones((nq, 4, 64))
+            if dtype == "bf16":
+                kv, sc = torch.zeros((4, 16, Hkv, 128), dtype=torch.bfloat16), None
+                kv[0, 0, :, :64] = -math.inf
+            else:
+                kv, sc = M.cache(4, 16, Hkv, 64, dtype, torch.Generator().manual_seed(0))
+                kv.view(torch.uint8)[0, 0, :, :64 * dtype // 8] = 0xfe if dtype == 8 else 0xff
+                sc[0, 0, :, :2] = 254
+            t = torch.tensor([[0, nq, 60, 1, -1, 2, 3]], dtype=torch.int32)
+            got = be.flash_attn_paged(q.cuda(), kv.cuda(), t.cuda(), scale=1.0, max_q=nq, **({} if sc is None else dict(scales=sc.cuda())))
+            assert torch.isnan(got).all(), (dtype, nq, Hkv)
