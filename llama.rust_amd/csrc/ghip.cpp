@@ -3632,7 +3632,7 @@ struct FapLayout {
 FapLayout fap_layout(FapParams &p, int type) {
     FapLayout L;
     const int G = p.H / p.H_kv;
-    const bool mx = mx_type(type), bf16 = type != GHIP_TYPE_F16;  // (codes are computed with as bfloat16)
+    const bool mx = mx_type(type), bf16 = !mx && type != GHIP_TYPE_F16;  // (tiles of codes are computed with as float16)
     L.DP = p.D <= 64 ? 64 : p.D <= 96 && !mx ? 96 : p.D <= 128 ? 128 : 256;
     // bytes of a head's key and value
     const double key_bytes = !mx ? 4.0 * p.D : type == GHIP_TYPE_E4M3 ? 2.0 * p.D + 2 * mx_scale_bytes(p.D) : p.D + 2.0 * mx_scale_bytes(p.D);
@@ -3655,18 +3655,22 @@ FapLayout fap_layout(FapParams &p, int type) {
     // dims).  Measured, us, one a CU and two: a 64-key tile of 64 / 96 / 128 / 256 dims
     // with 64 rows 1.5 1.6 1.8 2.6 and 1.8 2.1 2.5 -, with 128 rows 2.0 2.3 2.7 - and
     // 2.6 3.3 3.9 -, bf16 a quarter more; start 7 7 10 16 and 9 10 13 -, 10 11 14 - and
-    // 13 14 20 -.  The lines below go through these.
+    // 13 14 20 -.  The lines below go through these.  Of a quantized cache, 64 rows a quarter more (each
+    // fragment in LDS is read for half the products), and of 64 dims three a CU, a tile then 1.12 times the time of two.
     auto tiles = [&](int R, double blocks, int64_t keys, bool alone) {
-        const int64_t n = std::max<int64_t>(1, (keys + 63) / 64), slots = L.DP == 256 ? 256 : 512;
-        const double terms = bf16 ? 1.25 : 1.0;
+        const int64_t n = std::max<int64_t>(1, (keys + 63) / 64), slots = L.DP == 256 ? 256 : mx && L.DP == 64 ? 768 : 512;
+        const double terms = bf16 || (mx && R == 64) ? 1.25 : 1.0;
         const double start[2] = {R == 64 ? 4.0 + 6.0 * wide : 5.0 + 9.0 * wide, R == 64 ? 5.0 + 8.0 * wide : 6.0 + 14.0 * wide};
         const double tile[2] = {terms * (R == 64 ? 1.2 + 0.6 * wide : 1.35 + 1.3 * wide),
                                 terms * (R == 64 ? 1.0 + 1.5 * wide : 1.25 + 2.7 * wide)};
         Way best{1, 0};
         for (int z = 1; z <= 32 && z <= n; z++) {
             const double wgs = blocks * p.H_kv * z;
-            const int two = wgs > 256 && slots == 512;
-            const double us = std::max(1.0, std::ceil(wgs / slots - 0.1)) * (start[two] + (double)((n + z - 1) / z) * tile[two]) +
+            const int two = wgs > 256 && slots > 256;
+            const double each = wgs > 512 && slots > 512 ? 1.12 * tile[two] : tile[two];
+            // (a last round that is not full goes faster, and blocks see more keys or fewer: half of it)
+            const double full = std::max(1.0, std::ceil(wgs / slots - 0.1)), rounds = mx ? std::max(1.0, (full + wgs / slots) / 2) : full;
+            const double us = rounds * (start[two] + (double)((n + z - 1) / z) * each) +
                               (z > 1 || !alone ? join(z) : 0.0);
             if (z == 1 || us < best.us) best = {z, us};
         }
@@ -3680,7 +3684,10 @@ FapLayout fap_layout(FapParams &p, int type) {
         const int64_t wgs = (int64_t)p.B * p.H_kv, slots = L.DP == 256 ? 256 : 512;
         Way w;
         w.z = keys <= 512 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>({(1024 + wgs - 1) / wgs, (keys + 255) / 256, 32}));
-        // (a quantized cache by itself: splits by length, up to four times an even share for the longest)
+        // A quantized cache beside a shared prefix, which fills half of the slots: one round of splits (64 rows over
+        // 8192 keys and 40 .. 600 of their own: 54.7 us in two, 47.2).  By itself: splits by length, up to four
+        // times an even share for the longest.
+        if (mx && !alone) w.z = std::min<int>(w.z, (int)std::max<int64_t>(1, (512 + wgs - 1) / wgs));
         if (mx && alone) w.z = keys <= 256 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>({(4 * 768 + wgs - 1) / wgs, (keys + 127) / 128, 32}));
         const double steps = (double)((keys + 128 * w.z - 1) / (128 * w.z));
         w.us = std::max((double)((wgs * w.z + slots - 1) / slots) * (6.0 + steps * (1.2 + 0.8 * wide)), key_bytes * wgs * keys / mem) +
@@ -3781,8 +3788,11 @@ ghip_status fap_run(ghip_context *ctx, const char *call, const ghip_tensor *q, c
         if (p.zs_own > 1 && !p.wg_sh) {
             const int64_t slots = 256 * (few_rows > 16 ? 2 : L.DP == 64 ? 4 : L.DP == 128 ? 3 : few_rows <= 4 ? 2 : 1);
             const int64_t round = std::max<int64_t>(8, slots / p.H_kv / 8 * 8);
-            parts = p.wgs = (int)(std::max<int64_t>(1, (3 * (int64_t)p.B + round - 1) / round) * round);
+            parts = std::max<int64_t>(1, (3 * (int64_t)p.B + round - 1) / round) * round;
             p.least = 4;
+            // (no more than there can be of so many tiles)
+            const int64_t tiles = ((int64_t)p.per * p.page + 63) / 32 + 2;
+            parts = p.wgs = (int)std::min(parts, (p.B * ((tiles + p.least - 1) / p.least) + 7) / 8 * 8);
         }
         // The heads of the same keys follow one another on one XCD (workgroups go to the 8 XCDs in
         // turn), whose cache then has the keys' scales once: where the parts divide into eights, or nearly so.

@@ -662,17 +662,26 @@ DEV int prefix_of(const FapParams &p) {
 // L: how a tile comes into LDS.  L::Loads<DP> has
 //   ld.load_pages(t)     the page numbers of tile t's keys are on their way
 //   ld.find_tile(t)      where its rows are; ld.ok2, ld.bad2: its keys that are there, those on no page
-//   ld.load_part(t, f)   load f of DP / 16 of it goes out
-//   ld.loaded(t)         this wavefront's loads of it are in: LDS holds its rows, 0 for values of keys not in ok
-template <typename L, int DP, int RW>
+//   ld.load_part(t, u, f)  under fragment f of DP / 16 of half u of the tile before: loads of it go out
+//   ld.load_half(t, u)     all of those of half u
+//   ld.load_first(t)       the first tile's, of both (in after wait_loads and loaded())
+//   ld.middle(t)           between the halves
+//   ld.loaded(t)           this wavefront's loads of it are in: LDS holds its rows, 0 for values of keys not in ok
+//   L::LATE                half 1 has loads, and loads past the last tile do no harm (those of the tile found last)
+//   L::HOME_K            keys and values are in LDS 2^HOME_K times what they are
+//   L::NARROW            LDS cannot hold every tile: wide[t & 1] says that it does not hold tile t
+// BW: a block's rows, 64 each; RW of them are this pass's, from `half` on.  Returns whether
+// a tile was met that LDS cannot hold; then nothing has been stored.
+template <typename L, int DP, int BW>
 struct TileLds {
     uint8_t kvs[2][2][64 * DP * 2];  // this tile's K and V, the next one's
     typename L::Lds ld;
-    RowList<64 * RW> ls;
+    RowList<64 * BW> ls;
 };
-template <typename L, typename E, int DP, int RW, typename PARAMS>
-DEV void fap_tile(const PARAMS &p, TileLds<L, DP, RW> &lds) {
-    constexpr int KT = 64, R = 64 * RW;
+template <typename L, typename E, int DP, int RW, int BW = RW, typename PARAMS>
+DEV bool fap_tile(const PARAMS &p, TileLds<L, DP, BW> &lds, int half = 0) {
+    constexpr int KT = 64, R = 64 * BW;
+    constexpr float LESS = 1.0f / (1 << L::HOME_K);
     auto &kvs = lds.kvs;
     auto &ls = lds.ls;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, g = lane >> 4;
@@ -732,7 +741,7 @@ DEV void fap_tile(const PARAMS &p, TileLds<L, DP, RW> &lds) {
             __syncthreads();
             b = ls.found[0];
             bb = ls.found[1];
-            if (b < 0) return;
+            if (b < 0) return false;
         }
         r0 = bb * R;
         x0 = r0 / G;
@@ -755,7 +764,7 @@ DEV void fap_tile(const PARAMS &p, TileLds<L, DP, RW> &lds) {
             ps.p1 = max(ps.p1, ls.pos[k]);
             any = true;
         }
-    if (!__ballot(any)) return;
+    if (!__ballot(any)) return false;
 #pragma unroll
     for (int o = 32; o; o >>= 1) {
         ps.p0 = min(ps.p0, __shfl_xor(ps.p0, o, 64));
@@ -774,7 +783,7 @@ DEV void fap_tile(const PARAMS &p, TileLds<L, DP, RW> &lds) {
     };
     auto row_of = [&](int rt) {
         Row y;
-        const int r = r0 + 16 * (RW * w + rt) + n, k = r / G - x0;
+        const int r = r0 + 64 * half + 16 * (RW * w + rt) + n, k = r / G - x0;
         y.hd = hk * G + r % G;
         y.valid = ls.tok[k] >= 0;
         y.tok = y.valid ? ls.tok[k] : 0;
@@ -788,7 +797,7 @@ DEV void fap_tile(const PARAMS &p, TileLds<L, DP, RW> &lds) {
             const Row y = row_of(rt);
             if (y.valid && g == 0) stat_none(p, y.pi, y.pos >= table);
         }
-        return;
+        return false;
     }
     Rows<E, DP, RW> Q;
     RawRow<DP> raw[RW];
@@ -826,19 +835,25 @@ DEV void fap_tile(const PARAMS &p, TileLds<L, DP, RW> &lds) {
         ld.find_tile(t0);
         wait_lds();
         ld.load_pages(t0 + 2);
-        ld.load_tile(t0);
+        ld.load_first(t0);
         ld.ok = ld.ok2;
         ld.bad = ld.bad2;
         if (t0 + 1 < t1) ld.find_tile(t0 + 1);
     }
 #pragma unroll
-    for (int rt = 0; rt < RW; rt++) rows_start<E, DP, RW>(Q, rt, raw[rt], p.scale * kLog2e);
+    for (int rt = 0; rt < RW; rt++) {
+        rows_start<E, DP, RW>(Q, rt, raw[rt], p.scale * kLog2e);
+        if constexpr (L::HOME_K != 0) Q.unit[rt] *= LESS;
+    }
     if (t0 < t1) {
         wait_loads<0>();
         ld.loaded(t0);
     }
     __syncthreads();
     for (int t = t0; t < t1; t++) {
+        // (said before the last barrier; the next to say it in this place do so behind the next barrier)
+        if constexpr (L::NARROW)
+            if (__builtin_amdgcn_readfirstlane(lds.ld.wide[t & 1])) return true;
         const Tile tile = tile_at(ps.tl, t, KT);
         const uint64_t badc = ld.bad;
         const bool part = !tile_whole(tile, KT, ps, p.window, p.n_first);
@@ -853,13 +868,15 @@ DEV void fap_tile(const PARAMS &p, TileLds<L, DP, RW> &lds) {
             const int h0 = tile.k0 + 32 * u, h1 = min(h0 + 32, tile.ke);
             const bool need = work && (!part || (h0 < h1 && h0 <= w1 && (!p.window || h1 - 1 > w0 - p.window || h0 < p.n_first)));
             v4f s[2][RW];
+            if (u == 1 && more) ld.middle(t + 1);
+            const bool loads = L::LATE || (u == 0 && more);
             if (need) {
                 __builtin_amdgcn_s_setprio(1);
-                if (u == 0 && more) scores<E, DP, RW, 2>(Q, Kh, s, [&](int f) { ld.load_part(t + 1, f); });
+                if (loads) scores<E, DP, RW, 2>(Q, Kh, s, [&](int f) { ld.load_part(t + 1, u, f); });
                 else scores<E, DP, RW, 2>(Q, Kh, s, [](int) {});
                 __builtin_amdgcn_s_setprio(0);
-            } else if (u == 0 && more) {
-                ld.load_tile(t + 1);
+            } else if (loads) {
+                ld.load_half(t + 1, u);
             }
             if (need) {
                 if (part || badc) mask_scores<E, DP, RW, 2>(Q, s, tile.k0 + 32 * u, tile.ke, badc >> (32 * u), p.window, p.n_first);
@@ -888,6 +905,7 @@ DEV void fap_tile(const PARAMS &p, TileLds<L, DP, RW> &lds) {
         if (y.pos >= table) l = __builtin_nanf("");
         if (y.valid) {
             if (!p.part) finish_stat(p, y.hd, m, l, f);
+            if constexpr (L::HOME_K != 0) f *= LESS;
             float *out = p.part ? p.part + y.pi * p.D : p.dst + y.tok * p.d_nb2 + y.hd * p.d_nb1;
 #pragma unroll
             for (int dt = 0; dt < DP / 16; dt++) {
@@ -903,6 +921,7 @@ DEV void fap_tile(const PARAMS &p, TileLds<L, DP, RW> &lds) {
         }
         if (!p.part) rows_again<typename L::Again>(p, row + 3, again && y.pos < table, y.tok, y.hd, y.pos, [](int) { return true; });
     }
+    return false;
 }
 
 // ---- the splits' partials of a row -> dst, in the order of the splits

@@ -536,16 +536,21 @@ DEV void fapq_few(const FapMxParams &p, FewqLds<BITS, DP, CG, RW> &lds) {
 
 // How a tile comes into LDS: its codes go into registers, 16 elements a lane (load ii of wavefront
 // w: unit idx % U of key 16 w + idx / U, idx = 64 ii + lane), and from there as bfloat16 into LDS.
-template <int BITS>
+template <int BITS, typename E>
 struct Decoded {
     typedef Alone<BITS> Again;
+    typedef MxHalf<BITS> Half;
+    static constexpr bool NARROW = Frag<E>::SCALED, LATE = true;
+    static constexpr int HOME_K = NARROW ? Half::HOME : 0;
     struct Lds {
         int64_t offs[4][2][64];
+        int wide[2];
     };
+    typedef typename Frag<E>::v8 v8;
     template <int DP>
     struct Loads {
         static constexpr int KT = 64, CH = DP / 8, U = DP / 16, NL = 16 * U / 64, W = BITS / 2;
-        static_assert(2 * NL <= DP / 16, "one load under each of a half's fragments");
+        static_assert(NL <= DP / 16, "one load under each of a half's fragments");
         const FapMxParams &p;
         Lds &lds;
         uint8_t (&kvs)[2][2][64 * DP * 2];
@@ -555,13 +560,29 @@ struct Decoded {
         const uint8_t *kvh, *sch;
         uint64_t ok = 0, bad = 0, ok2 = 0, bad2 = 0;
         int pg[2];                        // page numbers of the tiles to be found next, a lane a key
-        const uint8_t *at[NL], *sat[NL];  // this lane's rows of the tile found last
-        uint32_t kw[NL][W], vw[NL][W], ks[NL], vs[NL];
+        // keys, then values, of the tile on its way
+        uint32_t x[NL][W], sc[NL];
         int unit;
         DEV_M Loads(const FapMxParams &p_, Lds &lds_, uint8_t (&kvs_)[2][2][64 * DP * 2], int hk, const int32_t *row_, int w_,
                     const PagedTiles &tl_, int t1_)
             : p(p_), lds(lds_), kvs(kvs_), row(row_), w(w_), t1(t1_), tl(tl_), kvh((const uint8_t *)p_.kv + hk * p_.kv_head),
               sch(p_.sc + hk * p_.sc_head), unit(min((int)(threadIdx.x & 63) % U, p_.D / 16 - 1)) {}
+        // a block's scale; what E cannot hold of a block that counts is seen in `wide`
+        DEV_M float scale_of(uint32_t byte, const uint32_t (&x)[W], bool counts, bool &wide) const {
+            if constexpr (!NARROW) {
+                return mx_scale(byte);
+            } else {
+                float f = mx_scale(byte + HOME_K);
+                if (byte - Half::FROM > Half::UP) {  // a block of zeros will do
+                    uint32_t any = byte == 255;
+#pragma unroll
+                    for (int i = 0; i < W; i++) any |= x[i] & (BITS == 8 ? 0x7f7f7f7f : 0x77777777);
+                    wide = wide || (any && counts);
+                    f = 1.0f;
+                }
+                return f;
+            }
+        }
         DEV_M int key(int ii) const { return 16 * w + (64 * ii + (int)(threadIdx.x & 63)) / U; }
         DEV_M void load_pages(int t) {
             const Tile tile = tile_at(tl, min(t, t1 - 1), KT);
@@ -572,43 +593,64 @@ struct Decoded {
         DEV_M void find_tile(int t) {
             // (the pages loaded last are those of the tile after t)
             find_keys_mx(p, tile_at(tl, t, KT), KT, pg[0], lds.offs[w][0], lds.offs[w][1], ok2, bad2);
+        }
+        DEV_M void load_unit(int kv, int ii, uint32_t (&to)[W], uint32_t &scale) {
+            load_words(to, kvh + lds.offs[w][0][key(ii)] + unit * (2 * BITS) + (kv ? p.D * BITS / 8 : 0));
+            scale = load_byte(sch + lds.offs[w][1][key(ii)] + unit / 2 + (kv ? p.S : 0));
+        }
+        DEV_M void load_part(int, int kv, int ii) {
+            if (ii < NL) load_unit(kv, ii, x[ii], sc[ii]);
+        }
+        DEV_M void load_half(int t, int kv) {
 #pragma unroll
-            for (int ii = 0; ii < NL; ii++) {
-                at[ii] = kvh + lds.offs[w][0][key(ii)] + unit * (2 * BITS);
-                sat[ii] = sch + lds.offs[w][1][key(ii)] + unit / 2;
-            }
+            for (int ii = 0; ii < NL; ii++) load_part(t, kv, ii);
         }
-        DEV_M void load_part(int t, int f) {
-            if (f < NL) {
-                load_words(kw[f], at[f]);
-                ks[f] = load_byte(sat[f]);
-            } else if (f < 2 * NL) {
-                load_words(vw[f - NL], at[f - NL] + p.D * BITS / 8);
-                vs[f - NL] = load_byte(sat[f - NL] + p.S);
-            }
-        }
-        DEV_M void load_tile(int t) {
+        DEV_M void load_first(int t) {
+            uint32_t y[NL][W], ysc[NL];
 #pragma unroll
-            for (int f = 0; f < 2 * NL; f++) load_part(t, f);
+            for (int ii = 0; ii < NL; ii++) load_unit(0, ii, y[ii], ysc[ii]);
+            load_half(t, 1);
+            decode(t, 0, ok2, y, ysc);
         }
-        DEV_M void loaded(int t) {
+        DEV_M void middle(int t) { decode(t, 0, ok2, x, sc); }
+        DEV_M void loaded(int t) { decode(t, 1, ok, x, sc); }
+        DEV_M void decode(int t, int kv, uint64_t ok, const uint32_t (&x)[NL][W], const uint32_t (&sc)[NL]) {
             const int u = (threadIdx.x & 63) % U;
+            bool wide = false;
 #pragma unroll
             for (int ii = 0; ii < NL; ii++) {
                 const int r = key(ii);
-                const float kf = mx_scale(ks[ii]), vf = mx_scale(vs[ii]);
-                uint8_t *K = kvs[t & 1][0] + 2 * r * DP, *V = kvs[t & 1][1] + 2 * r * DP;
-                *(mx_bf8 *)(K + 16 * k_swz<CH>(r, 2 * u)) = mx_eight<BITS>(&kw[ii][0], kf);
-                *(mx_bf8 *)(K + 16 * k_swz<CH>(r, 2 * u + 1)) = mx_eight<BITS>(&kw[ii][W / 2], kf);
-                mx_bf8 lo = mx_eight<BITS>(&vw[ii][0], vf), hi = mx_eight<BITS>(&vw[ii][W / 2], vf);
+                const bool there = (ok >> r) & 1;
+                const float f = scale_of(sc[ii], x[ii], there, wide);
+                v8 lo = mx_eight<BITS>(&x[ii][0], f, v8{}), hi = mx_eight<BITS>(&x[ii][W / 2], f, v8{});
                 // rows that were not there: no value of theirs may count
-                if (!((ok >> r) & 1)) lo = hi = mx_bf8{};
-                *(mx_bf8 *)(V + 16 * v_swz<CH>(r, 2 * u)) = lo;
-                *(mx_bf8 *)(V + 16 * v_swz<CH>(r, 2 * u + 1)) = hi;
+                if (!there) lo = hi = v8{};
+                uint8_t *to = kvs[t & 1][kv] + 2 * r * DP;
+                *(v8 *)(to + 16 * (kv ? v_swz<CH>(r, 2 * u) : k_swz<CH>(r, 2 * u))) = lo;
+                *(v8 *)(to + 16 * (kv ? v_swz<CH>(r, 2 * u + 1) : k_swz<CH>(r, 2 * u + 1))) = hi;
             }
+            if constexpr (NARROW)
+                if (wide) lds.wide[t & 1] = 1;
         }
     };
 };
+
+// Tiles of 64 BW rows: as float16, two terms of q and p for each of its products, and where a tile has blocks that
+// float16 does not hold (MxHalf) once more as bfloat16, three terms.
+template <int BITS, int DP, int BW>
+union FapqTileLds {
+    TileLds<Decoded<BITS, f16>, DP, BW> half;
+    TileLds<Decoded<BITS, bf16>, DP, BW> wide;
+};
+template <int BITS, int DP, int BW>
+DEV void fapq_tile(const FapMxParams &p, FapqTileLds<BITS, DP, BW> &lds) {
+    if (threadIdx.x < 2) lds.half.ld.wide[threadIdx.x] = 0;
+    if (!fap_tile<Decoded<BITS, f16>, f16, DP, BW>(p, lds.half)) return;
+    for (int half = 0; half < BW; half++) {  // (what the registers hold of three terms)
+        __syncthreads();
+        fap_tile<Decoded<BITS, bf16>, bf16, DP, 1, BW>(p, lds.wide, half);
+    }
+}
 
 extern "C" __global__ void __launch_bounds__(256) ghip_fapq_join_8(FapMxParams p) { fap_join<Alone<8>>(p); }
 extern "C" __global__ void __launch_bounds__(256) ghip_fapq_join_4(FapMxParams p) { fap_join<Alone<4>>(p); }
@@ -616,7 +658,7 @@ extern "C" __global__ void __launch_bounds__(256) ghip_fapq_join_4(FapMxParams p
 template <int BITS, int DP, int RW>
 union FapqLds {
     FewqLds<BITS, DP, 1, 1> few;
-    TileLds<Decoded<BITS>, DP, RW> tile;
+    FapqTileLds<BITS, DP, RW> tile;
 };
 // (ROWS: up to how many, 16 RW / CG; WG: workgroups a CU)
 #define FAPQ_FEW(B, DP, CG, RW, ROWS, WG)                                                                          \
@@ -627,16 +669,16 @@ union FapqLds {
 #define FAPQ_FEWS(B, DP, WG) FAPQ_FEW(B, DP, 4, 1, 4, WG) FAPQ_FEW(B, DP, 2, 1, 8, WG) FAPQ_FEW(B, DP, 1, 1, 16, WG)
 // (R: rows of a workgroup, 64 RW)
 #define FAPQ_TILE(B, DP, RW, R)                                                                                    \
-    extern "C" __global__ void __launch_bounds__(256, 2) ghip_fapq_tile##R##_##B##_##DP(FapMxParams p) {            \
-        __shared__ __attribute__((aligned(1024))) uint8_t lds[sizeof(TileLds<Decoded<B>, DP, RW>)];                 \
-        fap_tile<Decoded<B>, bf16, DP, RW>(p, *(TileLds<Decoded<B>, DP, RW> *)lds);                                 \
+    extern "C" __global__ void __launch_bounds__(256, DP == 64 ? 3 : 2) ghip_fapq_tile##R##_##B##_##DP(FapMxParams p) {            \
+        __shared__ __attribute__((aligned(1024))) uint8_t lds[sizeof(FapqTileLds<B, DP, RW>)];                      \
+        fapq_tile<B, DP, RW>(p, *(FapqTileLds<B, DP, RW> *)lds);                                                    \
     }                                                                                                              \
-    extern "C" __global__ void __launch_bounds__(256, 2) ghip_fapq_both##R##_##B##_##DP(FapMxParams p) {            \
+    extern "C" __global__ void __launch_bounds__(256, DP == 64 ? 3 : 2) ghip_fapq_both##R##_##B##_##DP(FapMxParams p) {            \
         __shared__ __attribute__((aligned(1024))) uint8_t lds[sizeof(FapqLds<B, DP, RW>)];                          \
-        if ((int)blockIdx.x < p.wg_sh) fap_tile<Decoded<B>, bf16, DP, RW>(p, *(TileLds<Decoded<B>, DP, RW> *)lds);  \
+        if ((int)blockIdx.x < p.wg_sh) fapq_tile<B, DP, RW>(p, *(FapqTileLds<B, DP, RW> *)lds);                     \
         else fapq_few<B, DP, 1, 1>(p, *(FewqLds<B, DP, 1, 1> *)lds);                                                      \
     }
 #define FAPQ_B(B)                                                                                                  \
     FAPQ_FEWS(B, 64, 3) FAPQ_FEW(B, 64, 1, 2, 32, 2) FAPQ_FEWS(B, 128, 3) FAPQ_FEW(B, 128, 1, 2, 32, 2) FAPQ_FEWS(B, 256, 1)                                                  \
-    FAPQ_TILE(B, 64, 1, 64) FAPQ_TILE(B, 128, 1, 64) FAPQ_TILE(B, 256, 1, 64) FAPQ_TILE(B, 64, 2, 128)
+    FAPQ_TILE(B, 64, 1, 64) FAPQ_TILE(B, 128, 1, 64) FAPQ_TILE(B, 256, 1, 64) FAPQ_TILE(B, 64, 2, 128) FAPQ_TILE(B, 128, 2, 128)
 FAPQ_B(8) FAPQ_B(4)

@@ -11,6 +11,8 @@
 
 typedef __bf16 mx_bf2 __attribute__((ext_vector_type(2)));
 typedef __bf16 mx_bf8 __attribute__((ext_vector_type(8)));
+typedef _Float16 mx_h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 mx_h8 __attribute__((ext_vector_type(8)));
 typedef float mx_f2 __attribute__((ext_vector_type(2)));
 typedef short mx_s2 __attribute__((ext_vector_type(2)));
 
@@ -66,7 +68,7 @@ DEV mx_f2 mx_pair(uint32_t w, float s) {
     else return __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, I);
 }
 template <int BITS>
-DEV mx_bf8 mx_eight(const uint32_t *w, float s) {
+DEV mx_bf8 mx_eight(const uint32_t *w, float s, mx_bf8) {
     mx_bf2 p[4];
     if constexpr (BITS == 8) {
         p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[0], s, false);
@@ -84,3 +86,34 @@ DEV mx_bf8 mx_eight(const uint32_t *w, float s) {
     for (int i = 0; i < 8; i++) r[i] = p[i / 2][i & 1];
     return r;
 }
+template <int BITS>
+DEV mx_h8 mx_eight(const uint32_t *w, float s, mx_h8) {
+    mx_h2 p[4];
+    if constexpr (BITS == 8) {
+        p[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[0], s, false);
+        p[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[0], s, true);
+        p[2] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[1], s, false);
+        p[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[1], s, true);
+    } else {
+        p[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w[0], s, 0);
+        p[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w[0], s, 1);
+        p[2] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w[0], s, 2);
+        p[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w[0], s, 3);
+    }
+    mx_h8 r;
+#pragma unroll
+    for (int i = 0; i < 8; i++) r[i] = p[i / 2][i & 1];
+    return r;
+}
+template <int BITS>
+DEV mx_bf8 mx_eight(const uint32_t *w, float s) { return mx_eight<BITS>(w, s, mx_bf8{}); }
+
+// float16 holds a code times 2^e exactly too, if e is in a range: with 8 bits, all of 2^-9 .. 448, -15 .. 7;
+// with 4, all of 0.5 .. 6, -23 .. 13.  A cache's elements are taken 2^HOME times, so that the
+// range lies about what they are like: blocks whose largest is 2^-12 .. 896, or 2^-21 .. 57344.
+// The byte of a scale is in range if byte - FROM (unsigned) <= UP.
+template <int BITS>
+struct MxHalf {
+    static constexpr int HOME = BITS == 8 ? 6 : 0;
+    static constexpr uint32_t FROM = 127 - (BITS == 8 ? 15 : 23) - HOME, UP = BITS == 8 ? 22 : 36;
+};

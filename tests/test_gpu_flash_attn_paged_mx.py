@@ -1,9 +1,9 @@
 """ghip_flash_attn_paged_mx against attention's formula in 64 bits over the values
 that a quantized cache's codes stand for (mx_oracle, paged_oracle).  A code's
-value is a bfloat16, so the bounds are those of a BF16 cache: every element within
-attention_tol, and the whole within 5 * 2^-22 in 2-norm (q and p in 24 bits as three
-terms, a score's sum, 2^x and the row's sum in 24: five roundings of at most 2^-22) for scores
-of about 1.  A score of size s is a 32-bit number too, whose last place is 2^-24 s:
+value is a bfloat16 (of most caches a float16 too), so the bounds are those of such a cache: every element
+within attention_tol, and the whole within 5 * 2^-22 in 2-norm (q and p as three
+terms of 8 bits or two of 11, a score's sum, 2^x and the row's sum in 24: five roundings of at most 2^-22) for
+scores of about 1.  A score of size s is a 32-bit number too, whose last place is 2^-24 s:
 that much of its p, and of what the row sums, 2^-24 s is added for the largest s
 (these caches' scales spread over 2^6, scores reach 40)."""
 import math
@@ -441,6 +441,85 @@ def test_workspace_of_the_caller(be, bits):
             own.flash_attn_paged(q, kv, seqs, scale=0.09, scales=sc, **kw)
         torch.cuda.synchronize()
         own.close()
+
+
+@BITS
+@pytest.mark.parametrize("D,nq", [(64, 150), (128, 150), (128, 40), (256, 40)])
+def test_scales_out_of_half_precisions_range(be, D, nq, bits):
+    """Tiles of rows are computed with as float16 where that holds a tile's blocks, else as bfloat16:
+    a block out of its range in one split of the keys, in all of them, in a shared prefix, and
+    blocks of zeros, whose scale is the least there is."""
+    S = M.scale_bytes(D)
+    for n_shared, seqs in ((0, [(nq, 5000), (20, 300)]), (256, [(nq, 900), (nq, 700)])):
+        for what in ("key", "value", "values", "zeros", "keys"):
+            q, kv, sc, table = make(seqs, 4, 2, D, bits, 16, n_shared, seed=5)
+            at = lambda j: (int(table[0, 3 + j // 16]), j % 16)
+            if what == "key":      # one block of keys, of 2^40 (the row's q there as small)
+                q[..., 32:64] *= 2.0 ** -44
+                sc[at(200)][1, 1] += 40
+            elif what == "value":  # values of about 2^30 and 2^-20 in one block each
+                sc[at(130)][0, S] += 30
+                sc[at(201)][1, S + 1] -= 20
+            elif what == "values":
+                sc[..., S + 1] -= 40
+            elif what == "keys":
+                q[..., :32] *= 2.0 ** 40
+                sc[..., 0] -= 40
+            else:
+                kv.view(torch.uint8)[..., 32 * bits // 8:64 * bits // 8] = 0
+                kv.view(torch.uint8)[..., D * bits // 8:(D + 32) * bits // 8] = 0
+                sc[..., 1], sc[..., S] = 27, 27
+            want, mag, wgt = P.attention(q, M.values(kv, sc, bits), table.tolist(), D ** -0.5)
+            print(what, D, nq, n_shared, flush=True)
+            for how in ways(n_shared):
+                got = be.flash_attn_paged(q.cuda(), kv.cuda(), table.cuda(), scale=D ** -0.5, n_shared=n_shared, max_q=nq, scales=sc.cuda()).cpu()
+                assert ((got.double() - want).abs() <= P.attention_tol(mag, wgt, D)).all()
+
+
+@BITS
+@pytest.mark.parametrize("D,H,Hkv,nq", [(128, 4, 1, 1), (64, 8, 1, 2), (128, 16, 1, 1), (128, 4, 1, 7), (64, 5, 1, 4), (256, 4, 2, 1)])
+def test_many_sequences_share_the_workgroups(be, D, H, Hkv, nq, bits):
+    """More sequences than a wavefront has lanes, long and short ones, idle ones among them and at the
+    end, whose splits go by length: a workspace full of NaN, rows no sequence has as they were."""
+    import ghip
+    page, B, pages = 16, 150, 400
+    g = torch.Generator().manual_seed(9)
+    kv, sc = M.cache(pages, page, Hkv, D, bits, g)
+    lens = [3000 if b in (3, 70, 140) else 0 if b % 7 == 5 or b >= 145 else 1 + 13 * b % 190 for b in range(B)]
+    table = torch.zeros((B, 3 + 190), dtype=torch.int32)
+    rows = []
+    for b, n in enumerate(lens):
+        m = min(nq, n)
+        table[b, :3] = torch.tensor([len(rows), m, n])
+        table[b, 3:] = torch.randint(0, pages, (190,), generator=g)
+        rows += [b] * m
+    for few in (0, 90):  # all, and up to 64 of them
+        t = table[few:]
+        q = torch.randn((len(rows) + 3, H, D), generator=g)
+        for window, n_first, sinks in ((0, 0, None), (1500, 5, torch.randn(H, generator=g))):
+            want, mag, wgt = P.attention(q, M.values(kv, sc, bits), t.tolist(), D ** -0.5, sinks, window, n_first)
+            print(D, H, nq, few, window, flush=True)
+            kw = dict(scale=D ** -0.5, max_q=nq, window=window, n_first=n_first, scales=sc.cuda(), sinks=None if sinks is None else sinks.cuda())
+            need = be.flash_attn_paged_workspace(q.cuda(), kv.cuda(), t.cuda(), scales=sc.cuda(), max_q=nq, window=window, n_first=n_first)
+            own = ghip.Backend(0)
+            if need:
+                own.set_workspace(torch.full((need // 4,), NAN, device="cuda").view(torch.uint8))
+            out = torch.full(q.shape, 7.0).cuda()
+            own.flash_attn_paged(q.cuda(), kv.cuda(), t.cuda(), out=out, **kw)
+            got = out.cpu()
+            own.close()
+            first, last = int(t[0, 0]), len(rows)
+            assert (got[:first] == 7).all() and (got[last:] == 7).all()
+            compare(got[first:last], want[first:last], mag[first:last], wgt[first:last], D)
+
+
+@BITS
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("nq,H", [(17, 1), (6, 4), (8, 4), (31, 1), (4, 8)])
+def test_up_to_32_rows_of_a_head(be, nq, H, D, bits):
+    """Two tiles of 16 rows in a wavefront: long keys in splits, windows, idle sequences between, sinks."""
+    check(be, [(nq, 4000), (0, 70), (max(nq - 2, 1), 90), (nq, nq), (1, 2500)], 2 * H, 2, D, bits, 64)
+    check(be, [(nq, 900), (nq, 40), (nq - 1, 333)], H, 1, D, bits, 24, window=100, n_first=6, sinks=True)
 
 
 @pytest.mark.parametrize("dtype", ["bf16", 8, 4])
