@@ -3395,7 +3395,7 @@ ghip_status ghip_kv_append_mx(ghip_context *ctx, const ghip_tensor *k, const ghi
     if (T > INT32_MAX) return bad("dimension too large");
     if (slots->type != GHIP_TYPE_I64 || !packed(slots, 8) || slots->ne[0] < T) return bad("slots must be I64, one for each token");
     AppendMxParams p;
-    p.P = 0;
+    p.P = p.tab.axes = 0;
     p.pos = nullptr;
     p.pos_nb1 = 0;
     p.factors = nullptr;

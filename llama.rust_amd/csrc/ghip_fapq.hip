@@ -147,6 +147,17 @@ constexpr int few_keys(int bits, int DP) { return DP == 256 || bits == 8 ? 32 : 
 struct Part {
     int b, z, of, t0, t1;
 };
+// sums over the lanes up to and with each; lane 63: over all
+DEV int lane_sums(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // of the lane 1 before in a row of 16, 2, 4, 8
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // of rows 0 and 2 to the next
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // of the first two rows to the others
+    return x;
+}
+DEV int lane_sum(int x) { return __builtin_amdgcn_readlane(lane_sums(x), 63); }
 template <int KT>
 DEV bool find_part(const FapMxParams &p, int no, Part &w) {
     const int lane = threadIdx.x & 63;
@@ -171,11 +182,9 @@ DEV bool find_part(const FapMxParams &p, int no, Part &w) {
     int live = 0;
     const int first = lane < p.B ? tiles_of(lane) : 0;
     for (int b0 = 0; b0 < p.B; b0 += 64) {
-        int n = b0 == 0 ? first : b0 + lane < p.B ? tiles_of(b0 + lane) : 0;
+        const int n = b0 == 0 ? first : b0 + lane < p.B ? tiles_of(b0 + lane) : 0;
         live += __popcll(__ballot(n > 0));
-#pragma unroll
-        for (int o = 32; o; o >>= 1) n += __shfl_xor(n, o, 64);
-        total += n;
+        total += lane_sum(n);
     }
     // The fewest tiles a part that need no more parts than there are workgroups: with total / (wgs - live)
     // they never do; up to 64 sequences the least is looked for.
@@ -185,10 +194,7 @@ DEV bool find_part(const FapMxParams &p, int no, Part &w) {
         int lo = max((int)((total + p.wgs - 1) / p.wgs), p.least), hi = (int)each;
         while (lo < hi) {
             const int mid = (lo + hi) / 2;
-            int parts = (first + mid - 1) / mid;
-#pragma unroll
-            for (int o = 32; o; o >>= 1) parts += __shfl_xor(parts, o, 64);
-            if (parts <= p.wgs) hi = mid;
+            if (lane_sum((first + mid - 1) / mid) <= p.wgs) hi = mid;
             else lo = mid + 1;
         }
         each = hi;
@@ -197,12 +203,7 @@ DEV bool find_part(const FapMxParams &p, int no, Part &w) {
     for (int b0 = 0; b0 < p.B && base <= no; b0 += 64) {
         const int n = b0 == 0 ? first : b0 + lane < p.B ? tiles_of(b0 + lane) : 0;
         const int parts = (int)min((n + each - 1) / each, (int64_t)p.zs_own);
-        int to = parts;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int y = __shfl_up(to, o, 64);
-            if (lane >= o) to += y;
-        }
+        const int to = lane_sums(parts);
         const uint64_t here = __ballot(base + to - parts <= no && no < base + to);
         if (here) {
             const int at = __builtin_ctzll(here), tiles = __builtin_amdgcn_readlane(n, at);
@@ -354,26 +355,17 @@ DEV void fapq_few(const FapMxParams &p, FewqLds<BITS, DP, CG, RW> &lds) {
     }
     if (t0 >= t1 && p.part) return;  // nothing in this split
     const float j1 = j >= 1, j2 = j >= 2;
-    for (int f = w; f < RW * DP / 32; f += 4) {
-        const int rt = f / (DP / 32), kk = f % (DP / 32), d = EL * (g + 4 * (kk / FU)) + 8 * (kk % FU);
+    // q: loaded here, worked on when the first tile is on its way
+    constexpr int NF = RW * DP / 32, QF = (NF + 3) / 4;
+    float x[QF][8];
+#pragma unroll
+    for (int i = 0; i < QF; i++) {
+        const int f = min(w + 4 * i, NF - 1), rt = f / (DP / 32), kk = f % (DP / 32), d = EL * (g + 4 * (kk / FU)) + 8 * (kk % FU);
         const Row y = row_of(rt);
-        float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        if (y.there && d < p.D && j < 3) __builtin_memcpy(x, p.q + y.tok * p.q_nb2 + y.hd * p.q_nb1 + d, 32);
-        Frag<bf16>::v8 terms[NM];
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            Frag<bf16>::v2 t[NM];
-            group_terms<CG>(v2f{x[2 * e], x[2 * e + 1]} * (p.scale * kLog2e), j1, j2, t);
-#pragma unroll
-            for (int m = 0; m < NM; m++) {
-                terms[m][2 * e] = t[m][0];
-                terms[m][2 * e + 1] = t[m][1];
-            }
-        }
-#pragma unroll
-        for (int m = 0; m < NM; m++) *(Frag<bf16>::v8 *)&lds.q[rt][kk][m][16 * lane] = terms[m];
+        for (int e = 0; e < 8; e++) x[i][e] = 0.0f;
+        if (y.there && d < p.D && j < 3) __builtin_memcpy(x[i], p.q + y.tok * p.q_nb2 + y.hd * p.q_nb1 + d, 32);
     }
-    __syncthreads();
     const uint8_t *kvh = (const uint8_t *)p.kv + hk * p.kv_head, *sch = p.sc + hk * p.sc_head;
     uint8_t *Vs = lds.v[w];
     const uint32_t va = lds_addr(Vs);
@@ -417,6 +409,25 @@ DEV void fapq_few(const FapMxParams &p, FewqLds<BITS, DP, CG, RW> &lds) {
         pg = load_page(first + 4);
         load_tile();
     }
+#pragma unroll
+    for (int i = 0; i < QF; i++) {
+        const int f = w + 4 * i, rt = f / (DP / 32), kk = f % (DP / 32);
+        if (f >= NF) break;
+        Frag<bf16>::v8 terms[NM];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            Frag<bf16>::v2 t[NM];
+            group_terms<CG>(v2f{x[i][2 * e], x[i][2 * e + 1]} * (p.scale * kLog2e), j1, j2, t);
+#pragma unroll
+            for (int m = 0; m < NM; m++) {
+                terms[m][2 * e] = t[m][0];
+                terms[m][2 * e + 1] = t[m][1];
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < NM; m++) *(Frag<bf16>::v8 *)&lds.q[rt][kk][m][16 * lane] = terms[m];
+    }
+    __syncthreads();
     for (int t = first; t < t1; t += 4) {
         const Tile tile = tile_at(ps.tl, t, KT);
         const uint64_t okc = ok, badc = bad;

@@ -154,11 +154,12 @@ DEV void append_mx(const AppendMxParams &p) {
         if (MODE == HALF) load8<E>(k + h * p.k_nb1 + to, y[i]);
         load8<E>(v + h * p.v_nb1, z[i]);
     }
+    int32_t at[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int a = 0; a < 4; a++)
+        if (a < p.tab.axes) at[a] = p.pos[a * p.pos_nb1 + t];
     if (slot < 0 || slot >= p.to.n_slots) return;  // padding, or a slot outside the cache
     if (turned) {
-        int32_t at[4];
-#pragma unroll
-        for (int a = 0; a < 4; a++) at[a] = a < p.tab.axes ? p.pos[a * p.pos_nb1 + t] : 0;
         double cs, sn;
         if (MODE == NORM) {
 #pragma unroll
