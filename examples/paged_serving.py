@@ -1,6 +1,6 @@
 """Attention of one decoder layer as a server runs it: a paged KV cache, prompts
 and generated tokens of several conversations in one batch, a system prompt that
-they share, a sliding window.
+they share, a sliding window; the cache in 16 bits, or quantized to 8 or 4.
 
     python examples/paged_serving.py
 
@@ -28,6 +28,14 @@ class Pages:
         self.tables[name] = self.tables[like][:shared // self.page] if like is not None else []
         self.length[name] = shared
 
+    def fork(self, name, like, n):
+        """A new conversation that goes on from `like`'s first n tokens: whole pages are shared -> the slots
+        of the cut page's rows, and where they are to be copied"""
+        cut = n // self.page * self.page
+        self.open(name, like, cut)
+        t = self.tables[like]
+        return [t[p // self.page] * self.page + p % self.page for p in range(cut, n)], self.extend(name, n - cut)[1]
+
     def extend(self, name, n):
         """Room for n more tokens -> (their positions, their slots)"""
         first, t = self.length[name], self.tables[name]
@@ -52,11 +60,26 @@ class Pages:
 
 
 class PagedAttention:
-    def __init__(self, be, weights, n_heads, n_kv, head, pages, page, rope, wtype=ghip.Q4_K, ctype=torch.float16, window=0, n_first=0):
-        """weights: {"q", "k", "v", "o"}: quantized blocks, rows by input"""
+    def __init__(self, be, weights, n_heads, n_kv, head, pages, page, rope, wtype=ghip.Q4_K, ctype=torch.float16, window=0, n_first=0,
+                 bits=16):
+        """weights: {"q", "k", "v", "o"}: quantized blocks, rows by input; bits: 16 (a cache of ctype), or 8 or 4"""
         self.be, self.w, self.ty, self.rope = be, weights, wtype, rope
         self.H, self.Hkv, self.D, self.window, self.n_first = n_heads, n_kv, head, window, n_first
-        self.kv = torch.zeros((pages, page, n_kv, 2 * head), dtype=ctype, device="cuda")
+        self.scales = None
+        if bits == 16:
+            self.kv = torch.zeros((pages, page, n_kv, 2 * head), dtype=ctype, device="cuda")
+        else:
+            self.kv, self.scales = ghip.mx_cache(pages, page, n_kv, head, bits)
+
+    def copy(self, src, dst):
+        """Rows of the cache, as they lie (a quantized row's values are those of its codes again)"""
+        src, dst = torch.tensor(src, device="cuda"), torch.tensor(dst, device="cuda")
+        if self.scales is None:
+            flat = self.kv.view(-1, *self.kv.shape[2:])
+            flat[dst] = flat[src]
+        else:
+            rows = self.be.kv_read(self.kv, src, self.scales)
+            self.be.kv_append(rows[..., :self.D], rows[..., self.D:], dst, self.kv, scales=self.scales)
 
     def __call__(self, x, b, n_shared=0):
         """x [T, hidden] f32 -> (attention's contribution to the residual, q, attention's output)"""
@@ -66,9 +89,9 @@ class PagedAttention:
         be.graph_compute([ghip.mul_mat_node(self.w[n], self.ty, hidden, x, y) for n, y in (("q", q), ("k", k), ("v", v))])
         q, k, v = q.view(T, self.H, D), k.view(T, self.Hkv, D), v.view(T, self.Hkv, D)
         be.rope(q, b["pos"], self.rope, out=q)
-        be.kv_append(k, v, b["slots"], self.kv, pos=b["pos"], rope=self.rope)
+        be.kv_append(k, v, b["slots"], self.kv, pos=b["pos"], rope=self.rope, scales=self.scales)
         o = be.flash_attn_paged(q, self.kv, b["seqs"], scale=D ** -0.5, window=self.window, n_first=self.n_first,
-                                n_shared=n_shared, max_q=b["max_q"])
+                                n_shared=n_shared, max_q=b["max_q"], scales=self.scales)
         return be.mul_mat(self.w["o"], self.ty, self.H * D, o.view(T, self.H * D)), q, o
 
 
@@ -79,9 +102,8 @@ def make(be, n_heads=8, n_kv=2, head=128, hidden=1024, pages=64, page=16, seed=0
     return PagedAttention(be, weights, n_heads, n_kv, head, pages, page, ghip.Rope(head, ghip.ROPE_NEOX, freq_base=500000.0), **kw), Pages(pages, page)
 
 
-def main():
-    be = ghip.Backend(0)
-    layer, pages = make(be)
+def converse(be, bits):
+    layer, pages = make(be, bits=bits)
     x = lambda n: torch.randn((n, 1024), device="cuda")
     pages.open("system")
     layer(x(48), pages.batch([("system", 48)]))
@@ -91,10 +113,19 @@ def main():
     # the users' first turns, of different length, then a few tokens each
     todo = list(zip(users, (20, 1, 33)))
     y, _, _ = layer(x(sum(n for _, n in todo)), pages.batch(todo), n_shared=48)
-    print("prompts", tuple(y.shape), float(y.abs().mean()))
+    print(f"{bits} bits: prompts", tuple(y.shape), float(y.abs().mean()))
     for _ in range(4):
         y, _, _ = layer(x(3), pages.batch([(u, 1) for u in users]), n_shared=48)
-    print("tokens", tuple(y.shape), float(y.abs().mean()))
+    # another answer to the first 60 tokens of a's
+    layer.copy(*pages.fork("d", "a", 60))
+    y, _, _ = layer(x(4), pages.batch([(u, 1) for u in users + ["d"]]), n_shared=48)
+    print(f"{bits} bits: tokens", tuple(y.shape), float(y.abs().mean()))
+
+
+def main():
+    be = ghip.Backend(0)
+    for bits in (16, 8, 4):
+        converse(be, bits)
 
 
 if __name__ == "__main__":
