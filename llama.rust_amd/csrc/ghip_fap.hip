@@ -319,14 +319,13 @@ struct Direct {
         // load f of 2 NI of tile t: one goes out under each fragment's products (bf16, 12
         // turns under 4001 keys, 128 rows: 125 us, and 130 with all of them at the step's
         // start; f16 the same)
-        DEV_M void load_part(int t, int u, int f) {
-            if (u) return;
+        DEV_M void load_part(int t, int f) {
             const int ii = f >> 1, kv = f & 1;
             load16(at[ii] + (kv ? 2 * p.D + rl.v_chunk(ii) : rl.k_chunk(ii)), lds_addr(kvs[t & 1][kv]) + 1024 * (NI * w + ii));
         }
-        DEV_M void load_half(int t, int u) {
+        DEV_M void load_half(int t, int) {
 #pragma unroll
-            for (int f = 0; f < 2 * NI; f++) load_part(t, u, f);
+            for (int f = 0; f < 2 * NI; f++) load_part(t, f);
         }
         DEV_M void load_first(int t) { load_half(t, 0); }
         DEV_M void middle(int) {}

@@ -662,12 +662,12 @@ DEV int prefix_of(const FapParams &p) {
 // L: how a tile comes into LDS.  L::Loads<DP> has
 //   ld.load_pages(t)     the page numbers of tile t's keys are on their way
 //   ld.find_tile(t)      where its rows are; ld.ok2, ld.bad2: its keys that are there, those on no page
-//   ld.load_part(t, u, f)  under fragment f of DP / 16 of half u of the tile before: loads of it go out
-//   ld.load_half(t, u)     all of those of half u
-//   ld.load_first(t)       the first tile's, of both (in after wait_loads and loaded())
-//   ld.middle(t)           between the halves
-//   ld.loaded(t)           this wavefront's loads of it are in: LDS holds its rows, 0 for values of keys not in ok
-//   L::LATE                half 1 has loads, and loads past the last tile do no harm (those of the tile found last)
+//   ld.load_part(t, f)   under fragment f of DP / 16 of the tile before's first half: a load of it goes out
+//   ld.load_half(t, u)   at the start of that tile's half u (not L::LATE: in place of all load_part): loads go out
+//   ld.load_first(t)     the first tile's loads, all of them (in after wait_loads and loaded())
+//   ld.middle(t)         between the halves
+//   ld.loaded(t)         this wavefront's loads of it are in: LDS holds its rows, 0 for values of keys not in ok
+//   L::LATE              both halves have loads, and past the last tile they do no harm (those of the tile found last)
 //   L::HOME_K            keys and values are in LDS 2^HOME_K times what they are
 //   L::NARROW            LDS cannot hold every tile: wide[t & 1] says that it does not hold tile t
 // BW: a block's rows, 64 each; RW of them are this pass's, from `half` on.  Returns whether
@@ -869,14 +869,15 @@ DEV bool fap_tile(const PARAMS &p, TileLds<L, DP, BW> &lds, int half = 0) {
             const bool need = work && (!part || (h0 < h1 && h0 <= w1 && (!p.window || h1 - 1 > w0 - p.window || h0 < p.n_first)));
             v4f s[2][RW];
             if (u == 1 && more) ld.middle(t + 1);
-            const bool loads = L::LATE || (u == 0 && more);
+            if (L::LATE) ld.load_half(t + 1, u);
+            const bool loads = !L::LATE && u == 0 && more;
             if (need) {
                 __builtin_amdgcn_s_setprio(1);
-                if (loads) scores<E, DP, RW, 2>(Q, Kh, s, [&](int f) { ld.load_part(t + 1, u, f); });
+                if (loads) scores<E, DP, RW, 2>(Q, Kh, s, [&](int f) { ld.load_part(t + 1, f); });
                 else scores<E, DP, RW, 2>(Q, Kh, s, [](int) {});
                 __builtin_amdgcn_s_setprio(0);
             } else if (loads) {
-                ld.load_half(t + 1, u);
+                ld.load_half(t + 1, 0);
             }
             if (need) {
                 if (part || badc) mask_scores<E, DP, RW, 2>(Q, s, tile.k0 + 32 * u, tile.ke, badc >> (32 * u), p.window, p.n_first);

@@ -1,5 +1,25 @@
 // ghip_fapq.hip -- attention over a quantized paged KV cache (codes and scales of ghip_mx.h).
 // The formula, tables, masks and partials are those of ghip_fap.hip.
+//
+// A code times its scale is exact in bfloat16, and where the scales are in a range (MxHalf) in float16
+// too, so the products are those over a 16-bit cache: q and p as three terms or two, the
+// error against 64 bits that of 32-bit arithmetic (0.15 .. 0.8e-6), whatever the codes' own rounding cost.
+//
+// Up to 32 rows a KV head (decode, drafted tokens): fapq_few, bound by memory, 264 bytes a key and value of
+// 128 dims in 8 bits, 136 in 4.  Long runs of keys reach 5.0 TB/s in 8 bits, what a large copy does;
+// in 4 bits 3.9, held by the conversions.  A wavefront takes tiles of its own, so
+// that nothing waits for the other three until the end, with the next tile's rows in registers.
+//   24 sequences of 500 .. 16384 keys, 32 heads over 8 of 128, 8 bits: 101 us, 4.4 TB/s
+//   64 sequences of 2000 .. 12000 keys, 4 bits: 125 us, 3.9 TB/s
+//   12 sequences of 5 or 6 drafted tokens, 900 .. 8192 keys, 8 bits: 44 us, 2.7 TB/s (20 of them launches, the
+//   first tile's latencies and the join)
+//
+// More rows: tiles of 64 or 128 rows, bound by the products and the vector work beside them.
+//   1702 rows of two prompts over 4000 .. 8192 keys, 8 bits: 400 us, 489 TFLOP/s of the formula's (two terms: twice
+//   that on the matrix cores); four of 2048 rows over 8192 keys: 580
+//   1290 rows of 64 heads over 8 of 64 in a window of 1024, 4 bits: 82 us
+// A prefix that the batch shares takes the tiles, the sequences' own keys the other way, in one launch:
+//   64 sequences over 8192 shared and 40 .. 600 own keys, 8 bits: 46 us with the join
 #include "ghip_fap_core.h"
 #include "ghip_mx.h"
 
@@ -123,7 +143,7 @@ DEV void find_keys_mx(const FapMxParams &p, const Tile &tl, int kt, int pg, int6
 }
 // Words and bytes of the cache.  The address has been through LDS, and of that the compiler cannot
 // tell that it is not LDS itself: said to be global memory, or the loads count as LDS's too
-// and each wait for LDS waits for memory (24 sequences of 500 .. 16384 keys: 118 us).
+// and each wait for LDS waits for memory (24 sequences of 500 .. 16384 keys: 118 us, 108 without).
 typedef const __attribute__((address_space(1))) uint8_t *in_memory;
 template <int W>
 DEV void load_words(uint32_t (&w)[W], const uint8_t *from) {
@@ -143,7 +163,7 @@ constexpr int few_keys(int bits, int DP) { return DP == 256 || bits == 8 ? 32 : 
 // Which part of the keys a workgroup takes: split z (of `of`) of sequence b, its tiles [t0, t1).
 // With p.wgs the sequences' tiles are shared out over that many workgroups, each sequence having
 // as many splits as its tiles are worth: of splits alike for all, the longest sequence's are the last to
-// end (24 sequences of 500 .. 16384 keys: 108 us).
+// end (24 sequences of 500 .. 16384 keys: 108 us, 102 so).
 struct Part {
     int b, z, of, t0, t1;
 };
@@ -378,7 +398,7 @@ DEV void fapq_few(const FapMxParams &p, FewqLds<BITS, DP, CG, RW> &lds) {
     const int units = (p.D + EL - 1) / EL, uv = min(lane % U, p.D / 16 - 1);
     // A tile is loaded as whole rows, 16 bytes a lane and a row's bytes in neighbouring lanes (loads of the
     // fragments' own places, 64 bytes of a line each, were twice the requests: 64 sequences of
-    // 8192 keys in 4 bits 162 us), and goes through LDS to the lanes that need it.
+    // 8192 keys in 4 bits: 162 us, 140 so), and goes through LDS to the lanes that need it.
     constexpr int RCH = DP * BITS / 64, RS = 16 * RCH, KPI = 64 / RCH, NLD = KT / KPI;
     uint32_t st[NLD][4], sc[SB / 4];  // (sc: a lane a key)
     const int chunk = 16 * min(lane % RCH, p.D * BITS / 64 - 1);
@@ -561,7 +581,6 @@ struct Decoded {
     template <int DP>
     struct Loads {
         static constexpr int KT = 64, CH = DP / 8, U = DP / 16, NL = 16 * U / 64, W = BITS / 2;
-        static_assert(NL <= DP / 16, "one load under each of a half's fragments");
         const FapMxParams &p;
         Lds &lds;
         uint8_t (&kvs)[2][2][64 * DP * 2];
@@ -573,11 +592,10 @@ struct Decoded {
         int pg[2];                        // page numbers of the tiles to be found next, a lane a key
         // keys, then values, of the tile on its way
         uint32_t x[NL][W], sc[NL];
-        int unit;
         DEV_M Loads(const FapMxParams &p_, Lds &lds_, uint8_t (&kvs_)[2][2][64 * DP * 2], int hk, const int32_t *row_, int w_,
                     const PagedTiles &tl_, int t1_)
             : p(p_), lds(lds_), kvs(kvs_), row(row_), w(w_), t1(t1_), tl(tl_), kvh((const uint8_t *)p_.kv + hk * p_.kv_head),
-              sch(p_.sc + hk * p_.sc_head), unit(min((int)(threadIdx.x & 63) % U, p_.D / 16 - 1)) {}
+              sch(p_.sc + hk * p_.sc_head) {}
         // a block's scale; what E cannot hold of a block that counts is seen in `wide`
         DEV_M float scale_of(uint32_t byte, const uint32_t (&x)[W], bool counts, bool &wide) const {
             if constexpr (!NARROW) {
@@ -594,7 +612,13 @@ struct Decoded {
                 return f;
             }
         }
-        DEV_M int key(int ii) const { return 16 * w + (64 * ii + (int)(threadIdx.x & 63)) / U; }
+        // (the lane as if it were another each time: or the addresses in LDS are worked out before the loop, into
+        // registers that the loop needs; 9 would spill)
+        static DEV_M int lane() {
+            int l = threadIdx.x & 63;
+            asm volatile("" : "+v"(l));
+            return l;
+        }
         DEV_M void load_pages(int t) {
             const Tile tile = tile_at(tl, min(t, t1 - 1), KT);
             const int j = min(tile.k0 + (int)(threadIdx.x & 63), tile.ke - 1);
@@ -606,15 +630,15 @@ struct Decoded {
             find_keys_mx(p, tile_at(tl, t, KT), KT, pg[0], lds.offs[w][0], lds.offs[w][1], ok2, bad2);
         }
         DEV_M void load_unit(int kv, int ii, uint32_t (&to)[W], uint32_t &scale) {
-            load_words(to, kvh + lds.offs[w][0][key(ii)] + unit * (2 * BITS) + (kv ? p.D * BITS / 8 : 0));
-            scale = load_byte(sch + lds.offs[w][1][key(ii)] + unit / 2 + (kv ? p.S : 0));
+            const int l = threadIdx.x & 63, key = 16 * w + (64 * ii + l) / U, unit = min(l % U, p.D / 16 - 1);
+            load_words(to, kvh + lds.offs[w][0][key] + unit * (2 * BITS) + (kv ? p.D * BITS / 8 : 0));
+            scale = load_byte(sch + lds.offs[w][1][key] + unit / 2 + (kv ? p.S : 0));
         }
-        DEV_M void load_part(int, int kv, int ii) {
-            if (ii < NL) load_unit(kv, ii, x[ii], sc[ii]);
-        }
-        DEV_M void load_half(int t, int kv) {
+        DEV_M void load_part(int, int) {}
+        // (before a half's products: among them they cost more, 1702 rows over 4000 .. 8192 keys 415 and 403 us)
+        DEV_M void load_half(int, int kv) {
 #pragma unroll
-            for (int ii = 0; ii < NL; ii++) load_part(t, kv, ii);
+            for (int ii = 0; ii < NL; ii++) load_unit(kv, ii, x[ii], sc[ii]);
         }
         DEV_M void load_first(int t) {
             uint32_t y[NL][W], ysc[NL];
@@ -626,11 +650,11 @@ struct Decoded {
         DEV_M void middle(int t) { decode(t, 0, ok2, x, sc); }
         DEV_M void loaded(int t) { decode(t, 1, ok, x, sc); }
         DEV_M void decode(int t, int kv, uint64_t ok, const uint32_t (&x)[NL][W], const uint32_t (&sc)[NL]) {
-            const int u = (threadIdx.x & 63) % U;
+            const int l = lane(), u = l % U;
             bool wide = false;
 #pragma unroll
             for (int ii = 0; ii < NL; ii++) {
-                const int r = key(ii);
+                const int r = 16 * w + (64 * ii + l) / U;
                 const bool there = (ok >> r) & 1;
                 const float f = scale_of(sc[ii], x[ii], there, wide);
                 v8 lo = mx_eight<BITS>(&x[ii][0], f, v8{}), hi = mx_eight<BITS>(&x[ii][W / 2], f, v8{});
@@ -646,8 +670,10 @@ struct Decoded {
     };
 };
 
-// Tiles of 64 BW rows: as float16, two terms of q and p for each of its products, and where a tile has blocks that
-// float16 does not hold (MxHalf) once more as bfloat16, three terms.
+// Tiles of 64 BW rows: as float16, two terms of q and p, and where a tile has blocks that float16 does not
+// hold (MxHalf) once more as bfloat16, three terms: the workgroup stops at such a tile and starts again.
+// (1702 rows over 4000 .. 8192 keys, 8 bits: 568 us as bfloat16 alone, 535 as float16 with 64 rows, 400 with 128,
+// whose fragments each serve four products.)
 template <int BITS, int DP, int BW>
 union FapqTileLds {
     TileLds<Decoded<BITS, f16>, DP, BW> half;
