@@ -3393,6 +3393,7 @@ ghip_status ghip_kv_append_mx(ghip_context *ctx, const ghip_tensor *k, const ghi
     if (const char *why = mx_cache(kv, scales, D)) return bad(why);
     if (kv->ne[1] != H) return bad("kv must be [2 D, H_kv, page, pages]");
     if (T > INT32_MAX) return bad("dimension too large");
+    if (T > (1ll << 32) / H) return bad("k too large");
     if (slots->type != GHIP_TYPE_I64 || !packed(slots, 8) || slots->ne[0] < T) return bad("slots must be I64, one for each token");
     AppendMxParams p;
     p.P = p.tab.axes = 0;

@@ -204,7 +204,7 @@ DEV bool find_part(const FapMxParams &p, int no, Part &w) {
     for (int b0 = 0; b0 < p.B; b0 += 64) {
         const int n = b0 == 0 ? first : b0 + lane < p.B ? tiles_of(b0 + lane) : 0;
         live += __popcll(__ballot(n > 0));
-        total += lane_sum(n);
+        total += (uint32_t)lane_sum(n);  // (2^25 tiles each at most)
     }
     // The fewest tiles a part that need no more parts than there are workgroups: with total / (wgs - live)
     // they never do; up to 64 sequences the least is looked for.

@@ -194,3 +194,13 @@ def test_paged_refuses(ctx):
     # the cache of the other call
     st = L.ghip_flash_attn_paged(ctx, args[0], args[1], args[3], None, args[5], args[6], None)
     assert st != 0 and "F16 or BF16" in L.ghip_last_error(ctx).decode()
+
+
+def test_append_of_more_than_can_be_counted(ctx):
+    """Tokens times heads past what 64 bits of threads hold (strides of 0)."""
+    import ghip
+    n = 2 ** 31 - 1
+    k, v = (T(0, [256, n, n], a, 4, [4, 0, 0, 0]) for a in (A[0], A[1]))
+    kv, sc = codes(ghip.E4M3, [512, n, 1, 1], A[3], [1, 0, 0, 0]), scales_of(256, n, 1, 1, A[5], [1, 0, 0, 0])
+    st, msg = run_append(ctx, D=256, Hkv=n, N=n, k=k, v=v, kv=kv, sc=sc, slots=T(ghip.I64, [n], A[2]), rope=False, pos=None)
+    assert st != 0 and "k too large" in msg, msg
