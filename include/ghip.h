@@ -393,8 +393,10 @@ ghip_status ghip_flash_attn_paged_workspace(const ghip_tensor *q, const ghip_ten
                                             const ghip_paged_params *params, const ghip_tensor *dst, size_t *bytes);
 
 /* The same over a quantized cache (ghip_kv_append_mx): attention over the values that its
- * codes stand for, to 32 bits as over a BF16 cache.  D a multiple of 16; all else as above.  A row that
- * sees a NaN block gives NaN, in full or where the value's is, as 32-bit arithmetic has it. */
+ * codes stand for, as close as 32-bit arithmetic brings it whatever the sizes of its blocks: q and p count in
+ * 24 bits, or in 22 where that moves no score by more than 2^-23 and no value outweighs it.  D a multiple of 16;
+ * all else as above.  A row that sees a NaN block gives NaN, in full or where the value's is, as 32-bit
+ * arithmetic has it. */
 ghip_status ghip_flash_attn_paged_mx(ghip_context *ctx, const ghip_tensor *q, const ghip_tensor *kv, const ghip_tensor *scales,
                                      const ghip_tensor *seqs, const ghip_tensor *sinks, const ghip_paged_params *params,
                                      const ghip_tensor *dst, void *stream);

@@ -184,9 +184,11 @@ DEV void raw_wait(RawRow<DP> &r) {
 #pragma unroll
         for (int e = 0; e < 8; e++) asm volatile("" : "+v"(r.x[kk][e]));
 }
+// Returns k of a scaled row's 2^k, 127 where that says nothing (all 0, infinite).
 template <typename E, int DP, int RW>
-DEV void rows_start(Rows<E, DP, RW> &R, int rt, const RawRow<DP> &r, float scale) {
+DEV int rows_start(Rows<E, DP, RW> &R, int rt, const RawRow<DP> &r, float scale) {
     int k = 0;
+    bool sized = false;
     if constexpr (Frag<E>::SCALED) {
         float mx = 0.0f;
 #pragma unroll
@@ -194,7 +196,8 @@ DEV void rows_start(Rows<E, DP, RW> &R, int rt, const RawRow<DP> &r, float scale
 #pragma unroll
             for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(r.x[kk][e] * scale));
         mx = row_max(mx);
-        if (mx > 0.0f && mx < __builtin_inff()) k = min(15 - __builtin_amdgcn_frexp_expf(mx), 100);
+        sized = mx > 0.0f && mx < __builtin_inff();
+        if (sized) k = min(15 - __builtin_amdgcn_frexp_expf(mx), 100);
     }
     R.unit[rt] = __builtin_amdgcn_ldexpf(1.0f, -k);
     R.zero = v4f{0, 0, 0, 0};
@@ -221,6 +224,7 @@ DEV void rows_start(Rows<E, DP, RW> &R, int rt, const RawRow<DP> &r, float scale
     R.mneg[rt] = typename Frag<E>::ref{};
     R.l[rt] = 0.0f;
     R.from[rt] = R.pos[rt] < 0 ? -__builtin_inff() : __builtin_inff();
+    return sized ? k : 127;
 }
 
 // Fragment reads.  The swizzles touch the low bits of a chunk's number alone, so
@@ -669,9 +673,11 @@ DEV int prefix_of(const FapParams &p) {
 //   ld.loaded(t)         this wavefront's loads of it are in: LDS holds its rows, 0 for values of keys not in ok
 //   L::LATE              both halves have loads, and past the last tile they do no harm (those of the tile found last)
 //   L::HOME_K            keys and values are in LDS 2^HOME_K times what they are
-//   L::NARROW            LDS cannot hold every tile: wide[t & 1] says that it does not hold tile t
+//   L::NARROW            E does not do for every tile:
+//   ld.rows_at(k)        this lane's rows' least k (rows_start)
+//   ld.beyond(t)         does it not do for tile t, or one before?  The same for all wavefronts
 // BW: a block's rows, 64 each; RW of them are this pass's, from `half` on.  Returns whether
-// a tile was met that LDS cannot hold; then nothing has been stored.
+// a tile was met that E does not do for; then nothing has been stored.
 template <typename L, int DP, int BW>
 struct TileLds {
     uint8_t kvs[2][2][64 * DP * 2];  // this tile's K and V, the next one's
@@ -840,20 +846,21 @@ DEV bool fap_tile(const PARAMS &p, TileLds<L, DP, BW> &lds, int half = 0) {
         ld.bad = ld.bad2;
         if (t0 + 1 < t1) ld.find_tile(t0 + 1);
     }
+    int k = 127;
 #pragma unroll
     for (int rt = 0; rt < RW; rt++) {
-        rows_start<E, DP, RW>(Q, rt, raw[rt], p.scale * kLog2e);
+        k = min(k, rows_start<E, DP, RW>(Q, rt, raw[rt], p.scale * kLog2e));
         if constexpr (L::HOME_K != 0) Q.unit[rt] *= LESS;
     }
+    if constexpr (L::NARROW) ld.rows_at(k);
     if (t0 < t1) {
         wait_loads<0>();
         ld.loaded(t0);
     }
     __syncthreads();
     for (int t = t0; t < t1; t++) {
-        // (said before the last barrier; the next to say it in this place do so behind the next barrier)
         if constexpr (L::NARROW)
-            if (__builtin_amdgcn_readfirstlane(lds.ld.wide[t & 1])) return true;
+            if (ld.beyond(t)) return true;
         const Tile tile = tile_at(ps.tl, t, KT);
         const uint64_t badc = ld.bad;
         const bool part = !tile_whole(tile, KT, ps, p.window, p.n_first);

@@ -1,9 +1,10 @@
 // ghip_fapq.hip -- attention over a quantized paged KV cache (codes and scales of ghip_mx.h).
 // The formula, tables, masks and partials are those of ghip_fap.hip.
 //
-// A code times its scale is exact in bfloat16, and where the scales are in a range (MxHalf) in float16
-// too, so the products are those over a 16-bit cache: q and p as three terms or two, the
-// error against 64 bits that of 32-bit arithmetic (0.15 .. 0.8e-6), whatever the codes' own rounding cost.
+// A code times its scale is exact in bfloat16, and where the scales are in a range in float16
+// too, so the products are those over a 16-bit cache: q and p as three terms or, of float16 and where that
+// costs no more than 32-bit arithmetic does (MxHalf), two; the error against 64 bits is that of 32-bit
+// arithmetic (0.15 .. 0.8e-6), whatever the codes' own rounding cost.
 //
 // Up to 32 rows a KV head (decode, drafted tokens): fapq_few, bound by memory, 264 bytes a key and value of
 // 128 dims in 8 bits, 136 in 4.  Long runs of keys reach 5.0 TB/s in 8 bits, what a large copy does;
@@ -178,6 +179,16 @@ DEV int lane_sums(int x) {
     return x;
 }
 DEV int lane_sum(int x) { return __builtin_amdgcn_readlane(lane_sums(x), 63); }
+// the largest of all lanes, x >= 0
+DEV int lane_max(int x) {
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false));
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false));
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false));
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false));
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));
+    return __builtin_amdgcn_readlane(x, 63);
+}
 template <int KT>
 DEV bool find_part(const FapMxParams &p, int no, Part &w) {
     const int lane = threadIdx.x & 63;
@@ -575,8 +586,15 @@ struct Decoded {
     static constexpr int HOME_K = NARROW ? Half::HOME : 0;
     struct Lds {
         int64_t offs[4][2][64];
-        int wide[2];
+        // Of the tiles in this place so far: the largest scale's byte of keys, or more where float16 will not do; the largest
+        // and 255 less the smallest of values.  And 127 less k of the rows.
+        alignas(16) int seen[2][4];
+        int news[2]; // the last one's number, and one, where `seen` of it holds more than what was known
     };
+    static DEV_M void start(Lds &l) {
+        if (threadIdx.x < 8) l.seen[threadIdx.x / 4][threadIdx.x % 4] = 0;
+        if (threadIdx.x < 2) l.news[threadIdx.x] = 0;
+    }
     typedef typename Frag<E>::v8 v8;
     template <int DP>
     struct Loads {
@@ -592,24 +610,69 @@ struct Decoded {
         int pg[2];                        // page numbers of the tiles to be found next, a lane a key
         // keys, then values, of the tile on its way
         uint32_t x[NL][W], sc[NL];
+        // What tiles up to this one have had, in one scalar register, a byte each: keys' scales from Half::KEYS on, values' least
+        // scale and how many there are from it on.
+        uint32_t known = 0;
         DEV_M Loads(const FapMxParams &p_, Lds &lds_, uint8_t (&kvs_)[2][2][64 * DP * 2], int hk, const int32_t *row_, int w_,
                     const PagedTiles &tl_, int t1_)
             : p(p_), lds(lds_), kvs(kvs_), row(row_), w(w_), t1(t1_), tl(tl_), kvh((const uint8_t *)p_.kv + hk * p_.kv_head),
               sch(p_.sc + hk * p_.sc_head) {}
-        // a block's scale; what E cannot hold of a block that counts is seen in `wide`
-        DEV_M float scale_of(uint32_t byte, const uint32_t (&x)[W], bool counts, bool &wide) const {
-            if constexpr (!NARROW) {
-                return mx_scale(byte);
-            } else {
-                float f = mx_scale(byte + HOME_K);
-                if (byte - Half::FROM > Half::UP) {  // a block of zeros will do
-                    uint32_t any = byte == 255;
+        DEV_M void rows_at(int k) {
+            const int x = lane_max(127 - k), i = threadIdx.x & 63;
+            if (i < 2) atomicMax(&lds.seen[i][3], x);
+        }
+        // (said before the last barrier; the next to say it in this place do so behind the next barrier)
+        DEV_M bool beyond(int t) {
+            if (__builtin_expect(__builtin_amdgcn_readfirstlane(lds.news[t & 1]) != t + 1, 1)) return false;
+            const int4 s = *(const int4 *)lds.seen[t & 1];
+            const int keys = max((int)(known & 255) + Half::KEYS - 1, __builtin_amdgcn_readfirstlane(s.x)), n = known >> 16,
+                      from = min(n ? (int)(known >> 8) & 255 : 255, 255 - __builtin_amdgcn_readfirstlane(s.z)),
+                      to = max(n ? ((int)(known >> 8) & 255) + n - 1 : 0, __builtin_amdgcn_readfirstlane(s.y));
+            known = max(to - from + 1, 0) << 16 | from << 8 | (keys + 1 - Half::KEYS);
+            return keys > Half::largest_scale(127 - __builtin_amdgcn_readfirstlane(s.w), p.D) || to - from > Half::APART;
+        }
+        // Is one of the codes of a unit's block, whose other half lane ^ 1 has, STRONG or more?
+        static DEV_M bool strong(const uint32_t (&x)[W]) {
+            const int y = (int)Half::strong(x);
+            return (y | __builtin_amdgcn_mov_dpp(y, 0xB1, 0xf, 0xf, true)) != 0;
+        }
+        // What decides about float16 of a tile's keys (values), a lane's units.  Hardly ever more than the comparisons with
+        // what is known; then those of rows that are there.
+        DEV_M void look(int t, int kv, uint64_t ok, const uint32_t (&x)[NL][W], const uint32_t (&sc)[NL]) {
+            const uint32_t least = kv ? (known >> 8) & 255 : Half::KEYS, n = kv ? known >> 16 : known & 255;
+            uint32_t most = 0;
+            bool news = false;
 #pragma unroll
-                    for (int i = 0; i < W; i++) any |= x[i] & (BITS == 8 ? 0x7f7f7f7f : 0x77777777);
-                    wide = wide || (any && counts);
-                    f = 1.0f;
+            for (int ii = 0; ii < NL; ii++) {
+                most = max(most, sc[ii] - least);
+                if (kv) news |= !strong(x[ii]);
+            }
+            if (__builtin_expect(!__ballot(news || most >= n), 1)) return;
+            const int l = lane();
+            auto there = [&](int ii) { return ((ok >> (16 * w + (64 * ii + l) / U)) & 1) != 0; };
+            int to = 0, from = 0, no = 0;
+#pragma unroll
+            for (int ii = 0; ii < NL; ii++) {
+                const int b = (int)sc[ii];
+                const bool weak = kv && !strong(x[ii]), counts = there(ii) && (kv || Half::any(x[ii]) || b == 255);
+                to = max(to, counts ? b : 0);
+                from = max(from, counts ? 255 - b : 0);
+                no = counts && (weak || b < (kv ? Half::VALUES : Half::KEYS) || b > Half::TO) ? 256 : no;
+            }
+            // (one lane for all: 64 atomics on one place take their turns)
+            no = lane_max(kv ? no : max(no, to));
+            if (kv) {
+                to = lane_max(to);
+                from = lane_max(from);
+            }
+            if (l == 0) {
+                int *seen = lds.seen[t & 1];
+                lds.news[t & 1] = t + 1;
+                if (no) atomicMax(&seen[0], no);
+                if (kv) {
+                    atomicMax(&seen[1], to);
+                    atomicMax(&seen[2], from);
                 }
-                return f;
             }
         }
         // (the lane as if it were another each time: or the addresses in LDS are worked out before the loop, into
@@ -651,12 +714,16 @@ struct Decoded {
         DEV_M void loaded(int t) { decode(t, 1, ok, x, sc); }
         DEV_M void decode(int t, int kv, uint64_t ok, const uint32_t (&x)[NL][W], const uint32_t (&sc)[NL]) {
             const int l = lane(), u = l % U;
-            bool wide = false;
+            if constexpr (NARROW) {
+                look(t, kv, ok, x, sc);
+                __builtin_amdgcn_sched_barrier(0);
+            }
 #pragma unroll
             for (int ii = 0; ii < NL; ii++) {
                 const int r = 16 * w + (64 * ii + l) / U;
                 const bool there = (ok >> r) & 1;
-                const float f = scale_of(sc[ii], x[ii], there, wide);
+                // (past float16's range 0 is to stay 0)
+                const float f = mx_scale(NARROW ? min(sc[ii] + HOME_K, 254u) : sc[ii]);
                 v8 lo = mx_eight<BITS>(&x[ii][0], f, v8{}), hi = mx_eight<BITS>(&x[ii][W / 2], f, v8{});
                 // rows that were not there: no value of theirs may count
                 if (!there) lo = hi = v8{};
@@ -664,14 +731,12 @@ struct Decoded {
                 *(v8 *)(to + 16 * (kv ? v_swz<CH>(r, 2 * u) : k_swz<CH>(r, 2 * u))) = lo;
                 *(v8 *)(to + 16 * (kv ? v_swz<CH>(r, 2 * u + 1) : k_swz<CH>(r, 2 * u + 1))) = hi;
             }
-            if constexpr (NARROW)
-                if (wide) lds.wide[t & 1] = 1;
         }
     };
 };
 
-// Tiles of 64 BW rows: as float16, two terms of q and p, and where a tile has blocks that float16 does not
-// hold (MxHalf) once more as bfloat16, three terms: the workgroup stops at such a tile and starts again.
+// Tiles of 64 BW rows: as float16, two terms of q and p, and where that does not do for the keys and values so
+// far (MxHalf) once more as bfloat16, three terms: the workgroup stops at such a tile and starts again.
 // (1702 rows over 4000 .. 8192 keys, 8 bits: 568 us as bfloat16 alone, 535 as float16 with 64 rows, 400 with 128,
 // whose fragments each serve four products.)
 template <int BITS, int DP, int BW>
@@ -681,7 +746,7 @@ union FapqTileLds {
 };
 template <int BITS, int DP, int BW>
 DEV void fapq_tile(const FapMxParams &p, FapqTileLds<BITS, DP, BW> &lds) {
-    if (threadIdx.x < 2) lds.half.ld.wide[threadIdx.x] = 0;
+    Decoded<BITS, f16>::start(lds.half.ld);
     if (!fap_tile<Decoded<BITS, f16>, f16, DP, BW>(p, lds.half)) return;
     for (int half = 0; half < BW; half++) {  // (what the registers hold of three terms)
         __syncthreads();

@@ -110,10 +110,40 @@ DEV mx_bf8 mx_eight(const uint32_t *w, float s) { return mx_eight<BITS>(w, s, mx
 
 // float16 holds a code times 2^e exactly too, if e is in a range: with 8 bits, all of 2^-9 .. 448, -15 .. 7;
 // with 4, all of 0.5 .. 6, -23 .. 13.  A cache's elements are taken 2^HOME times, so that the
-// range lies about what they are like: blocks whose largest is 2^-12 .. 896, or 2^-21 .. 57344.
-// The byte of a scale is in range if byte - FROM (unsigned) <= UP.
+// range lies about what they are like: blocks whose largest is 2^-14 .. 224, or 2^-21 .. 57344.
+// Exact elements are not all that a sum of products needs, so tiles are computed with as float16 only if
+//   keys:   what q's second term leaves off (2^-25 of units in which the row's largest element is 2^14 .. 2^15)
+//           moves no score by more than 2^-24, in log2 units: D 2^-25 times the largest code, scale and unit;
+//   values: what p's terms leave off (2^-25, of 2^8 or more that a row's largest p is) does not outweigh the
+//           rounding of a sum of as many products in 32 bits: the largest elements of all blocks lie within
+//           2^9 of one another (codes of STRONG or more, scales at most 2^APART apart).
+// And the matrix cores line products up as if an operand below 2^-14 were 2^-14, so a sum whose operands
+// are all smaller has fewer bits (measured: values of 2^-23 cost 2^-17 of the output).  So no value that is not 0 lies
+// below 2^-17 (2^-38 of p a product: 2^-21 of the element at worst); of keys it is 2^-23 a product, in units of
+// 2^-(k + HOME) of a score, of which k + HOME >= SMALL makes too little to count.
+// A block of zeros counts as a key of any scale, and as values too weak.
 template <int BITS>
 struct MxHalf {
-    static constexpr int HOME = BITS == 8 ? 6 : 0;
-    static constexpr uint32_t FROM = 127 - (BITS == 8 ? 15 : 23) - HOME, UP = BITS == 8 ? 22 : 36;
+    static constexpr int HOME = BITS == 8 ? 8 : 0, SMALL = 4;
+    // the bytes of scales, from .. to
+    static constexpr int KEYS = 127 - (BITS == 8 ? 15 : 23) - HOME, VALUES = 127 - (BITS == 8 ? 8 : 16) - HOME,
+                              TO = 127 + (BITS == 8 ? 7 : 13) - HOME;
+    static constexpr int LARGEST = BITS == 8 ? 448 : 6, STRONG = BITS == 8 ? 64 : 2, APART = BITS == 8 ? 6 : 7;
+    static_assert((LARGEST << APART) <= STRONG << 9, "values within 2^9 of one another");
+    // not 0: one of these BITS / 2 words' codes is STRONG or more
+    static __device__ __forceinline__ uint32_t strong(const uint32_t (&x)[BITS / 2]) {
+        uint32_t r = 0;
+#pragma unroll
+        for (int i = 0; i < BITS / 2; i++) r |= BITS == 8 ? (x[i] & 0x7f7f7f7f) + 0x18181818 : x[i];  // (0x68 is 64)
+        return r & (BITS == 8 ? 0x80808080 : 0x44444444);
+    }
+    // ... is not 0
+    static __device__ __forceinline__ uint32_t any(const uint32_t (&x)[BITS / 2]) {
+        uint32_t r = 0;
+#pragma unroll
+        for (int i = 0; i < BITS / 2; i++) r |= x[i];
+        return r & (BITS == 8 ? 0x7f7f7f7f : 0x77777777);
+    }
+    // The largest scale of keys for rows of q of which the largest is held 2^k times
+    static __device__ __forceinline__ int largest_scale(int k, int D) { return k + HOME < SMALL ? 0 : 128 + k - (32 - __builtin_clz(D * LARGEST - 1)); }
 };
