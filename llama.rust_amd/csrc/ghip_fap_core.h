@@ -294,15 +294,18 @@ template <typename E, int DP, int RW, int NT>
 DEV void mask_scores(const Rows<E, DP, RW> &R, v4f (&s)[NT][RW], int k0, int ke, uint64_t bad, int window, int n_first) {
     // (first: what a key on no page was scored with may be minus infinity too)
     if (bad) {
-        const uint64_t mine = bad >> (4 * ((threadIdx.x & 63) >> 4));
+        int g4 = 4 * ((threadIdx.x & 63) >> 4);
+        asm volatile("" : "+v"(g4));
 #pragma unroll
-        for (int t = 0; t < NT; t++)
+        for (int t = 0; t < NT; t++) {
+            const uint32_t mine = (uint32_t)(bad >> (16 * t)) >> g4;
 #pragma unroll
             for (int v = 0; v < 4; v++)
-                if ((mine >> (16 * t + v)) & 1) {
+                if ((mine >> v) & 1) {
 #pragma unroll
                     for (int rt = 0; rt < RW; rt++) s[t][rt][v] = __builtin_nanf("");
                 }
+        }
     }
     const int at = k0 + 4 * ((threadIdx.x & 63) >> 4);
     // seen(c, lo, hi): is this lane's key c in sight of a row?
