@@ -73,7 +73,7 @@ class PagedAttention:
 
     def copy(self, src, dst):
         """Rows of the cache, as they lie (a quantized row's values are those of its codes again)"""
-        src, dst = torch.tensor(src, device="cuda"), torch.tensor(dst, device="cuda")
+        src, dst = (torch.tensor(x, dtype=torch.int64).cuda() for x in (src, dst))
         if self.scales is None:
             flat = self.kv.view(-1, *self.kv.shape[2:])
             flat[dst] = flat[src]
