@@ -328,7 +328,8 @@ ghip_status ghip_kv_append(ghip_context *ctx, const ghip_tensor *k, const ghip_t
  *   scales:  E8M0 [2 S, H_kv, page, pages] (nb0 == 1), data and strides multiples of 2 S
  * For each slot and KV head scales hold a byte for every 32 elements of the key, in S
  * bytes, then of the value; S is D / 32 rounded up to 1, 2, 4 or 8.  An element is
- * its code times 2^(byte - 127); below 2^-126 it may count as 0.  A block with byte 255 is NaN.
+ * its code times 2^(byte - 127), as a number of 32 bits: below 2^-126 it may count as 0, from 2^128
+ * on it is infinite.  A block with byte 255 is NaN.
  *
  * Writing a block takes the least power of two from 2^-100 on that brings its largest
  * element to at most 448 (E4M3) or 7 (E2M1: what is over 6 becomes 6) and rounds each

@@ -11,14 +11,14 @@
 // in 4 bits 3.9, held by the conversions.  A wavefront takes tiles of its own, so
 // that nothing waits for the other three until the end, with the next tile's rows in registers.
 //   24 sequences of 500 .. 16384 keys, 32 heads over 8 of 128, 8 bits: 101 us, 4.4 TB/s
-//   64 sequences of 2000 .. 12000 keys, 4 bits: 125 us, 3.9 TB/s
+//   64 sequences of 2000 .. 12000 keys, 4 bits: 125 us, 3.9 TB/s, once the card runs steadily
 //   12 sequences of 5 or 6 drafted tokens, 900 .. 8192 keys, 8 bits: 44 us, 2.7 TB/s (20 of them launches, the
 //   first tile's latencies and the join)
 //
 // More rows: tiles of 64 or 128 rows, bound by the products and the vector work beside them.
 //   1702 rows of two prompts over 4000 .. 8192 keys, 8 bits: 400 us, 489 TFLOP/s of the formula's (two terms: twice
 //   that on the matrix cores); four of 2048 rows over 8192 keys: 580
-//   1290 rows of 64 heads over 8 of 64 in a window of 1024, 4 bits: 82 us
+//   1290 rows of 64 heads over 8 of 64 in a window of 1024, 4 bits: 80 us
 // A prefix that the batch shares takes the tiles, the sequences' own keys the other way, in one launch:
 //   64 sequences over 8192 shared and 40 .. 600 own keys, 8 bits: 46 us with the join
 #include "ghip_fap_core.h"
@@ -738,7 +738,8 @@ struct Decoded {
 // Tiles of 64 BW rows: as float16, two terms of q and p, and where that does not do for the keys and values so
 // far (MxHalf) once more as bfloat16, three terms: the workgroup stops at such a tile and starts again.
 // (1702 rows over 4000 .. 8192 keys, 8 bits: 568 us as bfloat16 alone, 535 as float16 with 64 rows, 400 with 128,
-// whose fragments each serve four products.)
+// whose fragments each serve four products.  All blocks out of range: 625, the two halves of 128 rows one after the
+// other as bfloat16; one block, of a late key of each sequence: 957, which is both passes.)
 template <int BITS, int DP, int BW>
 union FapqTileLds {
     TileLds<Decoded<BITS, f16>, DP, BW> half;
